@@ -130,6 +130,65 @@ int omni_mrope_kv_write_partials(void* qkv, int qkv_stride, const float* partial
 int omni_kv_copy_slot(void* pool, int n_layers, int pool_rows, int max_len, int row_halfs,
                       int src, int dst, int64_t length, int64_t* lengths, void* stream);
 
+/* The accepted path of each drafted tree (omni_tree_plan) made the end of its sequence: rows
+ * starts[s] + path[s][j] of pool row slots[s] (or s) move to starts[s] + j in every layer's K and
+ * V, j < emitted[s], and lengths[slot] = starts[s] + emitted[s] (at most max_len).  path int32
+ * [n][n_nodes] ascends from node 0; one that does not ascend within the tree ends there.  The
+ * sequences' pool rows are all different; one outside the pool is left alone. */
+int omni_kv_accept(void* pool, int n_layers, int pool_rows, int max_len, int row_halfs,
+                   const int64_t* slots, const int64_t* starts, const int* path,
+                   const int* emitted, int n, int n_nodes, int64_t* lengths, void* stream);
+
+/* K/V rows fp16 [tokens][row_halfs] (strides in halfs, multiples of 8; 16-byte aligned) to pool
+ * rows slots[t] at positions[t]; those outside the pool are skipped. */
+int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       void* k_cache, void* v_cache, const int64_t* slots,
+                       const int64_t* positions, int pool_rows, int max_len, int row_halfs,
+                       int tokens, void* stream);
+
+/* ---------------------------------------------------------------- drafted trees */
+
+/* The plan of a step over n drafted trees of n_nodes <= 64 nodes, behind the valid prefixes
+ * lengths[slots[s]] (slots NULL: pool row s).  parents int32 [n][n_nodes]: -1, or anything that
+ * is not an earlier node, for none; counts int32 [n] nodes in use (NULL: all); rope_delta int64
+ * per pool row or NULL.  Writes starts int64 [n] (the prefix lengths), ancestors uint64
+ * [n][n_nodes] (bit j: node j is the node or above it; 0 for a node not in use), positions int64
+ * [3][n * n_nodes] (starts + depth + rope_delta), token_slot / token_pos int64 [n * n_nodes] (where
+ * the nodes' K/V goes; token_slot -1: nowhere). */
+int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
+                   const int64_t* lengths, const int64_t* rope_delta, int n, int n_nodes,
+                   int pool_rows, int max_len, int64_t* starts, void* ancestors,
+                   int64_t* positions, int64_t* token_slot, int64_t* token_pos, void* stream);
+
+/* Attention of the trees' nodes over the pool: node i of sequence s (row s * n_nodes + i of q and
+ * out, fp16, strides in halfs) attends to keys [0, starts[s]) of its pool row and to starts[s] + j
+ * for its ancestors j; nodes not in use and sequences outside the pool leave their out rows as
+ * they were.  splits workgroups share a sequence's keys (1..256): splits > 1 leaves softmax states
+ * in workspace (fp32, n * n_nodes * n_heads * splits * 132 floats) for a second launch.  head_dim
+ * 128; scale a positive normal fp32; 16-byte aligned operands. */
+int omni_tree_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache,
+                        int pool_rows, int max_len, const int64_t* slots, const int64_t* starts,
+                        const void* ancestors, int n, int n_nodes, void* out, int out_stride,
+                        int n_heads, int n_kv_heads, int head_dim, float scale, int splits,
+                        float* workspace, int64_t workspace_floats, void* stream);
+
+/* Verification of drafted tokens.  logits [n][n_nodes][vocab] (dtype 0 fp16, 1 bf16, 2 fp32;
+ * strides in elements), tokens int64, uniforms fp32 [n][n_nodes]; parents int32 [n][n_nodes] for
+ * trees of proposed tokens, NULL for chains; draft (chains only) the logits [n][n_nodes - 1][vocab]
+ * that the tokens were drawn from; counts int32 [n] nodes in use or NULL; temperature fp32 [n], or
+ * NULL and temp for all (0: greedy, uniforms may then be NULL).  With p = softmax(logits /
+ * temperature) a node's child x stands if u (1 - p(tried siblings)) < p(x), with a draft if u q(x)
+ * < p(x); the next token is drawn with u_0 from what is left of p.  Writes path int32, out_tokens
+ * int64 [n][n_nodes] (-1 past emitted[s]) and emitted int32 [n].  workspace: doubles, as many as
+ * omni_spec_verify_work gives (-1: too many to count). */
+int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted);
+int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t row_stride,
+                     const void* draft, int64_t draft_seq_stride, int64_t draft_row_stride,
+                     const int64_t* tokens, const int* parents, const int* counts,
+                     const float* uniforms, const float* temperature, float temp, int n,
+                     int n_nodes, int vocab, int* path, int64_t* out_tokens, int* emitted,
+                     void* workspace, int64_t workspace_doubles, void* stream);
+
 /* ---------------------------------------------------------------- attention */
 
 /* _CacheView.flash_decode (cache/kv_prealloc.py:272-290): GQA decode attention over the

@@ -72,6 +72,14 @@ SIGNATURES = {
                                     _F, _I, _I, _P],
     "omni_prefill_attention_split": [_P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I,
                                      _F, _P],
+    "omni_tree_plan": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P],
+    "omni_kv_write_rows": [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "omni_tree_attention": [_P, _I, _P, _P, _I, _I, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _F, _I,
+                            _P, _I64, _P],
+    "omni_kv_accept": [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P],
+    "omni_spec_verify_work": [_I, _I, _I, _I],
+    "omni_spec_verify": [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _F, _I, _I, _I,
+                         _P, _P, _P, _P, _I64, _P],
     "omni_w4a16_gemm": [_P, _I, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
     "omni_f16_gemm": [_P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
     "omni_f16_gemm_tiled": [_P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P],
@@ -158,3 +166,15 @@ def require_cuda(*tensors, dtype=None, contiguous=True) -> None:
             raise TypeError(f"expected {dtype}, got {t.dtype}")
         if contiguous and not t.is_contiguous():
             raise ValueError("expected a contiguous tensor")
+
+
+def require_here(*tensors) -> None:
+    """Refuse tensors off the current device: launches go to its current stream."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("omniserver_amd ops run on the GPU only (got a CPU tensor)")
+        if t.device.index != torch._C._cuda_getDevice():
+            raise RuntimeError(f"tensor on {t.device}, but the current device is "
+                               f"cuda:{torch._C._cuda_getDevice()}")

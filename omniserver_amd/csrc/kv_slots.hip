@@ -73,3 +73,64 @@ extern "C" int omni_kv_copy_slot(void* pool, int n_layers, int pool_rows, int ma
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }
+
+// ---------------------------------------------------------------------------
+// The accepted path of a drafted tree made the end of its sequence: the K/V rows at starts[s] +
+// path[s][j] move to starts[s] + j in every layer, j < emitted[s], and lengths become starts +
+// emitted.  A path ascends from node 0, so path[j] >= j and a thread that moves its column of
+// every row, lowest first, reads each row before anything is written over it: a later row's
+// source lies above every row written so far.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void kv_accept_kernel(half_t* __restrict__ pool, int64_t seg_stride,
+                                                        int64_t row_stride, int row_halfs,
+                                                        const int64_t* __restrict__ slots,
+                                                        const int64_t* __restrict__ starts,
+                                                        const int* __restrict__ path,
+                                                        const int* __restrict__ emitted, int T,
+                                                        int64_t* __restrict__ lengths, int pool_rows,
+                                                        int max_len) {
+  const int s = blockIdx.y;
+  const int64_t slot = slots ? slots[s] : s;
+  if (slot < 0 || slot >= pool_rows) return;
+  const int64_t L = min(max(starts[s], (int64_t)0), (int64_t)max_len);
+  int len = min(max(emitted[s], 0), T);
+  if ((int64_t)len > max_len - L) len = (int)(max_len - L);
+  // a path that does not ascend within the tree ends there
+  int above = 0;
+  for (int j = 0; j < len; ++j) {
+    const int from = path[(int64_t)s * T + j];
+    if (from < above || from >= T || from >= max_len - L) {
+      len = j;
+      break;
+    }
+    above = from + 1;
+  }
+  half_t* seq = pool + blockIdx.x * seg_stride + slot * row_stride + L * row_halfs;
+  const int chunks = row_halfs >> 3;
+  for (int c = threadIdx.x; c < chunks; c += 256) {
+    half8_t* col = (half8_t*)seq + c;
+    for (int j = 0; j < len; ++j) {
+      const int from = path[(int64_t)s * T + j];
+      if (from != j) col[(int64_t)j * chunks] = col[(int64_t)from * chunks];
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) lengths[slot] = L + len;
+}
+
+extern "C" int omni_kv_accept(void* pool, int n_layers, int pool_rows, int max_len, int row_halfs,
+                              const int64_t* slots, const int64_t* starts, const int* path,
+                              const int* emitted, int n, int n_nodes, int64_t* lengths,
+                              void* stream) {
+  if (n_layers <= 0 || pool_rows <= 0 || max_len <= 0 || row_halfs <= 0 || n < 0 || n_nodes < 1)
+    return OMNI_EINVAL;
+  if ((row_halfs & 7) || n > 65535) return OMNI_EUNSUPPORTED;
+  if (!slots && n > pool_rows) return OMNI_EINVAL;
+  if (n == 0) return OMNI_OK;
+  if (!pool || !starts || !path || !emitted || !lengths || ((uintptr_t)pool & 15)) return OMNI_EINVAL;
+  const int64_t row_stride = (int64_t)max_len * row_halfs;
+  hipLaunchKernelGGL(kv_accept_kernel, dim3(2 * n_layers, n), dim3(256), 0, (hipStream_t)stream,
+                     (half_t*)pool, row_stride * pool_rows, row_stride, row_halfs, slots, starts,
+                     path, emitted, n_nodes, lengths, pool_rows, max_len);
+  OMNI_CHECK_LAUNCH();
+  return OMNI_OK;
+}

@@ -25,7 +25,7 @@ from typing import List, Sequence
 
 import torch
 
-from ._lib import call, ptr, require_cuda, stream
+from ._lib import call, ptr, require_cuda, require_here, stream
 from .hostio import to_device
 
 MAX_ATTN_SPLITS = 16
@@ -139,6 +139,12 @@ class PreallocatedKVCache:
         """Decode tokens and a prefill chunk in one forward (kv_prealloc.py:110-116): segment
         s appends new_lens[s] tokens to slot slots[s] at starts[s]."""
         return PackedPrefillWriter(self, slots, new_lens, starts)
+
+    def tree_cache(self, parents, counts=None, slots=None,
+                   rope_delta: torch.Tensor | None = None) -> "TreeCache":
+        """Drafted trees of the sequences in ``slots`` (default: rows [0, n)), appended behind
+        their valid prefixes: see TreeCache."""
+        return TreeCache(self, parents, counts, slots, rope_delta)
 
     # ---- kernel calls --------------------------------------------------------------
     def attend(self, q: torch.Tensor, q_stride: int, layer_idx: int, kv_len: torch.Tensor,
@@ -437,3 +443,169 @@ class ChunkedPrefillWriter(PackedPrefillWriter):
         if self.seg is None:
             self._build([int(T)])
         super().bind(T)
+
+
+TREE_MAX_NODES = 64
+
+
+class TreeCache(PackedPrefillWriter):
+    """Adapter for one forward over drafted trees: sequence s brings T nodes, node 0 its last
+    emitted token (not yet in the cache) and every other node the child of an earlier one.
+
+    ``parents`` [n, T]: each node's parent (-1: none; an entry that does not name an earlier node
+    counts as none), T <= 64.  ``counts`` [n]: nodes in use, the rest is padding (default T);
+    ``slots`` [n]: the sequences' pool rows, all different (default 0 .. n-1).  int32 / int32 /
+    int64 tensors on the pool's device are taken as they are and never read on the host, lists are
+    checked and uploaded.  ``rope_delta``: int64 per pool row, as for the decode views.
+
+    Node i's K/V goes to position lengths[slot] + i of its row and its rotary position is
+    lengths[slot] + depth + rope_delta (``positions`` [3, n * T]); it attends to the valid prefix,
+    itself and its ancestors, and to no other node, whatever that one holds.  The lengths are read
+    once, when the adapter is made (``starts``), and stay what they were until ``accept``: a tree
+    that is not accepted leaves nothing behind.  Nodes past the pool's max_len are neither stored
+    nor attended to.  Padding nodes' rows of an output are left as they were.
+
+    The packed rows are sequence-major: node i of sequence s is row s * T + i of the forward.  The
+    adapter's buffers belong to it, so two captured graphs never share them."""
+
+    def __init__(self, pool: PreallocatedKVCache, parents, counts=None, slots=None,
+                 rope_delta: torch.Tensor | None = None):
+        self.pool = pool
+        dev = pool.device
+        if not isinstance(parents, torch.Tensor):
+            parents = [[int(p) for p in row] for row in parents]
+            if any(len(row) != len(parents[0]) for row in parents):
+                raise ValueError("every tree has the same number of nodes (pad, and give counts)")
+            for row in parents:
+                if any(not -1 <= p < i for i, p in enumerate(row)):
+                    raise ValueError(f"parents {row}: each names an earlier node, or is -1")
+            n, T = len(parents), len(parents[0]) if parents else 0
+        else:
+            if parents.dim() != 2:
+                raise ValueError(f"parents of shape {tuple(parents.shape)}: expected [n, nodes]")
+            n, T = parents.shape
+        if n < 1 or not 1 <= T <= TREE_MAX_NODES:
+            raise ValueError(f"{n} trees of {T} nodes: at least one, of 1 to {TREE_MAX_NODES}")
+        if T > pool.max_len:
+            raise ValueError(f"{T} nodes do not fit max_len={pool.max_len}")
+        if slots is None and n > pool.max_batch:
+            raise ValueError(f"{n} sequences, the pool has {pool.max_batch} rows")
+        if slots is not None and not isinstance(slots, torch.Tensor):
+            slots = [int(s) for s in slots]
+            if any(not 0 <= s < pool.max_batch for s in slots) or len(set(slots)) != len(slots):
+                raise ValueError(f"slots {slots}: all different, within the pool's "
+                                 f"{pool.max_batch} rows")
+        if counts is not None and not isinstance(counts, torch.Tensor):
+            counts = [int(c) for c in counts]
+            if any(not 0 <= c <= T for c in counts):
+                raise ValueError(f"counts {counts}: nodes in use, 0 to {T}")
+        parents = _ints(parents, (n, T), torch.int32, dev, "parents")
+        self.counts = _ints(counts, (n,), torch.int32, dev, "counts")
+        self.slots = _ints(slots, (n,), torch.int64, dev, "slots")
+        rope_delta = _ints(rope_delta, None, torch.int64, dev, "rope_delta")
+        if rope_delta is not None and rope_delta.numel() < pool.max_batch:
+            raise ValueError(f"rope_delta holds one value per pool row ({pool.max_batch})")
+        require_here(parents, self.counts, self.slots, rope_delta)
+        self.n, self.nodes, self.T = n, T, n * T
+        # one block for the plan: starts, ancestors, positions, pool rows and positions
+        plan = torch.empty(n + 6 * n * T, device=dev, dtype=torch.int64)
+        self.starts = plan[:n]
+        self.ancestors = plan[n:n + n * T]
+        self.positions = plan[n + n * T:n + 4 * n * T].view(3, n * T)
+        self.token_slot = plan[n + 4 * n * T:n + 5 * n * T]
+        self.token_pos = plan[n + 5 * n * T:]
+        call("omni_tree_plan", ptr(parents), ptr(self.counts), ptr(self.slots), ptr(pool.lengths),
+             ptr(rope_delta), n, T, pool.max_batch, pool.max_len, ptr(self.starts),
+             ptr(self.ancestors), ptr(self.positions), ptr(self.token_slot), ptr(self.token_pos),
+             stream())
+        self._ws = None
+
+    def bind(self, T: int) -> None:
+        if T != self.T:
+            raise ValueError(f"the forward brings {T} tokens, the trees have {self.T} nodes")
+
+    def finish(self) -> None:
+        """The lengths move in accept, once it is known which nodes stand."""
+
+    def attend_qkv(self, qkv: torch.Tensor, layer_idx: int, scale: float,
+                   out: torch.Tensor) -> torch.Tensor:
+        """out [n * T, nh, hd] (fp16, contiguous): attention of the nodes whose queries are the
+        first nh * hd columns of the rows qkv; their K/V is in the pool (rope_and_write)."""
+        pool = self.pool
+        nh, hd = pool.n_heads, pool.head_dim
+        if qkv.dim() != 2 or qkv.shape[0] != self.T or qkv.shape[1] < nh * hd or qkv.stride(1) != 1:
+            raise ValueError(f"query rows of shape {tuple(qkv.shape)}: expected [{self.T}, >= "
+                             f"{nh * hd}] with contiguous columns")
+        if qkv.dtype != torch.float16 or out.dtype != torch.float16:
+            raise TypeError(f"the pool's attention is fp16 (got {qkv.dtype} -> {out.dtype})")
+        if out.numel() != self.T * nh * hd or not out.is_contiguous():
+            raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
+                             f"[{self.T}, {nh}, {hd}]")
+        require_here(qkv, out)
+        call("omni_tree_attention", ptr(qkv), qkv.stride(0), ptr(pool.k[layer_idx]),
+             ptr(pool.v[layer_idx]), pool.max_batch, pool.max_len, ptr(self.slots),
+             ptr(self.starts), ptr(self.ancestors), self.n, self.nodes, ptr(out), nh * hd, nh,
+             pool.n_kv_heads, hd, float(scale), 1, None, 0, stream())
+        return out
+
+    def flash_prefill(self, q, k, v, layer_idx, scale):
+        """The adapters' protocol on rotated tensors: q [n * T, nh, hd], k / v [n * T, nkv, hd].
+        Writes the nodes' K/V rows, then attends; padding nodes' rows are zero."""
+        pool = self.pool
+        nh, nkv, hd = pool.n_heads, pool.n_kv_heads, pool.head_dim
+        self.bind(q.shape[0])
+        if tuple(q.shape[1:]) != (nh, hd) or tuple(k.shape) != (self.T, nkv, hd) \
+                or k.shape != v.shape:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected "
+                             f"[{self.T}, {nh} / {nkv}, {hd}]")
+        if not q.dtype == k.dtype == v.dtype == torch.float16:
+            raise TypeError(f"the pool is fp16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+        q, k, v = (_head_rows(x) for x in (q, k, v))
+        require_here(q, k, v)
+        call("omni_kv_write_rows", ptr(k), k.stride(0), ptr(v), v.stride(0),
+             ptr(pool.k[layer_idx]), ptr(pool.v[layer_idx]), ptr(self.token_slot),
+             ptr(self.token_pos), pool.max_batch, pool.max_len, nkv * hd, self.T, stream())
+        make = torch.empty if self.counts is None and self.slots is None else torch.zeros
+        out = make(self.T, nh, hd, device=q.device, dtype=torch.float16)
+        return self.attend_qkv(q, layer_idx, scale, out)
+
+    def update(self, k, v, layer_idx, cache_kwargs=None):
+        raise NotImplementedError("a drafted tree has no causal window for the SDPA route")
+
+    def accept(self, path: torch.Tensor, emitted: torch.Tensor) -> None:
+        """Make the accepted nodes the end of their sequences: in every layer the K/V rows of nodes
+        path[s, :emitted[s]] (ascending, as ``speculative.verify`` gives them; a path that does not
+        ascend ends there) move to positions starts[s] .., and lengths[slot] = starts[s] +
+        emitted[s], up to max_len.  path int32 [n, T], emitted int32 [n], on the device.  The tree's
+        rows are consumed: a second call would move what the first one left."""
+        pool = self.pool
+        path = _ints(path, (self.n, self.nodes), torch.int32, pool.device, "path")
+        emitted = _ints(emitted, (self.n,), torch.int32, pool.device, "emitted")
+        require_here(path, emitted)
+        call("omni_kv_accept", ptr(pool.storage), pool.n_layers, pool.max_batch, pool.max_len,
+             pool.n_kv_heads * pool.head_dim, ptr(self.slots), ptr(self.starts), ptr(path),
+             ptr(emitted), self.n, self.nodes, ptr(pool.lengths), stream())
+        if self.slots is None:
+            pool._active = max(pool._active, self.n)
+
+
+def _ints(values, shape, dtype, device, name: str):
+    """values as a contiguous dtype tensor of shape on device: a tensor has to be one already, a
+    list is uploaded; None stays None."""
+    if values is None:
+        return None
+    if not isinstance(values, torch.Tensor):
+        values = to_device(values, dtype, device)
+    if values.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {values.dtype}")
+    if shape is not None and tuple(values.shape) != shape:
+        raise ValueError(f"{name} of shape {tuple(values.shape)}: expected {list(shape)}")
+    return values.contiguous()
+
+
+def _head_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [T, heads, hd] as rows [T, heads * hd] with contiguous, 16-byte aligned columns: a view
+    where x is a slice of a fused projection, else a copy."""
+    if x.stride(2) != 1 or x.stride(1) != x.shape[2] or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+    return x.as_strided((x.shape[0], x.shape[1] * x.shape[2]), (x.stride(0), 1))
