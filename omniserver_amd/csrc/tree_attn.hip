@@ -3,7 +3,7 @@
 // Sequence s has a valid prefix of starts[s] tokens in its pool row; node i of its tree (n_nodes
 // <= 64 of them, parents before children) has its K/V at position starts[s] + i and attends to
 // the prefix, itself and its ancestors.  The ancestors of a node are one 64-bit word.
-#include "common.h"
+#include "attn_rows.h"
 
 #define TREE_HD 128
 #define TREE_MAX 64
@@ -72,8 +72,17 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// One wave a (node, query head): 64 keys a step, one a lane for the scores, then two dims a lane
-// for the output, with the running maximum and sum of a softmax.
+// The tile structure and what bounds it are in attn_rows.h.  A workgroup takes one sequence, one
+// KV head, 32 R rows of its (node, query head) pairs, node-major, and one of `splits` shares of
+// the keys, which its S groups of R waves take in contiguous runs of KT-key tiles (each group has
+// its own LDS tiles, as in attn_rows.hip).  A K / V byte staged in LDS serves all query heads of
+// the group and up to 32 R / G nodes.
+//
+// The keys are the prefix and, behind it, the nodes.  Only tiles that reach past the prefix are
+// masked, with the row's ancestor word shifted to the tile.  A node that a row does not attend to
+// has probability 0 there, and 0 times an infinity or NaN in its V row is NaN: rows whose merged
+// outputs are not all finite are taken again, key by key and without the keys they do not
+// attend to (tree_row).  That costs the others the check and a barrier.
 // ---------------------------------------------------------------------------
 struct TreeArgs {
   const half_t* q;
@@ -81,59 +90,383 @@ struct TreeArgs {
   const half_t* k_cache;
   const half_t* v_cache;
   int pool_rows, max_len, nkv, G, T;
+  int items, rblocks, splits;  // (sequence, KV head, split) items, row blocks of each
   const int64_t* slots;        // [n] or null
   const int64_t* starts;       // [n]
   const uint64_t* ancestors;   // [n][T]
   half_t* out;
   int out_stride;
   float scale_log2;
+  float* states;               // [n * T * heads][splits][ATT_REC], splits > 1
 };
 
-__global__ __launch_bounds__(64) void tree_attn_kernel(TreeArgs a) {
-  const int lane = threadIdx.x;
-  const int t = blockIdx.x, head = blockIdx.y;
-  const int s = t / a.T;
-  const int64_t slot = a.slots ? a.slots[s] : s;
-  const uint64_t m = a.ancestors[t];
-  if (slot < 0 || slot >= a.pool_rows || !m) return;
-  const int64_t L = a.starts[s];
-  const int64_t end = min(L + a.T, (int64_t)a.max_len);
+// One row over keys [k0, k1) by one wave: 64 keys a step, a key a lane for the scores, then two
+// dims a lane for the output, hidden keys left out.
+__device__ __forceinline__ void tree_row(const TreeArgs& a, int64_t slot, int s, int g, int row, int L,
+                                         int k0, int k1, int sp) {
+  const int lane = threadIdx.x & 63;
+  const int node = row / a.G, head = g * a.G + row - node * a.G;
+  const int64_t tok = (int64_t)s * a.T + node;
+  const uint64_t mask = a.ancestors[tok];
   const int64_t tstride = (int64_t)a.nkv * TREE_HD;
-  const int64_t base = slot * a.max_len * tstride + (head / a.G) * TREE_HD;
-  const half_t* qp = a.q + (int64_t)t * a.q_stride + head * TREE_HD;
+  const int64_t base = slot * a.max_len * tstride + g * TREE_HD;
+  const half_t* qp = a.q + tok * a.q_stride + head * TREE_HD;
   float mr = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int64_t tb = 0; tb < end; tb += 64) {
-    const int64_t key = tb + lane;
-    const bool seen = key < end && (key < L || ((m >> (key - L)) & 1));
+#pragma unroll 1
+  for (int tb = k0; tb < k1; tb += 64) {
+    const int key = tb + lane;
+    const bool seen = key < k1 && (key < L || ((mask >> (key - L)) & 1));
     float sc = -INFINITY;
     if (seen) {
       const half_t* kp = a.k_cache + base + key * tstride;
       sc = 0.f;
-      for (int c = 0; c < 16; ++c) {
-        const half8_t kv = *(const half8_t*)(kp + 8 * c), qv = *(const half8_t*)(qp + 8 * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sc = fmaf((float)kv[e], (float)qv[e], sc);
-      }
+#pragma unroll 1
+      for (int c = 0; c < TREE_HD; ++c) sc = fmaf((float)kp[c], (float)qp[c], sc);
       sc *= a.scale_log2;
     }
-    const float mn = fmaxf(mr, wave_max(sc));
-    if (mn == -INFINITY) continue;
-    const float alpha = exp2f(mr - mn), p = seen ? exp2f(sc - mn) : 0.f;
+    const uint64_t all = __ballot(seen);
+    if (!all) continue;
+    const float mn = fmaxf(mr, wave_max(sc)), ref = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f(mr - ref), p = seen ? exp2f(sc - ref) : 0.f;
     mr = mn;
     l = l * alpha + wave_sum(p);
     o0 *= alpha;
     o1 *= alpha;
-    const uint64_t all = __ballot(seen);
+#pragma unroll 1
     for (int j = 0; j < 64; ++j) {
-      if (!((all >> j) & 1)) continue;
       const float pj = __shfl(p, j);
+      if (!((all >> j) & 1)) continue;
       const half2_t vv = *(const half2_t*)(a.v_cache + base + (tb + j) * tstride + 2 * lane);
       o0 = fmaf(pj, (float)vv[0], o0);
       o1 = fmaf(pj, (float)vv[1], o1);
     }
   }
-  const half2_t r = {(half_t)(l == 0.f ? 0.f : o0 / l), (half_t)(l == 0.f ? 0.f : o1 / l)};
-  *(half2_t*)(a.out + (int64_t)t * a.out_stride + head * TREE_HD + 2 * lane) = r;
+  if (a.splits > 1) {
+    float* rec = a.states + ((tok * (a.nkv * a.G) + head) * a.splits + sp) * ATT_REC;
+    *(float2*)(rec + 2 * lane) = make_float2(o0, o1);
+    if (lane == 0) *(float2*)(rec + 128) = make_float2(mr, l);
+  } else {
+    const half2_t r = {(half_t)(l == 0.f ? 0.f : o0 / l), (half_t)(l == 0.f ? 0.f : o1 / l)};
+    *(half2_t*)(a.out + tok * a.out_stride + head * TREE_HD + 2 * lane) = r;
+  }
+}
+
+template <int R, int S, int KT>
+__global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
+  constexpr int NBUF = R == 1 ? 1 : 2;
+  constexpr int TB = KT * TREE_HD * 2;              // bytes of a K (or V) tile
+  constexpr int NL = TB / 1024;                     // 1 KB (4-row) pieces of a tile
+  constexpr int NB = KT / 32;
+  constexpr int MB = R * S * 64 * 64 * 4;           // the merge's outputs
+  constexpr int SB = S * NBUF * 2 * TB > MB ? S * NBUF * 2 * TB : MB;
+  __shared__ __attribute__((aligned(16))) char smem[SB];
+  __shared__ float ml_lds[S][R][2][32];
+  __shared__ uint32_t bad_rows[R][S];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / R;                          // key group
+  const int rt = wave - grp * R;                     // row tile
+  const int l32 = lane & 31, h = lane >> 5;
+  // the row blocks of an item, which read the same keys, on one XCD (workgroup b on XCD b % 8)
+  const int y = blockIdx.x >> 3;
+  const int rb = y % a.rblocks;
+  const int item = (y / a.rblocks) * 8 + (blockIdx.x & 7);
+  if (item >= a.items) return;
+  const int sp = item % a.splits;
+  const int g = (item / a.splits) % a.nkv;
+  const int s = item / a.splits / a.nkv;
+  const int64_t slot = a.slots ? a.slots[s] : s;
+  if (slot < 0 || slot >= a.pool_rows) return;
+  const uint64_t word = lane < a.T ? a.ancestors[(int64_t)s * a.T + lane] : 0;
+  const int used = __popcll(__ballot(word != 0));    // nodes in use come first
+  const int nrows = used * a.G - 32 * R * rb;        // this block's
+  if (nrows <= 0) return;
+  const int64_t L64 = a.starts[s];
+  const int L = (int)(L64 < 0 ? 0 : L64 > a.max_len ? a.max_len : L64);
+  const int end = min(L + used, a.max_len);
+  const int row = min(32 * rt + l32, nrows - 1);
+  const int node = (32 * R * rb + row) / a.G;
+  const int u = 32 * R * rb + row - node * a.G;
+  const int64_t tok = (int64_t)s * a.T + node;
+  uint64_t mask = (uint64_t)(uint32_t)__shfl((int)(word & 0xffffffffu), node) |
+                  ((uint64_t)(uint32_t)__shfl((int)(word >> 32), node) << 32);
+  if (end - L < 64) mask &= (1ull << (end - L)) - 1;   // nodes behind the pool's end
+  const bool rows_here = 32 * rt < nrows;
+
+  half8_t qf[8];
+  {
+    const half_t* qp = a.q + tok * a.q_stride + (int64_t)(g * a.G + u) * TREE_HD + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = *(const half8_t*)(qp + 16 * ks);
+  }
+
+  const int ntiles = (end + KT - 1) / KT;
+  const int steps = (ntiles + S * a.splits - 1) / (S * a.splits);
+  const int tbeg = (sp * S + grp) * steps;
+  const int nt = min(steps, ntiles - tbeg);          // may be <= 0
+
+  const int cr = lane >> 4, cc = lane & 15;
+  const int64_t tstride = (int64_t)a.nkv * TREE_HD;  // halfs per token
+  const int64_t base = slot * (int64_t)a.max_len * tstride + g * TREE_HD;
+  const half_t* kb0 = a.k_cache + base;
+  const half_t* vb0 = a.v_cache + base;
+  half8_t kr[NL], vr[NL];
+  auto load_tile = [&](int tb) {                     // past the end: the last key again
+    const int64_t last = end - 1;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int64_t t = min((int64_t)tb + cr + 4 * j, last);
+      kr[j] = *(const half8_t*)(kb0 + t * tstride + cc * 8);
+      vr[j] = *(const half8_t*)(vb0 + t * tstride + cc * 8);
+    }
+  };
+  auto store_tile = [&](char* kt) {
+    char* vt = kt + TB;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int r = cr + 4 * j;
+      *(half8_t*)(kt + r * 256 + ((cc ^ (r & 15)) << 4)) = kr[j];
+      *(half8_t*)(vt + r * 256 + ((cc << 4) ^ ((r & 3) << 6))) = vr[j];
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  const int koff = l32 * 256 + ((h ^ (l32 & 15)) << 4);
+  const int i16 = lane & 15;
+  const int voff = (4 * h + (i16 >> 2)) * 256 + ((i16 >> 2) << 6) + ((lane >> 4) & 1) * 32 +
+                   (i16 & 3) * 8;
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  f32x16 sc[NB];
+  half8_t p[2 * NB];
+  auto scores = [&](const char* kt) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[b][i] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        sc[b] = mfma32x32x16(*(const half8_t*)(kt + 8192 * b + (koff ^ (ks << 5))), qf[ks], sc[b]);
+    // the first reads ahead, then one step's reads beside each step's MFMAs
+    __builtin_amdgcn_sched_group_barrier(0x100, 3 * NB, 0);
+#pragma unroll
+    for (int ks = 0; ks < 5; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 3 * NB, 0);
+  };
+  // bit j: the row attends to key tb + j
+  auto tile_word = [&](int tb) {
+    const int off = tb - L;
+    return off >= 0 ? mask >> off : (mask << -off) | ((1ull << -off) - 1);
+  };
+  auto hide = [&](int tb) {
+    if (tb + KT > L) {
+      const uint64_t w = tile_word(tb) >> (4 * h);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!((w >> (32 * b + 8 * (i >> 2) + (i & 3))) & 1)) sc[b][i] = -INFINITY;
+    }
+  };
+  auto output = [&](const char* vt) {
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const char* vp = vt + 4096 * t + (voff ^ (d << 6));
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)vp);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vp + 2048));
+        const half4_t a0 = __builtin_bit_cast(half4_t, lo), a1 = __builtin_bit_cast(half4_t, hi);
+        o[d] = mfma32x32x16((half8_t){a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
+                            p[t], o[d]);
+      }
+  };
+  char* gbuf = smem + grp * NBUF * 2 * TB;
+  auto dma_half = [&](int tb, char* dst, const half_t* src0, bool is_k) {
+    const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_offset(dst)) + rt * 1024;
+    const bool whole = tb + KT <= end;               // else the last key is repeated
+    const half_t* src = src0 + (int64_t)tb * tstride;
+#pragma unroll
+    for (int j = 0; j < NL / R; ++j) {
+      const int r0 = 4 * (rt + R * j), r = r0 + cr;
+      const int ch = is_k ? cc ^ (r & 15) : cc ^ ((r & 3) << 2);
+      const half_t* sp = whole ? src + (int64_t)r0 * tstride : src;
+      const int rr = whole ? cr : min(r, end - 1 - tb);
+      dma16(sp, (uint32_t)rr * (uint32_t)tstride * 2 + ch * 16, l0 + R * j * 1024);
+    }
+  };
+  auto dma_tile = [&](int tb, char* kt) {
+    dma_half(tb, kt, kb0, true);
+    dma_half(tb, kt + TB, vb0, false);
+  };
+  if (nt > 0) {
+    if constexpr (R > 1) dma_tile(tbeg * KT, gbuf);
+    else load_tile(tbeg * KT);
+  }
+  // Q has landed: without this the compiler counts the Q loads as outstanding inside the loop
+  // and makes every tile's first MFMAs wait for the transfers just requested
+  __builtin_amdgcn_s_waitcnt(0x0f70);
+  for (int it = 0; it < steps; ++it) {
+    char* kt = gbuf + (NBUF == 2 ? (it & 1) * 2 * TB : 0);
+    const int tb = (tbeg + it) * KT;
+    if constexpr (R > 1) {
+      vm_wait();             // this wave's part of tile it has landed; so, past the barrier,
+      lds_barrier();         // have the others', and tile it - 1's buffer is free
+      if (it + 1 < nt) dma_tile(tb + KT, gbuf + ((it + 1) & 1) * 2 * TB);
+    } else {
+      if (it < nt) store_tile(kt);
+      if (it + 1 < nt) load_tile(tb + KT);
+    }
+    if (it < nt && rows_here) {
+      scores(kt);
+      hide(tb);
+      softmax32<NB, 4>(sc, a.scale_log2, m_run, l_run, o, p);
+      output(kt + TB);
+    }
+  }
+
+  // Every group's unnormalised output and (max, sum) per row go to LDS; wave (rt, grp)
+  // merges its share of the 16 output quads (4 dims) of row tile rt over the S groups.
+  {
+    float x, y2;
+    half_pair(l_run, x, y2);
+    l_run = x + y2;
+  }
+  __syncthreads();
+  float* om = (float*)smem;
+  if (rows_here) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *(float4*)(om + (((grp * R + rt) * 16 + 4 * d + b) * 64 + lane) * 4) =
+            make_float4(o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]);
+    if (h == 0) {
+      ml_lds[grp][rt][0][l32] = m_run;
+      ml_lds[grp][rt][1][l32] = l_run;
+    }
+  }
+  __syncthreads();
+  const int64_t heads = a.nkv * a.G, head = g * a.G + u;
+  if (rows_here) {
+    float M = ml_lds[0][rt][0][l32];
+#pragma unroll
+    for (int k = 1; k < S; ++k) M = fmaxf(M, ml_lds[k][rt][0][l32]);
+    const float ref = M == -INFINITY ? 0.f : M;        // no key at all: factors 0
+    float f[S], den = 0.f;
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      f[k] = __builtin_amdgcn_exp2f(ml_lds[k][rt][0][l32] - ref);
+      den += ml_lds[k][rt][1][l32] * f[k];
+    }
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    const bool mine = 32 * rt + l32 < nrows;
+    float* rec = a.states + ((tok * heads + head) * a.splits + sp) * ATT_REC;
+    half_t* op = a.out + tok * a.out_stride + head * TREE_HD;
+    constexpr int NQ = 16 / S;
+    float bad = den * 0.f;                             // NaN where an output is not finite
+#pragma unroll
+    for (int k = 0; k < NQ; k += 2) {
+      unsigned w[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int quad = grp * NQ + k + e;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < S; ++m) {
+          const float4 v = *(const float4*)(om + (((m * R + rt) * 16 + quad) * 64 + lane) * 4);
+          acc.x = fmaf(v.x, f[m], acc.x);
+          acc.y = fmaf(v.y, f[m], acc.y);
+          acc.z = fmaf(v.z, f[m], acc.z);
+          acc.w = fmaf(v.w, f[m], acc.w);
+        }
+        bad = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, fmaf(acc.w, 0.f, bad))));
+        if (a.splits > 1) {                            // the state, for the merging launch
+          if (mine) *(float4*)(rec + 8 * quad + 4 * h) = acc;
+        } else {
+          const half2_t c0 = {(half_t)(acc.x * inv), (half_t)(acc.y * inv)};
+          const half2_t c1 = {(half_t)(acc.z * inv), (half_t)(acc.w * inv)};
+          w[e][0] = __builtin_bit_cast(unsigned, c0);
+          w[e][1] = __builtin_bit_cast(unsigned, c1);
+        }
+      }
+      if (a.splits == 1) {
+        // lane half h holds dims 8 quad + 4 h .. + 3 of quads k and k + 1: exchanged, half 0 has
+        // all 8 dims of quad k and half 1 those of quad k + 1
+        const auto r0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const u32x4 st = {r0[0], r1[0], r0[1], r1[1]};
+        if (mine) *(u32x4*)(op + 8 * (grp * NQ + k + h)) = st;
+      }
+    }
+    if (a.splits > 1 && mine && grp == 0 && h == 0) *(float2*)(rec + 128) = make_float2(M, den);
+    const uint64_t lanes = __ballot(bad != bad && mine);
+    if (lane == 0) bad_rows[rt][grp] = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+  }
+  if (!rows_here && lane == 0) bad_rows[rt][grp] = 0;
+  __syncthreads();
+  uint32_t again = 0;
+  for (int k = 0; k < S; ++k) again |= bad_rows[rt][k];
+  for (int i = 0; again; ++i, again &= again - 1) {
+    if (i % S != grp) continue;
+    const int r = 32 * rt + __ffs(again) - 1;
+    const int span = S * steps * KT, k0 = min(sp * span, end);
+    tree_row(a, slot, s, g, 32 * R * rb + r, L, k0, min(k0 + span, end), sp);
+  }
+}
+
+// The splits' states of a (node, query head) row to its output: one wave a row, two dims a lane.
+__global__ __launch_bounds__(256) void tree_merge_kernel(const float* __restrict__ states, int splits,
+                                                         int heads, int T, int64_t rows,
+                                                         const int64_t* __restrict__ slots,
+                                                         int pool_rows,
+                                                         const uint64_t* __restrict__ ancestors,
+                                                         half_t* __restrict__ out, int out_stride) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int64_t tok = r / heads;
+  const int head = (int)(r - tok * heads);
+  const int64_t slot = slots ? slots[tok / T] : 0;
+  if (slot < 0 || slot >= pool_rows || !ancestors[tok]) return;      // no state was written
+  const float* rec = states + r * splits * ATT_REC;
+  float M = -INFINITY;
+  for (int k = lane; k < splits; k += 64) M = fmaxf(M, rec[k * ATT_REC + 128]);
+  M = wave_max(M);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float o0 = 0.f, o1 = 0.f, den = 0.f;
+  for (int k0 = 0; k0 < splits; k0 += 8) {
+    float2 ml[8], v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float* at = rec + min(k0 + k, splits - 1) * ATT_REC;
+      ml[k] = *(const float2*)(at + 128);
+      v[k] = *(const float2*)(at + 2 * lane);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = k0 + k < splits ? exp2f(ml[k].x - ref) : 0.f;
+      if (k0 + k < splits) {
+        den = fmaf(f, ml[k].y, den);
+        o0 = fmaf(f, v[k].x, o0);
+        o1 = fmaf(f, v[k].y, o1);
+      }
+    }
+  }
+  const float inv = den == 0.f ? 0.f : 1.0f / den;
+  const half2_t h2 = {(half_t)(o0 * inv), (half_t)(o1 * inv)};
+  *(half2_t*)(out + tok * out_stride + head * TREE_HD + 2 * lane) = h2;
 }
 
 extern "C" int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
@@ -176,22 +509,25 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
                                    const int64_t* slots, const int64_t* starts,
                                    const void* ancestors, int n, int n_nodes, void* out,
                                    int out_stride, int n_heads, int n_kv_heads, int head_dim,
-                                   float scale, int splits, float* workspace,
+                                   float scale, int rows, int groups, int splits, float* workspace,
                                    int64_t workspace_floats, void* stream) {
   if (n < 0 || n_nodes < 1 || n_heads <= 0 || n_kv_heads <= 0 || pool_rows <= 0 || max_len <= 0)
     return OMNI_EINVAL;
   if (head_dim != TREE_HD || n_heads % n_kv_heads || n_nodes > TREE_MAX) return OMNI_EUNSUPPORTED;
   if (!(scale >= 0x1p-126f) || scale > 3e38f) return OMNI_EUNSUPPORTED;
+  const int form = rows == 128 && (groups == 1 || groups == 2) ? groups
+                   : rows == 64 && groups == 4 ? 4 : rows == 32 && groups == 8 ? 8 : 0;
+  if (!form) return OMNI_EINVAL;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
   if (splits < 1 || splits > 256 || (!slots && n > pool_rows)) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
   if (!q || !k_cache || !v_cache || !starts || !ancestors || !out) return OMNI_EINVAL;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return OMNI_EINVAL;
-  if (splits > 1 &&
-      (!workspace || workspace_floats < (int64_t)n * n_nodes * n_heads * splits * ATT_REC))
+  const int64_t nrec = (int64_t)n * n_nodes * n_heads;
+  if (splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
+                     workspace_floats < nrec * splits * ATT_REC))
     return OMNI_EINVAL;
-  if ((int64_t)n * n_nodes > 0x7fffffff || n_heads > 65535) return OMNI_EUNSUPPORTED;
   TreeArgs a;
   a.q = (const half_t*)q;
   a.q_stride = q_stride;
@@ -202,13 +538,36 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   a.nkv = n_kv_heads;
   a.G = n_heads / n_kv_heads;
   a.T = n_nodes;
+  a.splits = splits;
+  const int64_t items = (int64_t)n * n_kv_heads * splits;
+  const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
+  const int64_t grid = (items + 7) / 8 * 8 * rblocks;
+  if (grid > 0x7fffffff || nrec > 0x7fffffff) return OMNI_EUNSUPPORTED;
+  a.items = (int)items;
+  a.rblocks = (int)rblocks;
   a.slots = slots;
   a.starts = starts;
   a.ancestors = (const uint64_t*)ancestors;
   a.out = (half_t*)out;
   a.out_stride = out_stride;
   a.scale_log2 = scale * 1.4426950408889634f;
-  hipLaunchKernelGGL(tree_attn_kernel, dim3(n * n_nodes, n_heads), dim3(64), 0, (hipStream_t)stream, a);
+  a.states = workspace;
+  const dim3 gd((unsigned)grid);
+  hipStream_t st = (hipStream_t)stream;
+  if (form == 1)
+    hipLaunchKernelGGL((tree_attn_kernel<4, 1, 64>), gd, dim3(256), 0, st, a);
+  else if (form == 2)
+    hipLaunchKernelGGL((tree_attn_kernel<4, 2, 64>), gd, dim3(512), 0, st, a);
+  else if (form == 4)
+    hipLaunchKernelGGL((tree_attn_kernel<2, 4, 32>), gd, dim3(512), 0, st, a);
+  else
+    hipLaunchKernelGGL((tree_attn_kernel<1, 8, 32>), gd, dim3(512), 0, st, a);
   OMNI_CHECK_LAUNCH();
+  if (splits > 1) {
+    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((nrec + 3) / 4)), dim3(256), 0, st,
+                       workspace, splits, n_heads, n_nodes, nrec, slots, pool_rows,
+                       (const uint64_t*)ancestors, (half_t*)out, out_stride);
+    OMNI_CHECK_LAUNCH();
+  }
   return OMNI_OK;
 }

@@ -26,6 +26,7 @@ from typing import List, Sequence
 import torch
 
 from ._lib import call, ptr, require_cuda, require_here, stream
+from .attention import num_cus
 from .hostio import to_device
 
 MAX_ATTN_SPLITS = 16
@@ -448,6 +449,16 @@ class ChunkedPrefillWriter(PackedPrefillWriter):
 TREE_MAX_NODES = 64
 
 
+def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) -> tuple:
+    """(rows, key groups, splits) for omni_tree_attention over n trees in a pool of capacity
+    tokens a row."""
+    rows = nodes * (nh // nkv)
+    form = (32, 8) if rows <= 32 else (64, 4) if rows <= 64 else (128, 2)
+    items = n * nkv * -(-rows // form[0])
+    splits = max(1, min(cus // items, capacity // 256, 64))
+    return (*form, splits)
+
+
 class TreeCache(PackedPrefillWriter):
     """Adapter for one forward over drafted trees: sequence s brings T nodes, node 0 its last
     emitted token (not yet in the cache) and every other node the child of an earlier one.
@@ -518,7 +529,11 @@ class TreeCache(PackedPrefillWriter):
              ptr(rope_delta), n, T, pool.max_batch, pool.max_len, ptr(self.starts),
              ptr(self.ancestors), ptr(self.positions), ptr(self.token_slot), ptr(self.token_pos),
              stream())
-        self._ws = None
+        # (rows, groups, splits) of the attention and its split states, shared by the layers
+        # (launches on one stream are ordered)
+        self.plan = tree_plan(n, T, pool.n_heads, pool.n_kv_heads, pool.max_len, num_cus(dev))
+        self._ws = None if self.plan[2] == 1 else torch.empty(
+            n * T * pool.n_heads * self.plan[2] * 132, device=dev, dtype=torch.float32)
 
     def bind(self, T: int) -> None:
         if T != self.T:
@@ -542,10 +557,12 @@ class TreeCache(PackedPrefillWriter):
             raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
                              f"[{self.T}, {nh}, {hd}]")
         require_here(qkv, out)
+        rows, groups, splits = self.plan
         call("omni_tree_attention", ptr(qkv), qkv.stride(0), ptr(pool.k[layer_idx]),
              ptr(pool.v[layer_idx]), pool.max_batch, pool.max_len, ptr(self.slots),
              ptr(self.starts), ptr(self.ancestors), self.n, self.nodes, ptr(out), nh * hd, nh,
-             pool.n_kv_heads, hd, float(scale), 1, None, 0, stream())
+             pool.n_kv_heads, hd, float(scale), rows, groups, splits, ptr(self._ws),
+             0 if self._ws is None else self._ws.numel(), stream())
         return out
 
     def flash_prefill(self, q, k, v, layer_idx, scale):

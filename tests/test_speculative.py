@@ -20,16 +20,17 @@ def test_tree_attention_refusals():
     from omniserver_amd._lib import lib
 
     def rc(q=P, q_stride=1536, rows=4, max_len=256, starts=P, n=2, nodes=8, out=P, out_stride=1536,
-           nh=12, nkv=2, hd=128, scale=0.1, splits=1, ws=None, floats=0, slots=None):
+           nh=12, nkv=2, hd=128, scale=0.1, splits=1, ws=None, floats=0, slots=None, form=(64, 4)):
         return lib().omni_tree_attention(q, q_stride, P, P, rows, max_len, slots, starts, P, n,
-                                         nodes, out, out_stride, nh, nkv, hd, scale, splits, ws,
-                                         floats, None)
+                                         nodes, out, out_stride, nh, nkv, hd, scale, *form, splits,
+                                         ws, floats, None)
 
     assert rc(n=-1) == rc(nodes=0) == rc(nh=0) == rc(nkv=0) == rc(rows=0) == rc(max_len=0) == -1
     assert rc(nodes=65) == rc(hd=64) == rc(nh=13) == -2
     assert rc(scale=0.0) == rc(scale=-1.0) == rc(scale=float("nan")) == rc(scale=1e-39) == -2
     assert rc(scale=float("inf")) == -2
     assert rc(q_stride=1535) == rc(q_stride=1532) == rc(out_stride=8) == rc(out_stride=1540) == -1
+    assert rc(form=(64, 2)) == rc(form=(32, 1)) == rc(form=(0, 0)) == -1
     assert rc(splits=0) == rc(splits=257) == rc(n=5) == -1
     assert rc(q=None) == rc(out=None) == rc(starts=None) == -1
     assert rc(q=ctypes.c_void_p(24)) == rc(out=ctypes.c_void_p(8)) == -1
