@@ -154,26 +154,32 @@ int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v, int64_t v
  * per pool row or NULL.  Writes starts int64 [n] (the prefix lengths), ancestors uint64
  * [n][n_nodes] (bit j: node j is the node or above it; 0 for a node not in use), positions int64
  * [3][n * n_nodes] (starts + depth + rope_delta), token_slot / token_pos int64 [n * n_nodes] (where
- * the nodes' K/V goes; token_slot -1: nowhere). */
+ * the nodes' K/V goes; token_slot -1: nowhere), and schedule (int32, 16-byte aligned, 4 n + 8
+ * columns + 2 n n_kv_heads of them) for omni_tree_attention with the same n_kv_heads, (rows,
+ * groups), columns and least: the keys of all sequences and KV heads in equal stretches for that
+ * many columns of workgroups, none shorter than least steps of a workgroup; least 0: no cuts,
+ * columns = n n_kv_heads. */
 int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
                    const int64_t* lengths, const int64_t* rope_delta, int n, int n_nodes,
                    int pool_rows, int max_len, int64_t* starts, void* ancestors,
-                   int64_t* positions, int64_t* token_slot, int64_t* token_pos, void* stream);
+                   int64_t* positions, int64_t* token_slot, int64_t* token_pos, int n_kv_heads,
+                   int rows, int groups, int columns, int least, int* schedule,
+                   int64_t schedule_ints, void* stream);
 
 /* Attention of the trees' nodes over the pool: node i of sequence s (row s * n_nodes + i of q and
  * out, fp16, strides in halfs) attends to keys [0, starts[s]) of its pool row and to starts[s] + j
  * for its ancestors j; nodes not in use and sequences outside the pool leave their out rows as
  * they were.  (rows, groups) of a workgroup as in omni_prefill_attention_rows: (128, 1), (128, 2),
- * (64, 4) or (32, 8), any number of query heads per KV head.  splits workgroups share a sequence's
- * keys (1..256): splits > 1 leaves softmax states in workspace (fp32, 16-byte aligned, n * n_nodes
- * * n_heads * splits * 132 floats) for a second launch.  head_dim 128; scale a positive normal
- * fp32; 16-byte aligned operands. */
+ * (64, 4) or (32, 8), any number of query heads per KV head.  Where the plan cuts (least > 0) the
+ * softmax states of the pieces go through workspace (fp32, 16-byte aligned, columns * ceil(n_nodes
+ * * n_heads / n_kv_heads / rows) * 2 * rows * 132 floats) to a second launch.  head_dim 128; scale
+ * a positive normal fp32; 16-byte aligned operands. */
 int omni_tree_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache,
-                        int pool_rows, int max_len, const int64_t* slots, const int64_t* starts,
-                        const void* ancestors, int n, int n_nodes, void* out, int out_stride,
-                        int n_heads, int n_kv_heads, int head_dim, float scale, int rows,
-                        int groups, int splits, float* workspace, int64_t workspace_floats,
-                        void* stream);
+                        int pool_rows, int max_len, const int64_t* slots, const void* ancestors,
+                        int n, int n_nodes, void* out, int out_stride, int n_heads,
+                        int n_kv_heads, int head_dim, float scale, int rows, int groups,
+                        int columns, int least, const int* schedule, float* workspace,
+                        int64_t workspace_floats, void* stream);
 
 /* Verification of drafted tokens.  logits [n][n_nodes][vocab] (dtype 0 fp16, 1 bf16, 2 fp32;
  * strides in elements), tokens int64, uniforms fp32 [n][n_nodes]; parents int32 [n][n_nodes] for

@@ -14,26 +14,21 @@
 // first v whose running sum of weights exceeds u_0 times their total.  A NaN logit counts as
 // -inf; a row without a token above -inf accepts nothing and gives -1.
 //
-// Which token a random number falls on is decided by sums over the whole vocabulary, so all
-// weights and sums are 64-bit: the borders between 151936 tokens lie 1e-6 apart and closer, and
-// 32-bit sums would move one in a few hundred draws to a neighbour.
+// Every row is read once, in 32 bits: largest logit and sum of weights per 2048 tokens (the bound
+// is the rows' bytes).  A test that these sums leave open - they are good to 2^-18, so one in some
+// 10^5 - is decided by a 64-bit sum of its row.  Where a random number falls among 151936 tokens
+// is a matter of borders 1e-6 apart and closer, which 32-bit sums would move across one draw in a
+// few hundred: the one row per sequence that the next token comes from is summed and searched in
+// 64 bits.  Launches: row statistics; the walk, with the drawn row's 64-bit chunk sums; with a
+// draft, the chunk sums of max(p - q, 0), which need both rows' totals; the draw.
 #include "common.h"
 
 #define SV_MAX_NODES 64
-#define SV_THREADS 1024
+#define SV_CHUNK 2048              // tokens a wave sums: 32 a lane
+#define SV_WAVES 16                // waves of the walk's and the residual's workgroups
+#define SV_ERR 0x1p-18             // relative error of a row's 32-bit sum, with a factor 4 to spare
 
-template <int DT>   // 0 fp16, 1 bf16, 2 fp32
-__device__ __forceinline__ float sv_logit(const void* row, int64_t v) {
-  float x;
-  if (DT == 2) x = ((const float*)row)[v];
-  else x = ld16f<DT == 1>(((const unsigned short*)row)[v]);
-  return x == x ? x : -INFINITY;
-}
-
-// weight of logit x where m is the row's largest (1 there, infinite or not)
-__device__ __forceinline__ double sv_weight(float x, float m, double inv_t) {
-  return x == -INFINITY ? 0.0 : x == m ? 1.0 : exp(((double)x - (double)m) * inv_t);
-}
+enum { SV_DONE = 0, SV_TARGET = 1, SV_RESIDUAL = 2 };   // where the next token comes from
 
 struct SvArgs {
   const void* logits;
@@ -46,202 +41,622 @@ struct SvArgs {
   const float* uniforms;
   const float* temperature;
   float temp;
-  int n, T, V;
+  int n, T, V, chunks;
   int* path;
   int64_t* out_tokens;
   int* emitted;
+  float2* rec;             // [n T target rows, n (T - 1) draft rows][chunks] (largest, sum or index)
+  double* sums;            // [3][n][chunks]: target, draft, residual
+  struct SvSeq* seqs;      // [n]
 };
 
-struct SvRow {
-  const void* row;
-  float m;        // largest logit
-  int best;       // its first index
-  double z;       // sum of weights
+struct SvSeq {             // what the walk leaves for the draw
+  int mode, last, len;
+  float m, mq;             // largest logits of the drawn row and of the draft's
+  uint32_t tried[2];       // children tried at the last node
 };
 
 template <int DT>
-__device__ SvRow sv_stats(const void* row, int V, double inv_t, bool greedy) {
-  __shared__ float wm[16];
-  __shared__ int wi[16];
-  __shared__ double wz[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ constexpr int sv_size() { return DT == 2 ? 4 : 2; }
+
+template <int DT>   // 0 fp16, 1 bf16, 2 fp32; NaN as -inf
+__device__ __forceinline__ float sv_logit(const void* row, int64_t v) {
+  float x;
+  if (DT == 2) x = ((const float*)row)[v];
+  else x = ld16f<DT == 1>(((const unsigned short*)row)[v]);
+  return x == x ? x : -INFINITY;
+}
+
+template <int DT>
+__device__ __forceinline__ const void* sv_row(const SvArgs& a, int s, int i) {
+  return (const char*)a.logits + (s * a.seq_stride + i * a.row_stride) * sv_size<DT>();
+}
+template <int DT>
+__device__ __forceinline__ const void* sv_draft_row(const SvArgs& a, int s, int i) {
+  return (const char*)a.draft + (s * a.dseq_stride + i * a.drow_stride) * sv_size<DT>();
+}
+
+__device__ __forceinline__ float sv_temp(const SvArgs& a, int s) {
+  return a.temperature ? a.temperature[s] : a.temp;
+}
+__device__ __forceinline__ int sv_used(const SvArgs& a, int s) {
+  return a.counts ? min(max(a.counts[s], 0), a.T) : a.T;
+}
+
+// 2^t for t <= 0: t = n + f, |f| <= 1/2, 2^f by the polynomial through its values at the eleven
+// Chebyshev points of [-1/2, 1/2] (relative error 3e-16), 2^n by the exponent (0 far below).
+__device__ __forceinline__ double sv_exp2(double t) {
+#pragma clang fp contract(off)          // the same wherever it is inlined
+  const double n = rint(t), f = t - n;
+  double r = 0x1.e6063f7217bc6p-28;
+  r = fma(r, f, 0x1.b675bca4eeebbp-24);
+  r = fma(r, f, 0x1.62bfd47773353p-20);
+  r = fma(r, f, 0x1.ffcb54062e698p-17);
+  r = fma(r, f, 0x1.430913096fd9fp-13);
+  r = fma(r, f, 0x1.5d87fe9d7a584p-10);
+  r = fma(r, f, 0x1.3b2ab6fba1ddap-7);
+  r = fma(r, f, 0x1.c6b08d703ce49p-5);
+  r = fma(r, f, 0x1.ebfbdff82c598p-3);
+  r = fma(r, f, 0x1.62e42fefa3a19p-1);
+  r = fma(r, f, 1.0);
+  return ldexp(r, (int)fmax(n, -2000.0));
+}
+
+// weight of logit x in a row whose largest is m: 1 there, infinite or not
+__device__ __forceinline__ double sv_weight(float x, float m, double c) {
+#pragma clang fp contract(off)
+  const double w = sv_exp2(((double)x - (double)m) * c);
+  return x == m && m > -INFINITY ? 1.0 : x > -INFINITY && m < INFINITY ? w : 0.0;
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, OMNI_WAVE);
+  return v;
+}
+
+// A lane's 32 logits of a chunk, as they are stored, N in each of P 16-byte pieces; element e of
+// piece j is token chunk + at(lane, j) + e.
+template <int DT>
+struct SvPiece {
+  static constexpr int N = DT == 2 ? 4 : 8, P = 32 / N;
+  u32x4 w;
+  static __device__ __forceinline__ int at(int lane, int j) { return j * 64 * N + lane * N; }
+  __device__ __forceinline__ float get(int e) const {      // may be NaN
+    if (DT == 2) return __builtin_bit_cast(float, (uint32_t)w[e % N]);
+    return ld16f<DT == 1>((unsigned short)(w[e % N / 2] >> (16 * (e & 1))));
+  }
+  // tokens past the vocabulary: -inf
+  __device__ __forceinline__ void load(const void* row, int v0, int V, int lane, int j) {
+    const int v1 = v0 + at(lane, j);
+    if (v0 + SV_CHUNK <= V) {            // rows of an odd width are off every alignment
+      __builtin_memcpy(&w, (const char*)row + (int64_t)v1 * sv_size<DT>(), 16);
+      return;
+    }
+    constexpr uint32_t NONE = DT == 0 ? 0xfc00fc00u : DT == 1 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int v = v1 + d * N / 4;
+      uint32_t x = NONE;
+      if (DT == 2) {
+        if (v < V) x = ((const uint32_t*)row)[v];
+      } else {
+        const unsigned short* r = (const unsigned short*)row;
+        if (v < V) x = (x & 0xffff0000u) | r[v];
+        if (v + 1 < V) x = (x & 0xffffu) | (uint32_t)r[v + 1] << 16;
+      }
+      w[d] = x;
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Row statistics: one wave a 2048-token chunk of a row, rec = (largest logit, sum of weights
+// relative to it), for greedy rows (largest logit, its first index).
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(256) void sv_stats_kernel(SvArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int per = (a.chunks + 3) >> 2;
+  const int r = blockIdx.x / per, chunk = (blockIdx.x - r * per) * 4 + (threadIdx.x >> 6);
+  if (chunk >= a.chunks) return;
+  const int target_rows = a.n * a.T;
+  const bool is_draft = r >= target_rows;
+  const int T = is_draft ? a.T - 1 : a.T, rr = is_draft ? r - target_rows : r;
+  const int s = rr / T, i = rr - s * T;
+  const float temp = sv_temp(a, s);
+  const bool greedy = !(temp > 0.f);
+  const int used = sv_used(a, s);
+  if (is_draft ? (greedy || i + 1 >= used) : i >= used) return;
+  const void* row = is_draft ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
+  const int v0 = chunk * SV_CHUNK;
+  typedef SvPiece<DT> P;
+  P x[P::P];
+#pragma unroll
+  for (int j = 0; j < P::P; ++j) x[j].load(row, v0, a.V, lane, j);
   float m = -INFINITY;
-  int at = 0x7fffffff;
-  for (int v = tid; v < V; v += SV_THREADS) {
-    const float x = sv_logit<DT>(row, v);
-    if (x > m) {
-      m = x;
-      at = v;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) m = fmaxf(m, x[e / P::N].get(e));       // leaves a NaN out
+  m = wave_max(m);
+  float2* out = a.rec + (int64_t)r * a.chunks + chunk;
+  if (greedy) {
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int e = 31; e >= 0; --e)
+      if (x[e / P::N].get(e) == m) at = v0 + P::at(lane, e / P::N) + e % P::N;
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+    if (lane == 0) *out = make_float2(m, __builtin_bit_cast(float, at));
+    return;
+  }
+  // (x - m) c in two steps: c may be as large as fp32 goes, and an infinite m stays in order
+  const float c = fminf(1.4426950408889634f / temp, 1e38f);
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+  if (fabsf(m) < INFINITY) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float w = __builtin_amdgcn_exp2f((x[e / P::N].get(e) - m) * c);
+      z[e & 3] += w == w ? w : 0.f;
+    }
+  } else if (m == INFINITY) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) z[e & 3] += x[e / P::N].get(e) == m ? 1.f : 0.f;
+  }
+  const float sum = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
+  if (lane == 0) *out = make_float2(m, sum);
+}
+
+// A row's chunks together, by one wave: largest logit and 64-bit sum of their 32-bit sums
+// (greedy: first index).
+__device__ __forceinline__ void sv_combine(const float2* rec, int chunks, int lane, double c, bool greedy,
+                                           float& m, double& z, int& best) {
+  float2 keep[2];
+  m = -INFINITY;
+  for (int k = lane, j = 0; k < chunks; k += 64, ++j) {
+    const float2 v = rec[k];
+    if (j < 2) keep[j] = v;
+    m = fmaxf(m, v.x);
+  }
+  m = wave_max(m);
+  z = 0.0;
+  best = 0x7fffffff;
+  for (int k = lane, j = 0; k < chunks; k += 64, ++j) {
+    const float2 v = j < 2 ? keep[j] : rec[k];
+    if (greedy) {
+      if (v.x == m) best = min(best, __builtin_bit_cast(int, v.y));
+    } else {
+      z += (double)v.y * sv_weight(v.x, m, c);
+    }
+  }
+  if (greedy)
+    for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
+  else
+    z = wave_sum64(z);
+}
+
+// 64-bit sum of a chunk's weights, the tried tokens left out; by one wave.
+template <int DT>
+__device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V, int lane, float m,
+                                               double c, const int64_t* tok, uint64_t tried) {
+  typedef SvPiece<DT> P;
+  const int v0 = chunk * SV_CHUNK;
+  double z[2] = {0.0, 0.0};
+  P next;
+  next.load(row, v0, V, lane, 0);
+#pragma unroll 1
+  for (int j = 0; j < P::P; ++j) {
+    const P x = next;
+    if (j + 1 < P::P) next.load(row, v0, V, lane, j + 1);
+    uint32_t gone = 0;                                  // elements that hold a tried token
+    for (uint64_t b = tried; b; b &= b - 1) {
+      const int64_t t = tok[__ffsll((unsigned long long)b) - 1] - (v0 + P::at(lane, j));
+      if (t >= 0 && t < P::N) gone |= 1u << t;
+    }
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      const double w = sv_weight(x.get(e), m, c);
+      z[e & 1] += gone >> e & 1 ? 0.0 : w;
+    }
+  }
+  return wave_sum64(z[0] + z[1]);
+}
+
+// ---------------------------------------------------------------------------
+// The walk, by every workgroup of a sequence (part 0 writes it down), then this part's share of
+// the drawn row's chunk sums.  All nodes' tests are made at once, a lane each: a node's own test
+// depends on its earlier siblings' tokens, not on their fate.
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
+  __shared__ float ms[2][SV_MAX_NODES];
+  __shared__ double zs[2][SV_MAX_NODES];
+  __shared__ double wt[SV_MAX_NODES];
+  __shared__ int par[SV_MAX_NODES], best[SV_MAX_NODES];
+  __shared__ int64_t tok[SV_MAX_NODES];
+  __shared__ double part[SV_WAVES];
+  __shared__ uint64_t open_rows[2], tried_s;
+  __shared__ int last_s, len_s;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int parts = (a.chunks + SV_WAVES - 1) / SV_WAVES;
+  const int s = blockIdx.x / parts, mine = blockIdx.x - s * parts;
+  const int T = a.T, used = sv_used(a, s);
+  const float temp = sv_temp(a, s);
+  const bool greedy = !(temp > 0.f), chain_q = a.draft && !greedy;
+  const double c = greedy ? 1.0 : 1.4426950408889634073599 / (double)temp;
+  int* path = a.path + (int64_t)s * T;
+  int64_t* out = a.out_tokens + (int64_t)s * T;
+  if (used == 0) {
+    if (mine) return;
+    if (tid < T) {
+      path[tid] = -1;
+      out[tid] = -1;
+    }
+    if (tid == 0) {
+      a.emitted[s] = 0;
+      a.seqs[s].mode = SV_DONE;
+    }
+    return;
+  }
+  // a lane a node: its parent, token and random number, its logits at the parent's rows
+  int up = -1;
+  int64_t x = 0;
+  double u = 0.0;
+  float lp = -INFINITY, lq = -INFINITY;
+  if (lane < used) {
+    up = lane == 0 ? -1 : a.parents ? a.parents[(int64_t)s * T + lane] : lane - 1;
+    if (up < 0 || up >= lane) up = -1;
+    x = a.tokens[(int64_t)s * T + lane];
+    if (a.uniforms) u = (double)a.uniforms[(int64_t)s * T + lane];
+    if (up >= 0 && x >= 0 && x < a.V) {
+      lp = sv_logit<DT>(sv_row<DT>(a, s, up), x);
+      if (chain_q) lq = sv_logit<DT>(sv_draft_row<DT>(a, s, up), x);
+    }
+  }
+  for (int i = wave; i < used; i += SV_WAVES) {
+    float m;
+    double z;
+    int b;
+    sv_combine(a.rec + ((int64_t)s * T + i) * a.chunks, a.chunks, lane, c, greedy, m, z, b);
+    if (lane == 0) {
+      ms[0][i] = m;
+      zs[0][i] = z;
+      best[i] = b;
+    }
+    if (chain_q && i + 1 < used) {
+      sv_combine(a.rec + ((int64_t)a.n * T + (int64_t)s * (T - 1) + i) * a.chunks, a.chunks, lane, c,
+                 false, m, z, b);
+      if (lane == 0) {
+        ms[1][i] = m;
+        zs[1][i] = z;
+      }
+    }
+  }
+  if (wave == 0) {
+    par[lane] = up;
+    tok[lane] = x;
+  }
+  __syncthreads();
+
+  // exact: rows whose sums are 64-bit by now
+  uint64_t exact[2] = {0, 0};
+  while (true) {
+    bool stands = false, open = false;
+    if (wave == 0) {
+      double w = 0.0;
+      bool twice = up < 0;
+      if (up >= 0) {
+        for (int j = up + 1; j < lane; ++j) twice |= par[j] == up && tok[j] == x;
+        if (!twice && x >= 0 && x < a.V)
+          w = greedy ? (ms[0][up] > -INFINITY && x == best[up] ? 1.0 : 0.0)
+                     : sv_weight(lp, ms[0][up], c);
+      }
+      wt[lane] = w;                                       // read by this wave alone, in order
+      if (w > 0.0) {
+        if (greedy) {
+          stands = true;
+        } else if (chain_q) {
+          // u q / Zq < w / Z, both sides times Z Zq
+          const double a0 = u * sv_weight(lq, ms[1][up], c) * zs[0][up], a1 = w * zs[1][up];
+          stands = a0 < a1;
+          open = fabs(a0 - a1) <= 2.0 * SV_ERR * a1 && !((exact[0] & exact[1]) >> up & 1);
+          if (zs[1][up] == 0.0) stands = true, open = false;      // q is nowhere
+        } else {
+          double left = zs[0][up];
+          for (int j = up + 1; j < lane; ++j)
+            if (par[j] == up) left -= wt[j];
+          stands = u * left < w;
+          open = fabs(u * left - w) <= u * zs[0][up] * SV_ERR && !(exact[0] >> up & 1);
+        }
+      }
+      uint64_t rows = 0;
+      for (uint64_t b = __ballot(open); b; b &= b - 1)
+        rows |= 1ull << __shfl(up, __ffsll((unsigned long long)b) - 1);
+      if (lane == 0) open_rows[0] = rows;
+    }
+    __syncthreads();
+    const uint64_t todo = open_rows[0];
+    if (!todo) {
+      if (wave == 0) {
+        const uint64_t ok = __ballot(stands);
+        int here = 0, len = 1;
+        while (true) {
+          const uint64_t next = __ballot(up == here) & ok;
+          if (!next) break;
+          here = __ffsll((unsigned long long)next) - 1;
+          if (mine == 0 && lane == 0) {
+            path[len] = here;
+            out[len - 1] = tok[here];
+          }
+          ++len;
+        }
+        const uint64_t tried = __ballot(up == here);
+        if (lane == 0) {
+          last_s = here;
+          len_s = len;
+          tried_s = tried;
+        }
+      }
+      break;
+    }
+    // the open rows' sums in 64 bits, by the whole workgroup
+    for (uint64_t b = todo; b; b &= b - 1) {
+      const int i = __ffsll((unsigned long long)b) - 1;
+      for (int d = 0; d < (chain_q ? 2 : 1); ++d) {
+        const void* row = d ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
+        double z = 0.0;
+        for (int k = wave; k < a.chunks; k += SV_WAVES)
+          z += sv_chunk_sum<DT>(row, k, a.V, lane, ms[d][i], c, tok, 0);
+        if (lane == 0) part[wave] = z;
+        __syncthreads();
+        if (tid == 0) {
+          double t = 0.0;
+          for (int w = 0; w < SV_WAVES; ++w) t += part[w];
+          zs[d][i] = t;
+        }
+        __syncthreads();
+      }
+    }
+    exact[0] |= todo;
+    exact[1] |= todo;
+  }
+  __syncthreads();
+  const int last = last_s, len = len_s;
+  const uint64_t tried = tried_s;
+  const float m = ms[0][last];
+  const bool residual = chain_q && tried != 0;
+  const int mode = greedy || m == -INFINITY ? SV_DONE : residual ? SV_RESIDUAL : SV_TARGET;
+  if (mine == 0) {
+    if (tid == 0) {
+      path[0] = 0;
+      a.emitted[s] = len;
+      if (mode == SV_DONE) out[len - 1] = m == -INFINITY ? -1 : best[last];
+      SvSeq* q = a.seqs + s;
+      q->mode = mode;
+      q->last = last;
+      q->len = len;
+      q->m = m;
+      q->mq = residual ? ms[1][last] : 0.f;
+      q->tried[0] = (uint32_t)tried;
+      q->tried[1] = (uint32_t)(tried >> 32);
+    }
+    if (tid >= len && tid < T) {
+      path[tid] = -1;
+      out[tid] = -1;
+    }
+  }
+  const int chunk = mine * SV_WAVES + wave;
+  if (mode == SV_DONE || chunk >= a.chunks) return;
+  const double sp = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), chunk, a.V, lane, m, c, tok,
+                                     residual ? 0 : tried);
+  if (lane == 0) a.sums[(int64_t)s * a.chunks + chunk] = sp;
+  if (residual) {
+    const double sq = sv_chunk_sum<DT>(sv_draft_row<DT>(a, s, last), chunk, a.V, lane, ms[1][last], c,
+                                       tok, 0);
+    if (lane == 0) a.sums[((int64_t)a.n + s) * a.chunks + chunk] = sq;
+  }
+}
+
+// Sum of a sequence's chunk sums, by one wave.
+__device__ __forceinline__ double sv_total(const double* sums, int chunks, int lane) {
+  double z = 0.0;
+  for (int k = lane; k < chunks; k += 64) z += sums[k];
+  return wave_sum64(z);
+}
+
+// max(p - q, 0) of a token; zp, zq: 1 / totals
+__device__ __forceinline__ double sv_rest(float x, float y, float m, float mq, double c, double zp,
+                                          double zq) {
+#pragma clang fp contract(off)          // equal rows leave exactly nothing
+  const double d = sv_weight(x, m, c) * zp - sv_weight(y, mq, c) * zq;
+  return d > 0.0 ? d : 0.0;
+}
+
+template <int DT>
+__global__ __launch_bounds__(64 * SV_WAVES) void sv_residual_kernel(SvArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int parts = (a.chunks + SV_WAVES - 1) / SV_WAVES;
+  const int s = blockIdx.x / parts, chunk = (blockIdx.x - s * parts) * SV_WAVES + wave;
+  const SvSeq q = a.seqs[s];
+  if (q.mode != SV_RESIDUAL || chunk >= a.chunks) return;
+  const double c = 1.4426950408889634073599 / (double)sv_temp(a, s);
+  const double* sums = a.sums + (int64_t)s * a.chunks;
+  const double zp = 1.0 / sv_total(sums, a.chunks, lane);
+  const double tq = sv_total(sums + (int64_t)a.n * a.chunks, a.chunks, lane);
+  const double zq = tq > 0.0 ? 1.0 / tq : 0.0;
+  typedef SvPiece<DT> P;
+  const void* row = sv_row<DT>(a, s, q.last);
+  const void* drow = sv_draft_row<DT>(a, s, q.last);
+  const int v0 = chunk * SV_CHUNK;
+  double z[2] = {0.0, 0.0};
+  P nx, ny;
+  nx.load(row, v0, a.V, lane, 0);
+  ny.load(drow, v0, a.V, lane, 0);
+#pragma unroll 1
+  for (int j = 0; j < P::P; ++j) {
+    const P x = nx, y = ny;
+    if (j + 1 < P::P) {
+      nx.load(row, v0, a.V, lane, j + 1);
+      ny.load(drow, v0, a.V, lane, j + 1);
+    }
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) z[e & 1] += sv_rest(x.get(e), y.get(e), q.m, q.mq, c, zp, zq);
+  }
+  const double sum = wave_sum64(z[0] + z[1]);
+  if (lane == 0) a.sums[(2 * (int64_t)a.n + s) * a.chunks + chunk] = sum;
+}
+
+// Inclusive prefix sums of a lane's v over the wave.
+__device__ __forceinline__ double wave_scan64(double v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// The draw, one workgroup a sequence: the chunk that u_0 times the total falls into, then the token
+// within it, eight a thread.
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
+  __shared__ double wsum[4];
+  __shared__ double base_s, want_s;
+  __shared__ int chunk_s, pick[4], tail[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int s = blockIdx.x;
+  const SvSeq q = a.seqs[s];
+  if (q.mode == SV_DONE) return;
+  const double c = 1.4426950408889634073599 / (double)sv_temp(a, s);
+  const int64_t* tok = a.tokens + (int64_t)s * a.T;
+  const void* row = sv_row<DT>(a, s, q.last);
+  const void* drow = q.mode == SV_RESIDUAL ? sv_draft_row<DT>(a, s, q.last) : nullptr;
+  double* sums = a.sums + (int64_t)s * a.chunks;
+  double zp = 1.0, zq = 0.0;
+  if (drow) {
+    zp = 1.0 / sv_total(sums, a.chunks, lane);
+    const double tq = sv_total(sums + (int64_t)a.n * a.chunks, a.chunks, lane);
+    zq = tq > 0.0 ? 1.0 / tq : 0.0;
+    sums += 2 * (int64_t)a.n * a.chunks;
+  }
+  uint64_t tried = drow ? 0 : (uint64_t)q.tried[1] << 32 | q.tried[0];
+  if (!(sv_total(sums, a.chunks, lane) > 0.0)) {
+    // nothing is left: p itself, summed here
+    tried = 0;
+    drow = nullptr;
+    for (int k = wave; k < a.chunks; k += 4) {
+      const double z = sv_chunk_sum<DT>(row, k, a.V, lane, q.m, c, tok, 0);
+      if (lane == 0) sums[k] = z;
+    }
+    __syncthreads();                                    // the sums, too, are this workgroup's
+  }
+  if (wave == 0) {
+    double total = 0.0;
+    for (int k0 = 0; k0 < a.chunks; k0 += 64) {
+      const double v = wave_scan64(k0 + lane < a.chunks ? sums[k0 + lane] : 0.0, lane);
+      total += __shfl(v, 63);
+    }
+    const double want = (double)a.uniforms[(int64_t)s * a.T] * total;
+    double base = 0.0, at = 0.0;
+    int found = -1, full = 0;
+    for (int k0 = 0; k0 < a.chunks && found < 0; k0 += 64) {
+      const double own = k0 + lane < a.chunks ? sums[k0 + lane] : 0.0;
+      const double v = wave_scan64(own, lane) + base;
+      const uint64_t hit = __ballot(own > 0.0 && v > want), some = __ballot(own > 0.0);
+      const int l = hit ? __ffsll((unsigned long long)hit) - 1
+                    : some ? 63 - __clzll((long long)some) : -1;
+      if (l >= 0) {                                     // so far the last chunk with weight
+        full = k0 + l;
+        at = l ? __shfl(v, l - 1) : base;
+      }
+      if (hit) found = full;
+      base = __shfl(v, 63);
+    }
+    if (lane == 0) {
+      chunk_s = full;
+      base_s = at;
+      want_s = want;
+    }
+  }
+  __syncthreads();
+  const int v0 = chunk_s * SV_CHUNK + tid * 8;
+  double w[8], sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int v = v0 + e;
+    w[e] = 0.0;
+    if (v < a.V) {
+      const float x = sv_logit<DT>(row, v);
+      if (drow) {
+        w[e] = sv_rest(x, sv_logit<DT>(drow, v), q.m, q.mq, c, zp, zq);
+      } else {
+        w[e] = sv_weight(x, q.m, c);
+        for (uint64_t b = tried; b; b &= b - 1)
+          if (tok[__ffsll((unsigned long long)b) - 1] == v) w[e] = 0.0;
+      }
+    }
+    sum += w[e];
+  }
+  double run = wave_scan64(sum, lane);
+  if (lane == 63) wsum[wave] = run;
+  __syncthreads();
+  run -= sum;
+  for (int k = 0; k < wave; ++k) run += wsum[k];
+  run += base_s;
+  const double want = want_s;
+  int mine = 0x7fffffff, heavy = -1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    run += w[e];
+    if (w[e] > 0.0) {
+      heavy = v0 + e;
+      if (mine == 0x7fffffff && run > want) mine = v0 + e;
     }
   }
   for (int o = 32; o; o >>= 1) {
-    const float xm = __shfl_xor(m, o);
-    const int xi = __shfl_xor(at, o);
-    if (xm > m || (xm == m && xi < at)) {
-      m = xm;
-      at = xi;
-    }
+    mine = min(mine, __shfl_xor(mine, o));
+    heavy = max(heavy, __shfl_xor(heavy, o));
   }
-  __syncthreads();
   if (lane == 0) {
-    wm[wave] = m;
-    wi[wave] = at;
+    pick[wave] = mine;
+    tail[wave] = heavy;
   }
   __syncthreads();
-  for (int w = 0; w < 16; ++w)
-    if (wm[w] > m || (wm[w] == m && wi[w] < at)) {
-      m = wm[w];
-      at = wi[w];
+  if (tid == 0) {
+    for (int k = 1; k < 4; ++k) {
+      mine = min(mine, pick[k]);
+      heavy = max(heavy, tail[k]);
     }
-  SvRow r = {row, m, at, 1.0};
-  if (greedy) return r;
-  double z = 0.0;
-  for (int v = tid; v < V; v += SV_THREADS) z += sv_weight(sv_logit<DT>(row, v), m, inv_t);
-  for (int o = 32; o; o >>= 1) z += __shfl_xor(z, o);
-  if (lane == 0) wz[wave] = z;
-  __syncthreads();
-  r.z = 0.0;
-  for (int w = 0; w < 16; ++w) r.z += wz[w];
-  if (r.z == 0.0) r.z = 1.0;      // no token above -inf: every probability is 0
-  return r;
+    // rounding, or u_0 >= 1: the chunk's last token with weight
+    a.out_tokens[(int64_t)s * a.T + q.len - 1] = mine != 0x7fffffff ? mine : heavy;
+  }
 }
 
-// One workgroup a sequence, walking from the root.
-template <int DT>
-__global__ __launch_bounds__(SV_THREADS) void spec_verify_kernel(SvArgs a) {
-  constexpr int SIZE = DT == 2 ? 4 : 2;
-  __shared__ double part[SV_THREADS];
-  __shared__ int64_t found;
-  const int tid = threadIdx.x;
-  const int s = blockIdx.x;
-  const int used = a.counts ? min(max(a.counts[s], 0), a.T) : a.T;
-  const int64_t* tok = a.tokens + (int64_t)s * a.T;
-  const int* par = a.parents ? a.parents + (int64_t)s * a.T : nullptr;
-  const float* u = a.uniforms ? a.uniforms + (int64_t)s * a.T : nullptr;
-  int* path = a.path + (int64_t)s * a.T;
-  int64_t* out = a.out_tokens + (int64_t)s * a.T;
-  const float temp = a.temperature ? a.temperature[s] : a.temp;
-  const bool greedy = !(temp > 0.f);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)temp;
-  if (used == 0) {
-    for (int i = tid; i < a.T; i += SV_THREADS) {
-      path[i] = -1;
-      out[i] = -1;
-    }
-    if (tid == 0) a.emitted[s] = 0;
-    return;
-  }
-  int here = 0, len = 1;
-  uint64_t tried = 0;
-  SvRow p, q;
-  while (true) {
-    p = sv_stats<DT>((const char*)a.logits + (s * a.seq_stride + here * a.row_stride) * SIZE, a.V,
-                     inv_t, greedy);
-    const bool chain_q = a.draft && here + 1 < used && !greedy;
-    q.row = nullptr;
-    if (chain_q)
-      q = sv_stats<DT>((const char*)a.draft + (s * a.dseq_stride + here * a.drow_stride) * SIZE,
-                       a.V, inv_t, false);
-    tried = 0;
-    int taken = -1;
-    double left = p.z;
-    for (int i = here + 1; i < used && taken < 0 && p.m > -INFINITY; ++i) {
-      if ((par ? par[i] : i - 1) != here) continue;
-      const int64_t x = tok[i];
-      double w = 0.0;
-      bool twice = x < 0 || x >= a.V;
-      for (int j = here + 1; j < i; ++j) twice |= ((tried >> j) & 1) && tok[j] == x;
-      if (!twice) w = greedy ? (x == p.best ? 1.0 : 0.0) : sv_weight(sv_logit<DT>(p.row, x), p.m, inv_t);
-      bool ok;
-      if (greedy) ok = w > 0.0;
-      else if (chain_q)
-        ok = !twice && (double)u[i] * (sv_weight(sv_logit<DT>(q.row, x), q.m, inv_t) / q.z) < w / p.z;
-      else ok = (double)u[i] * left < w;
-      if (ok) taken = i;
-      tried |= 1ull << i;
-      left -= w;
-    }
-    if (taken < 0) break;
-    if (tid == 0) {
-      path[len] = taken;
-      out[len - 1] = tok[taken];
-    }
-    here = taken;
-    ++len;
-  }
-  // the next token
-  int64_t next = -1;
-  if (greedy || p.m == -INFINITY) {
-    next = p.m == -INFINITY ? -1 : p.best;
-  } else {
-    const int seg = (a.V + SV_THREADS - 1) / SV_THREADS;
-    const int lo = min(a.V, tid * seg), hi = min(a.V, lo + seg);
-    for (int full = 0; full < 2 && next < 0; ++full) {   // second: an empty residual, p itself
-      auto weight = [&](int v) {
-        const double w = sv_weight(sv_logit<DT>(p.row, v), p.m, inv_t);
-        if (full) return w;
-        if (q.row) {
-          const double d = w / p.z - sv_weight(sv_logit<DT>(q.row, v), q.m, inv_t) / q.z;
-          return d > 0.0 ? d : 0.0;
-        }
-        for (uint64_t b = tried; b; b &= b - 1)
-          if (tok[__ffsll((unsigned long long)b) - 1] == v) return 0.0;
-        return w;
-      };
-      double sum = 0.0;
-      for (int v = lo; v < hi; ++v) sum += weight(v);
-      __syncthreads();
-      part[tid] = sum;
-      if (tid == 0) found = 0x7fffffff;
-      __syncthreads();
-      double before = 0.0, total = 0.0;
-      for (int i = 0; i < SV_THREADS; ++i) {
-        if (i == tid) before = total;
-        total += part[i];
-      }
-      const double want = (double)u[0] * total;
-      int mine = 0x7fffffff, last = -1;
-      double run = before;
-      if (total > 0.0)
-        for (int v = lo; v < hi; ++v) {
-          const double w = weight(v);
-          if (w > 0.0) last = v;
-          run += w;
-          if (w > 0.0 && run > want) {
-            mine = v;
-            break;
-          }
-        }
-      if (mine != 0x7fffffff) atomicMin((unsigned long long*)&found, (unsigned long long)mine);
-      __syncthreads();
-      if (found != 0x7fffffff) {
-        next = found;
-      } else if (total > 0.0) {            // rounding, or u >= 1: the last token with weight
-        __syncthreads();
-        if (tid == 0) found = -1;
-        __syncthreads();
-        if (last >= 0) atomicMax((long long*)&found, (long long)last);
-        __syncthreads();
-        next = found;
-      }
-      __syncthreads();
-    }
-  }
-  if (tid == 0) {
-    path[0] = 0;
-    out[len - 1] = next;
-    a.emitted[s] = len;
-  }
-  for (int i = len + tid; i < a.T; i += SV_THREADS) {
-    path[i] = -1;
-    out[i] = -1;
-  }
+static int64_t sv_work(int64_t n, int64_t T, int64_t V, bool drafted) {
+  const int64_t chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
+  const int64_t rows = n * T + (drafted ? n * (T - 1) : 0);
+  return rows * chunks + 3 * n * chunks + 4 * n;        // records, sums, sequences, in doubles
 }
 
 extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted) {
   if (n < 0 || n_nodes < 1 || vocab < 1) return OMNI_EINVAL;
   if (n_nodes > SV_MAX_NODES) return OMNI_EUNSUPPORTED;
-  return 0;
+  const int64_t work = sv_work(n, n_nodes, vocab, drafted);
+  return work > 0x7fffffff ? OMNI_EUNSUPPORTED : (int)work;
+}
+
+template <int DT>
+static void sv_launch(const SvArgs& a, hipStream_t st) {
+  const int rows = a.n * a.T + (a.draft ? a.n * (a.T - 1) : 0);
+  const int parts = ceil_div(a.chunks, SV_WAVES);
+  hipLaunchKernelGGL((sv_stats_kernel<DT>), dim3(rows * ceil_div(a.chunks, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((sv_walk_kernel<DT>), dim3(a.n * parts), dim3(64 * SV_WAVES), 0, st, a);
+  if (a.uniforms) {                                     // else every row is greedy
+    if (a.draft)
+      hipLaunchKernelGGL((sv_residual_kernel<DT>), dim3(a.n * parts), dim3(64 * SV_WAVES), 0, st, a);
+    hipLaunchKernelGGL((sv_draw_kernel<DT>), dim3(a.n), dim3(256), 0, st, a);
+  }
 }
 
 extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t row_stride,
@@ -259,13 +674,38 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   if (!uniforms && (temperature || temp > 0.f)) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
   if (!logits || !tokens || !path || !out_tokens || !emitted) return OMNI_EINVAL;
-  const SvArgs a = {logits, seq_stride, row_stride, draft, draft_seq_stride, draft_row_stride, tokens,
-                    parents, counts, uniforms, temperature, temp, n, n_nodes, vocab, path, out_tokens,
-                    emitted};
+  if (n_nodes == 1) draft = nullptr;
+  const int64_t work = sv_work(n, n_nodes, vocab, draft != nullptr);
+  if (work > 0x7fffffff) return OMNI_EUNSUPPORTED;
+  if (!workspace || ((uintptr_t)workspace & 7) || workspace_doubles < work) return OMNI_EINVAL;
+  SvArgs a;
+  a.logits = logits;
+  a.seq_stride = seq_stride;
+  a.row_stride = row_stride;
+  a.draft = draft;
+  a.dseq_stride = draft_seq_stride;
+  a.drow_stride = draft_row_stride;
+  a.tokens = tokens;
+  a.parents = parents;
+  a.counts = counts;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.temp = temp;
+  a.n = n;
+  a.T = n_nodes;
+  a.V = vocab;
+  a.chunks = ceil_div(vocab, SV_CHUNK);
+  a.path = path;
+  a.out_tokens = out_tokens;
+  a.emitted = emitted;
+  a.rec = (float2*)workspace;
+  const int64_t rows = (int64_t)n * n_nodes + (draft ? (int64_t)n * (n_nodes - 1) : 0);
+  a.sums = (double*)workspace + rows * a.chunks;
+  a.seqs = (SvSeq*)(a.sums + 3 * (int64_t)n * a.chunks);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == 0) hipLaunchKernelGGL((spec_verify_kernel<0>), dim3(n), dim3(SV_THREADS), 0, st, a);
-  else if (dtype == 1) hipLaunchKernelGGL((spec_verify_kernel<1>), dim3(n), dim3(SV_THREADS), 0, st, a);
-  else hipLaunchKernelGGL((spec_verify_kernel<2>), dim3(n), dim3(SV_THREADS), 0, st, a);
+  if (dtype == 0) sv_launch<0>(a, st);
+  else if (dtype == 1) sv_launch<1>(a, st);
+  else sv_launch<2>(a, st);
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }

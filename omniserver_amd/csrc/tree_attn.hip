@@ -9,30 +9,115 @@
 #define TREE_MAX 64
 
 // ---------------------------------------------------------------------------
-// The plan of a step, once for all layers: per node its ancestors (itself included; bit j =
-// node j), its pool row and position (row -1: not in use, or past the pool), its rotary
-// position starts + depth + rope_delta on all three axes; per sequence the prefix length, a
-// copy, so that the plan stays what it was when the lengths move on.  A node whose parent does
-// not precede it is a root of its own.  One wave a sequence: lane i walks up from node i.
+// The plan of a step, once for all layers.
+//
+// Per node its ancestors (itself included; bit j = node j), its pool row and position (row -1: not
+// in use, or past the pool), its rotary position starts + depth + rope_delta on all three axes; per
+// sequence the prefix length, a copy, so that the plan stays what it was when the lengths move on.
+// A node whose parent does not precede it is a root of its own.
+//
+// And the attention's schedule.  A sequence's keys count in units of `unit` (what a workgroup takes
+// in a step), once per KV head; the units of all (sequence, KV head) items stand in one line,
+// which is cut into equal stretches, one per column of workgroups.  So a batch of one long and many
+// short contexts loads the workgroups as evenly as one of equal contexts, whatever the lengths
+// on the device are.  A stretch is at least `least` units; least 0: a column for each item.
+//   seqs[s]     (prefix length, nodes in use, units, -)
+//   columns[c]  (s, g, first unit there, units in all, prefix length, nodes in use)
+//   heads[s][g] (first column | 1 << 30 where the item is not the first that column sees, last)
+// One wave a sequence: lane i walks up from node i; every wave sums all sequences' units and
+// writes the columns that start in its own sequence.
 // ---------------------------------------------------------------------------
+struct TreeCols {
+  int* seqs;       // [n][4]
+  int* columns;    // [ncols][8]
+  int* heads;      // [n][nkv][2]
+  int ncols, nkv, unit, least;
+};
+
 __global__ __launch_bounds__(64) void tree_plan_kernel(
     const int* __restrict__ parents, const int* __restrict__ counts,
     const int64_t* __restrict__ slots, const int64_t* __restrict__ lengths,
     const int64_t* __restrict__ rope_delta, int n, int T, int pool_rows, int max_len,
     int64_t* __restrict__ starts, uint64_t* __restrict__ ancestors,
     int64_t* __restrict__ positions, int64_t* __restrict__ token_slot,
-    int64_t* __restrict__ token_pos) {
+    int64_t* __restrict__ token_pos, TreeCols tc) {
   __shared__ int up[TREE_MAX];
   const int s = blockIdx.x, i = threadIdx.x;
+  if (i < T) up[i] = parents[(int64_t)s * T + i];
+  auto prefix = [&](int r) {
+    const int64_t row = slots ? slots[r] : r;
+    const int64_t v = row >= 0 && row < pool_rows ? lengths[row] : 0;
+    return (int)(v < 0 ? 0 : v > max_len ? max_len : v);
+  };
+  auto in_use = [&](int r) { return counts ? min(max(counts[r], 0), T) : T; };
   const int64_t slot = slots ? slots[s] : s;
   const bool row_ok = slot >= 0 && slot < pool_rows;
-  int64_t L = row_ok ? lengths[slot] : 0;
-  L = L < 0 ? 0 : L > max_len ? max_len : L;
+  const int L = prefix(s), used = in_use(s);
   const int64_t delta = row_ok && rope_delta ? rope_delta[slot] : 0;
-  const int used = counts ? min(max(counts[s], 0), T) : T;
-  if (i < T) up[i] = parents[(int64_t)s * T + i];
+
+  // units of the sequences before this one, its own, and all
+  int64_t before = 0, all = 0;
+  int units = 0;
+  for (int r0 = 0; r0 < n; r0 += 64) {
+    const int r = r0 + i;
+    int w = 0;
+    if (r < n) {
+      const int64_t row = slots ? slots[r] : r;
+      const int m = in_use(r);
+      if (m && row >= 0 && row < pool_rows) w = ceil_div(min(prefix(r) + m, max_len), tc.unit);
+      if (r == s) units = w;
+    }
+    int lo = r < s ? w : 0;
+    for (int o = 32; o; o >>= 1) {
+      w += __shfl_xor(w, o);
+      lo += __shfl_xor(lo, o);
+    }
+    all += w;
+    before += lo;
+  }
+  units = __shfl(units, s & 63);
+  all *= tc.nkv;
+  before *= tc.nkv;
+  int64_t cols = tc.least ? min((int64_t)tc.ncols, max((int64_t)1, all / tc.least)) : tc.ncols;
+  auto cut = [&](int64_t c) { return c * all / cols; };        // first unit of column c
+  for (int c = i; c < tc.ncols; c += 64) {
+    int* col = tc.columns + 8 * c;
+    if (tc.least) {
+      const int64_t lo = c < cols ? cut(c) : all, cnt = c < cols ? cut(c + 1) - lo : 0;
+      if (cnt > 0 && lo >= before && lo < before + (int64_t)units * tc.nkv) {
+        const int g = (int)((lo - before) / units);
+        *(i32x4*)col = (i32x4){s, g, (int)(lo - before) - g * units, (int)cnt};
+        *(i32x4*)(col + 4) = (i32x4){L, used, 0, 0};
+      } else if (cnt <= 0 && s == 0) {
+        *(i32x4*)col = (i32x4){0, 0, 0, 0};
+      }
+    } else if (c / tc.nkv == s) {
+      *(i32x4*)col = (i32x4){s, c % tc.nkv, 0, units};
+      *(i32x4*)(col + 4) = (i32x4){L, used, 0, 0};
+    }
+  }
+  for (int g = i; g < tc.nkv; g += 64) {
+    int2 at = make_int2(0, 0);
+    if (units && tc.least) {
+      const int64_t lo = before + (int64_t)g * units, hi = lo + units - 1;
+      // the last column that starts at or before a unit
+      auto column = [&](int64_t x) {
+        int64_t c = x * cols / all;
+        while (c + 1 < cols && cut(c + 1) <= x) ++c;
+        while (cut(c) > x) --c;
+        return (int)c;
+      };
+      at.x = column(lo);
+      at.y = column(hi);
+      if (cut(at.x) < lo) at.x |= 1 << 30;
+    }
+    *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) = at;
+  }
+  if (i == 0) {
+    starts[s] = L;
+    *(i32x4*)(tc.seqs + 4 * s) = (i32x4){L, used, units, 0};
+  }
   __syncthreads();
-  if (i == 0) starts[s] = L;
   if (i >= T) return;
   uint64_t m = 0;
   if (i < used) {
@@ -72,11 +157,13 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// The tile structure and what bounds it are in attn_rows.h.  A workgroup takes one sequence, one
-// KV head, 32 R rows of its (node, query head) pairs, node-major, and one of `splits` shares of
-// the keys, which its S groups of R waves take in contiguous runs of KT-key tiles (each group has
-// its own LDS tiles, as in attn_rows.hip).  A K / V byte staged in LDS serves all query heads of
-// the group and up to 32 R / G nodes.
+// The tile structure and what bounds it are in attn_rows.h.  A workgroup takes 32 R (node, query
+// head) rows, node-major, of the sequences and KV heads that its column of the schedule runs
+// through, one stretch of keys after another; the S groups of R waves take contiguous runs of a
+// stretch's KT-key tiles (each group has its own LDS tiles, as in attn_rows.hip).  A K / V byte
+// staged in LDS serves all query heads of the group and up to 32 R / G nodes.  A stretch that is
+// an item's whole gives outputs, a part of one a softmax state for the merging launch: only a
+// column's first and last can be parts.
 //
 // The keys are the prefix and, behind it, the nodes.  Only tiles that reach past the prefix are
 // masked, with the row's ancestor word shifted to the tile.  A node that a row does not attend to
@@ -89,21 +176,23 @@ struct TreeArgs {
   int q_stride;
   const half_t* k_cache;
   const half_t* v_cache;
-  int pool_rows, max_len, nkv, G, T;
-  int items, rblocks, splits;  // (sequence, KV head, split) items, row blocks of each
+  int pool_rows, max_len, nkv, G, T, n;
+  int ncols, rblocks;          // columns of the schedule, row blocks (workgroups) of each
   const int64_t* slots;        // [n] or null
-  const int64_t* starts;       // [n]
   const uint64_t* ancestors;   // [n][T]
+  const int* seqs;
+  const int* columns;
   half_t* out;
   int out_stride;
   float scale_log2;
-  float* states;               // [n * T * heads][splits][ATT_REC], splits > 1
+  float* states;               // [ncols][rblocks][2][32 R][ATT_REC]
 };
 
 // One row over keys [k0, k1) by one wave: 64 keys a step, a key a lane for the scores, then two
 // dims a lane for the output, hidden keys left out.
+// rec: the row's state, or null for its output.
 __device__ __forceinline__ void tree_row(const TreeArgs& a, int64_t slot, int s, int g, int row, int L,
-                                         int k0, int k1, int sp) {
+                                         int k0, int k1, float* rec) {
   const int lane = threadIdx.x & 63;
   const int node = row / a.G, head = g * a.G + row - node * a.G;
   const int64_t tok = (int64_t)s * a.T + node;
@@ -141,8 +230,7 @@ __device__ __forceinline__ void tree_row(const TreeArgs& a, int64_t slot, int s,
       o1 = fmaf(pj, (float)vv[1], o1);
     }
   }
-  if (a.splits > 1) {
-    float* rec = a.states + ((tok * (a.nkv * a.G) + head) * a.splits + sp) * ATT_REC;
+  if (rec) {
     *(float2*)(rec + 2 * lane) = make_float2(o0, o1);
     if (lane == 0) *(float2*)(rec + 128) = make_float2(mr, l);
   } else {
@@ -168,23 +256,25 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   const int grp = wave / R;                          // key group
   const int rt = wave - grp * R;                     // row tile
   const int l32 = lane & 31, h = lane >> 5;
-  // the row blocks of an item, which read the same keys, on one XCD (workgroup b on XCD b % 8)
+  // the row blocks of a column, which read the same keys, on one XCD (workgroup b on XCD b % 8)
   const int y = blockIdx.x >> 3;
   const int rb = y % a.rblocks;
-  const int item = (y / a.rblocks) * 8 + (blockIdx.x & 7);
-  if (item >= a.items) return;
-  const int sp = item % a.splits;
-  const int g = (item / a.splits) % a.nkv;
-  const int s = item / a.splits / a.nkv;
-  const int64_t slot = a.slots ? a.slots[s] : s;
-  if (slot < 0 || slot >= a.pool_rows) return;
-  const uint64_t word = lane < a.T ? a.ancestors[(int64_t)s * a.T + lane] : 0;
-  const int used = __popcll(__ballot(word != 0));    // nodes in use come first
-  const int nrows = used * a.G - 32 * R * rb;        // this block's
-  if (nrows <= 0) return;
-  const int64_t L64 = a.starts[s];
-  const int L = (int)(L64 < 0 ? 0 : L64 > a.max_len ? a.max_len : L64);
+  const int col = (y / a.rblocks) * 8 + (blockIdx.x & 7);
+  if (col >= a.ncols) return;
+  const i32x4 c0 = *(const i32x4*)(a.columns + 8 * col), c1 = *(const i32x4*)(a.columns + 8 * col + 4);
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  int s = uniform(c0[0]), g = uniform(c0[1]), u0 = uniform(c0[2]), left = uniform(c0[3]);
+  int L = uniform(c1[0]), used = uniform(c1[1]);
+  constexpr int UNIT = S * KT;
+  for (int part = 0; left > 0; part = 1) {
   const int end = min(L + used, a.max_len);
+  const int ntiles = ceil_div(end, KT), units = ceil_div(end, UNIT);
+  const int steps = min(left, units - u0);
+  const bool whole = u0 == 0 && steps == units;
+  const int nrows = used * a.G - 32 * R * rb;        // this block's
+  if (nrows > 0) {
+  const int64_t slot = a.slots ? a.slots[s] : s;
+  const uint64_t word = lane < a.T ? a.ancestors[(int64_t)s * a.T + lane] : 0;
   const int row = min(32 * rt + l32, nrows - 1);
   const int node = (32 * R * rb + row) / a.G;
   const int u = 32 * R * rb + row - node * a.G;
@@ -201,9 +291,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
     for (int ks = 0; ks < 8; ++ks) qf[ks] = *(const half8_t*)(qp + 16 * ks);
   }
 
-  const int ntiles = (end + KT - 1) / KT;
-  const int steps = (ntiles + S * a.splits - 1) / (S * a.splits);
-  const int tbeg = (sp * S + grp) * steps;
+  const int tbeg = u0 * S + grp * steps;
   const int nt = min(steps, ntiles - tbeg);          // may be <= 0
 
   const int cr = lane >> 4, cc = lane & 15;
@@ -358,7 +446,8 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
     }
   }
   __syncthreads();
-  const int64_t heads = a.nkv * a.G, head = g * a.G + u;
+  const int64_t head = g * a.G + u;
+  float* state = a.states + ((int64_t)(col * a.rblocks + rb) * 2 + part) * (32 * R * ATT_REC);
   if (rows_here) {
     float M = ml_lds[0][rt][0][l32];
 #pragma unroll
@@ -372,7 +461,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
     }
     const float inv = den == 0.f ? 0.f : 1.0f / den;
     const bool mine = 32 * rt + l32 < nrows;
-    float* rec = a.states + ((tok * heads + head) * a.splits + sp) * ATT_REC;
+    float* rec = state + (32 * rt + l32) * ATT_REC;
     half_t* op = a.out + tok * a.out_stride + head * TREE_HD;
     constexpr int NQ = 16 / S;
     float bad = den * 0.f;                             // NaN where an output is not finite
@@ -392,7 +481,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
           acc.w = fmaf(v.w, f[m], acc.w);
         }
         bad = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, fmaf(acc.w, 0.f, bad))));
-        if (a.splits > 1) {                            // the state, for the merging launch
+        if (!whole) {                                  // the state, for the merging launch
           if (mine) *(float4*)(rec + 8 * quad + 4 * h) = acc;
         } else {
           const half2_t c0 = {(half_t)(acc.x * inv), (half_t)(acc.y * inv)};
@@ -401,7 +490,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
           w[e][1] = __builtin_bit_cast(unsigned, c1);
         }
       }
-      if (a.splits == 1) {
+      if (whole) {
         // lane half h holds dims 8 quad + 4 h .. + 3 of quads k and k + 1: exchanged, half 0 has
         // all 8 dims of quad k and half 1 those of quad k + 1
         const auto r0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
@@ -410,7 +499,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
         if (mine) *(u32x4*)(op + 8 * (grp * NQ + k + h)) = st;
       }
     }
-    if (a.splits > 1 && mine && grp == 0 && h == 0) *(float2*)(rec + 128) = make_float2(M, den);
+    if (!whole && mine && grp == 0 && h == 0) *(float2*)(rec + 128) = make_float2(M, den);
     const uint64_t lanes = __ballot(bad != bad && mine);
     if (lane == 0) bad_rows[rt][grp] = (uint32_t)lanes | (uint32_t)(lanes >> 32);
   }
@@ -421,28 +510,43 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   for (int i = 0; again; ++i, again &= again - 1) {
     if (i % S != grp) continue;
     const int r = 32 * rt + __ffs(again) - 1;
-    const int span = S * steps * KT, k0 = min(sp * span, end);
-    tree_row(a, slot, s, g, 32 * R * rb + r, L, k0, min(k0 + span, end), sp);
+    tree_row(a, slot, s, g, 32 * R * rb + r, L, u0 * UNIT, min((u0 + steps) * UNIT, end),
+             whole ? nullptr : state + r * ATT_REC);
+  }
+  __syncthreads();                                     // the LDS is the next stretch's
+  }
+  // on to the next item
+  left -= steps;
+  u0 = 0;
+  if (left > 0 && ++g == a.nkv) {
+    g = 0;
+    while (++s < a.n - 1 && uniform(a.seqs[4 * s + 2]) == 0) {}
+    L = uniform(a.seqs[4 * s]);
+    used = uniform(a.seqs[4 * s + 1]);
+  }
   }
 }
 
-// The splits' states of a (node, query head) row to its output: one wave a row, two dims a lane.
-__global__ __launch_bounds__(256) void tree_merge_kernel(const float* __restrict__ states, int splits,
-                                                         int heads, int T, int64_t rows,
-                                                         const int64_t* __restrict__ slots,
-                                                         int pool_rows,
-                                                         const uint64_t* __restrict__ ancestors,
-                                                         half_t* __restrict__ out, int out_stride) {
+// The states of a (node, query head) row to its output, for items that more than one column has
+// parts of: one wave a row, two dims a lane.
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, const int* __restrict__ heads,
+                                                         int block_rows, int64_t rows) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= rows) return;
-  const int64_t tok = r / heads;
-  const int head = (int)(r - tok * heads);
-  const int64_t slot = slots ? slots[tok / T] : 0;
-  if (slot < 0 || slot >= pool_rows || !ancestors[tok]) return;      // no state was written
-  const float* rec = states + r * splits * ATT_REC;
+  const int nh = a.nkv * a.G;
+  const int tok = (int)(r / nh), head = (int)(r - (int64_t)tok * nh);
+  const int s = tok / a.T, node = tok - s * a.T, g = head / a.G;
+  const i32x4 seq = *(const i32x4*)(a.seqs + 4 * s);
+  const int2 at = *(const int2*)(heads + 2 * (s * a.nkv + g));
+  const int first = at.x & ~(1 << 30), splits = at.y - first + 1;
+  if (node >= seq[1] || seq[2] == 0 || splits == 1) return;
+  const int row = node * a.G + head - g * a.G, rb = row / block_rows;
+  const int64_t block = (int64_t)block_rows * ATT_REC, step = a.rblocks * 2 * block;
+  const float* rec = a.states + (int64_t)first * step + rb * 2 * block + (row - rb * block_rows) * ATT_REC;
+  const int64_t skip = at.x >> 30 ? block : 0;       // in its first column the item is the second
   float M = -INFINITY;
-  for (int k = lane; k < splits; k += 64) M = fmaxf(M, rec[k * ATT_REC + 128]);
+  for (int k = lane; k < splits; k += 64) M = fmaxf(M, rec[k * step + (k ? 0 : skip) + 128]);
   M = wave_max(M);
   const float ref = M == -INFINITY ? 0.f : M;
   float o0 = 0.f, o1 = 0.f, den = 0.f;
@@ -450,39 +554,61 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const float* __restrict
     float2 ml[8], v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float* at = rec + min(k0 + k, splits - 1) * ATT_REC;
-      ml[k] = *(const float2*)(at + 128);
-      v[k] = *(const float2*)(at + 2 * lane);
+      const int at_k = min(k0 + k, splits - 1);
+      const float* from = rec + at_k * step + (at_k ? 0 : skip);
+      ml[k] = *(const float2*)(from + 128);
+      v[k] = *(const float2*)(from + 2 * lane);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float f = k0 + k < splits ? exp2f(ml[k].x - ref) : 0.f;
+    for (int k = 0; k < 8; ++k)
       if (k0 + k < splits) {
+        const float f = exp2f(ml[k].x - ref);
         den = fmaf(f, ml[k].y, den);
         o0 = fmaf(f, v[k].x, o0);
         o1 = fmaf(f, v[k].y, o1);
       }
-    }
   }
   const float inv = den == 0.f ? 0.f : 1.0f / den;
   const half2_t h2 = {(half_t)(o0 * inv), (half_t)(o1 * inv)};
-  *(half2_t*)(out + tok * out_stride + head * TREE_HD + 2 * lane) = h2;
+  *(half2_t*)(a.out + (int64_t)tok * a.out_stride + head * TREE_HD + 2 * lane) = h2;
+}
+
+// The workgroup forms, (rows, groups): 32 R rows, S key groups of KT-key tiles.
+static int tree_form(int rows, int groups, int* unit) {
+  const int form = rows == 128 && (groups == 1 || groups == 2) ? groups
+                   : rows == 64 && groups == 4 ? 4 : rows == 32 && groups == 8 ? 8 : 0;
+  *unit = groups * (form <= 2 ? 64 : 32);
+  return form;
+}
+
+// schedule: [n][4] seqs, [ncols][8] columns, [n][nkv][2] heads
+static int64_t tree_schedule_ints(int n, int nkv, int ncols) {
+  return 4 * (int64_t)n + 8 * (int64_t)ncols + 2 * (int64_t)n * nkv;
 }
 
 extern "C" int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
                               const int64_t* lengths, const int64_t* rope_delta, int n, int n_nodes,
                               int pool_rows, int max_len, int64_t* starts, void* ancestors,
                               int64_t* positions, int64_t* token_slot, int64_t* token_pos,
-                              void* stream) {
-  if (n < 0 || n_nodes < 1 || pool_rows <= 0 || max_len <= 0) return OMNI_EINVAL;
+                              int n_kv_heads, int rows, int groups, int columns, int least,
+                              int* schedule, int64_t schedule_ints, void* stream) {
+  if (n < 0 || n_nodes < 1 || pool_rows <= 0 || max_len <= 0 || n_kv_heads <= 0) return OMNI_EINVAL;
   if (n_nodes > TREE_MAX) return OMNI_EUNSUPPORTED;
   if (!slots && n > pool_rows) return OMNI_EINVAL;
+  int unit;
+  if (!tree_form(rows, groups, &unit) || columns < 1 || least < 0) return OMNI_EINVAL;
+  if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
+  if ((int64_t)n * n_kv_heads * ceil_div(max_len, unit) > 0x3fffffff || (columns >> 24)) return OMNI_EUNSUPPORTED;
   if (n == 0) return OMNI_OK;
-  if (!parents || !lengths || !starts || !ancestors || !positions || !token_slot || !token_pos)
+  if (!parents || !lengths || !starts || !ancestors || !positions || !token_slot || !token_pos ||
+      !schedule || ((uintptr_t)schedule & 15))
     return OMNI_EINVAL;
+  if (schedule_ints < tree_schedule_ints(n, n_kv_heads, columns)) return OMNI_EINVAL;
+  TreeCols tc = {schedule, schedule + 4 * (int64_t)n, schedule + 4 * (int64_t)n + 8 * (int64_t)columns,
+                 columns, n_kv_heads, unit, least};
   hipLaunchKernelGGL(tree_plan_kernel, dim3(n), dim3(64), 0, (hipStream_t)stream, parents, counts,
                      slots, lengths, rope_delta, n, n_nodes, pool_rows, max_len, starts,
-                     (uint64_t*)ancestors, positions, token_slot, token_pos);
+                     (uint64_t*)ancestors, positions, token_slot, token_pos, tc);
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }
@@ -506,29 +632,34 @@ extern "C" int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v
 
 extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_cache,
                                    const void* v_cache, int pool_rows, int max_len,
-                                   const int64_t* slots, const int64_t* starts,
-                                   const void* ancestors, int n, int n_nodes, void* out,
-                                   int out_stride, int n_heads, int n_kv_heads, int head_dim,
-                                   float scale, int rows, int groups, int splits, float* workspace,
+                                   const int64_t* slots, const void* ancestors, int n, int n_nodes,
+                                   void* out, int out_stride, int n_heads, int n_kv_heads,
+                                   int head_dim, float scale, int rows, int groups, int columns,
+                                   int least, const int* schedule, float* workspace,
                                    int64_t workspace_floats, void* stream) {
   if (n < 0 || n_nodes < 1 || n_heads <= 0 || n_kv_heads <= 0 || pool_rows <= 0 || max_len <= 0)
     return OMNI_EINVAL;
   if (head_dim != TREE_HD || n_heads % n_kv_heads || n_nodes > TREE_MAX) return OMNI_EUNSUPPORTED;
   if (!(scale >= 0x1p-126f) || scale > 3e38f) return OMNI_EUNSUPPORTED;
-  const int form = rows == 128 && (groups == 1 || groups == 2) ? groups
-                   : rows == 64 && groups == 4 ? 4 : rows == 32 && groups == 8 ? 8 : 0;
-  if (!form) return OMNI_EINVAL;
+  int unit;
+  const int form = tree_form(rows, groups, &unit);
+  if (!form || columns < 1 || least < 0) return OMNI_EINVAL;
+  if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
-  if (splits < 1 || splits > 256 || (!slots && n > pool_rows)) return OMNI_EINVAL;
+  if (!slots && n > pool_rows) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
-  if (!q || !k_cache || !v_cache || !starts || !ancestors || !out) return OMNI_EINVAL;
-  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return OMNI_EINVAL;
-  const int64_t nrec = (int64_t)n * n_nodes * n_heads;
-  if (splits > 1 && (!workspace || ((uintptr_t)workspace & 15) ||
-                     workspace_floats < nrec * splits * ATT_REC))
+  if (!q || !k_cache || !v_cache || !ancestors || !schedule || !out) return OMNI_EINVAL;
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)schedule) & 15)
     return OMNI_EINVAL;
   TreeArgs a;
+  a.G = n_heads / n_kv_heads;
+  const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
+  const int64_t grid = (columns + 7) / 8 * 8 * rblocks, out_rows = (int64_t)n * n_nodes * n_heads;
+  if (grid > 0x7fffffff || out_rows > 0x7fffffff) return OMNI_EUNSUPPORTED;
+  if (least && (!workspace || ((uintptr_t)workspace & 15) ||
+                workspace_floats < columns * rblocks * 2 * rows * ATT_REC))
+    return OMNI_EINVAL;
   a.q = (const half_t*)q;
   a.q_stride = q_stride;
   a.k_cache = (const half_t*)k_cache;
@@ -536,18 +667,14 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   a.pool_rows = pool_rows;
   a.max_len = max_len;
   a.nkv = n_kv_heads;
-  a.G = n_heads / n_kv_heads;
   a.T = n_nodes;
-  a.splits = splits;
-  const int64_t items = (int64_t)n * n_kv_heads * splits;
-  const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
-  const int64_t grid = (items + 7) / 8 * 8 * rblocks;
-  if (grid > 0x7fffffff || nrec > 0x7fffffff) return OMNI_EUNSUPPORTED;
-  a.items = (int)items;
+  a.n = n;
+  a.ncols = columns;
   a.rblocks = (int)rblocks;
   a.slots = slots;
-  a.starts = starts;
   a.ancestors = (const uint64_t*)ancestors;
+  a.seqs = schedule;
+  a.columns = schedule + 4 * (int64_t)n;
   a.out = (half_t*)out;
   a.out_stride = out_stride;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -563,10 +690,9 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   else
     hipLaunchKernelGGL((tree_attn_kernel<1, 8, 32>), gd, dim3(512), 0, st, a);
   OMNI_CHECK_LAUNCH();
-  if (splits > 1) {
-    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((nrec + 3) / 4)), dim3(256), 0, st,
-                       workspace, splits, n_heads, n_nodes, nrec, slots, pool_rows,
-                       (const uint64_t*)ancestors, (half_t*)out, out_stride);
+  if (least) {
+    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a,
+                       a.columns + 8 * (int64_t)columns, rows, out_rows);
     OMNI_CHECK_LAUNCH();
   }
   return OMNI_OK;

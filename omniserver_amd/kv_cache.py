@@ -450,13 +450,15 @@ TREE_MAX_NODES = 64
 
 
 def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) -> tuple:
-    """(rows, key groups, splits) for omni_tree_attention over n trees in a pool of capacity
-    tokens a row."""
+    """(rows, key groups, columns, least) for omni_tree_attention over n trees in a pool of
+    capacity tokens a row."""
     rows = nodes * (nh // nkv)
     form = (32, 8) if rows <= 32 else (64, 4) if rows <= 64 else (128, 2)
-    items = n * nkv * -(-rows // form[0])
-    splits = max(1, min(cus // items, capacity // 256, 64))
-    return (*form, splits)
+    unit = {1: 64, 2: 128, 4: 128, 8: 256}[form[1]]
+    if capacity <= 512:
+        return (*form, n * nkv, 0)
+    columns = max(1, min(cus // -(-rows // form[0]), n * nkv * -(-capacity // unit)))
+    return (*form, columns, 1)
 
 
 class TreeCache(PackedPrefillWriter):
@@ -518,6 +520,15 @@ class TreeCache(PackedPrefillWriter):
             raise ValueError(f"rope_delta holds one value per pool row ({pool.max_batch})")
         require_here(parents, self.counts, self.slots, rope_delta)
         self.n, self.nodes, self.T = n, T, n * T
+        # how the attention's workgroups share the keys; its split states' buffer serves all
+        # layers (launches on one stream are ordered)
+        self.form = rows, groups, columns, least = tree_plan(
+            n, T, pool.n_heads, pool.n_kv_heads, pool.max_len, num_cus(dev))
+        self._ws = None if not least else torch.empty(
+            columns * -(-T * (pool.n_heads // pool.n_kv_heads) // rows) * 2 * rows * 132,
+            device=dev, dtype=torch.float32)
+        self.schedule = torch.empty(4 * n + 8 * columns + 2 * n * pool.n_kv_heads, device=dev,
+                                    dtype=torch.int32)
         # one block for the plan: starts, ancestors, positions, pool rows and positions
         plan = torch.empty(n + 6 * n * T, device=dev, dtype=torch.int64)
         self.starts = plan[:n]
@@ -528,12 +539,8 @@ class TreeCache(PackedPrefillWriter):
         call("omni_tree_plan", ptr(parents), ptr(self.counts), ptr(self.slots), ptr(pool.lengths),
              ptr(rope_delta), n, T, pool.max_batch, pool.max_len, ptr(self.starts),
              ptr(self.ancestors), ptr(self.positions), ptr(self.token_slot), ptr(self.token_pos),
-             stream())
-        # (rows, groups, splits) of the attention and its split states, shared by the layers
-        # (launches on one stream are ordered)
-        self.plan = tree_plan(n, T, pool.n_heads, pool.n_kv_heads, pool.max_len, num_cus(dev))
-        self._ws = None if self.plan[2] == 1 else torch.empty(
-            n * T * pool.n_heads * self.plan[2] * 132, device=dev, dtype=torch.float32)
+             pool.n_kv_heads, rows, groups, columns, least, ptr(self.schedule),
+             self.schedule.numel(), stream())
 
     def bind(self, T: int) -> None:
         if T != self.T:
@@ -557,11 +564,10 @@ class TreeCache(PackedPrefillWriter):
             raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
                              f"[{self.T}, {nh}, {hd}]")
         require_here(qkv, out)
-        rows, groups, splits = self.plan
         call("omni_tree_attention", ptr(qkv), qkv.stride(0), ptr(pool.k[layer_idx]),
              ptr(pool.v[layer_idx]), pool.max_batch, pool.max_len, ptr(self.slots),
-             ptr(self.starts), ptr(self.ancestors), self.n, self.nodes, ptr(out), nh * hd, nh,
-             pool.n_kv_heads, hd, float(scale), rows, groups, splits, ptr(self._ws),
+             ptr(self.ancestors), self.n, self.nodes, ptr(out), nh * hd, nh, pool.n_kv_heads, hd,
+             float(scale), *self.form, ptr(self.schedule), ptr(self._ws),
              0 if self._ws is None else self._ws.numel(), stream())
         return out
 

@@ -19,11 +19,12 @@ def pool(max_batch=4, max_len=128, **kw):
 def test_tree_attention_refusals():
     from omniserver_amd._lib import lib
 
-    def rc(q=P, q_stride=1536, rows=4, max_len=256, starts=P, n=2, nodes=8, out=P, out_stride=1536,
-           nh=12, nkv=2, hd=128, scale=0.1, splits=1, ws=None, floats=0, slots=None, form=(64, 4)):
-        return lib().omni_tree_attention(q, q_stride, P, P, rows, max_len, slots, starts, P, n,
-                                         nodes, out, out_stride, nh, nkv, hd, scale, *form, splits,
-                                         ws, floats, None)
+    def rc(q=P, q_stride=1536, rows=4, max_len=256, plan=P, n=2, nodes=8, out=P, out_stride=1536,
+           nh=12, nkv=2, hd=128, scale=0.1, form=(64, 4), columns=4, least=0, ws=None, floats=0,
+           slots=None):
+        return lib().omni_tree_attention(q, q_stride, P, P, rows, max_len, slots, P, n, nodes, out,
+                                         out_stride, nh, nkv, hd, scale, *form, columns, least,
+                                         plan, ws, floats, None)
 
     assert rc(n=-1) == rc(nodes=0) == rc(nh=0) == rc(nkv=0) == rc(rows=0) == rc(max_len=0) == -1
     assert rc(nodes=65) == rc(hd=64) == rc(nh=13) == -2
@@ -31,22 +32,26 @@ def test_tree_attention_refusals():
     assert rc(scale=float("inf")) == -2
     assert rc(q_stride=1535) == rc(q_stride=1532) == rc(out_stride=8) == rc(out_stride=1540) == -1
     assert rc(form=(64, 2)) == rc(form=(32, 1)) == rc(form=(0, 0)) == -1
-    assert rc(splits=0) == rc(splits=257) == rc(n=5) == -1
-    assert rc(q=None) == rc(out=None) == rc(starts=None) == -1
-    assert rc(q=ctypes.c_void_p(24)) == rc(out=ctypes.c_void_p(8)) == -1
-    assert rc(splits=2) == rc(splits=2, ws=P, floats=2 * 8 * 12 * 2 * 132 - 1) == -1
+    assert rc(columns=0) == rc(columns=5) == rc(least=-1) == rc(n=5, columns=10) == -1
+    assert rc(q=None) == rc(out=None) == rc(plan=None) == -1
+    assert rc(q=ctypes.c_void_p(24)) == rc(out=ctypes.c_void_p(8)) == rc(plan=ctypes.c_void_p(4)) == -1
+    cut = {"least": 1, "columns": 3, "nodes": 16, "form": (64, 4)}
+    assert rc(**cut) == rc(**cut, ws=P, floats=3 * 2 * 2 * 64 * 132 - 1) == -1
     assert rc(n=0) == 0
 
 
 def test_tree_plan_and_row_write_refusals():
     from omniserver_amd._lib import lib
 
-    def plan(parents=P, lengths=P, n=2, nodes=8, rows=4, max_len=64, slots=None, starts=P):
+    def plan(parents=P, lengths=P, n=2, nodes=8, rows=4, max_len=64, slots=None, starts=P, nkv=2,
+             form=(64, 4), columns=4, least=0, ints=1 << 20):
         return lib().omni_tree_plan(parents, None, slots, lengths, None, n, nodes, rows, max_len,
-                                    starts, P, P, P, P, None)
+                                    starts, P, P, P, P, nkv, *form, columns, least, P, ints, None)
 
-    assert plan(n=-1) == plan(nodes=0) == plan(rows=0) == plan(max_len=0) == plan(n=5) == -1
-    assert plan(nodes=65) == -2
+    assert plan(n=-1) == plan(nodes=0) == plan(rows=0) == plan(max_len=0) == plan(nkv=0) == -1
+    assert plan(n=5, columns=10) == plan(columns=3) == plan(columns=0) == plan(least=-1) == -1
+    assert plan(form=(128, 4)) == plan(ints=4 * 2 + 8 * 4 + 2 * 2 * 2 - 1) == -1
+    assert plan(columns=1 << 24, least=1) == plan(nodes=65) == -2
     assert plan(parents=None) == plan(lengths=None) == plan(starts=None) == -1
     assert plan(n=0) == 0
 
