@@ -174,8 +174,9 @@ def require_here(*tensors) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise RuntimeError("omniserver_amd ops run on the GPU only (got a CPU tensor)")
-        if t.device.index != torch._C._cuda_getDevice():
+        if at != torch._C._cuda_getDevice():
             raise RuntimeError(f"tensor on {t.device}, but the current device is "
                                f"cuda:{torch._C._cuda_getDevice()}")

@@ -14,7 +14,7 @@
 // first v whose running sum of weights exceeds u_0 times their total.  A NaN logit counts as
 // -inf; a row without a token above -inf accepts nothing and gives -1.
 //
-// Every row is read once, in 32 bits: largest logit and sum of weights per 2048 tokens (the bound
+// Every row is read once, in 32 bits: largest logit and sum of weights per 8192 tokens (the bound
 // is the rows' bytes).  A test that these sums leave open - they are good to 2^-18, so one in some
 // 10^5 - is decided by a 64-bit sum of its row.  Where a random number falls among 151936 tokens
 // is a matter of borders 1e-6 apart and closer, which 32-bit sums would move across one draw in a
@@ -25,7 +25,8 @@
 
 #define SV_MAX_NODES 64
 #define SV_CHUNK 2048              // tokens a wave sums: 32 a lane
-#define SV_WAVES 16                // waves of the walk's and the residual's workgroups
+#define SV_WAVES 4                 // waves of a workgroup
+#define SV_BLOCK (SV_WAVES * SV_CHUNK)
 #define SV_ERR 0x1p-18             // relative error of a row's 32-bit sum, with a factor 4 to spare
 
 enum { SV_DONE = 0, SV_TARGET = 1, SV_RESIDUAL = 2 };   // where the next token comes from
@@ -41,11 +42,11 @@ struct SvArgs {
   const float* uniforms;
   const float* temperature;
   float temp;
-  int n, T, V, chunks;
+  int n, T, V, chunks, blocks;
   int* path;
   int64_t* out_tokens;
   int* emitted;
-  float2* rec;             // [n T target rows, n (T - 1) draft rows][chunks] (largest, sum or index)
+  float2* rec;             // [n T target rows, n (T - 1) draft rows][blocks] (largest, sum or index)
   double* sums;            // [3][n][chunks]: target, draft, residual
   struct SvSeq* seqs;      // [n]
 };
@@ -83,31 +84,41 @@ __device__ __forceinline__ int sv_used(const SvArgs& a, int s) {
   return a.counts ? min(max(a.counts[s], 0), a.T) : a.T;
 }
 
-// 2^t for t <= 0: t = n + f, |f| <= 1/2, 2^f by the polynomial through its values at the eleven
-// Chebyshev points of [-1/2, 1/2] (relative error 3e-16), 2^n by the exponent (0 far below).
+// 2^t for t <= 0: t = n + f, |f| <= 1/2, 2^f by the polynomial through its values at the nine
+// Chebyshev points of [-1/2, 1/2] (relative error 1.1e-12; 1 at 0), 2^n by the exponent (0 far
+// below).  That error moves a border between two tokens of 1e-6 each across one draw in 10^6.
 __device__ __forceinline__ double sv_exp2(double t) {
 #pragma clang fp contract(off)          // the same wherever it is inlined
   const double n = rint(t), f = t - n;
-  double r = 0x1.e6063f7217bc6p-28;
-  r = fma(r, f, 0x1.b675bca4eeebbp-24);
-  r = fma(r, f, 0x1.62bfd47773353p-20);
-  r = fma(r, f, 0x1.ffcb54062e698p-17);
-  r = fma(r, f, 0x1.430913096fd9fp-13);
-  r = fma(r, f, 0x1.5d87fe9d7a584p-10);
-  r = fma(r, f, 0x1.3b2ab6fba1ddap-7);
-  r = fma(r, f, 0x1.c6b08d703ce49p-5);
-  r = fma(r, f, 0x1.ebfbdff82c598p-3);
-  r = fma(r, f, 0x1.62e42fefa3a19p-1);
+  double r = 0x1.63d136366db24p-20;
+  r = fma(r, f, 0x1.00dc4a532fb8ep-16);
+  r = fma(r, f, 0x1.4308ac85aa947p-13);
+  r = fma(r, f, 0x1.5d8745a728441p-10);
+  r = fma(r, f, 0x1.3b2ab7181b755p-7);
+  r = fma(r, f, 0x1.c6b08dd6fd234p-5);
+  r = fma(r, f, 0x1.ebfbdff823cedp-3);
+  r = fma(r, f, 0x1.62e42fef84cf0p-1);
   r = fma(r, f, 1.0);
   return ldexp(r, (int)fmax(n, -2000.0));
 }
 
-// weight of logit x in a row whose largest is m: 1 there, infinite or not
-__device__ __forceinline__ double sv_weight(float x, float m, double c) {
+// The weights of a row whose largest logit is m, at log2(e) / temperature = c: 1 at m, infinite or
+// not, 0 at -inf and NaN.  Where m and c are ordinary a logit that counts for nothing is as good as
+// the lowest finite one.
+struct SvRow {
+  float m;
+  double c;
+  bool plain;
+  __device__ __forceinline__ SvRow(float m_, double c_)
+      : m(m_), c(c_), plain(fabsf(m_) < 3e38f && c_ > 1e-30 && c_ < 1e30) {}
+  __device__ __forceinline__ double weight(float x) const {
 #pragma clang fp contract(off)
-  const double w = sv_exp2(((double)x - (double)m) * c);
-  return x == m && m > -INFINITY ? 1.0 : x > -INFINITY && m < INFINITY ? w : 0.0;
-}
+    if (plain) return sv_exp2(((double)fmaxf(x, -3.4028234e38f) - (double)m) * c);
+    if (!(x > -INFINITY)) return 0.0;
+    if (x == m) return 1.0;
+    return m == INFINITY ? 0.0 : sv_exp2(((double)x - (double)m) * c);
+  }
+};
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -151,15 +162,14 @@ struct SvPiece {
 };
 
 // ---------------------------------------------------------------------------
-// Row statistics: one wave a 2048-token chunk of a row, rec = (largest logit, sum of weights
+// Row statistics: one workgroup 8192 tokens of a row, rec = (largest logit, sum of weights
 // relative to it), for greedy rows (largest logit, its first index).
 // ---------------------------------------------------------------------------
 template <int DT>
-__global__ __launch_bounds__(256) void sv_stats_kernel(SvArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int per = (a.chunks + 3) >> 2;
-  const int r = blockIdx.x / per, chunk = (blockIdx.x - r * per) * 4 + (threadIdx.x >> 6);
-  if (chunk >= a.chunks) return;
+__global__ __launch_bounds__(64 * SV_WAVES) void sv_stats_kernel(SvArgs a) {
+  __shared__ float wm[SV_WAVES], wz[SV_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = blockIdx.x / a.blocks, block = blockIdx.x - r * a.blocks;
   const int target_rows = a.n * a.T;
   const bool is_draft = r >= target_rows;
   const int T = is_draft ? a.T - 1 : a.T, rr = is_draft ? r - target_rows : r;
@@ -169,7 +179,7 @@ __global__ __launch_bounds__(256) void sv_stats_kernel(SvArgs a) {
   const int used = sv_used(a, s);
   if (is_draft ? (greedy || i + 1 >= used) : i >= used) return;
   const void* row = is_draft ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
-  const int v0 = chunk * SV_CHUNK;
+  const int v0 = block * SV_BLOCK + wave * SV_CHUNK;
   typedef SvPiece<DT> P;
   P x[P::P];
 #pragma unroll
@@ -178,65 +188,83 @@ __global__ __launch_bounds__(256) void sv_stats_kernel(SvArgs a) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) m = fmaxf(m, x[e / P::N].get(e));       // leaves a NaN out
   m = wave_max(m);
-  float2* out = a.rec + (int64_t)r * a.chunks + chunk;
+  // (x - m) c in two steps: c may be as large as fp32 goes, and an infinite m stays in order
+  const float c = greedy ? 0.f : fminf(1.4426950408889634f / temp, 1e38f);
+  float sum;
   if (greedy) {
     int at = 0x7fffffff;
 #pragma unroll
     for (int e = 31; e >= 0; --e)
       if (x[e / P::N].get(e) == m) at = v0 + P::at(lane, e / P::N) + e % P::N;
     for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
-    if (lane == 0) *out = make_float2(m, __builtin_bit_cast(float, at));
-    return;
-  }
-  // (x - m) c in two steps: c may be as large as fp32 goes, and an infinite m stays in order
-  const float c = fminf(1.4426950408889634f / temp, 1e38f);
-  float z[4] = {0.f, 0.f, 0.f, 0.f};
-  if (fabsf(m) < INFINITY) {
+    sum = __builtin_bit_cast(float, at);
+  } else {
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    if (fabsf(m) < INFINITY) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const float w = __builtin_amdgcn_exp2f((x[e / P::N].get(e) - m) * c);
-      z[e & 3] += w == w ? w : 0.f;
+      for (int e = 0; e < 32; ++e) {
+        const float w = __builtin_amdgcn_exp2f((x[e / P::N].get(e) - m) * c);
+        z[e & 3] += w == w ? w : 0.f;
+      }
+    } else if (m == INFINITY) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) z[e & 3] += x[e / P::N].get(e) == m ? 1.f : 0.f;
     }
-  } else if (m == INFINITY) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) z[e & 3] += x[e / P::N].get(e) == m ? 1.f : 0.f;
+    sum = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
   }
-  const float sum = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
-  if (lane == 0) *out = make_float2(m, sum);
+  if (lane == 0) {
+    wm[wave] = m;
+    wz[wave] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  float M = wm[0];
+  for (int w = 1; w < SV_WAVES; ++w) M = fmaxf(M, wm[w]);
+  if (greedy) {
+    int at = 0x7fffffff;
+    for (int w = 0; w < SV_WAVES; ++w)
+      if (wm[w] == M) at = min(at, __builtin_bit_cast(int, wz[w]));
+    sum = __builtin_bit_cast(float, at);
+  } else {
+    sum = 0.f;
+    for (int w = 0; w < SV_WAVES; ++w)
+      if (wz[w] > 0.f) sum += wz[w] * (wm[w] == M ? 1.f : __builtin_amdgcn_exp2f((wm[w] - M) * c));
+  }
+  a.rec[(int64_t)r * a.blocks + block] = make_float2(M, sum);
 }
 
-// A row's chunks together, by one wave: largest logit and 64-bit sum of their 32-bit sums
+// A row's blocks together, by half a wave: largest logit and 64-bit sum of their 32-bit sums
 // (greedy: first index).
-__device__ __forceinline__ void sv_combine(const float2* rec, int chunks, int lane, double c, bool greedy,
+__device__ __forceinline__ void sv_combine(const float2* rec, int blocks, int lane, double c, bool greedy,
                                            float& m, double& z, int& best) {
-  float2 keep[2];
-  m = -INFINITY;
-  for (int k = lane, j = 0; k < chunks; k += 64, ++j) {
-    const float2 v = rec[k];
-    if (j < 2) keep[j] = v;
-    m = fmaxf(m, v.x);
-  }
-  m = wave_max(m);
+  const int l = lane & 31;
+  const float2 own = l < blocks ? rec[l] : make_float2(-INFINITY, 0.f);
+  m = own.x;
+  for (int k = l + 32; k < blocks; k += 32) m = fmaxf(m, rec[k].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const SvRow row(m, c);
   z = 0.0;
   best = 0x7fffffff;
-  for (int k = lane, j = 0; k < chunks; k += 64, ++j) {
-    const float2 v = j < 2 ? keep[j] : rec[k];
+  for (int k = l; k < blocks; k += 32) {
+    const float2 v = k < 32 ? own : rec[k];
     if (greedy) {
       if (v.x == m) best = min(best, __builtin_bit_cast(int, v.y));
-    } else {
-      z += (double)v.y * sv_weight(v.x, m, c);
+    } else if (v.y > 0.f) {
+      z += (double)v.y * row.weight(v.x);
     }
   }
-  if (greedy)
-    for (int o = 32; o; o >>= 1) best = min(best, __shfl_xor(best, o));
-  else
-    z = wave_sum64(z);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    if (greedy) best = min(best, __shfl_xor(best, o));
+    else z += __shfl_xor(z, o);
+  }
 }
 
 // 64-bit sum of a chunk's weights, the tried tokens left out; by one wave.
 template <int DT>
-__device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V, int lane, float m,
-                                               double c, const int64_t* tok, uint64_t tried) {
+__device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V, int lane,
+                                               const SvRow& w, const int64_t* tok, uint64_t tried) {
   typedef SvPiece<DT> P;
   const int v0 = chunk * SV_CHUNK;
   double z[2] = {0.0, 0.0};
@@ -252,10 +280,7 @@ __device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V
       if (t >= 0 && t < P::N) gone |= 1u << t;
     }
 #pragma unroll
-    for (int e = 0; e < P::N; ++e) {
-      const double w = sv_weight(x.get(e), m, c);
-      z[e & 1] += gone >> e & 1 ? 0.0 : w;
-    }
+    for (int e = 0; e < P::N; ++e) z[e & 1] += w.weight(gone >> e & 1 ? -INFINITY : x.get(e));
   }
   return wave_sum64(z[0] + z[1]);
 }
@@ -312,23 +337,18 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
       if (chain_q) lq = sv_logit<DT>(sv_draft_row<DT>(a, s, up), x);
     }
   }
-  for (int i = wave; i < used; i += SV_WAVES) {
+  const int nrows = chain_q ? 2 * used - 1 : used;        // the target's rows, then the draft's
+  for (int r0 = 2 * wave; r0 < nrows; r0 += 2 * SV_WAVES) {
+    const int r = min(r0 + (lane >> 5), nrows - 1), d = r >= used, i = d ? r - used : r;
+    const int64_t at = d ? (int64_t)a.n * T + (int64_t)s * (T - 1) + i : (int64_t)s * T + i;
     float m;
     double z;
     int b;
-    sv_combine(a.rec + ((int64_t)s * T + i) * a.chunks, a.chunks, lane, c, greedy, m, z, b);
-    if (lane == 0) {
-      ms[0][i] = m;
-      zs[0][i] = z;
-      best[i] = b;
-    }
-    if (chain_q && i + 1 < used) {
-      sv_combine(a.rec + ((int64_t)a.n * T + (int64_t)s * (T - 1) + i) * a.chunks, a.chunks, lane, c,
-                 false, m, z, b);
-      if (lane == 0) {
-        ms[1][i] = m;
-        zs[1][i] = z;
-      }
+    sv_combine(a.rec + at * a.blocks, a.blocks, lane, c, greedy, m, z, b);
+    if ((lane & 31) == 0) {
+      ms[d][i] = m;
+      zs[d][i] = z;
+      if (!d) best[i] = b;
     }
   }
   if (wave == 0) {
@@ -348,7 +368,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
         for (int j = up + 1; j < lane; ++j) twice |= par[j] == up && tok[j] == x;
         if (!twice && x >= 0 && x < a.V)
           w = greedy ? (ms[0][up] > -INFINITY && x == best[up] ? 1.0 : 0.0)
-                     : sv_weight(lp, ms[0][up], c);
+                     : SvRow(ms[0][up], c).weight(lp);
       }
       wt[lane] = w;                                       // read by this wave alone, in order
       if (w > 0.0) {
@@ -356,7 +376,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
           stands = true;
         } else if (chain_q) {
           // u q / Zq < w / Z, both sides times Z Zq
-          const double a0 = u * sv_weight(lq, ms[1][up], c) * zs[0][up], a1 = w * zs[1][up];
+          const double a0 = u * SvRow(ms[1][up], c).weight(lq) * zs[0][up], a1 = w * zs[1][up];
           stands = a0 < a1;
           open = fabs(a0 - a1) <= 2.0 * SV_ERR * a1 && !((exact[0] & exact[1]) >> up & 1);
           if (zs[1][up] == 0.0) stands = true, open = false;      // q is nowhere
@@ -403,9 +423,10 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
       const int i = __ffsll((unsigned long long)b) - 1;
       for (int d = 0; d < (chain_q ? 2 : 1); ++d) {
         const void* row = d ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
+        const SvRow w(ms[d][i], c);
         double z = 0.0;
         for (int k = wave; k < a.chunks; k += SV_WAVES)
-          z += sv_chunk_sum<DT>(row, k, a.V, lane, ms[d][i], c, tok, 0);
+          z += sv_chunk_sum<DT>(row, k, a.V, lane, w, tok, 0);
         if (lane == 0) part[wave] = z;
         __syncthreads();
         if (tid == 0) {
@@ -446,12 +467,12 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
   }
   const int chunk = mine * SV_WAVES + wave;
   if (mode == SV_DONE || chunk >= a.chunks) return;
-  const double sp = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), chunk, a.V, lane, m, c, tok,
-                                     residual ? 0 : tried);
+  const double sp = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), chunk, a.V, lane, SvRow(m, c),
+                                     tok, residual ? 0 : tried);
   if (lane == 0) a.sums[(int64_t)s * a.chunks + chunk] = sp;
   if (residual) {
-    const double sq = sv_chunk_sum<DT>(sv_draft_row<DT>(a, s, last), chunk, a.V, lane, ms[1][last], c,
-                                       tok, 0);
+    const double sq = sv_chunk_sum<DT>(sv_draft_row<DT>(a, s, last), chunk, a.V, lane,
+                                       SvRow(ms[1][last], c), tok, 0);
     if (lane == 0) a.sums[((int64_t)a.n + s) * a.chunks + chunk] = sq;
   }
 }
@@ -464,10 +485,10 @@ __device__ __forceinline__ double sv_total(const double* sums, int chunks, int l
 }
 
 // max(p - q, 0) of a token; zp, zq: 1 / totals
-__device__ __forceinline__ double sv_rest(float x, float y, float m, float mq, double c, double zp,
+__device__ __forceinline__ double sv_rest(float x, float y, const SvRow& p, const SvRow& q, double zp,
                                           double zq) {
 #pragma clang fp contract(off)          // equal rows leave exactly nothing
-  const double d = sv_weight(x, m, c) * zp - sv_weight(y, mq, c) * zq;
+  const double d = p.weight(x) * zp - q.weight(y) * zq;
   return d > 0.0 ? d : 0.0;
 }
 
@@ -487,6 +508,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_residual_kernel(SvArgs a) {
   const void* row = sv_row<DT>(a, s, q.last);
   const void* drow = sv_draft_row<DT>(a, s, q.last);
   const int v0 = chunk * SV_CHUNK;
+  const SvRow wp(q.m, c), wq(q.mq, c);
   double z[2] = {0.0, 0.0};
   P nx, ny;
   nx.load(row, v0, a.V, lane, 0);
@@ -499,7 +521,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_residual_kernel(SvArgs a) {
       ny.load(drow, v0, a.V, lane, j + 1);
     }
 #pragma unroll
-    for (int e = 0; e < P::N; ++e) z[e & 1] += sv_rest(x.get(e), y.get(e), q.m, q.mq, c, zp, zq);
+    for (int e = 0; e < P::N; ++e) z[e & 1] += sv_rest(x.get(e), y.get(e), wp, wq, zp, zq);
   }
   const double sum = wave_sum64(z[0] + z[1]);
   if (lane == 0) a.sums[(2 * (int64_t)a.n + s) * a.chunks + chunk] = sum;
@@ -532,6 +554,7 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
   const int64_t* tok = a.tokens + (int64_t)s * a.T;
   const void* row = sv_row<DT>(a, s, q.last);
   const void* drow = q.mode == SV_RESIDUAL ? sv_draft_row<DT>(a, s, q.last) : nullptr;
+  const SvRow wp(q.m, c), wq(q.mq, c);
   double* sums = a.sums + (int64_t)s * a.chunks;
   double zp = 1.0, zq = 0.0;
   if (drow) {
@@ -546,7 +569,7 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
     tried = 0;
     drow = nullptr;
     for (int k = wave; k < a.chunks; k += 4) {
-      const double z = sv_chunk_sum<DT>(row, k, a.V, lane, q.m, c, tok, 0);
+      const double z = sv_chunk_sum<DT>(row, k, a.V, lane, wp, tok, 0);
       if (lane == 0) sums[k] = z;
     }
     __syncthreads();                                    // the sums, too, are this workgroup's
@@ -589,9 +612,9 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
     if (v < a.V) {
       const float x = sv_logit<DT>(row, v);
       if (drow) {
-        w[e] = sv_rest(x, sv_logit<DT>(drow, v), q.m, q.mq, c, zp, zq);
+        w[e] = sv_rest(x, sv_logit<DT>(drow, v), wp, wq, zp, zq);
       } else {
-        w[e] = sv_weight(x, q.m, c);
+        w[e] = wp.weight(x);
         for (uint64_t b = tried; b; b &= b - 1)
           if (tok[__ffsll((unsigned long long)b) - 1] == v) w[e] = 0.0;
       }
@@ -636,12 +659,13 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
 static int64_t sv_work(int64_t n, int64_t T, int64_t V, bool drafted) {
   const int64_t chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
   const int64_t rows = n * T + (drafted ? n * (T - 1) : 0);
-  return rows * chunks + 3 * n * chunks + 4 * n;        // records, sums, sequences, in doubles
+  const int64_t blocks = (V + SV_BLOCK - 1) / SV_BLOCK;
+  return rows * blocks + 3 * n * chunks + 4 * n;        // records, sums, sequences, in doubles
 }
 
 extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted) {
   if (n < 0 || n_nodes < 1 || vocab < 1) return OMNI_EINVAL;
-  if (n_nodes > SV_MAX_NODES) return OMNI_EUNSUPPORTED;
+  if (n_nodes > SV_MAX_NODES || vocab > 1 << 30) return OMNI_EUNSUPPORTED;
   const int64_t work = sv_work(n, n_nodes, vocab, drafted);
   return work > 0x7fffffff ? OMNI_EUNSUPPORTED : (int)work;
 }
@@ -650,7 +674,7 @@ template <int DT>
 static void sv_launch(const SvArgs& a, hipStream_t st) {
   const int rows = a.n * a.T + (a.draft ? a.n * (a.T - 1) : 0);
   const int parts = ceil_div(a.chunks, SV_WAVES);
-  hipLaunchKernelGGL((sv_stats_kernel<DT>), dim3(rows * ceil_div(a.chunks, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((sv_stats_kernel<DT>), dim3(rows * a.blocks), dim3(64 * SV_WAVES), 0, st, a);
   hipLaunchKernelGGL((sv_walk_kernel<DT>), dim3(a.n * parts), dim3(64 * SV_WAVES), 0, st, a);
   if (a.uniforms) {                                     // else every row is greedy
     if (a.draft)
@@ -667,7 +691,7 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
                                 int* emitted, void* workspace, int64_t workspace_doubles,
                                 void* stream) {
   if (n < 0 || n_nodes < 1 || vocab < 1 || dtype < 0 || dtype > 2) return OMNI_EINVAL;
-  if (n_nodes > SV_MAX_NODES) return OMNI_EUNSUPPORTED;
+  if (n_nodes > SV_MAX_NODES || vocab > 1 << 30) return OMNI_EUNSUPPORTED;
   if (seq_stride < 0 || row_stride < 0 || draft_seq_stride < 0 || draft_row_stride < 0) return OMNI_EINVAL;
   if (draft && parents) return OMNI_EUNSUPPORTED;
   if (!temperature && !(temp >= 0.f)) return OMNI_EINVAL;
@@ -695,12 +719,13 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   a.T = n_nodes;
   a.V = vocab;
   a.chunks = ceil_div(vocab, SV_CHUNK);
+  a.blocks = ceil_div(vocab, SV_BLOCK);
   a.path = path;
   a.out_tokens = out_tokens;
   a.emitted = emitted;
   a.rec = (float2*)workspace;
   const int64_t rows = (int64_t)n * n_nodes + (draft ? (int64_t)n * (n_nodes - 1) : 0);
-  a.sums = (double*)workspace + rows * a.chunks;
+  a.sums = (double*)workspace + rows * a.blocks;
   a.seqs = (SvSeq*)(a.sums + 3 * (int64_t)n * a.chunks);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) sv_launch<0>(a, st);

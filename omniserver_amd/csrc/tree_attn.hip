@@ -56,8 +56,7 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   const int64_t delta = row_ok && rope_delta ? rope_delta[slot] : 0;
 
   // units of the sequences before this one, its own, and all
-  int64_t before = 0, all = 0;
-  int units = 0;
+  int before = 0, all = 0, units = 0;
   for (int r0 = 0; r0 < n; r0 += 64) {
     const int r = r0 + i;
     int w = 0;
@@ -78,15 +77,17 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   units = __shfl(units, s & 63);
   all *= tc.nkv;
   before *= tc.nkv;
-  int64_t cols = tc.least ? min((int64_t)tc.ncols, max((int64_t)1, all / tc.least)) : tc.ncols;
-  auto cut = [&](int64_t c) { return c * all / cols; };        // first unit of column c
+  // column c starts at unit c all / cols (in two parts: all < 2^30, cols < 2^15)
+  const unsigned cols = tc.least ? min(tc.ncols, max(1, all / tc.least)) : tc.ncols;
+  const unsigned per = (unsigned)all / cols, over = (unsigned)all - per * cols;
+  auto cut = [&](unsigned c) { return (int)(c * per + c * over / cols); };
   for (int c = i; c < tc.ncols; c += 64) {
     int* col = tc.columns + 8 * c;
     if (tc.least) {
-      const int64_t lo = c < cols ? cut(c) : all, cnt = c < cols ? cut(c + 1) - lo : 0;
-      if (cnt > 0 && lo >= before && lo < before + (int64_t)units * tc.nkv) {
-        const int g = (int)((lo - before) / units);
-        *(i32x4*)col = (i32x4){s, g, (int)(lo - before) - g * units, (int)cnt};
+      const int lo = c < cols ? cut(c) : all, cnt = c < cols ? cut(c + 1) - lo : 0;
+      if (cnt > 0 && lo >= before && lo < before + units * tc.nkv) {
+        const int g = (lo - before) / units;
+        *(i32x4*)col = (i32x4){s, g, lo - before - g * units, cnt};
         *(i32x4*)(col + 4) = (i32x4){L, used, 0, 0};
       } else if (cnt <= 0 && s == 0) {
         *(i32x4*)col = (i32x4){0, 0, 0, 0};
@@ -99,10 +100,10 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   for (int g = i; g < tc.nkv; g += 64) {
     int2 at = make_int2(0, 0);
     if (units && tc.least) {
-      const int64_t lo = before + (int64_t)g * units, hi = lo + units - 1;
-      // the last column that starts at or before a unit
-      auto column = [&](int64_t x) {
-        int64_t c = x * cols / all;
+      const int lo = before + g * units, hi = lo + units - 1;
+      // the last column that starts at or before a unit: a guess and its neighbours
+      auto column = [&](int x) {
+        unsigned c = min(cols - 1, (unsigned)((float)x * (float)cols / (float)all));
         while (c + 1 < cols && cut(c + 1) <= x) ++c;
         while (cut(c) > x) --c;
         return (int)c;
@@ -528,11 +529,17 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
 }
 
 // The states of a (node, query head) row to its output, for items that more than one column has
-// parts of: one wave a row, two dims a lane.
+// parts of.  Half a wave takes a part's state, four dims a lane; a row's parts go round GROUPS
+// half waves, four in flight in each, and the groups meet in LDS.  One group a row for a handful
+// of parts, eight (a workgroup a row) for many: 32 at 4000 keys 7.2 us in one wave.
+template <int GROUPS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, const int* __restrict__ heads,
                                                          int block_rows, int64_t rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) float acc[GROUPS][TREE_HD];
+  __shared__ float ml[GROUPS][2];
+  const int half = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const int grp = half % GROUPS;
+  const int64_t r = (int64_t)blockIdx.x * (8 / GROUPS) + half / GROUPS;
   if (r >= rows) return;
   const int nh = a.nkv * a.G;
   const int tok = (int)(r / nh), head = (int)(r - (int64_t)tok * nh);
@@ -545,32 +552,65 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, const int* 
   const int64_t block = (int64_t)block_rows * ATT_REC, step = a.rblocks * 2 * block;
   const float* rec = a.states + (int64_t)first * step + rb * 2 * block + (row - rb * block_rows) * ATT_REC;
   const int64_t skip = at.x >> 30 ? block : 0;       // in its first column the item is the second
-  float M = -INFINITY;
-  for (int k = lane; k < splits; k += 64) M = fmaxf(M, rec[k * step + (k ? 0 : skip) + 128]);
-  M = wave_max(M);
-  const float ref = M == -INFINITY ? 0.f : M;
-  float o0 = 0.f, o1 = 0.f, den = 0.f;
-  for (int k0 = 0; k0 < splits; k0 += 8) {
-    float2 ml[8], v[8];
+  float M = -INFINITY, den = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = grp; k0 < splits; k0 += 4 * GROUPS) {
+    float2 st[4];
+    float4 v[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int at_k = min(k0 + k, splits - 1);
-      const float* from = rec + at_k * step + (at_k ? 0 : skip);
-      ml[k] = *(const float2*)(from + 128);
-      v[k] = *(const float2*)(from + 2 * lane);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k0 + k < splits) {
-        const float f = exp2f(ml[k].x - ref);
-        den = fmaf(f, ml[k].y, den);
-        o0 = fmaf(f, v[k].x, o0);
-        o1 = fmaf(f, v[k].y, o1);
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j * GROUPS;
+      st[j] = make_float2(-INFINITY, 0.f);
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < splits) {
+        const float* from = rec + k * step + (k ? 0 : skip);
+        st[j] = *(const float2*)(from + 128);
+        v[j] = *(const float4*)(from + 4 * l);
       }
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), M);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float f = exp2f(M - ref);
+    M = mn;
+    den *= f;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = exp2f(st[j].x - ref);
+      den = fmaf(e, st[j].y, den);
+      o.x = fmaf(e, v[j].x, o.x);
+      o.y = fmaf(e, v[j].y, o.y);
+      o.z = fmaf(e, v[j].z, o.z);
+      o.w = fmaf(e, v[j].w, o.w);
+    }
+  }
+  if (GROUPS > 1) {
+    *(float4*)&acc[grp][4 * l] = o;
+    if (l == 0) {
+      ml[grp][0] = M;
+      ml[grp][1] = den;
+    }
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k) M = fmaxf(M, ml[k][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    den = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      const float e = exp2f(ml[k][0] - ref);
+      const float4 v = *(const float4*)&acc[k][4 * l];
+      den = fmaf(e, ml[k][1], den);
+      o.x = fmaf(e, v.x, o.x);
+      o.y = fmaf(e, v.y, o.y);
+      o.z = fmaf(e, v.z, o.z);
+      o.w = fmaf(e, v.w, o.w);
+    }
   }
   const float inv = den == 0.f ? 0.f : 1.0f / den;
-  const half2_t h2 = {(half_t)(o0 * inv), (half_t)(o1 * inv)};
-  *(half2_t*)(a.out + (int64_t)tok * a.out_stride + head * TREE_HD + 2 * lane) = h2;
+  const half4_t h4 = {(half_t)(o.x * inv), (half_t)(o.y * inv), (half_t)(o.z * inv), (half_t)(o.w * inv)};
+  *(half4_t*)(a.out + (int64_t)tok * a.out_stride + head * TREE_HD + 4 * l) = h4;
 }
 
 // The workgroup forms, (rows, groups): 32 R rows, S key groups of KT-key tiles.
@@ -598,7 +638,8 @@ extern "C" int omni_tree_plan(const int* parents, const int* counts, const int64
   int unit;
   if (!tree_form(rows, groups, &unit) || columns < 1 || least < 0) return OMNI_EINVAL;
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
-  if ((int64_t)n * n_kv_heads * ceil_div(max_len, unit) > 0x3fffffff || (columns >> 24)) return OMNI_EUNSUPPORTED;
+  if ((int64_t)n * n_kv_heads * ceil_div(max_len, unit) > 0x3fffffff || (least && columns > 32767))
+    return OMNI_EUNSUPPORTED;
   if (n == 0) return OMNI_OK;
   if (!parents || !lengths || !starts || !ancestors || !positions || !token_slot || !token_pos ||
       !schedule || ((uintptr_t)schedule & 15))
@@ -691,8 +732,14 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
     hipLaunchKernelGGL((tree_attn_kernel<1, 8, 32>), gd, dim3(512), 0, st, a);
   OMNI_CHECK_LAUNCH();
   if (least) {
-    hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((out_rows + 3) / 4)), dim3(256), 0, st, a,
-                       a.columns + 8 * (int64_t)columns, rows, out_rows);
+    // parts of an item: at least one, some columns / items
+    const int* heads = a.columns + 8 * (int64_t)columns;
+    if (columns > 8 * n * n_kv_heads)
+      hipLaunchKernelGGL((tree_merge_kernel<8>), dim3((unsigned)out_rows), dim3(256), 0, st, a, heads,
+                         rows, out_rows);
+    else
+      hipLaunchKernelGGL((tree_merge_kernel<1>), dim3((unsigned)((out_rows + 7) / 8)), dim3(256), 0, st,
+                         a, heads, rows, out_rows);
     OMNI_CHECK_LAUNCH();
   }
   return OMNI_OK;

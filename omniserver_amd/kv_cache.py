@@ -457,7 +457,8 @@ def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) ->
     unit = {1: 64, 2: 128, 4: 128, 8: 256}[form[1]]
     if capacity <= 512:
         return (*form, n * nkv, 0)
-    columns = max(1, min(cus // -(-rows // form[0]), n * nkv * -(-capacity // unit)))
+    columns = cus // 8 // -(-rows // form[0]) * 8
+    columns = max(1, min(columns, n * nkv * -(-capacity // unit)))
     return (*form, columns, 1)
 
 
@@ -520,27 +521,52 @@ class TreeCache(PackedPrefillWriter):
             raise ValueError(f"rope_delta holds one value per pool row ({pool.max_batch})")
         require_here(parents, self.counts, self.slots, rope_delta)
         self.n, self.nodes, self.T = n, T, n * T
-        # how the attention's workgroups share the keys; its split states' buffer serves all
-        # layers (launches on one stream are ordered)
-        self.form = rows, groups, columns, least = tree_plan(
-            n, T, pool.n_heads, pool.n_kv_heads, pool.max_len, num_cus(dev))
+        nkv = pool.n_kv_heads
+        # how the attention's workgroups share the keys
+        self.form = rows, groups, columns, least = tree_plan(n, T, pool.n_heads, nkv, pool.max_len,
+                                                             num_cus(dev))
+        # one int64 block: starts, ancestors, positions, pool rows and positions, the attention's
+        # schedule (int32, on a 16-byte boundary)
+        ints = 4 * n + 8 * columns + 2 * n * nkv
+        words = n + 6 * n * T
+        words += words & 1
+        self._plan = torch.empty(words + (ints + 1) // 2, device=dev, dtype=torch.int64)
+        p = self._plan.data_ptr()
+        self._starts, self._ancestors, self._schedule = p, p + 8 * n, p + 8 * words
+        self._slot, self._pos = p + 8 * (n + 4 * n * T), p + 8 * (n + 5 * n * T)
+        call("omni_tree_plan", parents.data_ptr(), ptr(self.counts), ptr(self.slots),
+             pool.lengths.data_ptr(), ptr(rope_delta), n, T, pool.max_batch, pool.max_len, p,
+             self._ancestors, p + 8 * (n + n * T), self._slot, self._pos, nkv, rows, groups, columns,
+             least, self._schedule, ints, stream())
+        # the attention's split states, for all layers (launches on one stream are ordered)
         self._ws = None if not least else torch.empty(
-            columns * -(-T * (pool.n_heads // pool.n_kv_heads) // rows) * 2 * rows * 132,
-            device=dev, dtype=torch.float32)
-        self.schedule = torch.empty(4 * n + 8 * columns + 2 * n * pool.n_kv_heads, device=dev,
-                                    dtype=torch.int32)
-        # one block for the plan: starts, ancestors, positions, pool rows and positions
-        plan = torch.empty(n + 6 * n * T, device=dev, dtype=torch.int64)
-        self.starts = plan[:n]
-        self.ancestors = plan[n:n + n * T]
-        self.positions = plan[n + n * T:n + 4 * n * T].view(3, n * T)
-        self.token_slot = plan[n + 4 * n * T:n + 5 * n * T]
-        self.token_pos = plan[n + 5 * n * T:]
-        call("omni_tree_plan", ptr(parents), ptr(self.counts), ptr(self.slots), ptr(pool.lengths),
-             ptr(rope_delta), n, T, pool.max_batch, pool.max_len, ptr(self.starts),
-             ptr(self.ancestors), ptr(self.positions), ptr(self.token_slot), ptr(self.token_pos),
-             pool.n_kv_heads, rows, groups, columns, least, ptr(self.schedule),
-             self.schedule.numel(), stream())
+            columns * -(-T * (pool.n_heads // nkv) // rows) * 2 * rows * 132, device=dev,
+            dtype=torch.float32)
+
+    @property
+    def starts(self) -> torch.Tensor:
+        """int64 [n]: the prefix lengths the trees stand behind."""
+        return self._plan[:self.n]
+
+    @property
+    def ancestors(self) -> torch.Tensor:
+        """int64 [n, T]: bit j of a node's word is set where node j is the node or above it."""
+        return self._plan[self.n:self.n + self.T].view(self.n, self.nodes)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        """int64 [3, n * T]: rotary positions."""
+        return self._plan[self.n + self.T:self.n + 4 * self.T].view(3, self.T)
+
+    @property
+    def token_slot(self) -> torch.Tensor:
+        """int64 [n * T]: the nodes' pool rows, -1 where they are stored nowhere."""
+        return self._plan[self.n + 4 * self.T:self.n + 5 * self.T]
+
+    @property
+    def token_pos(self) -> torch.Tensor:
+        """int64 [n * T]: the nodes' positions in their rows."""
+        return self._plan[self.n + 5 * self.T:self.n + 6 * self.T]
 
     def bind(self, T: int) -> None:
         if T != self.T:
@@ -554,21 +580,27 @@ class TreeCache(PackedPrefillWriter):
         """out [n * T, nh, hd] (fp16, contiguous): attention of the nodes whose queries are the
         first nh * hd columns of the rows qkv; their K/V is in the pool (rope_and_write)."""
         pool = self.pool
-        nh, hd = pool.n_heads, pool.head_dim
-        if qkv.dim() != 2 or qkv.shape[0] != self.T or qkv.shape[1] < nh * hd or qkv.stride(1) != 1:
+        width = pool.n_heads * pool.head_dim
+        if qkv.dim() != 2 or qkv.shape[0] != self.T or qkv.shape[1] < width or qkv.stride(1) != 1:
             raise ValueError(f"query rows of shape {tuple(qkv.shape)}: expected [{self.T}, >= "
-                             f"{nh * hd}] with contiguous columns")
+                             f"{width}] with contiguous columns")
         if qkv.dtype != torch.float16 or out.dtype != torch.float16:
             raise TypeError(f"the pool's attention is fp16 (got {qkv.dtype} -> {out.dtype})")
-        if out.numel() != self.T * nh * hd or not out.is_contiguous():
+        if out.numel() != self.T * width or not out.is_contiguous():
             raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
-                             f"[{self.T}, {nh}, {hd}]")
+                             f"[{self.T}, {pool.n_heads}, {pool.head_dim}]")
         require_here(qkv, out)
-        call("omni_tree_attention", ptr(qkv), qkv.stride(0), ptr(pool.k[layer_idx]),
-             ptr(pool.v[layer_idx]), pool.max_batch, pool.max_len, ptr(self.slots),
-             ptr(self.ancestors), self.n, self.nodes, ptr(out), nh * hd, nh, pool.n_kv_heads, hd,
-             float(scale), *self.form, ptr(self.schedule), ptr(self._ws),
-             0 if self._ws is None else self._ws.numel(), stream())
+        stride = qkv.stride(0) if self.T > 1 else max(qkv.stride(0), width)
+        return self._attend(qkv.data_ptr(), stride, layer_idx, scale, out)
+
+    def _attend(self, q: int, q_stride: int, layer_idx: int, scale: float, out):
+        pool, ws = self.pool, self._ws
+        nh, hd = pool.n_heads, pool.head_dim
+        call("omni_tree_attention", q, q_stride, pool.k[layer_idx].data_ptr(),
+             pool.v[layer_idx].data_ptr(), pool.max_batch, pool.max_len, ptr(self.slots),
+             self._ancestors, self.n, self.nodes, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd,
+             float(scale), *self.form, self._schedule, ptr(ws), 0 if ws is None else ws.numel(),
+             stream())
         return out
 
     def flash_prefill(self, q, k, v, layer_idx, scale):
@@ -577,20 +609,19 @@ class TreeCache(PackedPrefillWriter):
         pool = self.pool
         nh, nkv, hd = pool.n_heads, pool.n_kv_heads, pool.head_dim
         self.bind(q.shape[0])
-        if tuple(q.shape[1:]) != (nh, hd) or tuple(k.shape) != (self.T, nkv, hd) \
-                or k.shape != v.shape:
+        if q.shape != (self.T, nh, hd) or k.shape != (self.T, nkv, hd) or k.shape != v.shape:
             raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: expected "
                              f"[{self.T}, {nh} / {nkv}, {hd}]")
         if not q.dtype == k.dtype == v.dtype == torch.float16:
             raise TypeError(f"the pool is fp16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-        q, k, v = (_head_rows(x) for x in (q, k, v))
+        (q, qs), (k, ks), (v, vs) = _head_rows(q), _head_rows(k), _head_rows(v)
         require_here(q, k, v)
-        call("omni_kv_write_rows", ptr(k), k.stride(0), ptr(v), v.stride(0),
-             ptr(pool.k[layer_idx]), ptr(pool.v[layer_idx]), ptr(self.token_slot),
-             ptr(self.token_pos), pool.max_batch, pool.max_len, nkv * hd, self.T, stream())
+        call("omni_kv_write_rows", k.data_ptr(), ks, v.data_ptr(), vs,
+             pool.k[layer_idx].data_ptr(), pool.v[layer_idx].data_ptr(), self._slot, self._pos,
+             pool.max_batch, pool.max_len, nkv * hd, self.T, stream())
         make = torch.empty if self.counts is None and self.slots is None else torch.zeros
         out = make(self.T, nh, hd, device=q.device, dtype=torch.float16)
-        return self.attend_qkv(q, layer_idx, scale, out)
+        return self._attend(q.data_ptr(), qs, layer_idx, scale, out)
 
     def update(self, k, v, layer_idx, cache_kwargs=None):
         raise NotImplementedError("a drafted tree has no causal window for the SDPA route")
@@ -605,9 +636,9 @@ class TreeCache(PackedPrefillWriter):
         path = _ints(path, (self.n, self.nodes), torch.int32, pool.device, "path")
         emitted = _ints(emitted, (self.n,), torch.int32, pool.device, "emitted")
         require_here(path, emitted)
-        call("omni_kv_accept", ptr(pool.storage), pool.n_layers, pool.max_batch, pool.max_len,
-             pool.n_kv_heads * pool.head_dim, ptr(self.slots), ptr(self.starts), ptr(path),
-             ptr(emitted), self.n, self.nodes, ptr(pool.lengths), stream())
+        call("omni_kv_accept", pool.storage.data_ptr(), pool.n_layers, pool.max_batch, pool.max_len,
+             pool.n_kv_heads * pool.head_dim, ptr(self.slots), self._starts, path.data_ptr(),
+             emitted.data_ptr(), self.n, self.nodes, pool.lengths.data_ptr(), stream())
         if self.slots is None:
             pool._active = max(pool._active, self.n)
 
@@ -621,14 +652,18 @@ def _ints(values, shape, dtype, device, name: str):
         values = to_device(values, dtype, device)
     if values.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {values.dtype}")
-    if shape is not None and tuple(values.shape) != shape:
+    if shape is not None and values.shape != shape:
         raise ValueError(f"{name} of shape {tuple(values.shape)}: expected {list(shape)}")
     return values.contiguous()
 
 
-def _head_rows(x: torch.Tensor) -> torch.Tensor:
-    """x [T, heads, hd] as rows [T, heads * hd] with contiguous, 16-byte aligned columns: a view
-    where x is a slice of a fused projection, else a copy."""
-    if x.stride(2) != 1 or x.stride(1) != x.shape[2] or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
-    return x.as_strided((x.shape[0], x.shape[1] * x.shape[2]), (x.stride(0), 1))
+def _head_rows(x: torch.Tensor) -> tuple:
+    """x [T, heads, hd] with each token's heads one after another, on 16-byte boundaries, and its
+    row stride: x itself where it is a slice of a fused projection, else a copy."""
+    T, heads, hd = x.shape
+    s0, s1, s2 = x.stride()
+    width = heads * hd
+    if s2 != 1 or (heads > 1 and s1 != hd) or x.data_ptr() % 16 or (T > 1 and (s0 % 8 or s0 < width)):
+        x = x.clone(memory_format=torch.contiguous_format)
+        return x, width
+    return x, s0 if T > 1 else width
