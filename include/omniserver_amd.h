@@ -169,17 +169,17 @@ int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
 /* Attention of the trees' nodes over the pool: node i of sequence s (row s * n_nodes + i of q and
  * out, fp16, strides in halfs) attends to keys [0, starts[s]) of its pool row and to starts[s] + j
  * for its ancestors j; nodes not in use and sequences outside the pool leave their out rows as
- * they were.  (rows, groups) of a workgroup as in omni_prefill_attention_rows: (128, 1), (128, 2),
- * (64, 4) or (32, 8), any number of query heads per KV head.  Where the plan cuts (least > 0) the
+ * they were.  (rows, groups) of a workgroup as in omni_prefill_attention_rows: (128, 2), (64, 4) or
+ * (32, 8), any number of query heads per KV head.  Where the plan cuts (least > 0) the
  * softmax states of the pieces go through workspace (fp32, 16-byte aligned, columns * ceil(n_nodes
  * * n_heads / n_kv_heads / rows) * 2 * rows * 132 floats) to a second launch.  head_dim 128; scale
  * a positive normal fp32; 16-byte aligned operands. */
 int omni_tree_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache,
-                        int pool_rows, int max_len, const int64_t* slots, const void* ancestors,
-                        int n, int n_nodes, void* out, int out_stride, int n_heads,
-                        int n_kv_heads, int head_dim, float scale, int rows, int groups,
-                        int columns, int least, const int* schedule, float* workspace,
-                        int64_t workspace_floats, void* stream);
+                        int pool_rows, int max_len, const void* ancestors, int n, int n_nodes,
+                        void* out, int out_stride, int n_heads, int n_kv_heads, int head_dim,
+                        float scale, int rows, int groups, int columns, int least,
+                        const int* schedule, float* workspace, int64_t workspace_floats,
+                        void* stream);
 
 /* Verification of drafted tokens.  logits [n][n_nodes][vocab] (dtype 0 fp16, 1 bf16, 2 fp32;
  * strides in elements), tokens int64, uniforms fp32 [n][n_nodes]; parents int32 [n][n_nodes] for

@@ -21,8 +21,8 @@
 // which is cut into equal stretches, one per column of workgroups.  So a batch of one long and many
 // short contexts loads the workgroups as evenly as one of equal contexts, whatever the lengths
 // on the device are.  A stretch is at least `least` units; least 0: a column for each item.
-//   seqs[s]     (prefix length, nodes in use, units, -)
-//   columns[c]  (s, g, first unit there, units in all, prefix length, nodes in use)
+//   seqs[s]     (prefix length, nodes in use, units, pool row)
+//   columns[c]  (s, g, first unit there, units in all, then of s: length, nodes, pool row)
 //   heads[s][g] (first column | 1 << 30 where the item is not the first that column sees, last)
 // One wave a sequence: lane i walks up from node i; every wave sums all sequences' units and
 // writes the columns that start in its own sequence.
@@ -88,13 +88,13 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
       if (cnt > 0 && lo >= before && lo < before + units * tc.nkv) {
         const int g = (lo - before) / units;
         *(i32x4*)col = (i32x4){s, g, lo - before - g * units, cnt};
-        *(i32x4*)(col + 4) = (i32x4){L, used, 0, 0};
+        *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
       } else if (cnt <= 0 && s == 0) {
         *(i32x4*)col = (i32x4){0, 0, 0, 0};
       }
     } else if (c / tc.nkv == s) {
       *(i32x4*)col = (i32x4){s, c % tc.nkv, 0, units};
-      *(i32x4*)(col + 4) = (i32x4){L, used, 0, 0};
+      *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
     }
   }
   for (int g = i; g < tc.nkv; g += 64) {
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   }
   if (i == 0) {
     starts[s] = L;
-    *(i32x4*)(tc.seqs + 4 * s) = (i32x4){L, used, units, 0};
+    *(i32x4*)(tc.seqs + 4 * s) = (i32x4){L, used, units, (int)slot};
   }
   __syncthreads();
   if (i >= T) return;
@@ -177,9 +177,8 @@ struct TreeArgs {
   int q_stride;
   const half_t* k_cache;
   const half_t* v_cache;
-  int pool_rows, max_len, nkv, G, T, n;
+  int max_len, nkv, G, T, n;
   int ncols, rblocks;          // columns of the schedule, row blocks (workgroups) of each
-  const int64_t* slots;        // [n] or null
   const uint64_t* ancestors;   // [n][T]
   const int* seqs;
   const int* columns;
@@ -192,14 +191,14 @@ struct TreeArgs {
 // One row over keys [k0, k1) by one wave: 64 keys a step, a key a lane for the scores, then two
 // dims a lane for the output, hidden keys left out.
 // rec: the row's state, or null for its output.
-__device__ __forceinline__ void tree_row(const TreeArgs& a, int64_t slot, int s, int g, int row, int L,
+__device__ __forceinline__ void tree_row(const TreeArgs& a, int slot, int s, int g, int row, int L,
                                          int k0, int k1, float* rec) {
   const int lane = threadIdx.x & 63;
   const int node = row / a.G, head = g * a.G + row - node * a.G;
   const int64_t tok = (int64_t)s * a.T + node;
   const uint64_t mask = a.ancestors[tok];
   const int64_t tstride = (int64_t)a.nkv * TREE_HD;
-  const int64_t base = slot * a.max_len * tstride + g * TREE_HD;
+  const int64_t base = (int64_t)slot * a.max_len * tstride + g * TREE_HD;
   const half_t* qp = a.q + tok * a.q_stride + head * TREE_HD;
   float mr = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll 1
@@ -265,7 +264,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   const i32x4 c0 = *(const i32x4*)(a.columns + 8 * col), c1 = *(const i32x4*)(a.columns + 8 * col + 4);
   auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   int s = uniform(c0[0]), g = uniform(c0[1]), u0 = uniform(c0[2]), left = uniform(c0[3]);
-  int L = uniform(c1[0]), used = uniform(c1[1]);
+  int L = uniform(c1[0]), used = uniform(c1[1]), slot = uniform(c1[2]);
   constexpr int UNIT = S * KT;
   for (int part = 0; left > 0; part = 1) {
   const int end = min(L + used, a.max_len);
@@ -274,7 +273,6 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   const bool whole = u0 == 0 && steps == units;
   const int nrows = used * a.G - 32 * R * rb;        // this block's
   if (nrows > 0) {
-  const int64_t slot = a.slots ? a.slots[s] : s;
   const uint64_t word = lane < a.T ? a.ancestors[(int64_t)s * a.T + lane] : 0;
   const int row = min(32 * rt + l32, nrows - 1);
   const int node = (32 * R * rb + row) / a.G;
@@ -297,7 +295,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
 
   const int cr = lane >> 4, cc = lane & 15;
   const int64_t tstride = (int64_t)a.nkv * TREE_HD;  // halfs per token
-  const int64_t base = slot * (int64_t)a.max_len * tstride + g * TREE_HD;
+  const int64_t base = (int64_t)slot * a.max_len * tstride + g * TREE_HD;
   const half_t* kb0 = a.k_cache + base;
   const half_t* vb0 = a.v_cache + base;
   half8_t kr[NL], vr[NL];
@@ -524,6 +522,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
     while (++s < a.n - 1 && uniform(a.seqs[4 * s + 2]) == 0) {}
     L = uniform(a.seqs[4 * s]);
     used = uniform(a.seqs[4 * s + 1]);
+    slot = uniform(a.seqs[4 * s + 3]);
   }
   }
 }
@@ -615,10 +614,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, const int* 
 
 // The workgroup forms, (rows, groups): 32 R rows, S key groups of KT-key tiles.
 static int tree_form(int rows, int groups, int* unit) {
-  const int form = rows == 128 && (groups == 1 || groups == 2) ? groups
-                   : rows == 64 && groups == 4 ? 4 : rows == 32 && groups == 8 ? 8 : 0;
-  *unit = groups * (form <= 2 ? 64 : 32);
-  return form;
+  *unit = groups * (groups == 2 ? 64 : 32);
+  return rows * groups == 256 && (groups == 2 || groups == 4 || groups == 8) ? groups : 0;
 }
 
 // schedule: [n][4] seqs, [ncols][8] columns, [n][nkv][2] heads
@@ -673,8 +670,8 @@ extern "C" int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v
 
 extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_cache,
                                    const void* v_cache, int pool_rows, int max_len,
-                                   const int64_t* slots, const void* ancestors, int n, int n_nodes,
-                                   void* out, int out_stride, int n_heads, int n_kv_heads,
+                                   const void* ancestors, int n, int n_nodes, void* out,
+                                   int out_stride, int n_heads, int n_kv_heads,
                                    int head_dim, float scale, int rows, int groups, int columns,
                                    int least, const int* schedule, float* workspace,
                                    int64_t workspace_floats, void* stream) {
@@ -688,7 +685,6 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
-  if (!slots && n > pool_rows) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
   if (!q || !k_cache || !v_cache || !ancestors || !schedule || !out) return OMNI_EINVAL;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)schedule) & 15)
@@ -705,14 +701,12 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   a.q_stride = q_stride;
   a.k_cache = (const half_t*)k_cache;
   a.v_cache = (const half_t*)v_cache;
-  a.pool_rows = pool_rows;
   a.max_len = max_len;
   a.nkv = n_kv_heads;
   a.T = n_nodes;
   a.n = n;
   a.ncols = columns;
   a.rblocks = (int)rblocks;
-  a.slots = slots;
   a.ancestors = (const uint64_t*)ancestors;
   a.seqs = schedule;
   a.columns = schedule + 4 * (int64_t)n;
@@ -722,9 +716,7 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   a.states = workspace;
   const dim3 gd((unsigned)grid);
   hipStream_t st = (hipStream_t)stream;
-  if (form == 1)
-    hipLaunchKernelGGL((tree_attn_kernel<4, 1, 64>), gd, dim3(256), 0, st, a);
-  else if (form == 2)
+  if (form == 2)
     hipLaunchKernelGGL((tree_attn_kernel<4, 2, 64>), gd, dim3(512), 0, st, a);
   else if (form == 4)
     hipLaunchKernelGGL((tree_attn_kernel<2, 4, 32>), gd, dim3(512), 0, st, a);

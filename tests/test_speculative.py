@@ -20,9 +20,8 @@ def test_tree_attention_refusals():
     from omniserver_amd._lib import lib
 
     def rc(q=P, q_stride=1536, rows=4, max_len=256, plan=P, n=2, nodes=8, out=P, out_stride=1536,
-           nh=12, nkv=2, hd=128, scale=0.1, form=(64, 4), columns=4, least=0, ws=None, floats=0,
-           slots=None):
-        return lib().omni_tree_attention(q, q_stride, P, P, rows, max_len, slots, P, n, nodes, out,
+           nh=12, nkv=2, hd=128, scale=0.1, form=(64, 4), columns=4, least=0, ws=None, floats=0):
+        return lib().omni_tree_attention(q, q_stride, P, P, rows, max_len, P, n, nodes, out,
                                          out_stride, nh, nkv, hd, scale, *form, columns, least,
                                          plan, ws, floats, None)
 
@@ -31,8 +30,8 @@ def test_tree_attention_refusals():
     assert rc(scale=0.0) == rc(scale=-1.0) == rc(scale=float("nan")) == rc(scale=1e-39) == -2
     assert rc(scale=float("inf")) == -2
     assert rc(q_stride=1535) == rc(q_stride=1532) == rc(out_stride=8) == rc(out_stride=1540) == -1
-    assert rc(form=(64, 2)) == rc(form=(32, 1)) == rc(form=(0, 0)) == -1
-    assert rc(columns=0) == rc(columns=5) == rc(least=-1) == rc(n=5, columns=10) == -1
+    assert rc(form=(64, 2)) == rc(form=(128, 1)) == rc(form=(0, 0)) == rc(form=(16, 16)) == -1
+    assert rc(columns=0) == rc(columns=5) == rc(least=-1) == -1
     assert rc(q=None) == rc(out=None) == rc(plan=None) == -1
     assert rc(q=ctypes.c_void_p(24)) == rc(out=ctypes.c_void_p(8)) == rc(plan=ctypes.c_void_p(4)) == -1
     cut = {"least": 1, "columns": 3, "nodes": 16, "form": (64, 4)}
