@@ -19,14 +19,19 @@
 // 10^5 - is decided by a 64-bit sum of its row.  Where a random number falls among 151936 tokens
 // is a matter of borders 1e-6 apart and closer, which 32-bit sums would move across one draw in a
 // few hundred: the one row per sequence that the next token comes from is summed and searched in
-// 64 bits.  Launches: row statistics; the walk, with the drawn row's 64-bit chunk sums; with a
-// draft, the chunk sums of max(p - q, 0), which need both rows' totals; the draw.
+// 64 bits.  Launches: row statistics; the walk, with the drawn row's 64-bit chunk sums; the draw.
+//
+// max(p - q, 0) is summed without knowing both rows' 64-bit totals first: with weights p, q not yet
+// normalised it is max(p - r q, 0), r = the totals' ratio.  From the 32-bit ratio r0 the walk sums
+// max(p - r0 q, 0) and the q of its positive terms, and the draw moves the sums by (r0 - r) times
+// the latter: exact but for the terms whose sign changes between r0 and r, 1e-12 of the total.
 #include "common.h"
 
 #define SV_MAX_NODES 64
-#define SV_CHUNK 2048              // tokens a wave sums: 32 a lane
 #define SV_WAVES 4                 // waves of a workgroup
-#define SV_BLOCK (SV_WAVES * SV_CHUNK)
+#define SV_BLOCK 8192              // tokens of a workgroup in 32 bits: 32 a lane
+#define SV_CHUNK 1024              // tokens a wave sums in 64 bits: 16 a lane
+#define SV_PARTS 768              // workgroups of the walk in all: more walk again what others walk
 #define SV_ERR 0x1p-18             // relative error of a row's 32-bit sum, with a factor 4 to spare
 
 enum { SV_DONE = 0, SV_TARGET = 1, SV_RESIDUAL = 2 };   // where the next token comes from
@@ -43,11 +48,12 @@ struct SvArgs {
   const float* temperature;
   float temp;
   int n, T, V, chunks, blocks;
+  int parts;               // workgroups of the walk for a sequence
   int* path;
   int64_t* out_tokens;
   int* emitted;
   float2* rec;             // [n T target rows, n (T - 1) draft rows][blocks] (largest, sum or index)
-  double* sums;            // [3][n][chunks]: target, draft, residual
+  double* sums;            // [4][n][chunks]: target, draft, residual at r0, its draft weights
   struct SvSeq* seqs;      // [n]
 };
 
@@ -55,6 +61,8 @@ struct SvSeq {             // what the walk leaves for the draw
   int mode, last, len;
   float m, mq;             // largest logits of the drawn row and of the draft's
   uint32_t tried[2];       // children tried at the last node
+  uint32_t pad;
+  double r0;               // the drawn rows' ratio of 32-bit sums, target / draft
 };
 
 template <int DT>
@@ -84,12 +92,13 @@ __device__ __forceinline__ int sv_used(const SvArgs& a, int s) {
   return a.counts ? min(max(a.counts[s], 0), a.T) : a.T;
 }
 
-// 2^t for t <= 0: t = n + f, |f| <= 1/2, 2^f by the polynomial through its values at the nine
-// Chebyshev points of [-1/2, 1/2] (relative error 1.1e-12; 1 at 0), 2^n by the exponent (0 far
-// below).  That error moves a border between two tokens of 1e-6 each across one draw in 10^6.
+// 2^t for -2100 <= t <= 0: t = n + f, |f| <= 1/2, n from the low word of t + 1.5 2^52, 2^f by the
+// polynomial through its values at the nine Chebyshev points of [-1/2, 1/2] (relative error
+// 1.1e-12), 2^n by the exponent (0 far below).  That error moves a border between two tokens of 1e-6
+// each across one draw in 10^6.
 __device__ __forceinline__ double sv_exp2(double t) {
 #pragma clang fp contract(off)          // the same wherever it is inlined
-  const double n = rint(t), f = t - n;
+  const double a = t + 0x1.8p52, f = t - (a - 0x1.8p52);
   double r = 0x1.63d136366db24p-20;
   r = fma(r, f, 0x1.00dc4a532fb8ep-16);
   r = fma(r, f, 0x1.4308ac85aa947p-13);
@@ -99,38 +108,92 @@ __device__ __forceinline__ double sv_exp2(double t) {
   r = fma(r, f, 0x1.ebfbdff823cedp-3);
   r = fma(r, f, 0x1.62e42fef84cf0p-1);
   r = fma(r, f, 1.0);
-  return ldexp(r, (int)fmax(n, -2000.0));
+  return ldexp(r, (int)(uint32_t)__builtin_bit_cast(uint64_t, a));
 }
 
-// The weights of a row whose largest logit is m, at log2(e) / temperature = c: 1 at m, infinite or
-// not, 0 at -inf and NaN.  Where m and c are ordinary a logit that counts for nothing is as good as
-// the lowest finite one.
+// log2(e) / temperature, and 2000 / that: so far below the largest logit every weight is 0.
+struct SvScale {
+  double c, span;
+  __device__ __forceinline__ explicit SvScale(float temp)
+      : c(1.4426950408889634073599 / (double)temp), span(1386.2943611198906 * (double)temp) {}
+};
+
+// The weights of a row whose largest logit is m: 1 at m, infinite or not, 0 at -inf and NaN.  Where m
+// and the scale are ordinary, whatever lies `span` below m is as good as a finite logit there.
 struct SvRow {
-  float m;
-  double c;
+  float m, low;
+  double c, mc;
   bool plain;
-  __device__ __forceinline__ SvRow(float m_, double c_)
-      : m(m_), c(c_), plain(fabsf(m_) < 3e38f && c_ > 1e-30 && c_ < 1e30) {}
+  __device__ __forceinline__ SvRow(float m_, const SvScale& t) : m(m_), c(t.c), mc(m_ * t.c) {
+    low = (float)((double)m - t.span);
+    plain = fabsf(m) < 1e30f && c > 1e-25 && c < 1e25 && ((double)m - (double)low) * c > 1100.0;
+  }
   __device__ __forceinline__ double weight(float x) const {
 #pragma clang fp contract(off)
-    if (plain) return sv_exp2(((double)fmaxf(x, -3.4028234e38f) - (double)m) * c);
+    if (plain) return sv_exp2(fma((double)fmaxf(x, low), c, -mc));
     if (!(x > -INFINITY)) return 0.0;
     if (x == m) return 1.0;
-    return m == INFINITY ? 0.0 : sv_exp2(((double)x - (double)m) * c);
+    return m == INFINITY ? 0.0 : sv_exp2(fmax(((double)x - (double)m) * c, -2000.0));
   }
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, OMNI_WAVE);
-  return v;
+// Reductions and prefix sums by data-parallel moves within rows of 16 lanes (a move is a VALU
+// operation; through LDS, as wave_sum does it, a step takes some 100 cycles and these kernels are
+// chains of such steps).  SHR + k: lane l gets lane l - k of its row, or 0; ROR + k: rotated.
+enum { DPP_SHR = 0x110, DPP_ROR = 0x120, DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143 };
+
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float v, float other = 0.f) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+      __builtin_bit_cast(int, other), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp(double v, double other = 0.0) {
+  const int2 x = __builtin_bit_cast(int2, v), o = __builtin_bit_cast(int2, other);
+  return __builtin_bit_cast(double,
+                            make_int2(__builtin_amdgcn_update_dpp(o.x, x.x, CTRL, ROWS, 0xf, false),
+                                      __builtin_amdgcn_update_dpp(o.y, x.y, CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const int2 x = __builtin_bit_cast(int2, v);
+  return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(x.x, lane),
+                                              __builtin_amdgcn_readlane(x.y, lane)));
 }
 
-// A lane's 32 logits of a chunk, as they are stored, N in each of P 16-byte pieces; element e of
-// piece j is token chunk + at(lane, j) + e.
+// Inclusive prefix sums over the wave.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp<DPP_SHR + 1>(v);
+  v += dpp<DPP_SHR + 2>(v);
+  v += dpp<DPP_SHR + 4>(v);
+  v += dpp<DPP_SHR + 8>(v);
+  v += dpp<DPP_BCAST15, 0xa>(v);       // a row's total into the next row
+  v += dpp<DPP_BCAST31, 0xc>(v);       // the lower half's into the upper
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) {
+  return lane_of(wave_scan(v), 63);
+}
+__device__ __forceinline__ float row_max(float v) {         // over 16 lanes, in all of them
+  v = fmaxf(v, dpp<DPP_ROR + 1>(v));
+  v = fmaxf(v, dpp<DPP_ROR + 2>(v));
+  v = fmaxf(v, dpp<DPP_ROR + 4>(v));
+  return fmaxf(v, dpp<DPP_ROR + 8>(v));
+}
+__device__ __forceinline__ float wave_top(float v) {
+  v = row_max(v);
+  return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
+}
+
+// A lane's logits as they are stored, N in a 16-byte piece; element e of piece j is token v0 +
+// at(lane, j) + e.
 template <int DT>
 struct SvPiece {
-  static constexpr int N = DT == 2 ? 4 : 8, P = 32 / N;
+  static constexpr int N = DT == 2 ? 4 : 8;
   u32x4 w;
   static __device__ __forceinline__ int at(int lane, int j) { return j * 64 * N + lane * N; }
   __device__ __forceinline__ float get(int e) const {      // may be NaN
@@ -140,7 +203,7 @@ struct SvPiece {
   // tokens past the vocabulary: -inf
   __device__ __forceinline__ void load(const void* row, int v0, int V, int lane, int j) {
     const int v1 = v0 + at(lane, j);
-    if (v0 + SV_CHUNK <= V) {            // rows of an odd width are off every alignment
+    if (v0 + (j + 1) * 64 * N <= V) {    // rows of an odd width are off every alignment
       __builtin_memcpy(&w, (const char*)row + (int64_t)v1 * sv_size<DT>(), 16);
       return;
     }
@@ -179,15 +242,16 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_stats_kernel(SvArgs a) {
   const int used = sv_used(a, s);
   if (is_draft ? (greedy || i + 1 >= used) : i >= used) return;
   const void* row = is_draft ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
-  const int v0 = block * SV_BLOCK + wave * SV_CHUNK;
+  constexpr int PER = SV_BLOCK / SV_WAVES;
+  const int v0 = block * SV_BLOCK + wave * PER;
   typedef SvPiece<DT> P;
-  P x[P::P];
+  P x[32 / P::N];
 #pragma unroll
-  for (int j = 0; j < P::P; ++j) x[j].load(row, v0, a.V, lane, j);
+  for (int j = 0; j < 32 / P::N; ++j) x[j].load(row, v0, a.V, lane, j);
   float m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < 32; ++e) m = fmaxf(m, x[e / P::N].get(e));       // leaves a NaN out
-  m = wave_max(m);
+  m = wave_top(m);
   // (x - m) c in two steps: c may be as large as fp32 goes, and an infinite m stays in order
   const float c = greedy ? 0.f : fminf(1.4426950408889634f / temp, 1e38f);
   float sum;
@@ -210,7 +274,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_stats_kernel(SvArgs a) {
 #pragma unroll
       for (int e = 0; e < 32; ++e) z[e & 3] += x[e / P::N].get(e) == m ? 1.f : 0.f;
     }
-    sum = wave_sum((z[0] + z[1]) + (z[2] + z[3]));
+    sum = wave_total((z[0] + z[1]) + (z[2] + z[3]));
   }
   if (lane == 0) {
     wm[wave] = m;
@@ -235,15 +299,15 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_stats_kernel(SvArgs a) {
 
 // A row's blocks together, by half a wave: largest logit and 64-bit sum of their 32-bit sums
 // (greedy: first index).
-__device__ __forceinline__ void sv_combine(const float2* rec, int blocks, int lane, double c, bool greedy,
-                                           float& m, double& z, int& best) {
+__device__ __forceinline__ void sv_combine(const float2* rec, int blocks, int lane, const SvScale& t,
+                                           bool greedy, float& m, double& z, int& best) {
   const int l = lane & 31;
   const float2 own = l < blocks ? rec[l] : make_float2(-INFINITY, 0.f);
   m = own.x;
   for (int k = l + 32; k < blocks; k += 32) m = fmaxf(m, rec[k].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const SvRow row(m, c);
+  m = row_max(m);
+  m = fmaxf(m, __shfl_xor(m, 16));
+  const SvRow row(m, t);
   z = 0.0;
   best = 0x7fffffff;
   for (int k = l; k < blocks; k += 32) {
@@ -254,11 +318,16 @@ __device__ __forceinline__ void sv_combine(const float2* rec, int blocks, int la
       z += (double)v.y * row.weight(v.x);
     }
   }
+  if (greedy) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if (greedy) best = min(best, __shfl_xor(best, o));
-    else z += __shfl_xor(z, o);
+    for (int o = 16; o; o >>= 1) best = min(best, __shfl_xor(best, o));
+    return;
   }
+  z += dpp<DPP_ROR + 1>(z);
+  z += dpp<DPP_ROR + 2>(z);
+  z += dpp<DPP_ROR + 4>(z);
+  z += dpp<DPP_ROR + 8>(z);
+  z += __shfl_xor(z, 16);
 }
 
 // 64-bit sum of a chunk's weights, the tried tokens left out; by one wave.
@@ -271,9 +340,9 @@ __device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V
   P next;
   next.load(row, v0, V, lane, 0);
 #pragma unroll 1
-  for (int j = 0; j < P::P; ++j) {
+  for (int j = 0; j < 16 / P::N; ++j) {
     const P x = next;
-    if (j + 1 < P::P) next.load(row, v0, V, lane, j + 1);
+    if (j + 1 < 16 / P::N) next.load(row, v0, V, lane, j + 1);
     uint32_t gone = 0;                                  // elements that hold a tried token
     for (uint64_t b = tried; b; b &= b - 1) {
       const int64_t t = tok[__ffsll((unsigned long long)b) - 1] - (v0 + P::at(lane, j));
@@ -282,32 +351,61 @@ __device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V
 #pragma unroll
     for (int e = 0; e < P::N; ++e) z[e & 1] += w.weight(gone >> e & 1 ? -INFINITY : x.get(e));
   }
-  return wave_sum64(z[0] + z[1]);
+  return wave_total(z[0] + z[1]);
+}
+
+// A chunk's 64-bit sums of p, of q, of max(p - r0 q, 0) and of the q of its positive terms.
+template <int DT>
+__device__ __forceinline__ void sv_residual_sums(const void* row, const void* drow, int chunk, int V,
+                                                 int lane, const SvRow& wp, const SvRow& wq, double r0,
+                                                 double (&z)[4]) {
+#pragma clang fp contract(off)          // equal rows leave exactly nothing
+  typedef SvPiece<DT> P;
+  const int v0 = chunk * SV_CHUNK;
+  z[0] = z[1] = z[2] = z[3] = 0.0;
+  P nx, ny;
+  nx.load(row, v0, V, lane, 0);
+  ny.load(drow, v0, V, lane, 0);
+#pragma unroll 1
+  for (int j = 0; j < 16 / P::N; ++j) {
+    const P x = nx, y = ny;
+    if (j + 1 < 16 / P::N) {
+      nx.load(row, v0, V, lane, j + 1);
+      ny.load(drow, v0, V, lane, j + 1);
+    }
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      const double p = wp.weight(x.get(e)), q = wq.weight(y.get(e)), d = p - r0 * q;
+      z[0] += p;
+      z[1] += q;
+      z[2] += d > 0.0 ? d : 0.0;
+      z[3] += d > 0.0 ? q : 0.0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) z[k] = wave_total(z[k]);
 }
 
 // ---------------------------------------------------------------------------
 // The walk, by every workgroup of a sequence (part 0 writes it down), then this part's share of
-// the drawn row's chunk sums.  All nodes' tests are made at once, a lane each: a node's own test
-// depends on its earlier siblings' tokens, not on their fate.
+// the drawn row's chunk sums.  A lane a node: all nodes' weights at their parents' rows at once; then
+// one wave goes from the root, children in index order.
 // ---------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
   __shared__ float ms[2][SV_MAX_NODES];
   __shared__ double zs[2][SV_MAX_NODES];
-  __shared__ double wt[SV_MAX_NODES];
-  __shared__ int par[SV_MAX_NODES], best[SV_MAX_NODES];
+  __shared__ int best[SV_MAX_NODES];
   __shared__ int64_t tok[SV_MAX_NODES];
   __shared__ double part[SV_WAVES];
-  __shared__ uint64_t open_rows[2], tried_s;
-  __shared__ int last_s, len_s;
+  __shared__ uint64_t tried_s;
+  __shared__ int open_s, last_s, len_s;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int parts = (a.chunks + SV_WAVES - 1) / SV_WAVES;
-  const int s = blockIdx.x / parts, mine = blockIdx.x - s * parts;
+  const int s = blockIdx.x / a.parts, mine = blockIdx.x - s * a.parts;
   const int T = a.T, used = sv_used(a, s);
   const float temp = sv_temp(a, s);
   const bool greedy = !(temp > 0.f), chain_q = a.draft && !greedy;
-  const double c = greedy ? 1.0 : 1.4426950408889634073599 / (double)temp;
   int* path = a.path + (int64_t)s * T;
   int64_t* out = a.out_tokens + (int64_t)s * T;
   if (used == 0) {
@@ -323,20 +421,22 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
     return;
   }
   // a lane a node: its parent, token and random number, its logits at the parent's rows
-  int up = -1;
+  int up = -1, id = -1;
   int64_t x = 0;
   double u = 0.0;
   float lp = -INFINITY, lq = -INFINITY;
-  if (lane < used) {
+  if (lane < T) {
     up = lane == 0 ? -1 : a.parents ? a.parents[(int64_t)s * T + lane] : lane - 1;
-    if (up < 0 || up >= lane) up = -1;
     x = a.tokens[(int64_t)s * T + lane];
     if (a.uniforms) u = (double)a.uniforms[(int64_t)s * T + lane];
-    if (up >= 0 && x >= 0 && x < a.V) {
-      lp = sv_logit<DT>(sv_row<DT>(a, s, up), x);
-      if (chain_q) lq = sv_logit<DT>(sv_draft_row<DT>(a, s, up), x);
+    if (up < 0 || up >= lane || lane >= used) up = -1;
+    if (x >= 0 && x < a.V) id = (int)x;
+    if (up >= 0 && id >= 0) {
+      lp = sv_logit<DT>(sv_row<DT>(a, s, up), id);
+      if (chain_q) lq = sv_logit<DT>(sv_draft_row<DT>(a, s, up), id);
     }
   }
+  const SvScale scale(greedy ? 1.f : temp);
   const int nrows = chain_q ? 2 * used - 1 : used;        // the target's rows, then the draft's
   for (int r0 = 2 * wave; r0 < nrows; r0 += 2 * SV_WAVES) {
     const int r = min(r0 + (lane >> 5), nrows - 1), d = r >= used, i = d ? r - used : r;
@@ -344,107 +444,121 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
     float m;
     double z;
     int b;
-    sv_combine(a.rec + at * a.blocks, a.blocks, lane, c, greedy, m, z, b);
+    sv_combine(a.rec + at * a.blocks, a.blocks, lane, scale, greedy, m, z, b);
     if ((lane & 31) == 0) {
       ms[d][i] = m;
       zs[d][i] = z;
       if (!d) best[i] = b;
     }
   }
-  if (wave == 0) {
-    par[lane] = up;
-    tok[lane] = x;
-  }
+  if (wave == 0) tok[lane] = x;
   __syncthreads();
 
-  // exact: rows whose sums are 64-bit by now
-  uint64_t exact[2] = {0, 0};
+  uint64_t exact = 0;                                     // rows whose sums are 64-bit by now
   while (true) {
-    bool stands = false, open = false;
     if (wave == 0) {
       double w = 0.0;
-      bool twice = up < 0;
-      if (up >= 0) {
-        for (int j = up + 1; j < lane; ++j) twice |= par[j] == up && tok[j] == x;
-        if (!twice && x >= 0 && x < a.V)
-          w = greedy ? (ms[0][up] > -INFINITY && x == best[up] ? 1.0 : 0.0)
-                     : SvRow(ms[0][up], c).weight(lp);
-      }
-      wt[lane] = w;                                       // read by this wave alone, in order
-      if (w > 0.0) {
-        if (greedy) {
-          stands = true;
-        } else if (chain_q) {
+      if (up >= 0 && id >= 0)
+        w = greedy ? (ms[0][up] > -INFINITY && id == best[up] ? 1.0 : 0.0)
+                   : SvRow(ms[0][up], scale).weight(lp);
+      int here = 0, len = 1, doubt = -1;
+      uint64_t tried = 0;
+      if (greedy || chain_q) {
+        bool stands = w > 0.0, open = false;
+        if (chain_q && stands && zs[1][up] > 0.0) {       // else the draft's row is empty: q = 0
           // u q / Zq < w / Z, both sides times Z Zq
-          const double a0 = u * SvRow(ms[1][up], c).weight(lq) * zs[0][up], a1 = w * zs[1][up];
+          const double a0 = u * SvRow(ms[1][up], scale).weight(lq) * zs[0][up], a1 = w * zs[1][up];
           stands = a0 < a1;
-          open = fabs(a0 - a1) <= 2.0 * SV_ERR * a1 && !((exact[0] & exact[1]) >> up & 1);
-          if (zs[1][up] == 0.0) stands = true, open = false;      // q is nowhere
-        } else {
-          double left = zs[0][up];
-          for (int j = up + 1; j < lane; ++j)
-            if (par[j] == up) left -= wt[j];
-          stands = u * left < w;
-          open = fabs(u * left - w) <= u * zs[0][up] * SV_ERR && !(exact[0] >> up & 1);
+          open = fabs(a0 - a1) <= 2.0 * SV_ERR * a1 && !(exact >> up & 1);
         }
-      }
-      uint64_t rows = 0;
-      for (uint64_t b = __ballot(open); b; b &= b - 1)
-        rows |= 1ull << __shfl(up, __ffsll((unsigned long long)b) - 1);
-      if (lane == 0) open_rows[0] = rows;
-    }
-    __syncthreads();
-    const uint64_t todo = open_rows[0];
-    if (!todo) {
-      if (wave == 0) {
-        const uint64_t ok = __ballot(stands);
-        int here = 0, len = 1;
+        const uint64_t ok = __ballot(stands), unsure = __ballot(open);
         while (true) {
-          const uint64_t next = __ballot(up == here) & ok;
+          tried = __ballot(up == here);
+          const uint64_t next = tried & (ok | unsure);
           if (!next) break;
-          here = __ffsll((unsigned long long)next) - 1;
+          const int i = __ffsll((unsigned long long)next) - 1;
+          if (unsure >> i & 1) {
+            doubt = here;
+            break;
+          }
+          here = i;
           if (mine == 0 && lane == 0) {
             path[len] = here;
             out[len - 1] = tok[here];
           }
           ++len;
         }
-        const uint64_t tried = __ballot(up == here);
-        if (lane == 0) {
-          last_s = here;
-          len_s = len;
-          tried_s = tried;
+      } else {
+        for (int taken = 0; taken >= 0;) {
+          taken = -1;
+          tried = 0;
+          const double z = zs[0][here];
+          const bool sure = exact >> here & 1;
+          double left = z;
+          for (uint64_t kids = __ballot(up == here); kids; kids &= kids - 1) {
+            const int i = __ffsll((unsigned long long)kids) - 1;
+            const double ui = lane_of(u, i);
+            // a token that a sibling has tried has no mass left
+            const bool twice = __ballot(id == __builtin_amdgcn_readlane(id, i)) & tried;
+            const double wi = twice ? 0.0 : lane_of(w, i), by = ui * left - wi;
+            tried |= 1ull << i;
+            if (wi > 0.0) {
+              if (!sure && fabs(by) <= ui * z * SV_ERR) {
+                doubt = here;
+                break;
+              }
+              if (by < 0.0) {
+                taken = i;
+                break;
+              }
+            }
+            left -= wi;
+          }
+          if (doubt >= 0) break;
+          if (taken >= 0) {
+            here = taken;
+            if (mine == 0 && lane == 0) {
+              path[len] = here;
+              out[len - 1] = tok[here];
+            }
+            ++len;
+          }
         }
       }
-      break;
-    }
-    // the open rows' sums in 64 bits, by the whole workgroup
-    for (uint64_t b = todo; b; b &= b - 1) {
-      const int i = __ffsll((unsigned long long)b) - 1;
-      for (int d = 0; d < (chain_q ? 2 : 1); ++d) {
-        const void* row = d ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
-        const SvRow w(ms[d][i], c);
-        double z = 0.0;
-        for (int k = wave; k < a.chunks; k += SV_WAVES)
-          z += sv_chunk_sum<DT>(row, k, a.V, lane, w, tok, 0);
-        if (lane == 0) part[wave] = z;
-        __syncthreads();
-        if (tid == 0) {
-          double t = 0.0;
-          for (int w = 0; w < SV_WAVES; ++w) t += part[w];
-          zs[d][i] = t;
-        }
-        __syncthreads();
+      if (lane == 0) {
+        open_s = doubt;
+        last_s = here;
+        len_s = len;
+        tried_s = tried;
       }
     }
-    exact[0] |= todo;
-    exact[1] |= todo;
+    __syncthreads();
+    const int i = open_s;
+    if (i < 0) break;
+    // the open row's sums in 64 bits, by the whole workgroup
+    for (int d = 0; d < (chain_q ? 2 : 1); ++d) {
+      const void* row = d ? sv_draft_row<DT>(a, s, i) : sv_row<DT>(a, s, i);
+      const SvRow w(ms[d][i], scale);
+      double z = 0.0;
+      for (int k = wave; k < a.chunks; k += SV_WAVES)
+        z += sv_chunk_sum<DT>(row, k, a.V, lane, w, tok, 0);
+      if (lane == 0) part[wave] = z;
+      __syncthreads();
+      if (tid == 0) {
+        double t = 0.0;
+        for (int k = 0; k < SV_WAVES; ++k) t += part[k];
+        zs[d][i] = t;
+      }
+      __syncthreads();
+    }
+    exact |= 1ull << i;
   }
-  __syncthreads();
   const int last = last_s, len = len_s;
   const uint64_t tried = tried_s;
   const float m = ms[0][last];
   const bool residual = chain_q && tried != 0;
+  // a draft row without a token: q is nowhere
+  const double r0 = residual && zs[1][last] > 0.0 ? zs[0][last] / zs[1][last] : 0.0;
   const int mode = greedy || m == -INFINITY ? SV_DONE : residual ? SV_RESIDUAL : SV_TARGET;
   if (mine == 0) {
     if (tid == 0) {
@@ -457,6 +571,7 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
       q->len = len;
       q->m = m;
       q->mq = residual ? ms[1][last] : 0.f;
+      q->r0 = r0;
       q->tried[0] = (uint32_t)tried;
       q->tried[1] = (uint32_t)(tried >> 32);
     }
@@ -465,84 +580,31 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
       out[tid] = -1;
     }
   }
-  const int chunk = mine * SV_WAVES + wave;
-  if (mode == SV_DONE || chunk >= a.chunks) return;
-  const double sp = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), chunk, a.V, lane, SvRow(m, c),
-                                     tok, residual ? 0 : tried);
-  if (lane == 0) a.sums[(int64_t)s * a.chunks + chunk] = sp;
-  if (residual) {
-    const double sq = sv_chunk_sum<DT>(sv_draft_row<DT>(a, s, last), chunk, a.V, lane,
-                                       SvRow(ms[1][last], c), tok, 0);
-    if (lane == 0) a.sums[((int64_t)a.n + s) * a.chunks + chunk] = sq;
-  }
-}
-
-// Sum of a sequence's chunk sums, by one wave.
-__device__ __forceinline__ double sv_total(const double* sums, int chunks, int lane) {
-  double z = 0.0;
-  for (int k = lane; k < chunks; k += 64) z += sums[k];
-  return wave_sum64(z);
-}
-
-// max(p - q, 0) of a token; zp, zq: 1 / totals
-__device__ __forceinline__ double sv_rest(float x, float y, const SvRow& p, const SvRow& q, double zp,
-                                          double zq) {
-#pragma clang fp contract(off)          // equal rows leave exactly nothing
-  const double d = p.weight(x) * zp - q.weight(y) * zq;
-  return d > 0.0 ? d : 0.0;
-}
-
-template <int DT>
-__global__ __launch_bounds__(64 * SV_WAVES) void sv_residual_kernel(SvArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int parts = (a.chunks + SV_WAVES - 1) / SV_WAVES;
-  const int s = blockIdx.x / parts, chunk = (blockIdx.x - s * parts) * SV_WAVES + wave;
-  const SvSeq q = a.seqs[s];
-  if (q.mode != SV_RESIDUAL || chunk >= a.chunks) return;
-  const double c = 1.4426950408889634073599 / (double)sv_temp(a, s);
-  const double* sums = a.sums + (int64_t)s * a.chunks;
-  const double zp = 1.0 / sv_total(sums, a.chunks, lane);
-  const double tq = sv_total(sums + (int64_t)a.n * a.chunks, a.chunks, lane);
-  const double zq = tq > 0.0 ? 1.0 / tq : 0.0;
-  typedef SvPiece<DT> P;
-  const void* row = sv_row<DT>(a, s, q.last);
-  const void* drow = sv_draft_row<DT>(a, s, q.last);
-  const int v0 = chunk * SV_CHUNK;
-  const SvRow wp(q.m, c), wq(q.mq, c);
-  double z[2] = {0.0, 0.0};
-  P nx, ny;
-  nx.load(row, v0, a.V, lane, 0);
-  ny.load(drow, v0, a.V, lane, 0);
-#pragma unroll 1
-  for (int j = 0; j < P::P; ++j) {
-    const P x = nx, y = ny;
-    if (j + 1 < P::P) {
-      nx.load(row, v0, a.V, lane, j + 1);
-      ny.load(drow, v0, a.V, lane, j + 1);
+  if (mode == SV_DONE) return;
+  const SvRow wp(m, scale), wq(residual ? ms[1][last] : 0.f, scale);
+  double* sums = a.sums + (int64_t)s * a.chunks;
+  const int64_t next = (int64_t)a.n * a.chunks;
+  for (int k = mine * SV_WAVES + wave; k < a.chunks; k += a.parts * SV_WAVES) {
+    if (residual) {
+      double z[4];
+      sv_residual_sums<DT>(sv_row<DT>(a, s, last), sv_draft_row<DT>(a, s, last), k, a.V, lane, wp, wq,
+                           r0, z);
+      if (lane == 0)
+        for (int d = 0; d < 4; ++d) sums[d * next + k] = z[d];
+    } else {
+      const double z = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), k, a.V, lane, wp, tok, tried);
+      if (lane == 0) sums[k] = z;
     }
-#pragma unroll
-    for (int e = 0; e < P::N; ++e) z[e & 1] += sv_rest(x.get(e), y.get(e), wp, wq, zp, zq);
   }
-  const double sum = wave_sum64(z[0] + z[1]);
-  if (lane == 0) a.sums[(2 * (int64_t)a.n + s) * a.chunks + chunk] = sum;
-}
-
-// Inclusive prefix sums of a lane's v over the wave.
-__device__ __forceinline__ double wave_scan64(double v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(v, o);
-    if (lane >= o) v += up;
-  }
-  return v;
 }
 
 // ---------------------------------------------------------------------------
 // The draw, one workgroup a sequence: the chunk that u_0 times the total falls into, then the token
-// within it, eight a thread.
+// within it, four a thread.  Where nothing is left of p, from p itself (the second turn).
 // ---------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
+  static_assert(SV_CHUNK == 4 * 256, "four tokens a thread");
   __shared__ double wsum[4];
   __shared__ double base_s, want_s;
   __shared__ int chunk_s, pick[4], tail[4];
@@ -550,117 +612,149 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
   const int s = blockIdx.x;
   const SvSeq q = a.seqs[s];
   if (q.mode == SV_DONE) return;
-  const double c = 1.4426950408889634073599 / (double)sv_temp(a, s);
+  const SvScale scale(sv_temp(a, s));
+  const double u0 = (double)a.uniforms[(int64_t)s * a.T];
   const int64_t* tok = a.tokens + (int64_t)s * a.T;
   const void* row = sv_row<DT>(a, s, q.last);
-  const void* drow = q.mode == SV_RESIDUAL ? sv_draft_row<DT>(a, s, q.last) : nullptr;
-  const SvRow wp(q.m, c), wq(q.mq, c);
+  const SvRow wp(q.m, scale), wq(q.mq, scale);
   double* sums = a.sums + (int64_t)s * a.chunks;
-  double zp = 1.0, zq = 0.0;
-  if (drow) {
-    zp = 1.0 / sv_total(sums, a.chunks, lane);
-    const double tq = sv_total(sums + (int64_t)a.n * a.chunks, a.chunks, lane);
-    zq = tq > 0.0 ? 1.0 / tq : 0.0;
-    sums += 2 * (int64_t)a.n * a.chunks;
-  }
-  uint64_t tried = drow ? 0 : (uint64_t)q.tried[1] << 32 | q.tried[0];
-  if (!(sv_total(sums, a.chunks, lane) > 0.0)) {
-    // nothing is left: p itself, summed here
-    tried = 0;
-    drow = nullptr;
-    for (int k = wave; k < a.chunks; k += 4) {
-      const double z = sv_chunk_sum<DT>(row, k, a.V, lane, wp, tok, 0);
-      if (lane == 0) sums[k] = z;
-    }
-    __syncthreads();                                    // the sums, too, are this workgroup's
-  }
-  if (wave == 0) {
-    double total = 0.0;
-    for (int k0 = 0; k0 < a.chunks; k0 += 64) {
-      const double v = wave_scan64(k0 + lane < a.chunks ? sums[k0 + lane] : 0.0, lane);
-      total += __shfl(v, 63);
-    }
-    const double want = (double)a.uniforms[(int64_t)s * a.T] * total;
-    double base = 0.0, at = 0.0;
-    int found = -1, full = 0;
-    for (int k0 = 0; k0 < a.chunks && found < 0; k0 += 64) {
-      const double own = k0 + lane < a.chunks ? sums[k0 + lane] : 0.0;
-      const double v = wave_scan64(own, lane) + base;
-      const uint64_t hit = __ballot(own > 0.0 && v > want), some = __ballot(own > 0.0);
-      const int l = hit ? __ffsll((unsigned long long)hit) - 1
-                    : some ? 63 - __clzll((long long)some) : -1;
-      if (l >= 0) {                                     // so far the last chunk with weight
-        full = k0 + l;
-        at = l ? __shfl(v, l - 1) : base;
+  const int64_t next = (int64_t)a.n * a.chunks;
+  for (int turn = 0; turn < 2; ++turn) {
+    const bool residual = turn == 0 && q.mode == SV_RESIDUAL;
+    const uint64_t tried = turn || residual ? 0 : (uint64_t)q.tried[1] << 32 | q.tried[0];
+    const void* drow = residual ? sv_draft_row<DT>(a, s, q.last) : nullptr;
+    if (turn) {
+      for (int k = wave; k < a.chunks; k += 4) {
+        const double z = sv_chunk_sum<DT>(row, k, a.V, lane, wp, tok, 0);
+        if (lane == 0) sums[k] = z;
       }
-      if (hit) found = full;
-      base = __shfl(v, 63);
+      __syncthreads();                                  // both turns' sums are this workgroup's
     }
-    if (lane == 0) {
-      chunk_s = full;
-      base_s = at;
-      want_s = want;
+    double ratio = 0.0;
+    if (residual) {
+      double zp = 0.0, zq = 0.0;
+      for (int k = lane; k < a.chunks; k += 64) {
+        zp += sums[k];
+        zq += sums[next + k];
+      }
+      zq = wave_total(zq);
+      ratio = zq > 0.0 ? wave_total(zp) / zq : 0.0;
     }
-  }
-  __syncthreads();
-  const int v0 = chunk_s * SV_CHUNK + tid * 8;
-  double w[8], sum = 0.0;
+    auto chunk_sum = [&](int k) {
+#pragma clang fp contract(off)
+      if (k >= a.chunks) return 0.0;
+      if (!residual) return sums[k];
+      return fmax(sums[2 * next + k] + (q.r0 - ratio) * sums[3 * next + k], 0.0);
+    };
+    if (wave == 0) {
+      // 256 chunks at a time: their sums' loads together
+      double own[4], total = 0.0, base = 0.0, at = 0.0;
+      int full = -1;
+      for (int k0 = 0; k0 < a.chunks; k0 += 256) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int v = v0 + e;
-    w[e] = 0.0;
-    if (v < a.V) {
-      const float x = sv_logit<DT>(row, v);
-      if (drow) {
-        w[e] = sv_rest(x, sv_logit<DT>(drow, v), wp, wq, zp, zq);
-      } else {
-        w[e] = wp.weight(x);
-        for (uint64_t b = tried; b; b &= b - 1)
-          if (tok[__ffsll((unsigned long long)b) - 1] == v) w[e] = 0.0;
+        for (int j = 0; j < 4; ++j) own[j] = chunk_sum(k0 + 64 * j + lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total += wave_total(own[j]);
+      }
+      const double want = u0 * total;
+      bool found = false;
+      for (int k0 = 0; k0 < a.chunks && !found; k0 += 256) {
+        if (a.chunks > 256) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) own[j] = chunk_sum(k0 + 64 * j + lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double v = wave_scan(own[j]) + base;
+          const uint64_t hit = __ballot(own[j] > 0.0 && v > want), some = __ballot(own[j] > 0.0);
+          const int l = hit ? __ffsll((unsigned long long)hit) - 1
+                        : some ? 63 - __clzll((long long)some) : -1;
+          if (!found && l >= 0) {                       // so far the last chunk with weight
+            full = k0 + 64 * j + l;
+            at = l ? lane_of(v, l - 1) : base;
+          }
+          found |= hit != 0;
+          base = lane_of(v, 63);
+        }
+      }
+      if (lane == 0) {
+        chunk_s = full;
+        base_s = at;
+        want_s = want;
       }
     }
-    sum += w[e];
-  }
-  double run = wave_scan64(sum, lane);
-  if (lane == 63) wsum[wave] = run;
-  __syncthreads();
-  run -= sum;
-  for (int k = 0; k < wave; ++k) run += wsum[k];
-  run += base_s;
-  const double want = want_s;
-  int mine = 0x7fffffff, heavy = -1;
+    __syncthreads();
+    int mine = 0x7fffffff, heavy = -1;
+    if (chunk_s >= 0) {
+      const int v0 = chunk_s * SV_CHUNK + tid * 4;
+      float x[4], y[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    run += w[e];
-    if (w[e] > 0.0) {
-      heavy = v0 + e;
-      if (mine == 0x7fffffff && run > want) mine = v0 + e;
-    }
-  }
-  for (int o = 32; o; o >>= 1) {
-    mine = min(mine, __shfl_xor(mine, o));
-    heavy = max(heavy, __shfl_xor(heavy, o));
-  }
-  if (lane == 0) {
-    pick[wave] = mine;
-    tail[wave] = heavy;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int k = 1; k < 4; ++k) {
-      mine = min(mine, pick[k]);
-      heavy = max(heavy, tail[k]);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = v0 + e < a.V ? sv_logit<DT>(row, v0 + e) : -INFINITY;
+        y[e] = drow && v0 + e < a.V ? sv_logit<DT>(drow, v0 + e) : -INFINITY;
+      }
+      for (uint64_t b = tried; b; b &= b - 1) {
+        const int64_t t = tok[__ffsll((unsigned long long)b) - 1] - v0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t == e) x[e] = -INFINITY;
+      }
+      double w[4], sum = 0.0;
+      {
+#pragma clang fp contract(off)          // equal rows leave exactly nothing
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = wp.weight(x[e]);
+          if (residual) w[e] = fmax(w[e] - ratio * wq.weight(y[e]), 0.0);
+          sum += w[e];
+        }
+      }
+      double run = wave_scan(sum);
+      if (lane == 63) wsum[wave] = run;
+      __syncthreads();
+      run -= sum;
+      for (int k = 0; k < wave; ++k) run += wsum[k];
+      run += base_s;
+      const double want = want_s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        run += w[e];
+        if (w[e] > 0.0) {
+          heavy = v0 + e;
+          if (mine == 0x7fffffff && run > want) mine = v0 + e;
+        }
+      }
+      for (int o = 32; o; o >>= 1) {
+        mine = min(mine, __shfl_xor(mine, o));
+        heavy = max(heavy, __shfl_xor(heavy, o));
+      }
+      if (lane == 0) {
+        pick[wave] = mine;
+        tail[wave] = heavy;
+      }
+      __syncthreads();
+      for (int k = 0; k < 4; ++k) {
+        mine = min(mine, pick[k]);
+        heavy = max(heavy, tail[k]);
+      }
     }
     // rounding, or u_0 >= 1: the chunk's last token with weight
-    a.out_tokens[(int64_t)s * a.T + q.len - 1] = mine != 0x7fffffff ? mine : heavy;
+    const int token = mine != 0x7fffffff ? mine : heavy;
+    if (token >= 0) {
+      if (tid == 0) a.out_tokens[(int64_t)s * a.T + q.len - 1] = token;
+      return;
+    }
+    __syncthreads();
   }
 }
+
+static_assert(sizeof(SvSeq) == 40, "five doubles");
 
 static int64_t sv_work(int64_t n, int64_t T, int64_t V, bool drafted) {
   const int64_t chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
   const int64_t rows = n * T + (drafted ? n * (T - 1) : 0);
   const int64_t blocks = (V + SV_BLOCK - 1) / SV_BLOCK;
-  return rows * blocks + 3 * n * chunks + 4 * n;        // records, sums, sequences, in doubles
+  return rows * blocks + 4 * n * chunks + 5 * n;        // records, sums, sequences, in doubles
 }
 
 extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted) {
@@ -673,14 +767,10 @@ extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted)
 template <int DT>
 static void sv_launch(const SvArgs& a, hipStream_t st) {
   const int rows = a.n * a.T + (a.draft ? a.n * (a.T - 1) : 0);
-  const int parts = ceil_div(a.chunks, SV_WAVES);
   hipLaunchKernelGGL((sv_stats_kernel<DT>), dim3(rows * a.blocks), dim3(64 * SV_WAVES), 0, st, a);
-  hipLaunchKernelGGL((sv_walk_kernel<DT>), dim3(a.n * parts), dim3(64 * SV_WAVES), 0, st, a);
-  if (a.uniforms) {                                     // else every row is greedy
-    if (a.draft)
-      hipLaunchKernelGGL((sv_residual_kernel<DT>), dim3(a.n * parts), dim3(64 * SV_WAVES), 0, st, a);
+  hipLaunchKernelGGL((sv_walk_kernel<DT>), dim3(a.n * a.parts), dim3(64 * SV_WAVES), 0, st, a);
+  if (a.uniforms)                                       // else every row is greedy
     hipLaunchKernelGGL((sv_draw_kernel<DT>), dim3(a.n), dim3(256), 0, st, a);
-  }
 }
 
 extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t row_stride,
@@ -720,13 +810,14 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   a.V = vocab;
   a.chunks = ceil_div(vocab, SV_CHUNK);
   a.blocks = ceil_div(vocab, SV_BLOCK);
+  a.parts = max(1, min(ceil_div(a.chunks, SV_WAVES), SV_PARTS / max(n, 1)));
   a.path = path;
   a.out_tokens = out_tokens;
   a.emitted = emitted;
   a.rec = (float2*)workspace;
   const int64_t rows = (int64_t)n * n_nodes + (draft ? (int64_t)n * (n_nodes - 1) : 0);
   a.sums = (double*)workspace + rows * a.blocks;
-  a.seqs = (SvSeq*)(a.sums + 3 * (int64_t)n * a.chunks);
+  a.seqs = (SvSeq*)(a.sums + 4 * (int64_t)n * a.chunks);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) sv_launch<0>(a, st);
   else if (dtype == 1) sv_launch<1>(a, st);
