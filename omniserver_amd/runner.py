@@ -26,6 +26,10 @@ prefilled chunk by chunk into the reserve slot (pool row ``max_running``), each 
 attending to the chunks before it; ``mixed_step`` runs the running sequences' decode
 tokens and one chunk in a single forward.  After the last chunk the prompt's KV prefix
 is copied into the next decode slot.
+
+Speculative decoding: ``speculate`` takes a drafted tree of tokens per running sequence (from
+any draft: prompt lookup, extra heads, a smaller model), scores all of them in one forward and
+advances every sequence by the drafted tokens that stand and one more.
 """
 
 from __future__ import annotations
@@ -40,6 +44,7 @@ from .hostio import to_device
 from .kv_cache import PreallocatedKVCache
 from .linear import weights_epoch
 from .request import Sequence, Status
+from .speculative import MAX_NODES, verify
 
 
 class ModelRunner(abc.ABC):
@@ -120,6 +125,7 @@ class MultimodalRunner(ModelRunner):
         self._prefill_graphs: Dict[tuple, dict] = {}
         self._prefill_epoch = weights_epoch()
         self._graphs_sampled: Dict[int, tuple] = {}
+        self._spec_graphs: Dict[tuple, dict] = {}
         self._eager: Dict[int, dict] = {}
         self._dev_ids_for = None              # batch whose next ids already sit on device
         self._pinned_ids = torch.zeros(max_running + 1, dtype=torch.int64).pin_memory()
@@ -242,13 +248,14 @@ class MultimodalRunner(ModelRunner):
         weights they were captured with, so call this after replacing weight tensors (a
         GPTQ linear's release_f16 is noticed by itself: see _prefill_graphed)."""
         self._prefill_graphs.clear()
+        self._spec_graphs.clear()
 
     def _prefill_graphed(self, packed, pos, slots, seg_lens):
         key = tuple(int(L) for L in seg_lens)
         graphs = self._prefill_graphs
         epoch = weights_epoch()
         if epoch != self._prefill_epoch:         # a resident fp16 expansion was released
-            graphs.clear()
+            self.drop_prefill_graphs()
             self._prefill_epoch = epoch
         ent = graphs.pop(key, None)
         dev = self.device
@@ -426,6 +433,135 @@ class MultimodalRunner(ModelRunner):
                     self._decode_eager(seqs, n, greedy)
                 else:
                     self._decode_forward(seqs, n)
+
+    # ---- speculative decoding --------------------------------------------------------
+    # Steps run as HIP graphs (with use_graph) keyed by the number of sequences, the nodes of a
+    # tree and the kind of verification: up to this many are kept, each with its activations and
+    # logits (0 disables).
+    spec_graph_layouts = 4
+
+    @torch.inference_mode()
+    def speculate(self, seqs: List[Sequence], drafts, draft_logits=None) -> List[int]:
+        """Advance every running sequence by the drafted tokens that stand and one more.
+
+        ``drafts``: per sequence (in the order of ``seqs``) either a list of tokens to follow one
+        another, or (tokens, parents) with each token's parent in that list (-1: the sequence's
+        last token), parents first; at most 63.  ``draft_logits`` [n, D, V] on the device (logits'
+        type fp16, D = the most tokens of a draft): row j of a sequence the logits its token j was
+        drawn from, for chains alone; without them the tokens are proposals.  Greedy sequences
+        keep the tokens that decode() would have produced, sampled ones are distributed as its.
+        Returns the number of tokens each sequence has gained (a stop token or the length limit
+        ends a sequence early)."""
+        self.settle()
+        n = len(seqs)
+        if len(drafts) != n:
+            raise ValueError(f"{len(drafts)} drafts for {n} sequences")
+        if n == 0:
+            return []
+        order = sorted(range(n), key=lambda i: seqs[i].kv_handle["slot"])
+        if [seqs[i].kv_handle["slot"] for i in order] != list(range(n)):
+            raise AssertionError("speculate expects the running sequences in slots [0, n)")
+        trees = [self._draft_tree(drafts[i], draft_logits is not None) for i in order]
+        T = 1 + max(len(t) for t, _ in trees)
+        if T > MAX_NODES:
+            raise ValueError(f"a draft of {T - 1} tokens: at most {MAX_NODES - 1}")
+        vocab = self.adapter.model.cfg.vocab_size
+        if draft_logits is not None and tuple(draft_logits.shape) != (n, T - 1, vocab):
+            raise ValueError(f"draft_logits {tuple(draft_logits.shape)}: expected "
+                             f"{(n, T - 1, vocab)}")
+        ids, parents, counts, temps = [], [], [], []
+        for slot, i in enumerate(order):
+            tokens, ups = trees[slot]
+            if any(not 0 <= t < vocab for t in tokens):
+                raise ValueError(f"drafted tokens {tokens}: outside the vocabulary of {vocab}")
+            room = self._pool.max_len - self._kv_len[slot]
+            if room < 1:
+                raise RuntimeError(f"sequence in slot {slot} reached max_len={self._pool.max_len}")
+            pad = T - 1 - len(tokens)
+            # padding nodes are scored like others (no row of the forward is left undefined) and
+            # never stand: counts ends before them, and before nodes that the pool cannot hold
+            ids += [seqs[i].last_token_id()] + tokens + [0] * pad
+            parents += [-1] + [p + 1 for p in ups] + [0] * pad
+            counts.append(min(1 + len(tokens), room))
+            temps.append(float(seqs[i].request.sampling.temperature))
+        dev = self.device
+        host = to_device(ids + parents + counts, torch.int64, dev)
+        step = {"ids": host[:n * T].view(n, T),
+                "parents": host[n * T:2 * n * T].view(n, T).to(torch.int32),
+                "counts": host[2 * n * T:].to(torch.int32)}
+        if any(t != 0.0 for t in temps):
+            step["temps"] = to_device(temps, torch.float32, dev)
+            step["uniforms"] = torch.rand(n, T, device=dev)
+            if draft_logits is not None and T > 1:
+                step["draft"] = draft_logits.index_select(0, to_device(order, torch.int64, dev))
+        run = self._spec_graphed if self._use_graph and self.spec_graph_layouts else self._spec_step
+        v = run(step)
+        out = torch.cat([v.tokens, v.emitted.to(torch.int64).unsqueeze(1)], 1).tolist()
+        self._dev_ids_for = None
+        gained = [0] * n
+        for slot, i in enumerate(order):
+            seq, new = seqs[i], out[slot][:out[slot][T]]
+            self._kv_len[slot] += len(new)
+            for t in new:
+                if t < 0:
+                    raise RuntimeError(f"no token is left to draw for the sequence in slot {slot}")
+                seq.append_token(t)
+                gained[i] += 1
+                if seq.maybe_finish():
+                    break
+        return gained
+
+    @staticmethod
+    def _draft_tree(draft, chain: bool):
+        """(tokens, parents within them) of a draft."""
+        tokens, up = draft if isinstance(draft, tuple) else (draft, None)
+        tokens = [int(t) for t in tokens]
+        if up is None:
+            return tokens, list(range(-1, len(tokens) - 1))
+        up = [int(p) for p in up]
+        if len(up) != len(tokens) or any(not -1 <= p < i for i, p in enumerate(up)):
+            raise ValueError(f"parents {up} of {len(tokens)} drafted tokens: one each, before it")
+        if chain and up != list(range(-1, len(tokens) - 1)):
+            raise ValueError("draft_logits are for chains")
+        return tokens, up
+
+    def _spec_step(self, step: dict):
+        """The step on device tensors: forward over the trees, verification, acceptance."""
+        n, T = step["ids"].shape
+        emb = self.adapter.embed_tokens(step["ids"].reshape(-1)).unsqueeze(0)
+        cache = self._pool.tree_cache(step["parents"], rope_delta=self._rope_delta)
+        logits = self.adapter.llm(emb, cache.positions.view(3, 1, n * T), None, cache)[0]
+        tree = ({"draft_logits": step["draft"]} if "draft" in step
+                else {"parents": step["parents"]})
+        v = verify(logits.view(n, T, -1), step["ids"], step.get("uniforms"),
+                   step.get("temps", 0.0), counts=step["counts"], **tree)
+        cache.accept(v.path, v.emitted)
+        return v
+
+    def _spec_graphed(self, step: dict):
+        """_spec_step as a graph per layout: the first call runs eagerly and is captured after."""
+        epoch = weights_epoch()
+        if epoch != self._prefill_epoch:
+            self.drop_prefill_graphs()
+            self._prefill_epoch = epoch
+        key = (*step["ids"].shape, *sorted(step))
+        ent = self._spec_graphs.pop(key, None)
+        if ent is not None:
+            self._spec_graphs[key] = ent                          # most recently used last
+            for name, t in step.items():
+                ent["in"][name].copy_(t)
+            ent["graph"].replay()
+            return ent["out"]
+        with torch.inference_mode(False):
+            ent = {"in": {name: t.clone() for name, t in step.items()}}
+            v = self._spec_step(ent["in"])
+            ent["graph"] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(ent["graph"]):
+                ent["out"] = self._spec_step(ent["in"])
+        self._spec_graphs[key] = ent
+        while len(self._spec_graphs) > self.spec_graph_layouts:
+            self._spec_graphs.pop(next(iter(self._spec_graphs)))
+        return v
 
     # ---- decode paths ----------------------------------------------------------------
     def _load_ids(self, seqs, n, dst: torch.Tensor) -> None:

@@ -500,3 +500,147 @@ def test_step_in_graphs(gpu):
             for x, y in zip(res, want):
                 assert torch.equal(x, y), turn
             spec_step(pool, layers, *sets[turn % 2])
+
+
+# ----------------------------------------------------------------------------- the runner
+def corrupt(rng, tokens, vocab, rate):
+    return [rng.randrange(vocab) if rng.random() < rate else t for t in tokens]
+
+
+@pytest.mark.parametrize("quant,use_graph", [(None, False), (None, True), ("gptq", True)])
+def test_runner_speculates_greedily(gpu, quant, use_graph):
+    """Drafts taken from the decoded stream, some tokens replaced, as chains and as trees with
+    the right token on one branch: every emitted token the oracle's wherever it is decisive, more
+    than one a step, and decode() goes on from there."""
+    from omniserver_amd import synth
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    from omniserver_amd.runner import NativeQwenVLRunner
+    from tests.helpers import (check_stream, compare_logits, oracle_from_fp16, oracle_from_gptq,
+                               oracle_stream_logits, record_sampled_logits)
+    say(f"runner speculates quant={quant} use_graph={use_graph}")
+    shape = synth.DecoderShape()
+    gen = synth.gptq_decoder if quant else synth.fp16_decoder
+    w = gen(shape, seed=5, num_layers=2)
+    prompts = [synth.random_ids(L, shape.vocab_size, 5, f"p{L}").tolist() for L in (40, 17, 65)]
+    steps = 14
+
+    def start():
+        r = NativeQwenVLRunner(max_running=4, max_len=256, use_graph=use_graph, weights=w,
+                               quant=quant)
+        seen = record_sampled_logits(r)
+        seqs = [Sequence(Request(prompt=p, sampling=SamplingParams(max_new_tokens=steps)))
+                for p in prompts]
+        for s in seqs:
+            r.tokenize(s)
+        r.prefill(seqs)
+        return r, seqs, seen
+
+    plain, ref_seqs, seen = start()
+    while any(s.num_output_tokens < steps for s in ref_seqs):
+        plain.decode(ref_seqs)
+    streams = [list(s.output_token_ids) for s in ref_seqs]
+    runner, seqs, _ = start()
+    rng = random.Random(1)
+    gained = calls = 0
+    while min(s.num_output_tokens for s in seqs) < steps - 5:
+        drafts = []
+        for b, s in enumerate(seqs):
+            at = s.num_output_tokens
+            right = streams[b][at:at + 3] if s.output_token_ids == streams[b][:at] else [1, 2, 3]
+            if calls % 3 == 2:                       # two branches, the right one second
+                wrong = corrupt(rng, right, shape.vocab_size, 1.0)
+                drafts.append((wrong + right, [-1] + list(range(len(right) - 1))
+                               + [-1] + list(range(len(right), 2 * len(right) - 1))))
+            else:
+                drafts.append(corrupt(rng, right[:rng.randint(0, 3)], shape.vocab_size, 0.2))
+        before = [s.num_output_tokens for s in seqs]
+        got = runner.speculate(seqs, drafts)
+        assert got == [s.num_output_tokens - x for s, x in zip(seqs, before)]
+        assert runner.pool.lengths[:3].tolist() == runner._kv_len
+        gained += sum(got)
+        calls += 1
+    runner.decode(seqs)
+    orc = oracle_from_gptq(w, shape) if quant else oracle_from_fp16(w, shape)
+    rows = [oracle_stream_logits(orc, p, s.output_token_ids, 256) for p, s in zip(prompts, seqs)]
+    err, _ = compare_logits(seen[0], torch.stack([r[0] for r in rows]))
+    total = sum(check_stream(s.output_token_ids, r, 2 * err + 1e-3, 0, f"seq {b}")
+                for b, (s, r) in enumerate(zip(seqs, rows)))
+    assert total >= sum(s.num_output_tokens for s in seqs) // 2
+    say(f"  {gained} tokens in {calls} calls for 3 sequences")
+    assert gained > 1.5 * 3 * calls
+
+
+def test_runner_speculates_sampled(gpu):
+    """Sampled and greedy sequences, chains with draft logits and proposals without: graph and
+    eager steps give the same tokens for the same random numbers; a sequence given in another order
+    than its slot gets its own draft."""
+    from omniserver_amd import synth
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    from omniserver_amd.runner import NativeQwenVLRunner
+    say("runner speculates, sampled")
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=6, num_layers=2)
+    V = shape.vocab_size
+    results = []
+    for use_graph in (False, True):
+        r = NativeQwenVLRunner(max_running=4, max_len=128, use_graph=use_graph, weights=w)
+        seqs = [Sequence(Request(prompt=synth.random_ids(20 + b, V, 6, f"s{b}").tolist(),
+                                 sampling=SamplingParams(max_new_tokens=60, temperature=t)))
+                for b, t in enumerate((0.8, 0.0, 1.2))]
+        for s in seqs:
+            r.tokenize(s)
+        torch.manual_seed(9)
+        r.prefill(seqs)
+        g = torch.Generator().manual_seed(4)
+        shuffled = [seqs[2], seqs[0], seqs[1]]
+        for step in range(5):
+            draft = (torch.randn(3, 3, V, generator=g) * 2).half()
+            tokens = torch.multinomial(torch.softmax(draft.float(), -1).view(9, V), 1,
+                                       generator=g).view(3, 3).tolist()
+            r.speculate(shuffled, tokens, draft_logits=draft.to(gpu))
+            r.speculate(shuffled, [(t, [-1, -1, 0]) for t in tokens])
+        r.decode(seqs)
+        results.append([list(s.output_token_ids) for s in seqs])
+        assert r.pool.lengths[:3].tolist() == r._kv_len
+    assert results[0] == results[1]
+
+
+def test_runner_speculate_limits(gpu):
+    """The pool's end, the token limit and a stop token inside a draft; refusals."""
+    from omniserver_amd import synth
+    from omniserver_amd.request import Request, SamplingParams, Sequence, Status
+    from omniserver_amd.runner import NativeQwenVLRunner
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=7, num_layers=1)
+    r = NativeQwenVLRunner(max_running=2, max_len=48, use_graph=False, weights=w)
+    mk = lambda L, **kw: Sequence(Request(  # noqa: E731
+        prompt=synth.random_ids(L, shape.vocab_size, 7, f"l{L}").tolist(),
+        sampling=SamplingParams(**kw)))
+    a, b = mk(45, max_new_tokens=99), mk(9, max_new_tokens=3)
+    for s in (a, b):
+        r.tokenize(s)
+    r.prefill([a, b])
+    for bad in ([[1]], [[1], [2], [3]], [[1], [shape.vocab_size]], [[1], [-1]],
+                [[1] * 64, [1]], [([1, 2], [-1, 1]), [1]], [([1, 2], [-1]), [1]]):
+        with pytest.raises(ValueError):
+            r.speculate([a, b], bad)
+    with pytest.raises(ValueError):
+        r.speculate([a, b], [[1], [2]], draft_logits=torch.zeros(2, 2, shape.vocab_size))
+    with pytest.raises(AssertionError):
+        r.speculate([b], [[1]])
+    assert r.speculate([], []) == []
+    # greedy continuation of both, by decoding copies of them
+    twin = NativeQwenVLRunner(max_running=2, max_len=64, use_graph=False, weights=w)
+    ta, tb = mk(45, max_new_tokens=99), mk(9, max_new_tokens=99)
+    for s in (ta, tb):
+        twin.tokenize(s)
+    twin.prefill([ta, tb])
+    for _ in range(5):
+        twin.decode([ta, tb])
+    got = r.speculate([a, b], [ta.output_token_ids[1:6], tb.output_token_ids[1:6]])
+    assert got[0] <= 3 and r._kv_len[0] <= 48          # positions 45, 46, 47
+    assert b.num_output_tokens <= 3
+    if got == [3, 2]:                                   # no near tie on the way
+        assert b.status == Status.FINISHED
+        with pytest.raises(RuntimeError):
+            r.speculate([a, b], [[], []])
