@@ -378,24 +378,48 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
         o[d] = mfma32x32x16((half8_t){a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
                             p[t], o[d]);
       }
+    // V of the first 16 keys ahead, then each 16 keys' MFMAs beside the next 16's exponentials
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
+#pragma unroll
+    for (int t = 0; t < 2 * NB - 1; ++t)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
+      }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
   };
   char* gbuf = smem + grp * NBUF * 2 * TB;
-  auto dma_half = [&](int tb, char* dst, const half_t* src0, bool is_k) {
-    const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_offset(dst)) + rt * 1024;
-    const bool whole = tb + KT <= end;               // else the last key is repeated
-    const half_t* src = src0 + (int64_t)tb * tstride;
-#pragma unroll
-    for (int j = 0; j < NL / R; ++j) {
-      const int r0 = 4 * (rt + R * j), r = r0 + cr;
-      const int ch = is_k ? cc ^ (r & 15) : cc ^ ((r & 3) << 2);
-      const half_t* sp = whole ? src + (int64_t)r0 * tstride : src;
-      const int rr = whole ? cr : min(r, end - 1 - tb);
-      dma16(sp, (uint32_t)rr * (uint32_t)tstride * 2 + ch * 16, l0 + R * j * 1024);
-    }
-  };
+  // R > 1 stages straight to LDS, 1 KB (4 rows) per instruction, the swizzle in the source
+  // addresses: they are a lane's constant, for R = 2 but for one bit, off uniform bases.
+  const uint32_t kv_row = (uint32_t)tstride * 2;
+  const uint32_t koffs = cr * kv_row + ((cc ^ (4 * rt + cr)) << 4);
+  const uint32_t voffs = cr * kv_row + ((cc ^ (cr << 2)) << 4);
   auto dma_tile = [&](int tb, char* kt) {
-    dma_half(tb, kt, kb0, true);
-    dma_half(tb, kt + TB, vb0, false);
+    const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_offset(kt)) + rt * 1024;
+    if (tb + KT <= end) {
+      const int64_t first = (int64_t)(tb + 4 * rt) * kv_row;
+      const char* kp = (const char*)kb0 + first;
+      const char* vp = (const char*)vb0 + first;
+#pragma unroll
+      for (int j = 0; j < NL / R; ++j) {
+        const uint32_t flip = (4 * R * j & 15) << 4;     // of the rows' swizzle
+        dma16(kp + (int64_t)(4 * R * j) * kv_row, koffs ^ flip, l0 + R * j * 1024);
+        dma16(vp + (int64_t)(4 * R * j) * kv_row, voffs, l0 + TB + R * j * 1024);
+      }
+    } else {                                             // past the end: the last key again
+      const char* kp = (const char*)kb0 + (int64_t)tb * kv_row;
+      const char* vp = (const char*)vb0 + (int64_t)tb * kv_row;
+#pragma unroll
+      for (int j = 0; j < NL / R; ++j) {
+        const int r = 4 * (rt + R * j) + cr;
+        const uint32_t at = (uint32_t)min(r, end - 1 - tb) * kv_row;
+        dma16(kp, at + ((cc ^ (r & 15)) << 4), l0 + R * j * 1024);
+        dma16(vp, at + ((cc ^ ((r & 3) << 2)) << 4), l0 + TB + R * j * 1024);
+      }
+    }
   };
   if (nt > 0) {
     if constexpr (R > 1) dma_tile(tbeg * KT, gbuf);
