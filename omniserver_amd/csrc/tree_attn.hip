@@ -178,6 +178,7 @@ struct TreeArgs {
   const half_t* k_cache;
   const half_t* v_cache;
   int max_len, nkv, G, T, n;
+  unsigned magic;              // row / G = high word of row * magic (G > 1)
   int ncols, rblocks;          // columns of the schedule, row blocks (workgroups) of each
   const uint64_t* ancestors;   // [n][T]
   const int* seqs;
@@ -261,11 +262,16 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   const int rb = y % a.rblocks;
   const int col = (y / a.rblocks) * 8 + (blockIdx.x & 7);
   if (col >= a.ncols) return;
-  const i32x4 c0 = *(const i32x4*)(a.columns + 8 * col), c1 = *(const i32x4*)(a.columns + 8 * col + 4);
-  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  int s = uniform(c0[0]), g = uniform(c0[1]), u0 = uniform(c0[2]), left = uniform(c0[3]);
-  int L = uniform(c1[0]), used = uniform(c1[1]), slot = uniform(c1[2]);
+  // through the scalar cache: the plan wrote it in an earlier launch
+  typedef const __attribute__((address_space(4))) int plan_int;
+  const plan_int* column = (const plan_int*)a.columns + 8 * col;
+  const plan_int* seqs = (const plan_int*)a.seqs;
+  int s = column[0], g = column[1], u0 = column[2], left = column[3];
+  int L = column[4], used = column[5], slot = column[6];
   constexpr int UNIT = S * KT;
+  const int cr = lane >> 4, cc = lane & 15;
+  const int64_t tstride = (int64_t)a.nkv * TREE_HD;  // halfs per token
+  const uint32_t kv_row = (uint32_t)tstride * 2;     // bytes
   for (int part = 0; left > 0; part = 1) {
   const int end = min(L + used, a.max_len);
   const int ntiles = ceil_div(end, KT), units = ceil_div(end, UNIT);
@@ -273,39 +279,32 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   const bool whole = u0 == 0 && steps == units;
   const int nrows = used * a.G - 32 * R * rb;        // this block's
   if (nrows > 0) {
-  const uint64_t word = lane < a.T ? a.ancestors[(int64_t)s * a.T + lane] : 0;
-  const int row = min(32 * rt + l32, nrows - 1);
-  const int node = (32 * R * rb + row) / a.G;
-  const int u = 32 * R * rb + row - node * a.G;
-  const int64_t tok = (int64_t)s * a.T + node;
-  uint64_t mask = (uint64_t)(uint32_t)__shfl((int)(word & 0xffffffffu), node) |
-                  ((uint64_t)(uint32_t)__shfl((int)(word >> 32), node) << 32);
-  if (end - L < 64) mask &= (1ull << (end - L)) - 1;   // nodes behind the pool's end
-  const bool rows_here = 32 * rt < nrows;
-
-  half8_t qf[8];
-  {
-    const half_t* qp = a.q + tok * a.q_stride + (int64_t)(g * a.G + u) * TREE_HD + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qf[ks] = *(const half8_t*)(qp + 16 * ks);
-  }
-
   const int tbeg = u0 * S + grp * steps;
   const int nt = min(steps, ntiles - tbeg);          // may be <= 0
-
-  const int cr = lane >> 4, cc = lane & 15;
-  const int64_t tstride = (int64_t)a.nkv * TREE_HD;  // halfs per token
   const int64_t base = (int64_t)slot * a.max_len * tstride + g * TREE_HD;
   const half_t* kb0 = a.k_cache + base;
   const half_t* vb0 = a.v_cache + base;
+
+  // R = 1 stages through registers (its one buffer is free only once the tile is used): chunk
+  // lane + 64 j of a tile is row cr + 4 j, 16-byte chunk cc.
   half8_t kr[NL], vr[NL];
-  auto load_tile = [&](int tb) {                     // past the end: the last key again
-    const int64_t last = end - 1;
+  auto load_tile = [&](int tb) {
+    const char* kp = (const char*)kb0 + (int64_t)tb * kv_row;
+    const char* vp = (const char*)vb0 + (int64_t)tb * kv_row;
+    if (tb + KT <= end) {
+      const uint32_t at = cr * kv_row + cc * 16;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int64_t t = min((int64_t)tb + cr + 4 * j, last);
-      kr[j] = *(const half8_t*)(kb0 + t * tstride + cc * 8);
-      vr[j] = *(const half8_t*)(vb0 + t * tstride + cc * 8);
+      for (int j = 0; j < NL; ++j) {
+        kr[j] = *(const half8_t*)(kp + 4 * j * (int64_t)kv_row + at);
+        vr[j] = *(const half8_t*)(vp + 4 * j * (int64_t)kv_row + at);
+      }
+    } else {                                         // past the end: the last key again
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const uint32_t at = (uint32_t)min(cr + 4 * j, end - 1 - tb) * kv_row + cc * 16;
+        kr[j] = *(const half8_t*)(kp + at);
+        vr[j] = *(const half8_t*)(vp + at);
+      }
     }
   };
   auto store_tile = [&](char* kt) {
@@ -317,6 +316,55 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
       *(half8_t*)(vt + r * 256 + ((cc << 4) ^ ((r & 3) << 6))) = vr[j];
     }
   };
+
+  char* gbuf = smem + grp * NBUF * 2 * TB;
+  // R > 1 stages straight to LDS, 1 KB (4 rows) per instruction, the swizzle in the source
+  // addresses: they are a lane's constant, for R = 2 but for one bit, off uniform bases.
+  const uint32_t koffs = cr * kv_row + ((cc ^ (4 * rt + cr)) << 4);
+  const uint32_t voffs = cr * kv_row + ((cc ^ (cr << 2)) << 4);
+  auto dma_tile = [&](int tb, char* kt) {
+    const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_offset(kt)) + rt * 1024;
+    if (tb + KT <= end) {
+      const int64_t first = (int64_t)(tb + 4 * rt) * kv_row;
+      const char* kp = (const char*)kb0 + first;
+      const char* vp = (const char*)vb0 + first;
+#pragma unroll
+      for (int j = 0; j < NL / R; ++j) {
+        const uint32_t flip = (4 * R * j & 15) << 4;     // of the rows' swizzle
+        dma16(kp + (int64_t)(4 * R * j) * kv_row, koffs ^ flip, l0 + R * j * 1024);
+        dma16(vp + (int64_t)(4 * R * j) * kv_row, voffs, l0 + TB + R * j * 1024);
+      }
+    } else {                                             // past the end: the last key again
+      const char* kp = (const char*)kb0 + (int64_t)tb * kv_row;
+      const char* vp = (const char*)vb0 + (int64_t)tb * kv_row;
+#pragma unroll
+      for (int j = 0; j < NL / R; ++j) {
+        const int r = 4 * (rt + R * j) + cr;
+        const uint32_t at = (uint32_t)min(r, end - 1 - tb) * kv_row;
+        dma16(kp, at + ((cc ^ (r & 15)) << 4), l0 + R * j * 1024);
+        dma16(vp, at + ((cc ^ ((r & 3) << 2)) << 4), l0 + TB + R * j * 1024);
+      }
+    }
+  };
+  // the first tile's transfers go out before anything else is asked for
+  if (nt > 0) {
+    if constexpr (R > 1) dma_tile(tbeg * KT, gbuf);
+    else load_tile(tbeg * KT);
+  }
+
+  const int row = min(32 * rt + l32, nrows - 1);
+  const int node = a.G == 1 ? 32 * R * rb + row : (int)__umulhi(32 * R * rb + row, a.magic);
+  const int u = 32 * R * rb + row - node * a.G;
+  const int64_t tok = (int64_t)s * a.T + node;
+  const bool rows_here = 32 * rt < nrows;
+  uint64_t mask = a.ancestors[tok];
+  half8_t qf[8];
+  {
+    const half_t* qp = a.q + tok * a.q_stride + (int64_t)(g * a.G + u) * TREE_HD + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = *(const half8_t*)(qp + 16 * ks);
+  }
+  if (end - L < 64) mask &= (1ull << (end - L)) - 1;   // nodes behind the pool's end
 
   float m_run = -INFINITY, l_run = 0.f;
   f32x16 o[4];
@@ -391,40 +439,6 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
       }
     __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
   };
-  char* gbuf = smem + grp * NBUF * 2 * TB;
-  // R > 1 stages straight to LDS, 1 KB (4 rows) per instruction, the swizzle in the source
-  // addresses: they are a lane's constant, for R = 2 but for one bit, off uniform bases.
-  const uint32_t kv_row = (uint32_t)tstride * 2;
-  const uint32_t koffs = cr * kv_row + ((cc ^ (4 * rt + cr)) << 4);
-  const uint32_t voffs = cr * kv_row + ((cc ^ (cr << 2)) << 4);
-  auto dma_tile = [&](int tb, char* kt) {
-    const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds_offset(kt)) + rt * 1024;
-    if (tb + KT <= end) {
-      const int64_t first = (int64_t)(tb + 4 * rt) * kv_row;
-      const char* kp = (const char*)kb0 + first;
-      const char* vp = (const char*)vb0 + first;
-#pragma unroll
-      for (int j = 0; j < NL / R; ++j) {
-        const uint32_t flip = (4 * R * j & 15) << 4;     // of the rows' swizzle
-        dma16(kp + (int64_t)(4 * R * j) * kv_row, koffs ^ flip, l0 + R * j * 1024);
-        dma16(vp + (int64_t)(4 * R * j) * kv_row, voffs, l0 + TB + R * j * 1024);
-      }
-    } else {                                             // past the end: the last key again
-      const char* kp = (const char*)kb0 + (int64_t)tb * kv_row;
-      const char* vp = (const char*)vb0 + (int64_t)tb * kv_row;
-#pragma unroll
-      for (int j = 0; j < NL / R; ++j) {
-        const int r = 4 * (rt + R * j) + cr;
-        const uint32_t at = (uint32_t)min(r, end - 1 - tb) * kv_row;
-        dma16(kp, at + ((cc ^ (r & 15)) << 4), l0 + R * j * 1024);
-        dma16(vp, at + ((cc ^ ((r & 3) << 2)) << 4), l0 + TB + R * j * 1024);
-      }
-    }
-  };
-  if (nt > 0) {
-    if constexpr (R > 1) dma_tile(tbeg * KT, gbuf);
-    else load_tile(tbeg * KT);
-  }
   // Q has landed: without this the compiler counts the Q loads as outstanding inside the loop
   // and makes every tile's first MFMAs wait for the transfers just requested
   __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -543,10 +557,10 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   u0 = 0;
   if (left > 0 && ++g == a.nkv) {
     g = 0;
-    while (++s < a.n - 1 && uniform(a.seqs[4 * s + 2]) == 0) {}
-    L = uniform(a.seqs[4 * s]);
-    used = uniform(a.seqs[4 * s + 1]);
-    slot = uniform(a.seqs[4 * s + 3]);
+    while (++s < a.n - 1 && seqs[4 * s + 2] == 0) {}
+    L = seqs[4 * s];
+    used = seqs[4 * s + 1];
+    slot = seqs[4 * s + 3];
   }
   }
 }
@@ -715,6 +729,7 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
     return OMNI_EINVAL;
   TreeArgs a;
   a.G = n_heads / n_kv_heads;
+  a.magic = 0xffffffffu / a.G + 1;                     // exact for rows below 2^32 / G
   const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
   const int64_t grid = (columns + 7) / 8 * 8 * rblocks, out_rows = (int64_t)n * n_nodes * n_heads;
   if (grid > 0x7fffffff || out_rows > 0x7fffffff) return OMNI_EUNSUPPORTED;

@@ -101,6 +101,80 @@ def test_tree_attention(gpu, n, T, nh, nkv, span, kind, ragged):
     assert torch.equal(out, again)
 
 
+CUT = [
+    # n, T, nh, nkv, starts, capacity, the plan's (rows, groups, least)
+    (1, 8, 12, 2, (3000, 3000), 4096, (64, 4, 1)),
+    (5, 10, 12, 2, (0, 1700), 2048, (64, 4, 1)),
+    (70, 3, 8, 1, (0, 150), 1600, (32, 8, 1)),        # more sequences than lanes
+    (33, 2, 12, 2, (0, 300), 4096, (32, 8, 1)),
+    (9, 40, 12, 2, (0, 900), 8192, (128, 2, 1)),
+    (2, 64, 28, 4, (1200, 1800), 16384, (128, 2, 1)),
+    (3, 64, 64, 1, (0, 200), 2000, (128, 2, 1)),      # 32 row blocks
+    (1, 64, 64, 1, (500, 500), 1024, (32, 8, 0)),     # 128 row blocks, enough to leave uncut
+]
+
+
+@pytest.mark.parametrize("n,T,nh,nkv,span,capacity,form", CUT)
+def test_tree_attention_cut(gpu, n, T, nh, nkv, span, capacity, form):
+    """Long pools, where the keys of all sequences are cut evenly over the workgroups: very
+    different contexts, sequences without nodes, rows outside the pool, every cut merged."""
+    say(f"tree attention cut: n={n} T={T} heads {nh}/{nkv} starts {span} capacity {capacity}")
+    rng = random.Random(n * 100 + T)
+    starts = [rng.randint(*span) for _ in range(n)]
+    counts = [rng.randint(0, T) if n > 2 else T for _ in range(n)]
+    parents = trees(rng, n, T, "tree")
+    pool, g = make_pool(gpu, 1, n, nh, nkv, 16, T)
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    pool = PreallocatedKVCache(1, n, nkv, capacity, HD, gpu, n_heads=nh)
+    most = max(starts) + T
+    pool.storage[:, :, :, :most].copy_(torch.randn(1, 2, n, most, nkv, HD, generator=g).half())
+    slots = rng.sample(range(n), n)
+    pool.lengths[torch.tensor(slots, device=gpu)] = torch.tensor(starts, device=gpu)
+    given = torch.tensor(slots, device=gpu)
+    if n > 8:
+        given[4], given[n - 1] = -1, n + 7
+        counts[4] = counts[n - 1] = 0
+    q = torch.randn(n * T, nh * HD, generator=g).half()
+    used = i32([max(c, 1) if s in (4, n - 1) else c for s, c in enumerate(counts)], gpu)
+    cache = pool.tree_cache(parents, counts=used, slots=given)
+    assert (*cache.form[:2], cache.form[3]) == form
+    for _ in range(2):
+        out = torch.full((n * T, nh, HD), 7.0, device=gpu, dtype=torch.float16)
+        cache.attend_qkv(q.to(gpu), 0, HD ** -0.5, out)
+        if n > 8:
+            check = [0 if s in (4, n - 1) else c for s, c in enumerate(counts)]
+        else:
+            check = counts
+        check_attention(out.view(n, T, nh, HD), q.view(n, T, nh, HD), pool, 0, starts, parents,
+                        check, slots, 7.0)
+
+
+def test_tree_attention_cut_keeps_infinities_apart(gpu):
+    """As test_tree_attention_nodes_keep_to_themselves, where the rows' states are merged."""
+    T, start = 30, 1500
+    rng = random.Random(3)
+    parents = trees(rng, 2, T, "tree")
+    pool, g = make_pool(gpu, 1, 2, 12, 2, 2048, 5)
+    pool.lengths.copy_(torch.tensor([start, 40]))
+    clean = set(ref.lineage(parents[0], T - 1))
+    for j in range(T):
+        if j not in clean:
+            pool.v[0][0, start + j] = math.inf if j % 2 else math.nan
+            pool.k[0][0, start + j] = math.nan
+    q = torch.randn(2 * T, 12 * HD, generator=g).half()
+    cache = pool.tree_cache(parents)
+    assert cache.form[3] == 1
+    out = torch.zeros(2 * T, 12, HD, device=gpu, dtype=torch.float16)
+    cache.attend_qkv(q.to(gpu), 0, HD ** -0.5, out)
+    rows = [i for i in range(T) if set(ref.lineage(parents[0], i)) <= clean]
+    want, mag, seen = ref.tree_attention(q.view(2, T, 12, HD), pool.k[0].cpu(), pool.v[0].cpu(),
+                                         [start, 40], parents, [T, T], [0, 1], HD ** -0.5)
+    v = pool.v[0].cpu().float()
+    bound = ref.attention_bound(want, mag, seen, v[v.isfinite()].abs().max().item())
+    err = (out.view(2, T, 12, HD).cpu().double() - want).abs() / bound
+    assert len(rows) > 3 and err[0, rows].max().item() <= 1.0 and err[1].max().item() <= 1.0
+
+
 def test_tree_plan(gpu):
     """Ancestors, positions and where the K/V goes; bad parents are roots, rows outside the pool
     and nodes past it go nowhere."""

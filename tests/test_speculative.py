@@ -125,6 +125,24 @@ def test_tree_cache_refusals():
         p.tree_cache(ok)
 
 
+def test_tree_plan_rule():
+    """What the attention's plan asks for is what the C entry points take, at any size."""
+    from omniserver_amd.kv_cache import tree_plan
+    for n in (1, 2, 3, 7, 32, 100, 1000):
+        for T in (1, 2, 8, 17, 64):
+            for nh, nkv in ((12, 2), (28, 4), (16, 16), (64, 1), (8, 8)):
+                for capacity in (64, 512, 513, 1536, 1537, 4096, 131072):
+                    rows, groups, columns, least = tree_plan(n, T, nh, nkv, capacity, 256)
+                    assert (rows, groups) in ((32, 8), (64, 4), (128, 2))
+                    if least == 0:
+                        assert columns == n * nkv
+                        continue
+                    blocks = -(-T * (nh // nkv) // rows)
+                    assert 1 <= columns <= 256 and (blocks > 32 or columns * blocks <= 256)
+                    assert columns <= n * nkv or columns % (n * nkv) == 0 \
+                        or columns == n * nkv * -(-capacity // (256 if groups == 8 else 128))
+
+
 def test_verify_refusals():
     from omniserver_amd.speculative import verify
     L, tok, u = torch.zeros(2, 4, 9), torch.zeros(2, 4, dtype=torch.int64), torch.rand(2, 4)
