@@ -58,19 +58,29 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | 
 
     A NaN logit counts as -inf; where no token is above -inf the next token is -1.  All weights and
     sums are 64-bit, in a fixed order: the same inputs give the same tokens."""
-    if logits.dim() != 3:
-        raise ValueError(f"logits of shape {tuple(logits.shape)}: expected [n, nodes, vocab]")
+    checked = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
     n, T, V = logits.shape
-    out = tokens.new_empty(n, T)
-    path = torch.empty(n, T, device=tokens.device, dtype=torch.int32)
-    emitted = torch.empty(n, device=tokens.device, dtype=torch.int32)
-    return verify_out(logits, tokens, uniforms, temperature, Verified(path, out, emitted),
-                      parents, draft_logits, counts)
+    dev = logits.device
+    out = Verified(torch.empty(n, T, device=dev, dtype=torch.int32),
+                   torch.empty(n, T, device=dev, dtype=torch.int64),
+                   torch.empty(n, device=dev, dtype=torch.int32))
+    return _launch(logits, tokens, uniforms, temperature, out, parents, counts, *checked)
 
 
 def verify_out(logits, tokens, uniforms, temperature, out: Verified, parents=None,
                draft_logits=None, counts=None) -> Verified:
     """verify into the caller's tensors."""
+    checked = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
+    n, T, V = logits.shape
+    _is(out.path, (n, T), torch.int32, "path")
+    _is(out.tokens, (n, T), torch.int64, "out tokens")
+    _is(out.emitted, (n,), torch.int32, "emitted")
+    require_here(*out)
+    return _launch(logits, tokens, uniforms, temperature, out, parents, counts, *checked)
+
+
+def _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts) -> tuple:
+    """Refuse what the kernels do not take; (draft logits or None, doubles of workspace)."""
     if logits.dim() != 3:
         raise ValueError(f"logits of shape {tuple(logits.shape)}: expected [n, nodes, vocab]")
     n, T, V = logits.shape
@@ -88,8 +98,6 @@ def verify_out(logits, tokens, uniforms, temperature, out: Verified, parents=Non
                              f"expected [{n}, {T - 1}, {V}] {logits.dtype}")
         if draft_logits.stride(2) != 1 and V > 1:
             raise ValueError("the draft logits' columns have to be contiguous")
-        if T == 1:
-            draft_logits = None
     per_row = isinstance(temperature, torch.Tensor)
     if not per_row and not 0.0 <= float(temperature) < float("inf"):
         raise ValueError(f"temperature {temperature}: zero or above, finite")
@@ -99,22 +107,29 @@ def verify_out(logits, tokens, uniforms, temperature, out: Verified, parents=Non
     _is(uniforms, (n, T), torch.float32, "uniforms")
     _is(parents, (n, T), torch.int32, "parents")
     _is(counts, (n,), torch.int32, "counts")
-    _is(temperature if per_row else None, (n,), torch.float32, "temperature")
-    _is(out.path, (n, T), torch.int32, "path")
-    _is(out.tokens, (n, T), torch.int64, "out tokens")
-    _is(out.emitted, (n,), torch.int32, "emitted")
-    require_here(logits, draft_logits, tokens, uniforms, parents, counts, *out,
-                 temperature if per_row else None)
+    if per_row:
+        _is(temperature, (n,), torch.float32, "temperature")
+        require_here(temperature)
+    require_here(logits, draft_logits, tokens, uniforms, parents, counts)
+    if T == 1:
+        draft_logits = None
     work = lib().omni_spec_verify_work(n, T, V, int(draft_logits is not None))
     if work < 0:
         raise ValueError(f"{n} sequences of {T} nodes over a vocabulary of {V}: too large")
+    return draft_logits, work
+
+
+def _launch(logits, tokens, uniforms, temperature, out, parents, counts, draft, work) -> Verified:
+    n, T, V = logits.shape
     ws = torch.empty(work, device=logits.device, dtype=torch.float64)
-    ds = (0, 0) if draft_logits is None else draft_logits.stride()[:2]
-    call("omni_spec_verify", ptr(logits), _DTYPES[logits.dtype], logits.stride(0),
-         logits.stride(1), ptr(draft_logits), *ds, ptr(tokens), ptr(parents), ptr(counts),
-         ptr(uniforms), ptr(temperature) if per_row else None,
-         0.0 if per_row else float(temperature), n, T, V, ptr(out.path), ptr(out.tokens),
-         ptr(out.emitted), ptr(ws), work, stream())
+    per_row = isinstance(temperature, torch.Tensor)
+    s0, s1, _ = logits.stride()
+    d0, d1, _ = (0, 0, 1) if draft is None else draft.stride()
+    call("omni_spec_verify", logits.data_ptr(), _DTYPES[logits.dtype], s0, s1, ptr(draft), d0, d1,
+         tokens.data_ptr(), ptr(parents), ptr(counts), ptr(uniforms),
+         temperature.data_ptr() if per_row else None, 0.0 if per_row else float(temperature), n, T,
+         V, out.path.data_ptr(), out.tokens.data_ptr(), out.emitted.data_ptr(), ws.data_ptr(), work,
+         stream())
     return out
 
 
@@ -123,5 +138,5 @@ def _is(t, shape, dtype, name: str) -> None:
         return
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} of shape {tuple(t.shape)}: expected a contiguous {list(shape)}")

@@ -378,7 +378,8 @@ def test_verify(gpu, n, T, V, dtype, mode):
     say(f"  emitted {total.tolist()}")
 
 
-def test_verify_borders(gpu):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_verify_borders(gpu, dtype):
     """Random numbers 0 and just below 1, tokens proposed twice or outside the vocabulary, masked
     rows, NaN and infinities, nothing left to draw from."""
     g = torch.Generator().manual_seed(3)
@@ -414,12 +415,37 @@ def test_verify_borders(gpu):
                 for u1 in (0.0, 0.5, below):
                     case(row, [0, 17, 17, 30, 5, -1], [u0] + [u1] * 5, temp)
                     case(row, [0, V, 5, 0, 3, 17], [u0] + [u1] * 5, temp)
-    logits = torch.stack(rows)
+    logits = torch.stack(rows).to(dtype)
     check_verify(gpu, logits, toks, us, temps, parents=pars)
     # chains against their own distribution, another one, a masked one and an empty one
-    draft = torch.stack([(base, two, only, none, nan, inf)[k % 6][:T - 1] for k in range(len(rows))])
+    draft = torch.stack([(base, two, only, none, nan, inf)[k % 6][:T - 1] for k in range(len(rows))]).to(dtype)
     check_verify(gpu, logits, toks, us, temps, draft=draft)
     check_verify(gpu, logits, toks, us, temps, draft=logits[:, :T - 1].contiguous())
+
+
+def test_verify_open_tests(gpu):
+    """Random numbers on the border of a test, where the rows' 32-bit sums leave it open: the 64-bit
+    sum decides, as the oracle does, for trees and chains, at the first node and further down."""
+    g = torch.Generator().manual_seed(12)
+    n, T, V = 48, 4, 9001
+    logits = rows_like_a_model(g, n, T, V, torch.float16)
+    draft = (logits[:, :T - 1].float() + 0.3 * torch.randn(n, T - 1, V, generator=g)).half()
+    tokens = logits.float().argmax(-1).roll(1, 1)
+    p = torch.softmax(logits.double(), -1)
+    q = torch.softmax(draft.double(), -1)
+    at = tokens[:, 1:, None]
+    px, qx = p[:, :-1].gather(2, at)[..., 0], q.gather(2, at)[..., 0]
+    for d, parents in ((None, [[-1, 0, 1, 2]] * n), (draft, None)):
+        border = px / (1.0 if d is None else qx)
+        u = torch.rand(n, T, generator=g)
+        for k in range(1, T):
+            # on one node a sequence the nearest fp32 number to the border, or its neighbours
+            u[:, 1:] = torch.where(torch.arange(1, T) < k, torch.zeros(()), u[:, 1:])
+            near = border[:, k - 1].float().clamp(max=1 - 2.0 ** -24)
+            step = torch.tensor([-1, 0, 1])[torch.arange(n) % 3]
+            u[:, k] = torch.where(step == 0, near, torch.nextafter(near, near + step.float()))
+            u[:, k].clamp_(0, 1 - 2.0 ** -24)
+            check_verify(gpu, logits, tokens, u, [1.0] * n, parents=parents, draft=d)
 
 
 def test_verify_scalars_strides_and_repeats(gpu):
