@@ -156,7 +156,7 @@ int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v, int64_t v
  * [3][n * n_nodes] (starts + depth + rope_delta), token_slot / token_pos int64 [n * n_nodes] (where
  * the nodes' K/V goes; token_slot -1: nowhere), and schedule (int32, 16-byte aligned, 4 n + 8
  * columns + 2 n n_kv_heads of them) for omni_tree_attention with the same n_kv_heads, (rows,
- * groups), columns and least: the keys of all sequences and KV heads in equal stretches for that
+ * groups), columns and least: the keys of all sequences and KV heads in equal pieces for that
  * many columns of workgroups, none shorter than least steps of a workgroup; least 0: no cuts,
  * columns = n n_kv_heads. */
 int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,

@@ -17,10 +17,13 @@
 // A node whose parent does not precede it is a root of its own.
 //
 // And the attention's schedule.  A sequence's keys count in units of `unit` (what a workgroup takes
-// in a step), once per KV head; the units of all (sequence, KV head) items stand in one line,
-// which is cut into equal stretches, one per column of workgroups.  So a batch of one long and many
-// short contexts loads the workgroups as evenly as one of equal contexts, whatever the lengths
-// on the device are.  A stretch is at least `least` units; least 0: a column for each item.
+// in a step), once per KV head.  Where the (sequence, KV head) items are of about one length, the
+// longest within a fifth of the mean, each is cut into as many equal pieces as there are columns of
+// workgroups for it.  Otherwise the units of all items stand in one line that is cut into equal
+// stretches, so that one long and many short contexts load the workgroups evenly, whatever the
+// lengths on the device are; a stretch that runs over an item's end costs its workgroup another
+// start and merge, some 4 us, which the even case is spared.  A piece is at least `least` units;
+// least 0: a column for each item.
 //   seqs[s]     (prefix length, nodes in use, units, pool row)
 //   columns[c]  (s, g, first unit there, units in all, then of s: length, nodes, pool row)
 //   heads[s][g] (first column | 1 << 30 where the item is not the first that column sees, last)
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   const int64_t delta = row_ok && rope_delta ? rope_delta[slot] : 0;
 
   // units of the sequences before this one, its own, and all
-  int before = 0, all = 0, units = 0;
+  int before = 0, all = 0, units = 0, longest = 0;
   for (int r0 = 0; r0 < n; r0 += 64) {
     const int r = r0 + i;
     int w = 0;
@@ -66,53 +69,69 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
       if (m && row >= 0 && row < pool_rows) w = ceil_div(min(prefix(r) + m, max_len), tc.unit);
       if (r == s) units = w;
     }
-    int lo = r < s ? w : 0;
+    int lo = r < s ? w : 0, hi = w;
     for (int o = 32; o; o >>= 1) {
       w += __shfl_xor(w, o);
       lo += __shfl_xor(lo, o);
+      hi = max(hi, __shfl_xor(hi, o));
     }
+    longest = max(longest, hi);
     all += w;
     before += lo;
   }
   units = __shfl(units, s & 63);
   all *= tc.nkv;
   before *= tc.nkv;
-  // column c starts at unit c all / cols (in two parts: all < 2^30, cols < 2^15)
-  const unsigned cols = tc.least ? min(tc.ncols, max(1, all / tc.least)) : tc.ncols;
-  const unsigned per = (unsigned)all / cols, over = (unsigned)all - per * cols;
-  auto cut = [&](unsigned c) { return (int)(c * per + c * over / cols); };
-  for (int c = i; c < tc.ncols; c += 64) {
+  const int items = n * tc.nkv;
+  auto column = [&](int c, int g, int first, int count) {
     int* col = tc.columns + 8 * c;
-    if (tc.least) {
+    *(i32x4*)col = (i32x4){s, g, first, count};
+    *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
+  };
+  if (!tc.least || (items <= tc.ncols && (int64_t)longest * items * 5 <= (int64_t)all * 6)) {
+    const int each = tc.ncols / items;
+    const int pieces = tc.least ? min(each, max(1, units / tc.least)) : 1;
+    for (int k = i; k < tc.nkv * each; k += 64) {
+      const int g = k / each, j = k - g * each;
+      const int lo = j < pieces ? j * units / pieces : 0, hi = j < pieces ? (j + 1) * units / pieces : 0;
+      column((s * tc.nkv + g) * each + j, g, lo, hi - lo);
+    }
+    for (int c = items * each + i; c < tc.ncols && s == 0; c += 64) column(c, 0, 0, 0);
+    for (int g = i; g < tc.nkv; g += 64) {
+      const int c = (s * tc.nkv + g) * each;
+      *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) = make_int2(c, c + pieces - 1);
+    }
+  } else {
+    // column c starts at unit c all / cols (in two parts: all < 2^30, cols < 2^15)
+    const unsigned cols = min(tc.ncols, max(1, all / tc.least));
+    const unsigned per = (unsigned)all / cols, over = (unsigned)all - per * cols;
+    auto cut = [&](unsigned c) { return (int)(c * per + c * over / cols); };
+    for (int c = i; c < tc.ncols; c += 64) {
       const int lo = c < cols ? cut(c) : all, cnt = c < cols ? cut(c + 1) - lo : 0;
       if (cnt > 0 && lo >= before && lo < before + units * tc.nkv) {
         const int g = (lo - before) / units;
-        *(i32x4*)col = (i32x4){s, g, lo - before - g * units, cnt};
-        *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
+        column(c, g, lo - before - g * units, cnt);
       } else if (cnt <= 0 && s == 0) {
-        *(i32x4*)col = (i32x4){0, 0, 0, 0};
+        column(c, 0, 0, 0);
       }
-    } else if (c / tc.nkv == s) {
-      *(i32x4*)col = (i32x4){s, c % tc.nkv, 0, units};
-      *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
     }
-  }
-  for (int g = i; g < tc.nkv; g += 64) {
-    int2 at = make_int2(0, 0);
-    if (units && tc.least) {
-      const int lo = before + g * units, hi = lo + units - 1;
-      // the last column that starts at or before a unit: a guess and its neighbours
-      auto column = [&](int x) {
-        unsigned c = min(cols - 1, (unsigned)((float)x * (float)cols / (float)all));
-        while (c + 1 < cols && cut(c + 1) <= x) ++c;
-        while (cut(c) > x) --c;
-        return (int)c;
-      };
-      at.x = column(lo);
-      at.y = column(hi);
-      if (cut(at.x) < lo) at.x |= 1 << 30;
+    for (int g = i; g < tc.nkv; g += 64) {
+      int2 at = make_int2(0, 0);
+      if (units) {
+        const int lo = before + g * units, hi = lo + units - 1;
+        // the last column that starts at or before a unit: a guess and its neighbours
+        auto column_of = [&](int x) {
+          unsigned c = min(cols - 1, (unsigned)((float)x * (float)cols / (float)all));
+          while (c + 1 < cols && cut(c + 1) <= x) ++c;
+          while (cut(c) > x) --c;
+          return (int)c;
+        };
+        at.x = column_of(lo);
+        at.y = column_of(hi);
+        if (cut(at.x) < lo) at.x |= 1 << 30;
+      }
+      *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) = at;
     }
-    *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) = at;
   }
   if (i == 0) {
     starts[s] = L;
