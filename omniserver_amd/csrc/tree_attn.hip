@@ -17,13 +17,13 @@
 // A node whose parent does not precede it is a root of its own.
 //
 // And the attention's schedule.  A sequence's keys count in units of `unit` (what a workgroup takes
-// in a step), once per KV head.  Where the (sequence, KV head) items are of about one length, the
-// longest within a fifth of the mean, each is cut into as many equal pieces as there are columns of
-// workgroups for it.  Otherwise the units of all items stand in one line that is cut into equal
-// stretches, so that one long and many short contexts load the workgroups evenly, whatever the
-// lengths on the device are; a stretch that runs over an item's end costs its workgroup another
-// start and merge, some 4 us, which the even case is spared.  A piece is at least `least` units;
-// least 0: a column for each item.
+// in a step), once per KV head.  Every (sequence, KV head) item gets one of the ncols columns of
+// workgroups and a share of the others by its length, and is cut into as many equal pieces: none
+// of a batch of one length runs over an item's end.  Where that would leave some column more than
+// three units above the mean, the units of all items stand in one line instead, cut into equal
+// stretches: as even for one long and many short contexts, whatever the lengths on the device
+// are, but a stretch that runs over an item's end costs its workgroup another start and merge, some
+// 4 us.  No piece is under `least` units; least 0: a column for each item.
 //   seqs[s]     (prefix length, nodes in use, units, pool row)
 //   columns[c]  (s, g, first unit there, units in all, then of s: length, nodes, pool row)
 //   heads[s][g] (first column | 1 << 30 where the item is not the first that column sees, last)
@@ -58,28 +58,23 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
   const int L = prefix(s), used = in_use(s);
   const int64_t delta = row_ok && rope_delta ? rope_delta[slot] : 0;
 
+  auto units_of = [&](int r) {
+    const int64_t row = slots ? slots[r] : r;
+    const int m = in_use(r);
+    return m && row >= 0 && row < pool_rows ? ceil_div(min(prefix(r) + m, max_len), tc.unit) : 0;
+  };
   // units of the sequences before this one, its own, and all
-  int before = 0, all = 0, units = 0, longest = 0;
+  int before = 0, all = 0;
   for (int r0 = 0; r0 < n; r0 += 64) {
-    const int r = r0 + i;
-    int w = 0;
-    if (r < n) {
-      const int64_t row = slots ? slots[r] : r;
-      const int m = in_use(r);
-      if (m && row >= 0 && row < pool_rows) w = ceil_div(min(prefix(r) + m, max_len), tc.unit);
-      if (r == s) units = w;
-    }
-    int lo = r < s ? w : 0, hi = w;
+    int w = r0 + i < n ? units_of(r0 + i) : 0, lo = r0 + i < s ? w : 0;
     for (int o = 32; o; o >>= 1) {
       w += __shfl_xor(w, o);
       lo += __shfl_xor(lo, o);
-      hi = max(hi, __shfl_xor(hi, o));
     }
-    longest = max(longest, hi);
     all += w;
     before += lo;
   }
-  units = __shfl(units, s & 63);
+  const int units = units_of(s);
   all *= tc.nkv;
   before *= tc.nkv;
   const int items = n * tc.nkv;
@@ -88,19 +83,43 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(
     *(i32x4*)col = (i32x4){s, g, first, count};
     *(i32x4*)(col + 4) = (i32x4){L, used, (int)slot, 0};
   };
-  if (!tc.least || (items <= tc.ncols && (int64_t)longest * items * 5 <= (int64_t)all * 6)) {
-    const int each = tc.ncols / items;
-    const int pieces = tc.least ? min(each, max(1, units / tc.least)) : 1;
-    for (int k = i; k < tc.nkv * each; k += 64) {
-      const int g = k / each, j = k - g * each;
-      const int lo = j < pieces ? j * units / pieces : 0, hi = j < pieces ? (j + 1) * units / pieces : 0;
-      column((s * tc.nkv + g) * each + j, g, lo, hi - lo);
+  // pieces of an item; the columns before this sequence's, and all; the longest piece
+  auto pieces_of = [&](int w) {
+    if (!w || !tc.least) return w ? 1 : 0;
+    const int more = (int)((uint64_t)w * (uint64_t)(tc.ncols - items) / (uint64_t)all);
+    return min(1 + more, max(1, w / tc.least));
+  };
+  bool apart = !tc.least;
+  int first = 0, taken = 0;
+  if (items <= tc.ncols) {
+    int most = 0;
+    for (int r0 = 0; r0 < n; r0 += 64) {
+      const int w = r0 + i < n ? units_of(r0 + i) : 0;
+      int c = pieces_of(w), lo = r0 + i < s ? c : 0, hi = c ? ceil_div(w, c) : 0;
+      for (int o = 32; o; o >>= 1) {
+        c += __shfl_xor(c, o);
+        lo += __shfl_xor(lo, o);
+        hi = max(hi, __shfl_xor(hi, o));
+      }
+      taken += c;
+      first += lo;
+      most = max(most, hi);
     }
-    for (int c = items * each + i; c < tc.ncols && s == 0; c += 64) column(c, 0, 0, 0);
-    for (int g = i; g < tc.nkv; g += 64) {
-      const int c = (s * tc.nkv + g) * each;
-      *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) = make_int2(c, c + pieces - 1);
+    apart |= most <= all / tc.ncols + 3;
+    taken *= tc.nkv;
+    first *= tc.nkv;
+  }
+  if (apart) {
+    const int pieces = pieces_of(units);
+    for (int k = i; k < tc.nkv * pieces; k += 64) {
+      const int g = k / pieces, j = k - g * pieces;
+      const int lo = j * units / pieces;
+      column(first + k, g, lo, (j + 1) * units / pieces - lo);
     }
+    for (int c = taken + i; c < tc.ncols && s == 0; c += 64) column(c, 0, 0, 0);
+    for (int g = i; g < tc.nkv; g += 64)
+      *(int2*)(tc.heads + 2 * (s * tc.nkv + g)) =
+          make_int2(first + g * pieces, first + max(g * pieces + pieces - 1, 0));
   } else {
     // column c starts at unit c all / cols (in two parts: all < 2^30, cols < 2^15)
     const unsigned cols = min(tc.ncols, max(1, all / tc.least));

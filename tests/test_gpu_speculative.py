@@ -110,6 +110,7 @@ CUT = [
     (9, 40, 12, 2, (0, 900), 8192, (128, 2, 1)),
     (2, 64, 28, 4, (1200, 1800), 16384, (128, 2, 1)),
     (3, 64, 64, 1, (0, 200), 2000, (128, 2, 1)),      # 32 row blocks
+    (150, 2, 12, 2, (0, 700), 4096, (32, 8, 1)),      # more items than columns
     (1, 64, 64, 1, (500, 500), 1024, (32, 8, 0)),     # 128 row blocks, enough to leave uncut
 ]
 
@@ -147,6 +148,28 @@ def test_tree_attention_cut(gpu, n, T, nh, nkv, span, capacity, form):
             check = counts
         check_attention(out.view(n, T, nh, HD), q.view(n, T, nh, HD), pool, 0, starts, parents,
                         check, slots, 7.0)
+
+
+@pytest.mark.parametrize("n,T,nkv,long", [(100, 3, 2, 3900), (60, 9, 2, 4000), (40, 6, 6, 3000)])
+def test_tree_attention_cut_one_long(gpu, n, T, nkv, long):
+    """One long context among short ones: its keys go over many columns, which others end in."""
+    say(f"tree attention, one of {n} sequences {long} tokens long, T={T} nkv={nkv}")
+    rng = random.Random(n)
+    starts = [rng.randint(0, 60) for _ in range(n)]
+    starts[n // 3], starts[n - 1] = long, long // 3
+    parents = trees(rng, n, T, "tree")
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    pool = PreallocatedKVCache(1, n, nkv, 4096, HD, gpu, n_heads=12)
+    g = torch.Generator(device=gpu).manual_seed(n)
+    pool.storage.normal_(generator=g)
+    pool.lengths.copy_(torch.tensor(starts))
+    q = torch.randn(n * T, 12 * HD, device=gpu, generator=g).half()
+    cache = pool.tree_cache(parents)
+    assert cache.form[3] == 1
+    out = torch.full((n * T, 12, HD), 7.0, device=gpu, dtype=torch.float16)
+    cache.attend_qkv(q, 0, HD ** -0.5, out)
+    check_attention(out.view(n, T, 12, HD), q.cpu().view(n, T, 12, HD), pool, 0, starts, parents,
+                    [T] * n, list(range(n)), 7.0)
 
 
 def test_tree_attention_cut_keeps_infinities_apart(gpu):
