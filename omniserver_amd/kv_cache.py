@@ -452,34 +452,35 @@ TREE_MAX_NODES = 64
 def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) -> tuple:
     """(rows, key groups, columns, least) for omni_tree_attention over n trees in a pool of
     capacity tokens a row (see its header: least 0 keeps every sequence's keys together, else they
-    are cut evenly over the columns and merged by a second launch).
+    are cut over the columns and merged by a second launch).
 
     us, MI355X, 12 heads / 2 KV heads: fewer rows a workgroup and more key groups while the
-    workgroups fit one round of the CUs, their key chains being the shorter; together where the
+    workgroups fit one round of the CUs, their key chains being the shorter.  Together where the
     contexts are short (8 nodes at 250 keys 9.2 against 10.6 cut) or the workgroups many enough
-    (16 x 32 nodes at 1000 18.6 / 21.6), cut where they are few (8 x 8 at 4000 16.7, together
-    33) or their contexts may differ most (32 x 64 at 200-4000 59, together 78; all at 4000 93
-    / 86)."""
+    (16 x 32 nodes at 1000 17.1 / 19.0), cut where they are few (8 x 8 at 4000 15.0, together 33)
+    or their contexts may differ most (32 x 64 at 200-4000 64, together 75; all at 4000 86 / 81).
+    Cut: 64 rows; 128 where 64 would leave more than eight steps of 128 keys for every CU (32 x 16
+    at 4000 41.4 against 44; 4 x 64 28 / 23); 32 where they suffice and many sequences may be
+    short (32 x 4 at 50-1000 13.0 against 17.5, all at 1000 15.3 / 14.7)."""
     rows, items = nodes * (nh // nkv), n * nkv
     blocks = lambda r: -(-rows // r)
     form = next((f for f in ((32, 8), (64, 4)) if items * blocks(f[0]) <= cus), (128, 2))
     if capacity <= 512 or (capacity <= 1536 and items * blocks(form[0]) >= 3 * cus // 8):
         return (*form, items, 0)
-    # cut: 64 rows; 128 where that leaves two steps of 128 keys and more for every CU (4 x 32
-    # nodes at 4000 21.0 against 26.0; 1 x 64 17.8 / 16.0); 32 where they suffice and many
-    # sequences may be short (32 x 4 nodes at 50-1000 13.0 against 17.5, all at 1000 15.3 / 14.7)
+    steps = items * blocks(64) * -(-capacity // 128)
     if rows <= 32 and items >= 32:
-        form = (32, 8)
-    elif rows > 128 and items * blocks(64) * -(-capacity // 128) >= 2 * cus:
-        form = (128, 2)
+        form, unit, least = (32, 8), 256, 1
+    elif rows > 64 and steps > 8 * cus:
+        form, unit, least = (128, 2), 128, 1
     else:
-        form = (64, 4)
+        # no single steps where there are enough for every CU (16 x 8 at 1000 13.9 against 15.2)
+        form, unit, least = (64, 4), 128, 2 if steps >= cus else 1
     # one round of workgroups, in whole eights for the row blocks of a column to share an XCD, and
     # a multiple of the items, so that equal contexts are cut at their ends
     columns = max(1, cus // 8 // blocks(form[0])) * 8
     if columns > items:
         columns -= columns % items
-    return (*form, min(columns, items * -(-capacity // (256 if form[1] == 8 else 128))), 1)
+    return (*form, min(columns, items * -(-capacity // unit)), least)
 
 
 class TreeCache(PackedPrefillWriter):
