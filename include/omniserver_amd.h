@@ -173,8 +173,8 @@ int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
  * (32, 8), any number of query heads per KV head.  Where the plan cuts (least > 0) the
  * softmax states of the pieces go through workspace (fp32, 16-byte aligned, columns * ceil(n_nodes
  * * n_heads / n_kv_heads / rows) * 2 * rows * 132 floats) to a second launch.  head_dim 128; scale
- * a positive normal fp32; 16-byte aligned operands. */
-int omni_tree_attention(const void* q, int q_stride, const void* k_cache, const void* v_cache,
+ * from 2^-126 to 2^126; 16-byte aligned operands. */
+int omni_tree_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                         int pool_rows, int max_len, const void* ancestors, int n, int n_nodes,
                         void* out, int out_stride, int n_heads, int n_kv_heads, int head_dim,
                         float scale, int rows, int groups, int columns, int least,

@@ -75,7 +75,7 @@ SIGNATURES = {
     "omni_tree_plan": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
                        _P, _I64, _P],
     "omni_kv_write_rows": [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I, _P],
-    "omni_tree_attention": [_P, _I, _P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _F, _I, _I,
+    "omni_tree_attention": [_P, _I64, _P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I, _F, _I, _I,
                             _I, _I, _P, _P, _I64, _P],
     "omni_kv_accept": [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "omni_spec_verify_work": [_I, _I, _I, _I],

@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 // ---------------------------------------------------------------------------
 struct TreeArgs {
   const half_t* q;
-  int q_stride;
+  int64_t q_stride;
   const half_t* k_cache;
   const half_t* v_cache;
   int max_len, nkv, G, T, n;
@@ -694,6 +694,13 @@ static int tree_form(int rows, int groups, int* unit) {
   return rows * groups == 256 && (groups == 2 || groups == 4 || groups == 8) ? groups : 0;
 }
 
+// 32-bit positions, indexes into the schedule, products of a column and an item's units hold.
+static bool tree_size_ok(int64_t n, int64_t nkv, int64_t columns, int max_len, int unit, int least) {
+  const int64_t units = ((int64_t)max_len + unit - 1) / unit;
+  return max_len <= 1 << 30 && n * nkv <= 1 << 24 && columns <= 1 << 24 && n * nkv * units <= 0x3fffffff &&
+         (!least || (columns <= 32767 && columns * units <= 0x7fffffff));
+}
+
 // schedule: [n][4] seqs, [ncols][8] columns, [n][nkv][2] heads
 static int64_t tree_schedule_ints(int n, int nkv, int ncols) {
   return 4 * (int64_t)n + 8 * (int64_t)ncols + 2 * (int64_t)n * nkv;
@@ -711,8 +718,7 @@ extern "C" int omni_tree_plan(const int* parents, const int* counts, const int64
   int unit;
   if (!tree_form(rows, groups, &unit) || columns < 1 || least < 0) return OMNI_EINVAL;
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
-  if ((int64_t)n * n_kv_heads * ceil_div(max_len, unit) > 0x3fffffff || (least && columns > 32767))
-    return OMNI_EUNSUPPORTED;
+  if (!tree_size_ok(n, n_kv_heads, columns, max_len, unit, least)) return OMNI_EUNSUPPORTED;
   if (n == 0) return OMNI_OK;
   if (!parents || !lengths || !starts || !ancestors || !positions || !token_slot || !token_pos ||
       !schedule || ((uintptr_t)schedule & 15))
@@ -744,7 +750,7 @@ extern "C" int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v
   return OMNI_OK;
 }
 
-extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_cache,
+extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* k_cache,
                                    const void* v_cache, int pool_rows, int max_len,
                                    const void* ancestors, int n, int n_nodes, void* out,
                                    int out_stride, int n_heads, int n_kv_heads,
@@ -753,12 +759,14 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
                                    int64_t workspace_floats, void* stream) {
   if (n < 0 || n_nodes < 1 || n_heads <= 0 || n_kv_heads <= 0 || pool_rows <= 0 || max_len <= 0)
     return OMNI_EINVAL;
-  if (head_dim != TREE_HD || n_heads % n_kv_heads || n_nodes > TREE_MAX) return OMNI_EUNSUPPORTED;
-  if (!(scale >= 0x1p-126f) || scale > 3e38f) return OMNI_EUNSUPPORTED;
+  if (head_dim != TREE_HD || n_heads % n_kv_heads || n_heads > 65536 || n_nodes > TREE_MAX)
+    return OMNI_EUNSUPPORTED;
+  if (!(scale >= 0x1p-126f) || scale > 0x1p126f) return OMNI_EUNSUPPORTED;
   int unit;
   const int form = tree_form(rows, groups, &unit);
   if (!form || columns < 1 || least < 0) return OMNI_EINVAL;
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
+  if (!tree_size_ok(n, n_kv_heads, columns, max_len, unit, least)) return OMNI_EUNSUPPORTED;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
@@ -803,7 +811,7 @@ extern "C" int omni_tree_attention(const void* q, int q_stride, const void* k_ca
   if (least) {
     // parts of an item: at least one, some columns / items
     const int* heads = a.columns + 8 * (int64_t)columns;
-    if (columns > 8 * n * n_kv_heads)
+    if (columns > 8 * (int64_t)n * n_kv_heads)
       hipLaunchKernelGGL((tree_merge_kernel<8>), dim3((unsigned)out_rows), dim3(256), 0, st, a, heads,
                          rows, out_rows);
     else

@@ -501,7 +501,8 @@ class TreeCache(PackedPrefillWriter):
     nor attended to.  Padding nodes' rows of an output are left as they were.
 
     The packed rows are sequence-major: node i of sequence s is row s * T + i of the forward.  The
-    adapter's buffers belong to it, so two captured graphs never share them."""
+    adapter's buffers belong to it, so two captured graphs never share them; its layers run on one
+    stream, one after another."""
 
     def __init__(self, pool: PreallocatedKVCache, parents, counts=None, slots=None,
                  rope_delta: torch.Tensor | None = None):
@@ -540,7 +541,7 @@ class TreeCache(PackedPrefillWriter):
         rope_delta = _ints(rope_delta, None, torch.int64, dev, "rope_delta")
         if rope_delta is not None and rope_delta.numel() < pool.max_batch:
             raise ValueError(f"rope_delta holds one value per pool row ({pool.max_batch})")
-        require_here(parents, self.counts, self.slots, rope_delta)
+        require_here(pool.lengths, parents, self.counts, self.slots, rope_delta)
         self.n, self.nodes, self.T = n, T, n * T
         nkv = pool.n_kv_heads
         # how the attention's workgroups share the keys
@@ -610,7 +611,7 @@ class TreeCache(PackedPrefillWriter):
         if out.numel() != self.T * width or not out.is_contiguous():
             raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
                              f"[{self.T}, {pool.n_heads}, {pool.head_dim}]")
-        require_here(qkv, out)
+        require_here(pool.storage, qkv, out)
         stride = qkv.stride(0) if self.T > 1 else max(qkv.stride(0), width)
         return self._attend(qkv.data_ptr(), stride, layer_idx, scale, out)
 
@@ -618,9 +619,9 @@ class TreeCache(PackedPrefillWriter):
         pool, ws = self.pool, self._ws
         nh, hd = pool.n_heads, pool.head_dim
         call("omni_tree_attention", q, q_stride, pool.k[layer_idx].data_ptr(),
-             pool.v[layer_idx].data_ptr(), pool.max_batch, pool.max_len, self._ancestors, self.n, self.nodes, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd,
-             float(scale), *self.form, self._schedule, ptr(ws), 0 if ws is None else ws.numel(),
-             stream())
+             pool.v[layer_idx].data_ptr(), pool.max_batch, pool.max_len, self._ancestors, self.n,
+             self.nodes, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd, float(scale), *self.form,
+             self._schedule, ptr(ws), 0 if ws is None else ws.numel(), stream())
         return out
 
     def flash_prefill(self, q, k, v, layer_idx, scale):
@@ -635,7 +636,7 @@ class TreeCache(PackedPrefillWriter):
         if not q.dtype == k.dtype == v.dtype == torch.float16:
             raise TypeError(f"the pool is fp16 (got {q.dtype}, {k.dtype}, {v.dtype})")
         (q, qs), (k, ks), (v, vs) = _head_rows(q), _head_rows(k), _head_rows(v)
-        require_here(q, k, v)
+        require_here(pool.storage, q, k, v)
         call("omni_kv_write_rows", k.data_ptr(), ks, v.data_ptr(), vs,
              pool.k[layer_idx].data_ptr(), pool.v[layer_idx].data_ptr(), self._slot, self._pos,
              pool.max_batch, pool.max_len, nkv * hd, self.T, stream())
@@ -655,7 +656,7 @@ class TreeCache(PackedPrefillWriter):
         pool = self.pool
         path = _ints(path, (self.n, self.nodes), torch.int32, pool.device, "path")
         emitted = _ints(emitted, (self.n,), torch.int32, pool.device, "emitted")
-        require_here(path, emitted)
+        require_here(pool.storage, path, emitted)
         call("omni_kv_accept", pool.storage.data_ptr(), pool.n_layers, pool.max_batch, pool.max_len,
              pool.n_kv_heads * pool.head_dim, ptr(self.slots), self._starts, path.data_ptr(),
              emitted.data_ptr(), self.n, self.nodes, pool.lengths.data_ptr(), stream())

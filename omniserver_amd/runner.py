@@ -499,9 +499,10 @@ class MultimodalRunner(ModelRunner):
         out = torch.cat([v.tokens, v.emitted.to(torch.int64).unsqueeze(1)], 1).tolist()
         self._dev_ids_for = None
         gained = [0] * n
+        for slot in range(n):
+            self._kv_len[slot] += out[slot][T]
         for slot, i in enumerate(order):
             seq, new = seqs[i], out[slot][:out[slot][T]]
-            self._kv_len[slot] += len(new)
             for t in new:
                 if t < 0:
                     raise RuntimeError(f"no token is left to draw for the sequence in slot {slot}")

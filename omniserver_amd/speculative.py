@@ -56,8 +56,9 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | 
     also what is not above 0) puts all mass on the first maximum, and needs no random numbers.
     counts int32 [n]: nodes in use (default T).
 
-    A NaN logit counts as -inf; where no token is above -inf the next token is -1.  All weights and
-    sums are 64-bit, in a fixed order: the same inputs give the same tokens."""
+    A NaN logit counts as -inf; where no token is above -inf the next token is -1.  The same
+    inputs give the same tokens: those of 64-bit weights and sums, which the 32-bit sums of the rows
+    stand for only where they cannot change what is decided."""
     checked = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
     n, T, V = logits.shape
     dev = logits.device

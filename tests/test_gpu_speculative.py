@@ -329,6 +329,41 @@ def test_tree_attention_strides_and_streams(gpu):
         cache.attend_qkv(wide.view(-1)[4:4 + 20 * 1536].view(20, 1536), 0, 0.1, out)
 
 
+def test_tree_attention_far_rows(gpu):
+    """Query rows further apart than 32-bit offsets reach."""
+    pool, g = make_pool(gpu, 1, 1, 2, 1, 64, 12)
+    pool.lengths[0] = 33
+    q = torch.randn(2, 2 * HD, generator=g).half()
+    far = (1 << 31) + 8
+    room = torch.empty(far + 2 * HD, device=gpu, dtype=torch.float16)
+    rows = room.as_strided((2, 2 * HD), (far, 1))
+    rows.copy_(q.to(gpu))
+    cache = pool.tree_cache([[-1, 0]])
+    out = torch.zeros(2, 2, HD, device=gpu, dtype=torch.float16)
+    cache.attend_qkv(rows, 0, HD ** -0.5, out)
+    check_attention(out.view(1, 2, 2, HD), q.view(1, 2, 2, HD), pool, 0, [33], [[-1, 0]], [2], [0],
+                    0.0)
+
+
+def test_pool_off_the_current_device(gpu):
+    """Whatever the tensors are, a pool elsewhere is refused before a launch."""
+    pool, _ = make_pool(gpu, 1, 2, 12, 2, 64, 13)
+    parents = i32([[-1, 0], [-1, 0]], gpu)
+    cache = pool.tree_cache(parents)
+    rows = torch.zeros(4, 16 * HD, device=gpu, dtype=torch.float16)
+    q = rows[:, :12 * HD].view(4, 12, HD)
+    kv = rows[:, 12 * HD:14 * HD].view(4, 2, HD)
+    pool.storage, pool.lengths = pool.storage.cpu(), pool.lengths.cpu()
+    with pytest.raises(RuntimeError):
+        pool.tree_cache(parents)
+    with pytest.raises(RuntimeError):
+        cache.attend_qkv(rows, 0, 0.1, torch.zeros(4, 12, HD, device=gpu, dtype=torch.float16))
+    with pytest.raises(RuntimeError):
+        cache.flash_prefill(q, kv, kv, 0, 0.1)
+    with pytest.raises(RuntimeError):
+        cache.accept(i32([[0, -1]] * 2, gpu), i32([1, 1], gpu))
+
+
 # ----------------------------------------------------------------------------- verification
 def rows_like_a_model(g, n, T, V, dtype, std=2.0):
     x = torch.randn(n, T, V, generator=g) * std
@@ -767,3 +802,29 @@ def test_runner_speculate_limits(gpu):
         assert b.status == Status.FINISHED
         with pytest.raises(RuntimeError):
             r.speculate([a, b], [[], []])
+
+
+def test_runner_speculate_without_a_token(gpu, monkeypatch):
+    """A sequence that nothing can be drawn for is an error, and the others' lengths still hold."""
+    from omniserver_amd import runner as runner_mod
+    from omniserver_amd import synth
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    shape = synth.DecoderShape()
+    r = runner_mod.NativeQwenVLRunner(max_running=2, max_len=48, use_graph=False,
+                                      weights=synth.fp16_decoder(shape, seed=8, num_layers=1))
+    seqs = [Sequence(Request(prompt=synth.random_ids(L, shape.vocab_size, 8, f"n{L}").tolist(),
+                             sampling=SamplingParams(max_new_tokens=9))) for L in (5, 11)]
+    for s in seqs:
+        r.tokenize(s)
+    r.prefill(seqs)
+    verify = runner_mod.verify
+
+    def without(*a, **kw):
+        v = verify(*a, **kw)
+        v.tokens[0].fill_(-1)
+        return v
+
+    monkeypatch.setattr(runner_mod, "verify", without)
+    with pytest.raises(RuntimeError):
+        r.speculate(seqs, [[1, 2], [3, 4]])
+    assert r.pool.lengths[:2].tolist() == r._kv_len[:2]

@@ -28,7 +28,11 @@ def test_tree_attention_refusals():
     assert rc(n=-1) == rc(nodes=0) == rc(nh=0) == rc(nkv=0) == rc(rows=0) == rc(max_len=0) == -1
     assert rc(nodes=65) == rc(hd=64) == rc(nh=13) == -2
     assert rc(scale=0.0) == rc(scale=-1.0) == rc(scale=float("nan")) == rc(scale=1e-39) == -2
-    assert rc(scale=float("inf")) == -2
+    assert rc(scale=float("inf")) == rc(scale=2.5e38) == -2       # x log2(e) is infinite
+    big = {"nodes": 1, "q_stride": 1 << 31, "out_stride": (1 << 31) - 8}
+    assert rc(nh=1 << 17, nkv=1, **big) == -2
+    assert rc(n=1 << 24, columns=1 << 25) == rc(columns=1 << 15, least=1) == -2
+    assert rc(n=1 << 12, columns=1 << 13, max_len=(1 << 31) - 1) == -2
     assert rc(q_stride=1535) == rc(q_stride=1532) == rc(out_stride=8) == rc(out_stride=1540) == -1
     assert rc(form=(64, 2)) == rc(form=(128, 1)) == rc(form=(0, 0)) == rc(form=(16, 16)) == -1
     assert rc(columns=0) == rc(columns=5) == rc(least=-1) == -1
@@ -51,6 +55,8 @@ def test_tree_plan_and_row_write_refusals():
     assert plan(n=5, columns=10) == plan(columns=3) == plan(columns=0) == plan(least=-1) == -1
     assert plan(form=(128, 4)) == plan(ints=4 * 2 + 8 * 4 + 2 * 2 * 2 - 1) == -1
     assert plan(columns=1 << 24, least=1) == plan(nodes=65) == -2
+    assert plan(columns=32767, least=1, max_len=(1 << 31) - 1) == -2
+    assert plan(n=1 << 24, rows=1 << 24, columns=1 << 25) == -2
     assert plan(parents=None) == plan(lengths=None) == plan(starts=None) == -1
     assert plan(n=0) == 0
 
