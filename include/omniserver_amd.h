@@ -133,7 +133,7 @@ int omni_kv_copy_slot(void* pool, int n_layers, int pool_rows, int max_len, int 
 /* The accepted path of each drafted tree (omni_tree_plan) made the end of its sequence: rows
  * starts[s] + path[s][j] of pool row slots[s] (or s) move to starts[s] + j in every layer's K and
  * V, j < emitted[s], and lengths[slot] = starts[s] + emitted[s] (at most max_len).  path int32
- * [n][n_nodes] ascends from node 0; one that does not ascend within the tree ends there.  The
+ * [n][n_nodes <= 64] ascends from node 0; one that does not ascend within the tree ends there.  The
  * sequences' pool rows are all different; one outside the pool is left alone. */
 int omni_kv_accept(void* pool, int n_layers, int pool_rows, int max_len, int row_halfs,
                    const int64_t* slots, const int64_t* starts, const int* path,

@@ -77,9 +77,10 @@ extern "C" int omni_kv_copy_slot(void* pool, int n_layers, int pool_rows, int ma
 // ---------------------------------------------------------------------------
 // The accepted path of a drafted tree made the end of its sequence: the K/V rows at starts[s] +
 // path[s][j] move to starts[s] + j in every layer, j < emitted[s], and lengths become starts +
-// emitted.  A path ascends from node 0, so path[j] >= j and a thread that moves its column of
-// every row, lowest first, reads each row before anything is written over it: a later row's
-// source lies above every row written so far.
+// emitted.  Eight rows of 32 16-byte columns a turn: all of a turn's rows are read before any is
+// written.  A path ascends from node 0, so path[j] >= j, and the next turn's sources lie above
+// whatever this one wrote: no wait between turns.  Latency bound (path, rows, stores): 32 paths of
+// 6 of 26 nodes in 28 layers, 11 MB, 4.4 us; a thread a column, row after row, 6.3.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void kv_accept_kernel(half_t* __restrict__ pool, int64_t seg_stride,
                                                         int64_t row_stride, int row_halfs,
@@ -89,29 +90,30 @@ __global__ __launch_bounds__(256) void kv_accept_kernel(half_t* __restrict__ poo
                                                         const int* __restrict__ emitted, int T,
                                                         int64_t* __restrict__ lengths, int pool_rows,
                                                         int max_len) {
-  const int s = blockIdx.y;
+  const int s = blockIdx.y, lane = threadIdx.x & 63;
   const int64_t slot = slots ? slots[s] : s;
+  // every wave a node a lane
+  const int from = lane < T ? path[(int64_t)s * T + lane] : -1;
   if (slot < 0 || slot >= pool_rows) return;
   const int64_t L = min(max(starts[s], (int64_t)0), (int64_t)max_len);
-  int len = min(max(emitted[s], 0), T);
-  if ((int64_t)len > max_len - L) len = (int)(max_len - L);
-  // a path that does not ascend within the tree ends there
-  int above = 0;
-  for (int j = 0; j < len; ++j) {
-    const int from = path[(int64_t)s * T + j];
-    if (from < above || from >= T || from >= max_len - L) {
-      len = j;
-      break;
-    }
-    above = from + 1;
-  }
-  half_t* seq = pool + blockIdx.x * seg_stride + slot * row_stride + L * row_halfs;
+  const int room = (int)min((int64_t)T, max_len - L);
+  const int before = __shfl_up(from, 1);
+  // a path that does not ascend within the tree and the pool ends there
+  const bool ok = from > (lane ? before : -1) && from < room;
+  const uint64_t bad = __ballot(!ok);
+  const int len = min(min(max(emitted[s], 0), T), bad ? __ffsll((unsigned long long)bad) - 1 : 64);
+  half8_t* seq = (half8_t*)(pool + blockIdx.x * seg_stride + slot * row_stride + L * row_halfs);
   const int chunks = row_halfs >> 3;
-  for (int c = threadIdx.x; c < chunks; c += 256) {
-    half8_t* col = (half8_t*)seq + c;
-    for (int j = 0; j < len; ++j) {
-      const int from = path[(int64_t)s * T + j];
-      if (from != j) col[(int64_t)j * chunks] = col[(int64_t)from * chunks];
+  const int r = threadIdx.x >> 5, c0 = threadIdx.x & 31;
+  for (int j0 = 0; j0 < len; j0 += 8) {
+    const int j = j0 + r, at = __shfl(from, min(j, len - 1));
+    for (int c1 = 0; c1 < chunks; c1 += 32) {
+      const int c = c1 + c0;
+      const bool moves = j < len && c < chunks && at != j;
+      half8_t v;
+      if (moves) v = seq[(int64_t)at * chunks + c];
+      __syncthreads();
+      if (moves) seq[(int64_t)j * chunks + c] = v;
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) lengths[slot] = L + len;
@@ -123,7 +125,7 @@ extern "C" int omni_kv_accept(void* pool, int n_layers, int pool_rows, int max_l
                               void* stream) {
   if (n_layers <= 0 || pool_rows <= 0 || max_len <= 0 || row_halfs <= 0 || n < 0 || n_nodes < 1)
     return OMNI_EINVAL;
-  if ((row_halfs & 7) || n > 65535) return OMNI_EUNSUPPORTED;
+  if ((row_halfs & 7) || n > 65535 || n_nodes > 64) return OMNI_EUNSUPPORTED;
   if (!slots && n > pool_rows) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
   if (!pool || !starts || !path || !emitted || !lengths || ((uintptr_t)pool & 15)) return OMNI_EINVAL;

@@ -81,7 +81,7 @@ def test_kv_accept_refusals():
 
     assert rc(layers=0) == rc(rows=0) == rc(max_len=0) == rc(halfs=0) == rc(n=-1) == -1
     assert rc(nodes=0) == rc(n=5) == -1
-    assert rc(halfs=252) == rc(n=70000, slots=P) == -2
+    assert rc(halfs=252) == rc(n=70000, slots=P) == rc(nodes=65) == -2
     assert rc(kv=None) == rc(starts=None) == rc(path=None) == rc(lengths=None) == -1
     assert rc(kv=ctypes.c_void_p(8)) == -1
     assert rc(n=0) == 0
