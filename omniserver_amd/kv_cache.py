@@ -14,8 +14,12 @@ Mirrors omniserve/cache/kv_prealloc.py:
   and its query i attends to keys ``[0, start+i]`` (cached prefix + the segment, causal);
   ``lengths[slot] = start + new_len``.  A decode token is a segment of one.
 
+Beyond the reference, ``tree_cache`` / ``TreeCache``: the adapter for one forward over drafted trees
+of tokens (speculative decoding), whose ``accept`` keeps the K/V rows of the nodes that stand.
+
 Attention, the K/V writes and the slot copies run on the HIP kernels
-(omni_decode_attention, omni_mrope_kv_write, omni_prefill_attention, omni_kv_copy_slot);
+(omni_decode_attention, omni_mrope_kv_write, omni_prefill_attention, omni_tree_attention, omni_kv_copy_slot,
+omni_kv_accept);
 snapshots for prefix reuse are torch clones.
 """
 
