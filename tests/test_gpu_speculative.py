@@ -616,11 +616,13 @@ def spec_step(pool, layers, parents, tokens, u, temps, q, k, v, logits):
     return outs, got
 
 
-def test_step_in_graphs(gpu):
+@pytest.mark.parametrize("capacity", [200, 2048])      # keys whole, and cut with a merge
+def test_step_in_graphs(gpu, capacity):
     """Two captured steps of one pool, replayed in turn with eager work between the replays, give
     what the eager step gives."""
     n, T, layers, V = 3, 12, 2, 5003
-    pool, g = make_pool(gpu, layers, n, 12, 2, 200, 6)
+    pool, g = make_pool(gpu, layers, n, 12, 2, capacity, 6)
+    assert (pool.tree_cache([[-1] * T] * n).form[3] > 0) == (capacity > 512)
     rng = random.Random(6)
     starts = torch.tensor([30, 0, 111], device=gpu)
     sets = []
