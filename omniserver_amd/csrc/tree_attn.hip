@@ -213,11 +213,11 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 // attend to (tree_row).  That costs the others the check and a barrier.
 //
 // MI355X, 12 / 2 heads.  A launch has some 8 us of its own (column and Q loads, first tile, LDS
-// merge).  128 rows: a step of 128 keys 1.90 us on up to 144 workgroups (matrix 40 %, vector 50 % of
-// the cycles, waits), 2.2 on 192, 2.5 on 240: the chip's power holds the products at 800 TFLOP/s,
-// whether K and V come from memory or cache; wave priorities, by group or by phase, change nothing.
+// merge).  128 rows: a step of 128 keys 1.85 us on up to 144 workgroups (matrix 40 %, vector 50 % of
+// the cycles, waits), 2.0 on 192, 2.4 on 240: the chip's power holds the products at 800
+// TFLOP/s, whether K and V come from memory or cache; wave priorities change nothing.
 // 64 rows: a step 1.3 us on 2 workgroups, 3.15 on 256 = 5.3 TB/s, memory's.  32 x 64 nodes at 4000
-// tokens 77 us with 4.8 of merge, 32 x 8 at 2048 18 + 4.8, 1 x 26 at 4000 10.3 + 4.2.
+// tokens 74 + 4.8 of merge, 32 x 8 at 2048 18 + 4.8, 1 x 26 at 4000 10.3 + 4.2.
 // ---------------------------------------------------------------------------
 struct TreeArgs {
   const half_t* q;
@@ -489,13 +489,22 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
   // Q has landed: without this the compiler counts the Q loads as outstanding inside the loop
   // and makes every tile's first MFMAs wait for the transfers just requested
   __builtin_amdgcn_s_waitcnt(0x0f70);
+  // Eight waves' transfers take the CU's load path some 1100 cycles to accept, and a wave waits
+  // there.  One wave of every SIMD issues its own at the start of a step, the other (wave + 4)
+  // behind its softmax: so one is at its products while the other waits.
+  const bool late = R > 1 && wave >= 4;
+  auto next_tile = [&](int it) {
+    if constexpr (R > 1) {
+      if (it + 1 < nt) dma_tile((tbeg + it + 1) * KT, gbuf + ((it + 1) & 1) * 2 * TB);
+    }
+  };
   for (int it = 0; it < steps; ++it) {
     char* kt = gbuf + (NBUF == 2 ? (it & 1) * 2 * TB : 0);
     const int tb = (tbeg + it) * KT;
     if constexpr (R > 1) {
       vm_wait();             // this wave's part of tile it has landed; so, past the barrier,
       lds_barrier();         // have the others', and tile it - 1's buffer is free
-      if (it + 1 < nt) dma_tile(tb + KT, gbuf + ((it + 1) & 1) * 2 * TB);
+      if (!late) next_tile(it);
     } else {
       if (it < nt) store_tile(kt);
       if (it + 1 < nt) load_tile(tb + KT);
@@ -504,7 +513,10 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
       scores(kt);
       hide(tb);
       softmax32<NB, 4>(sc, a.scale_log2, m_run, l_run, o, p);
+      if (late) next_tile(it);
       output(kt + TB);
+    } else if (late) {
+      next_tile(it);
     }
   }
 
