@@ -1,5 +1,5 @@
-// Attention on 32-row tiles: what the decoder's prefill (attn_rows.hip), the drafted trees'
-// attention (tree_attn.hip) and the vision tower's (vit.hip) share.
+// Attention on 32-row tiles: what the decoder's prefill (attn_rows.hip) and the vision
+// tower's attention (vit.hip) share.
 #pragma once
 
 #include "common.h"
@@ -36,9 +36,8 @@ __device__ __forceinline__ void half_pair(float v, float& a, float& b) {
 
 // One key tile's scores s (NB blocks of 32 keys) to probabilities p (the B operands of
 // 2 NB 16-key steps), with the row state m_run (log2 units) and l_run (this lane half's part
-// of the sum) updated and the NO output blocks rescaled where a maximum has moved, or, with SLACK,
-// has grown by more than 2^SLACK: the largest P is then up to that, not 1.
-template <int NB, int NO, int SLACK = 0>
+// of the sum) updated and the NO output blocks rescaled where a maximum has moved.
+template <int NB, int NO>
 __device__ __forceinline__ void softmax32(const f32x16 (&s)[NB], float scale_log2, float& m_run,
                                           float& l_run, f32x16 (&o)[NO], half8_t (&p)[2 * NB]) {
   float mx = s[0][0];
@@ -49,7 +48,7 @@ __device__ __forceinline__ void softmax32(const f32x16 (&s)[NB], float scale_log
   float ma, mb;
   half_pair(mx, ma, mb);
   const float mt = fmaxf(ma, mb) * scale_log2;            // scale > 0: the scaled maximum
-  if (__any(SLACK ? mt > m_run + (float)SLACK : mt > m_run)) {
+  if (__any(mt > m_run)) {
     const float m_new = fmaxf(m_run, mt);
     // -inf: a row none of whose keys has been seen (a key group that starts past its limit)
     const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));

@@ -212,14 +212,9 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 // outputs are not all finite are taken again, key by key and without the keys they do not
 // attend to (tree_row).  That costs the others the check and a barrier.
 //
-// The outputs are rescaled only once a row's maximum has grown by 2^8: among 32 rows some maximum
-// moves in most tiles, and 64 multiplies a tile are a twentieth of the vector work (32 x 64 nodes 84
-// -> 82 us, 1 x 48 with 28 heads 47.5 -> 45.5, 8 x 16 15.6 -> 15.2).  P up to 256 is rounded to fp16
-// as P up to 1 is, by 2^-11 of itself; only a key that takes all of a row's mass is no longer exact.
-//
 // MI355X, 12 / 2 heads.  A launch has some 8 us of its own (column and Q loads, first tile, LDS
-// merge).  128 rows: a step of 128 keys 1.76 us on up to 144 workgroups (matrix 40 %, vector 50 % of
-// the cycles, waits), 1.95 on 192, 2.5 on 240: the chip's power holds the products at 800
+// merge).  128 rows: a step of 128 keys 1.85 us on up to 144 workgroups (matrix 40 %, vector 50 % of
+// the cycles, waits), 2.0 on 192, 2.4 on 240: the chip's power holds the products at 800
 // TFLOP/s, whether K and V come from memory or cache; wave priorities change nothing.
 // 64 rows: a step 1.3 us on 2 workgroups, 3.15 on 256 = 5.3 TB/s, memory's.  32 x 64 nodes at 4000
 // tokens 74 + 4.8 of merge, 32 x 8 at 2048 18 + 4.8, 1 x 26 at 4000 10.3 + 4.2.
@@ -517,7 +512,7 @@ __global__ __launch_bounds__(64 * R * S, 2) void tree_attn_kernel(TreeArgs a) {
     if (it < nt && rows_here) {
       scores(kt);
       hide(tb);
-      softmax32<NB, 4, 8>(sc, a.scale_log2, m_run, l_run, o, p);
+      softmax32<NB, 4>(sc, a.scale_log2, m_run, l_run, o, p);
       if (late) next_tile(it);
       output(kt + TB);
     } else if (late) {

@@ -1,0 +1,106 @@
+"""Speculative decoding's operators on the GPU where their numerics turn: maxima that grow from tile
+to tile."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import speculative_ref as ref
+from tests.test_gpu_speculative import HD, i32, say, trees
+
+pytestmark = pytest.mark.gpu
+
+LOG2E = 1.0 / math.log(2.0)
+
+GROWING = [
+    # n, T, start, capacity, the plan's (rows, groups), cut or not: two to four tiles a key group
+    (2, 5, 490, 512, (32, 8, False)),
+    (20, 33, 470, 512, (64, 4, False)),
+    (32, 64, 448, 512, (128, 2, False)),
+    (33, 2, 1500, 4096, (32, 8, True)),
+    (32, 8, 2000, 4096, (64, 4, True)),
+    (9, 40, 1800, 4096, (128, 2, True)),
+]
+
+
+def growing_pool(gpu, n, T, start, capacity):
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    pool = PreallocatedKVCache(1, n, 2, capacity, HD, gpu, n_heads=12)
+    pool.storage.zero_()
+    pool.lengths.fill_(start)
+    g = torch.Generator().manual_seed(n + T + start)
+    return pool, g, trees(random.Random(n + T), n, T, "tree")
+
+
+@pytest.mark.parametrize("rise", [2.75, 6.1, 7.9, 8.1, 20.0])
+@pytest.mark.parametrize("n,T,start,capacity,form", GROWING)
+def test_tree_attention_growing_maximum(gpu, n, T, start, capacity, form, rise):
+    """One key in 32 lies `rise` to 1.5 `rise` (row by row) powers of two above the one 32 before
+    it, the others far below; every key of a (sequence, KV head) has the same V row, so each output
+    is that row.
+
+    Exactly: a row's largest probability rounds to 1; the next are some 2^-2.75, 2^-5.5, .. of it
+    (k[0]'s own rounding moves a rise by 0.13 at most, where rises are small), 0.2 together, each off
+    by at most 2^-11 of itself in fp16, 2^-13.3 of the sum.  A score of up to 2^11 in log2 units is
+    off by 2^-13 at most against the sum's, in fp32, 2^-13.5 of the largest probability.  Together
+    under 2^-12, half a step of any fp16 value at least."""
+    say(f"growing maximum: n={n} T={T} start={start} capacity={capacity} rise={rise}")
+    pool, g, parents = growing_pool(gpu, n, T, start, capacity)
+    scale = HD ** -0.5
+    # dims 0 and 1 carry the score: 16 (1 + r) k[0] - 64 k[1]
+    steps = torch.arange(start, device=gpu) // 32
+    on = torch.arange(start, device=gpu) % 32 == 5
+    k = pool.k[0]
+    k[:, :, :, 1] = 60.0                                  # off: far below
+    k[:, :start, :, 1] = torch.where(on, 0.0, 60.0).half()[None, :, None]
+    unit = rise / (16.0 * scale * LOG2E)
+    k[:, :start, :, 0] = torch.where(on, steps * unit, torch.zeros(())).half()[None, :, None]
+    v = torch.randn(n, 1, 2, HD, generator=g).half().to(gpu)
+    pool.v[0].copy_(v.expand_as(pool.v[0]))
+    q = torch.zeros(n, T, 12, HD)
+    q[..., 0] = 16.0 * (1.0 + 0.5 * torch.rand(n, T, 12, generator=g))
+    q[..., 1] = -64.0
+    q = q.half().to(gpu)
+    cache = pool.tree_cache(i32(parents, gpu))
+    assert (*cache.form[:2], cache.form[3] > 0) == form
+    out = torch.zeros(n * T, 12, HD, device=gpu, dtype=torch.float16)
+    cache.attend_qkv(q.view(n * T, 12 * HD), 0, scale, out)
+    want = v.repeat_interleave(6, 2).expand(n, T, 12, HD)
+    off = (out.view(n, T, 12, HD) != want).sum().item()
+    say(f"  {off} of {out.numel()} outputs differ")
+    assert off == 0
+
+
+@pytest.mark.parametrize("n,T,start,capacity,form", GROWING)
+def test_tree_attention_wide_scores(gpu, n, T, start, capacity, form):
+    """Scores of some 8 standard deviations, keys boosted late in the context for some sequences:
+    maxima grow in most tiles, by less and by more than 2^8.  The bound is the oracle's and, twice
+    (numerator and denominator), that of a score's fp32 products and sums: 128 roundings of at
+    most sum |q k|."""
+    say(f"wide scores: n={n} T={T} start={start} capacity={capacity}")
+    pool, g, parents = growing_pool(gpu, n, T, start, capacity)
+    scale = HD ** -0.5
+    most = start + T
+    pool.storage[:, :, :, :most] = torch.randn(1, 2, n, most, 2, HD, generator=g).half().to(gpu)
+    pool.k[0][::2, start - 40:start - 20] *= 2.0
+    q = (8 * torch.randn(n, T, 12, HD, generator=g)).half()
+    few = sorted(random.Random(n).sample(range(n), min(n, 4)))
+    cache = pool.tree_cache(i32(parents, gpu))
+    assert (*cache.form[:2], cache.form[3] > 0) == form
+    out = torch.zeros(n * T, 12, HD, device=gpu, dtype=torch.float16)
+    cache.attend_qkv(q.to(gpu).view(n * T, 12 * HD), 0, scale, out)
+    out = out.view(n, T, 12, HD)[few].cpu().double()
+    assert out.isfinite().all()
+    k, v = pool.k[0][few].cpu(), pool.v[0][few].cpu()
+    want, mag, seen = ref.tree_attention(q[few], k, v, [start] * len(few), [parents[s] for s in few],
+                                         [T] * len(few), list(range(len(few))), scale)
+    products = (q[few].float().abs().view(len(few), T, 2, 6, HD).permute(0, 2, 1, 3, 4)
+                .reshape(len(few), 2, T * 6, HD)
+                @ k[:, :most].float().abs().permute(0, 2, 3, 1).contiguous()).amax().item()
+    score = 128 * 2.0 ** -24 * products * scale
+    bound = ref.attention_bound(want, mag, seen, v.float().abs().max().item()) + 2 * score * mag
+    worst = ((out - want).abs() / bound).max().item()
+    say(f"  worst error {worst:.2f} of the bound")
+    assert worst <= 1.0
