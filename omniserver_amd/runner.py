@@ -451,7 +451,9 @@ class MultimodalRunner(ModelRunner):
         drawn from, for chains alone; without them the tokens are proposals.  Greedy sequences
         keep the tokens that decode() would have produced, sampled ones are distributed as its.
         Returns the number of tokens each sequence has gained (a stop token or the length limit
-        ends a sequence early)."""
+        ends a sequence early).  Where nothing is left to draw a sequence's next token from (all
+        of its logits NaN or -inf) every other one advances as ever, that one by the drafted tokens
+        that stand, and a RuntimeError names its slot."""
         self.settle()
         n = len(seqs)
         if len(drafts) != n:
@@ -498,18 +500,24 @@ class MultimodalRunner(ModelRunner):
         v = run(step)
         out = torch.cat([v.tokens, v.emitted.to(torch.int64).unsqueeze(1)], 1).tolist()
         self._dev_ids_for = None
-        gained = [0] * n
-        for slot in range(n):
-            self._kv_len[slot] += out[slot][T]
+        gained, dry = [0] * n, []
         for slot, i in enumerate(order):
             seq, new = seqs[i], out[slot][:out[slot][T]]
+            if -1 in new:
+                # nothing to draw the next token from: the sequence keeps the drafted tokens that
+                # stand, the last of them still to be scored
+                new = new[:new.index(-1)]
+                dry.append(slot)
+            self._kv_len[slot] += len(new)
             for t in new:
-                if t < 0:
-                    raise RuntimeError(f"no token is left to draw for the sequence in slot {slot}")
                 seq.append_token(t)
                 gained[i] += 1
                 if seq.maybe_finish():
                     break
+        if dry:
+            self._pool.lengths[:n].copy_(to_device(self._kv_len[:n], torch.int64, dev))
+            raise RuntimeError(f"no token is left to draw for the sequences in slots {dry} (the others "
+                               f"have advanced)")
         return gained
 
     @staticmethod

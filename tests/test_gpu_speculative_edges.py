@@ -1,5 +1,5 @@
-"""Speculative decoding's operators on the GPU where their numerics turn: maxima that grow from tile
-to tile."""
+"""Speculative decoding on the GPU at its edges: attention maxima that grow from tile to tile, steps
+in which a sequence has nothing to draw from."""
 
 import math
 import random
@@ -104,3 +104,61 @@ def test_tree_attention_wide_scores(gpu, n, T, start, capacity, form):
     worst = ((out - want).abs() / bound).max().item()
     say(f"  worst error {worst:.2f} of the bound")
     assert worst <= 1.0
+
+
+# ----------------------------------------------------------------------------- the runner
+def started(shape, w, prompts, **kw):
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    from omniserver_amd.runner import NativeQwenVLRunner
+    r = NativeQwenVLRunner(max_running=len(prompts), max_len=128, weights=w, **kw)
+    seqs = [Sequence(Request(prompt=list(p), sampling=SamplingParams(max_new_tokens=40)))
+            for p in prompts]
+    for s in seqs:
+        r.tokenize(s)
+    r.prefill(seqs)
+    return r, seqs
+
+
+def test_runner_speculate_others_go_on(gpu, monkeypatch):
+    """The rows of one sequence NaN, at its last token or behind drafted ones that stand: it keeps
+    those, the others gain what they gain without it, and all decode on from there."""
+    from omniserver_amd import runner as runner_mod
+    from omniserver_amd import synth
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=9, num_layers=2)
+    prompts = [synth.random_ids(L, shape.vocab_size, 9, f"o{L}").tolist() for L in (9, 21, 33)]
+    r, seqs = started(shape, w, prompts)
+    for _ in range(4):
+        r.decode(seqs)
+    drafts = [s.output_token_ids[1:4] for s in seqs]
+    verify = runner_mod.verify
+
+    def run(node):
+        r, seqs = started(shape, w, prompts)
+        first = seqs[1].output_token_ids[0]
+
+        def tainted(logits, *a, **kw):
+            logits[1, torch.arange(3), torch.tensor(drafts[1])] = 60000.0    # the draft stands
+            if node is not None:
+                logits[1, node:] = math.nan
+            return verify(logits, *a, **kw)
+
+        monkeypatch.setattr(runner_mod, "verify", tainted)
+        if node is None:
+            r.speculate(seqs, drafts)
+        else:
+            with pytest.raises(RuntimeError, match=r"\[1\]"):
+                r.speculate(seqs, drafts)
+            assert seqs[1].output_token_ids == [first] + drafts[1][:node]
+        monkeypatch.setattr(runner_mod, "verify", verify)
+        for _ in range(2):
+            assert r._kv_len == [s.total_len - 1 for s in seqs]
+            assert r.pool.lengths[:3].tolist() == r._kv_len
+            r.decode(seqs)
+        return [list(s.output_token_ids) for s in seqs]
+
+    want = run(None)
+    for node in (0, 1, 3):
+        say(f"rows of one sequence NaN from node {node} on")
+        got = run(node)
+        assert got[0] == want[0] and got[2] == want[2]

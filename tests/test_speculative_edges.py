@@ -1,0 +1,53 @@
+"""Speculative decoding without a GPU where it ends badly: what the runner leaves behind."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+VOCAB = 50
+
+
+def bare_runner(lengths, emitted_tokens):
+    """A runner over a CPU pool, its step replaced: emitted_tokens [n][..] is what verification
+    gives, the pool's lengths move as acceptance moves them."""
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    from omniserver_amd.runner import MultimodalRunner
+    from omniserver_amd.speculative import Verified
+    n = len(lengths)
+    r = MultimodalRunner.__new__(MultimodalRunner)
+    r.adapter = SimpleNamespace(model=SimpleNamespace(cfg=SimpleNamespace(vocab_size=VOCAB)))
+    r.device = torch.device("cpu")
+    r._pool = PreallocatedKVCache(1, n + 1, 2, 64, 128, "cpu", n_heads=12)
+    r._pool.lengths[:n] = torch.tensor(lengths)
+    r._kv_len = list(lengths)
+    r._use_graph, r._ahead, r._dev_ids_for = False, None, None
+    seqs = [Sequence(Request(prompt=list(range(L)), sampling=SamplingParams(max_new_tokens=9)),
+                     prompt_token_ids=list(range(L)), kv_handle={"slot": s, "rope_delta": 0})
+            for s, L in enumerate(lengths)]
+    for s in seqs:
+        s.append_token(7)
+
+    def step(step):
+        T = step["ids"].shape[1]
+        tokens = torch.tensor([row + [-1] * (T - len(row)) for row in emitted_tokens])
+        emitted = torch.tensor([len(row) for row in emitted_tokens], dtype=torch.int32)
+        r._pool.lengths[:n] += emitted
+        return Verified(torch.zeros(n, T, dtype=torch.int32), tokens, emitted)
+
+    r._spec_step = step
+    return r, seqs
+
+
+def test_speculate_keeps_the_others_tokens():
+    """Sequences that nothing can be drawn for, one of them after a drafted token that stands: the
+    others have their tokens, everyone's cached rows are its tokens but the last."""
+    lengths = [10, 11, 12, 13]
+    emitted = [[5, 6], [-1], [8, -1], [9, 3, 4]]
+    r, seqs = bare_runner(lengths, emitted)
+    with pytest.raises(RuntimeError, match=r"\[1, 2\]"):
+        r.speculate(seqs, [[3, 0]] * 4)
+    assert [s.output_token_ids for s in seqs] == [[7, 5, 6], [7], [7, 8], [7, 9, 3, 4]]
+    assert r._kv_len == [s.total_len - 1 for s in seqs]
+    assert r._pool.lengths[:4].tolist() == r._kv_len
