@@ -497,8 +497,14 @@ class MultimodalRunner(ModelRunner):
             if draft_logits is not None and T > 1:
                 step["draft"] = draft_logits.index_select(0, to_device(order, torch.int64, dev))
         run = self._spec_graphed if self._use_graph and self.spec_graph_layouts else self._spec_step
-        v = run(step)
-        out = torch.cat([v.tokens, v.emitted.to(torch.int64).unsqueeze(1)], 1).tolist()
+        try:
+            v = run(step)
+            out = torch.cat([v.tokens, v.emitted.to(torch.int64).unsqueeze(1)], 1).tolist()
+        except BaseException:
+            # acceptance may have moved the lengths already (a capture behind the eager step that
+            # fails): without its tokens the step has not been
+            self._pool.lengths[:n].copy_(to_device(self._kv_len[:n], torch.int64, dev))
+            raise
         self._dev_ids_for = None
         gained, dry = [0] * n, []
         for slot, i in enumerate(order):

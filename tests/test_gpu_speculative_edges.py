@@ -162,3 +162,35 @@ def test_runner_speculate_others_go_on(gpu, monkeypatch):
         say(f"rows of one sequence NaN from node {node} on")
         got = run(node)
         assert got[0] == want[0] and got[2] == want[2]
+
+
+def test_runner_speculate_capture_that_fails(gpu):
+    """The first step of a layout runs, its capture fails: the call can be made again and gives
+    what it gives without the failure."""
+    from omniserver_amd import synth
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=10, num_layers=1)
+    prompts = [synth.random_ids(L, shape.vocab_size, 10, f"c{L}").tolist() for L in (9, 21)]
+    results = []
+    for fails in (False, True):
+        r, seqs = started(shape, w, prompts, use_graph=True)
+        if fails:
+            real, calls = r._spec_step, []
+
+            def step(s):
+                calls.append(0)
+                if len(calls) == 2:
+                    raise MemoryError("no room for the graph")
+                return real(s)
+
+            r._spec_step = step
+            before = r.pool.lengths.tolist()
+            with pytest.raises(MemoryError):
+                r.speculate(seqs, [[1, 2], [3]])
+            assert r.pool.lengths.tolist() == before and r._kv_len == before[:2]
+            assert [s.num_output_tokens for s in seqs] == [1, 1]
+        for _ in range(3):
+            r.speculate(seqs, [[1, 2], [3]])
+            assert r.pool.lengths[:2].tolist() == r._kv_len == [s.total_len - 1 for s in seqs]
+        results.append([list(s.output_token_ids) for s in seqs])
+    assert results[0] == results[1]

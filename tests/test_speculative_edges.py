@@ -51,3 +51,23 @@ def test_speculate_keeps_the_others_tokens():
     assert [s.output_token_ids for s in seqs] == [[7, 5, 6], [7], [7, 8], [7, 9, 3, 4]]
     assert r._kv_len == [s.total_len - 1 for s in seqs]
     assert r._pool.lengths[:4].tolist() == r._kv_len
+
+
+def test_speculate_that_fails_behind_acceptance():
+    """An error once the lengths have moved (a capture out of memory): the lengths as before, so
+    that the same call can be made again."""
+    r, seqs = bare_runner([10, 11], [[5, 6], [4]])
+    step = r._spec_step
+
+    def fails(s):
+        step(s)
+        raise MemoryError
+
+    r._spec_step = fails
+    with pytest.raises(MemoryError):
+        r.speculate(seqs, [[3], [3]])
+    assert r._pool.lengths[:2].tolist() == r._kv_len == [10, 11]
+    assert [s.output_token_ids for s in seqs] == [[7], [7]]
+    r._spec_step = step
+    assert r.speculate(seqs, [[3], [3]]) == [2, 1]
+    assert r._pool.lengths[:2].tolist() == r._kv_len == [12, 12]
