@@ -446,8 +446,8 @@ class MultimodalRunner(ModelRunner):
 
         ``drafts``: per sequence (in the order of ``seqs``) either a list of tokens to follow one
         another, or (tokens, parents) with each token's parent in that list (-1: the sequence's
-        last token), parents first; at most 63.  ``draft_logits`` [n, D, V] on the device (logits'
-        type fp16, D = the most tokens of a draft): row j of a sequence the logits its token j was
+        last token), parents first; at most 63.  ``draft_logits`` fp16 [n, D, V] on the device (D =
+        the most tokens of a draft): row j of a sequence the logits its token j was
         drawn from, for chains alone; without them the tokens are proposals.  Greedy sequences
         keep the tokens that decode() would have produced, sampled ones are distributed as its.
         Returns the number of tokens each sequence has gained (a stop token or the length limit
@@ -471,6 +471,9 @@ class MultimodalRunner(ModelRunner):
         if draft_logits is not None and tuple(draft_logits.shape) != (n, T - 1, vocab):
             raise ValueError(f"draft_logits {tuple(draft_logits.shape)}: expected "
                              f"{(n, T - 1, vocab)}")
+        if draft_logits is not None and draft_logits.dtype != torch.float16:
+            # (rounded to the logits' type they would no longer be what the tokens were drawn from)
+            raise TypeError(f"draft_logits are fp16, as the logits (got {draft_logits.dtype})")
         ids, parents, counts, temps = [], [], [], []
         for slot, i in enumerate(order):
             tokens, ups = trees[slot]

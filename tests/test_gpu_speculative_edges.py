@@ -194,3 +194,22 @@ def test_runner_speculate_capture_that_fails(gpu):
             assert r.pool.lengths[:2].tolist() == r._kv_len == [s.total_len - 1 for s in seqs]
         results.append([list(s.output_token_ids) for s in seqs])
     assert results[0] == results[1]
+
+
+def test_runner_speculate_draft_logits_of_another_type(gpu):
+    """Refused alike before a layout's first step, between that and a replay, and after."""
+    from omniserver_amd import synth
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=10, num_layers=1)
+    prompts = [synth.random_ids(L, shape.vocab_size, 10, f"c{L}").tolist() for L in (9, 21)]
+    r, seqs = started(shape, w, prompts, use_graph=True)
+    for s in seqs:
+        s.request.sampling.temperature = 0.9
+    draft = torch.randn(2, 2, shape.vocab_size, device=gpu)
+    for _ in range(3):
+        before = [list(s.output_token_ids) for s in seqs]
+        for other in (draft, draft.bfloat16()):
+            with pytest.raises(TypeError):
+                r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=other)
+        assert [s.output_token_ids for s in seqs] == before
+        r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=draft.half())

@@ -71,3 +71,13 @@ def test_speculate_that_fails_behind_acceptance():
     r._spec_step = step
     assert r.speculate(seqs, [[3], [3]]) == [2, 1]
     assert r._pool.lengths[:2].tolist() == r._kv_len == [12, 12]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_speculate_refuses_draft_logits_of_another_type(dtype):
+    r, seqs = bare_runner([10, 11], [[5], [4]])
+    for temperature in (0.0, 0.7):
+        seqs[0].request.sampling.temperature = temperature
+        with pytest.raises(TypeError):
+            r.speculate(seqs, [[3], [3]], draft_logits=torch.zeros(2, 1, VOCAB, dtype=dtype))
+    assert r._pool.lengths[:2].tolist() == r._kv_len == [10, 11]
