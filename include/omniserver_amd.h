@@ -170,7 +170,7 @@ int omni_tree_plan(const int* parents, const int* counts, const int64_t* slots,
  * out, fp16, strides in halfs) attends to keys [0, starts[s]) of its pool row and to starts[s] + j
  * for its ancestors j; nodes not in use and sequences outside the pool leave their out rows as
  * they were.  (rows, groups) of a workgroup as in omni_prefill_attention_rows: (128, 2), (64, 4) or
- * (32, 8), any number of query heads per KV head.  Where the plan cuts (least > 0) the
+ * (32, 8), G query heads per KV head with n_nodes G^2 up to 2^32.  Where the plan cuts (least > 0) the
  * softmax states of the pieces go through workspace (fp32, 16-byte aligned, columns * ceil(n_nodes
  * * n_heads / n_kv_heads / rows) * 2 * rows * 132 floats) to a second launch.  head_dim 128; scale
  * from 2^-126 to 2^126; 16-byte aligned operands. */

@@ -722,6 +722,11 @@ static bool tree_size_ok(int64_t n, int64_t nkv, int64_t columns, int max_len, i
          (!least || (columns <= 32767 && columns * units <= 0x7fffffff));
 }
 
+// A workgroup divides its (node, query head) rows by the heads' ratio through a 32-bit reciprocal.
+static bool tree_heads_ok(int n_nodes, int64_t ratio) {
+  return n_nodes * ratio * ratio <= (int64_t)1 << 32;
+}
+
 // schedule: [n][4] seqs, [ncols][8] columns, [n][nkv][2] heads
 static int64_t tree_schedule_ints(int n, int nkv, int ncols) {
   return 4 * (int64_t)n + 8 * (int64_t)ncols + 2 * (int64_t)n * nkv;
@@ -788,6 +793,7 @@ extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* 
   if (!form || columns < 1 || least < 0) return OMNI_EINVAL;
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
   if (!tree_size_ok(n, n_kv_heads, columns, max_len, unit, least)) return OMNI_EUNSUPPORTED;
+  if (!tree_heads_ok(n_nodes, n_heads / n_kv_heads)) return OMNI_EUNSUPPORTED;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
@@ -796,7 +802,7 @@ extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* 
     return OMNI_EINVAL;
   TreeArgs a;
   a.G = n_heads / n_kv_heads;
-  a.magic = 0xffffffffu / a.G + 1;                     // exact for rows below 2^32 / G
+  a.magic = 0xffffffffu / a.G + 1;                     // exact for rows below 2^32 / G: tree_heads_ok
   const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
   const int64_t grid = (columns + 7) / 8 * 8 * rblocks, out_rows = (int64_t)n * n_nodes * n_heads;
   if (grid > 0x7fffffff || out_rows > 0x7fffffff) return OMNI_EUNSUPPORTED;

@@ -1,11 +1,15 @@
-"""Speculative decoding without a GPU where it ends badly: what the runner leaves behind."""
+"""Speculative decoding without a GPU where it ends badly: what the runner leaves behind, sizes that
+the kernels do not take."""
 
+import ctypes
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 import torch
 
 VOCAB = 50
+P = ctypes.c_void_p(16)          # never read: the checks fail first
 
 
 def bare_runner(lengths, emitted_tokens):
@@ -81,3 +85,29 @@ def test_speculate_refuses_draft_logits_of_another_type(dtype):
         with pytest.raises(TypeError):
             r.speculate(seqs, [[3], [3]], draft_logits=torch.zeros(2, 1, VOCAB, dtype=dtype))
     assert r._pool.lengths[:2].tolist() == r._kv_len == [10, 11]
+
+
+# ----------------------------------------------------------------------------- sizes
+def attention_rc(n=2, nodes=8, nh=12, nkv=2, form=(64, 4), columns=4, least=0, q=None):
+    from omniserver_amd._lib import lib
+    return lib().omni_tree_attention(q, nh * 128, P, P, max(n, 1), 256, P, n, nodes, P, nh * 128, nh,
+                                     nkv, 128, 0.1, *form, columns, least, P, None, 0, None)
+
+
+@pytest.mark.parametrize("nodes,widest", [(64, 8192), (63, 8256), (17, 15894), (1, 65536)])
+def test_tree_attention_head_ratio(nodes, widest):
+    """Up to the widest ratio that is taken every row's node comes out right by the 32-bit
+    reciprocal; wider ones are refused (q is null: what passes the sizes ends there, -1)."""
+    for ratio in (widest, widest - 1, 6):
+        rows, magic = np.arange(nodes * ratio, dtype=np.uint64), np.uint64(0xffffffff // ratio + 1)
+        assert (rows * magic >> np.uint64(32) == rows // np.uint64(ratio)).all()
+        assert attention_rc(nodes=nodes, nh=ratio, nkv=1, columns=2) == -1
+    assert attention_rc(nodes=nodes, nh=widest + 1, nkv=1, columns=2) == -2
+
+
+def test_tree_attention_head_ratio_goes_wrong():
+    """Why: 64 nodes and a ratio of 16383 put row 278510 one node too far."""
+    row, ratio = 278510, 16383
+    assert row < 64 * ratio
+    assert row * (0xffffffff // ratio + 1) >> 32 == row // ratio + 1
+    assert attention_rc(nodes=64, nh=ratio, nkv=1, columns=2) == -2
