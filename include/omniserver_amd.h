@@ -140,7 +140,7 @@ int omni_kv_accept(void* pool, int n_layers, int pool_rows, int max_len, int row
                    const int* emitted, int n, int n_nodes, int64_t* lengths, void* stream);
 
 /* K/V rows fp16 [tokens][row_halfs] (strides in halfs, multiples of 8; 16-byte aligned) to pool
- * rows slots[t] at positions[t]; those outside the pool are skipped. */
+ * rows slots[t] at positions[t]; those outside the pool are skipped.  Up to 2^24 - 1 tokens. */
 int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                        void* k_cache, void* v_cache, const int64_t* slots,
                        const int64_t* positions, int pool_rows, int max_len, int row_halfs,
@@ -189,7 +189,7 @@ int omni_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
  * temperature) a node's child x stands if u (1 - p(tried siblings)) < p(x), with a draft if u q(x)
  * < p(x); the next token is drawn with u_0 from what is left of p.  Writes path int32, out_tokens
  * int64 [n][n_nodes] (-1 past emitted[s]) and emitted int32 [n].  workspace: doubles, as many as
- * omni_spec_verify_work gives (-1: too many to count). */
+ * omni_spec_verify_work gives (-2: too many rows for one launch). */
 int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted);
 int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t row_stride,
                      const void* draft, int64_t draft_seq_stride, int64_t draft_row_stride,

@@ -753,23 +753,28 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
 
 static_assert(sizeof(SvSeq) == 40, "five doubles");
 
+static int64_t sv_rows(int64_t n, int64_t T, bool drafted) {
+  return n * T + (drafted ? n * (T - 1) : 0);
+}
+
+// Doubles of workspace, -1 where they do not count in 32 bits or the statistics' threads do not.
 static int64_t sv_work(int64_t n, int64_t T, int64_t V, bool drafted) {
   const int64_t chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
-  const int64_t rows = n * T + (drafted ? n * (T - 1) : 0);
-  const int64_t blocks = (V + SV_BLOCK - 1) / SV_BLOCK;
-  return rows * blocks + 4 * n * chunks + 5 * n;        // records, sums, sequences, in doubles
+  const int64_t records = sv_rows(n, T, drafted) * ((V + SV_BLOCK - 1) / SV_BLOCK);
+  const int64_t work = records + 4 * n * chunks + 5 * n;        // records, sums, sequences
+  return work > 0x7fffffff || records * 64 * SV_WAVES > 0xffffffff ? -1 : work;
 }
 
 extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted) {
   if (n < 0 || n_nodes < 1 || vocab < 1) return OMNI_EINVAL;
   if (n_nodes > SV_MAX_NODES || vocab > 1 << 30) return OMNI_EUNSUPPORTED;
   const int64_t work = sv_work(n, n_nodes, vocab, drafted);
-  return work > 0x7fffffff ? OMNI_EUNSUPPORTED : (int)work;
+  return work < 0 ? OMNI_EUNSUPPORTED : (int)work;
 }
 
 template <int DT>
 static void sv_launch(const SvArgs& a, hipStream_t st) {
-  const int rows = a.n * a.T + (a.draft ? a.n * (a.T - 1) : 0);
+  const int rows = (int)sv_rows(a.n, a.T, a.draft);
   hipLaunchKernelGGL((sv_stats_kernel<DT>), dim3(rows * a.blocks), dim3(64 * SV_WAVES), 0, st, a);
   hipLaunchKernelGGL((sv_walk_kernel<DT>), dim3(a.n * a.parts), dim3(64 * SV_WAVES), 0, st, a);
   if (a.uniforms)                                       // else every row is greedy
@@ -793,7 +798,7 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   if (!logits || !tokens || !path || !out_tokens || !emitted) return OMNI_EINVAL;
   if (n_nodes == 1) draft = nullptr;
   const int64_t work = sv_work(n, n_nodes, vocab, draft != nullptr);
-  if (work > 0x7fffffff) return OMNI_EUNSUPPORTED;
+  if (work < 0) return OMNI_EUNSUPPORTED;
   if (!workspace || ((uintptr_t)workspace & 7) || workspace_doubles < work) return OMNI_EINVAL;
   SvArgs a;
   a.logits = logits;
@@ -818,8 +823,7 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   a.out_tokens = out_tokens;
   a.emitted = emitted;
   a.rec = (float2*)workspace;
-  const int64_t rows = (int64_t)n * n_nodes + (draft ? (int64_t)n * (n_nodes - 1) : 0);
-  a.sums = (double*)workspace + rows * a.blocks;
+  a.sums = (double*)workspace + sv_rows(n, n_nodes, draft) * a.blocks;
   a.seqs = (SvSeq*)(a.sums + 4 * (int64_t)n * a.chunks);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) sv_launch<0>(a, st);

@@ -764,7 +764,7 @@ extern "C" int omni_kv_write_rows(const void* k, int64_t k_stride, const void* v
                                   const int64_t* positions, int pool_rows, int max_len,
                                   int row_halfs, int tokens, void* stream) {
   if (tokens < 0 || pool_rows <= 0 || max_len <= 0 || row_halfs <= 0) return OMNI_EINVAL;
-  if ((row_halfs & 7) || (k_stride & 7) || (v_stride & 7)) return OMNI_EUNSUPPORTED;
+  if ((row_halfs & 7) || (k_stride & 7) || (v_stride & 7) || tokens > 0xffffff) return OMNI_EUNSUPPORTED;
   if (k_stride < row_halfs || v_stride < row_halfs) return OMNI_EINVAL;
   if (tokens == 0) return OMNI_OK;
   if (!k || !v || !k_cache || !v_cache || !slots || !positions) return OMNI_EINVAL;
@@ -794,6 +794,14 @@ extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* 
   if (!least && columns != (int64_t)n * n_kv_heads && n) return OMNI_EINVAL;
   if (!tree_size_ok(n, n_kv_heads, columns, max_len, unit, least)) return OMNI_EUNSUPPORTED;
   if (!tree_heads_ok(n_nodes, n_heads / n_kv_heads)) return OMNI_EUNSUPPORTED;
+  const int64_t rblocks = ((int64_t)n_nodes * (n_heads / n_kv_heads) + rows - 1) / rows;
+  const int64_t grid = (columns + 7) / 8 * 8 * rblocks, out_rows = (int64_t)n * n_nodes * n_heads;
+  // the merge: parts of an item are at least one, some columns / items
+  const bool wide = columns > 8 * (int64_t)n * n_kv_heads;
+  const int64_t merges = !least ? 0 : wide ? out_rows : (out_rows + 7) / 8;
+  // a launch counts its threads in 32 bits
+  if (512 * grid > 0xffffffff || 256 * merges > 0xffffffff || out_rows > 0x7fffffff)
+    return OMNI_EUNSUPPORTED;
   if (q_stride < n_heads * TREE_HD || (q_stride & 7)) return OMNI_EINVAL;
   if (out_stride < n_heads * TREE_HD || (out_stride & 7)) return OMNI_EINVAL;
   if (n == 0) return OMNI_OK;
@@ -803,9 +811,6 @@ extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* 
   TreeArgs a;
   a.G = n_heads / n_kv_heads;
   a.magic = 0xffffffffu / a.G + 1;                     // exact for rows below 2^32 / G: tree_heads_ok
-  const int64_t rblocks = ((int64_t)n_nodes * a.G + rows - 1) / rows;
-  const int64_t grid = (columns + 7) / 8 * 8 * rblocks, out_rows = (int64_t)n * n_nodes * n_heads;
-  if (grid > 0x7fffffff || out_rows > 0x7fffffff) return OMNI_EUNSUPPORTED;
   if (least && (!workspace || ((uintptr_t)workspace & 15) ||
                 workspace_floats < columns * rblocks * 2 * rows * ATT_REC))
     return OMNI_EINVAL;
@@ -836,14 +841,13 @@ extern "C" int omni_tree_attention(const void* q, int64_t q_stride, const void* 
     hipLaunchKernelGGL((tree_attn_kernel<1, 8, 32>), gd, dim3(512), 0, st, a);
   OMNI_CHECK_LAUNCH();
   if (least) {
-    // parts of an item: at least one, some columns / items
     const int* heads = a.columns + 8 * (int64_t)columns;
-    if (columns > 8 * (int64_t)n * n_kv_heads)
-      hipLaunchKernelGGL((tree_merge_kernel<8>), dim3((unsigned)out_rows), dim3(256), 0, st, a, heads,
+    if (wide)
+      hipLaunchKernelGGL((tree_merge_kernel<8>), dim3((unsigned)merges), dim3(256), 0, st, a, heads,
                          rows, out_rows);
     else
-      hipLaunchKernelGGL((tree_merge_kernel<1>), dim3((unsigned)((out_rows + 7) / 8)), dim3(256), 0, st,
-                         a, heads, rows, out_rows);
+      hipLaunchKernelGGL((tree_merge_kernel<1>), dim3((unsigned)merges), dim3(256), 0, st, a, heads,
+                         rows, out_rows);
     OMNI_CHECK_LAUNCH();
   }
   return OMNI_OK;

@@ -111,3 +111,25 @@ def test_tree_attention_head_ratio_goes_wrong():
     assert row < 64 * ratio
     assert row * (0xffffffff // ratio + 1) >> 32 == row // ratio + 1
     assert attention_rc(nodes=64, nh=ratio, nkv=1, columns=2) == -2
+
+
+def test_launches_that_do_not_count_in_32_bits():
+    """A launch counts its threads in 32 bits: more rows are refused before any of a call's launches
+    goes out."""
+    from omniserver_amd._lib import lib
+    work = lib().omni_spec_verify_work
+    assert work((1 << 18) - 1, 64, 100, 0) > 0 and work(1 << 18, 64, 100, 0) == -2
+    assert work((1 << 18) - 1, 33, 100, 1) == -2 and work(1 << 12, 64, 8192 * 64, 0) == -2
+    assert work(1 << 17, 64, 8192, 0) > 0 and work(1 << 17, 64, 8193, 0) == -2
+    for n, rc in (((1 << 18) - 1, -1), (1 << 18, -2)):          # without a workspace
+        assert lib().omni_spec_verify(P, 0, 6400, 100, None, 0, 0, P, None, None, None, None, 0.0, n,
+                                      64, 100, P, P, P, None, 0, None) == rc
+    write = lambda n: lib().omni_kv_write_rows(None, 256, P, 256, P, P, P, P, 4, 64, 256, n, None)  # noqa: E731
+    assert write((1 << 24) - 1) == -1 and write(1 << 24) == -2
+    # 8 workgroups a column at 64 nodes of 16 heads, columns in eights
+    wide = {"nodes": 64, "nkv": 16, "nh": 256, "form": (128, 2)}
+    assert attention_rc(n=(1 << 16) - 2, columns=16 * ((1 << 16) - 2), **wide) == -1
+    assert attention_rc(n=1 << 16, columns=1 << 20, **wide) == -2
+    # a merge of a wave's half a row, eight rows a workgroup
+    cut = {"nodes": 64, "nkv": 8, "nh": 64, "form": (128, 2), "columns": 32760, "least": 1}
+    assert attention_rc(n=(1 << 15) - 1, **cut) == -1 and attention_rc(n=1 << 15, **cut) == -2
