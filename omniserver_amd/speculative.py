@@ -59,25 +59,22 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | 
     A NaN logit counts as -inf; where no token is above -inf the next token is -1.  The same
     inputs give the same tokens: those of 64-bit weights and sums, which the 32-bit sums of the rows
     stand for only where they cannot change what is decided."""
-    checked = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
+    draft, work = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
     n, T, V = logits.shape
     dev = logits.device
     out = Verified(torch.empty(n, T, device=dev, dtype=torch.int32),
                    torch.empty(n, T, device=dev, dtype=torch.int64),
                    torch.empty(n, device=dev, dtype=torch.int32))
-    return _launch(logits, tokens, uniforms, temperature, out, parents, counts, *checked)
-
-
-def verify_out(logits, tokens, uniforms, temperature, out: Verified, parents=None,
-               draft_logits=None, counts=None) -> Verified:
-    """verify into the caller's tensors."""
-    checked = _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
-    n, T, V = logits.shape
-    _is(out.path, (n, T), torch.int32, "path")
-    _is(out.tokens, (n, T), torch.int64, "out tokens")
-    _is(out.emitted, (n,), torch.int32, "emitted")
-    require_here(*out)
-    return _launch(logits, tokens, uniforms, temperature, out, parents, counts, *checked)
+    ws = torch.empty(work, device=dev, dtype=torch.float64)
+    per_row = isinstance(temperature, torch.Tensor)
+    s0, s1, _ = logits.stride()
+    d0, d1, _ = (0, 0, 1) if draft is None else draft.stride()
+    call("omni_spec_verify", logits.data_ptr(), _DTYPES[logits.dtype], s0, s1, ptr(draft), d0, d1,
+         tokens.data_ptr(), ptr(parents), ptr(counts), ptr(uniforms),
+         temperature.data_ptr() if per_row else None, 0.0 if per_row else float(temperature), n, T,
+         V, out.path.data_ptr(), out.tokens.data_ptr(), out.emitted.data_ptr(), ws.data_ptr(), work,
+         stream())
+    return out
 
 
 def _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts) -> tuple:
@@ -118,20 +115,6 @@ def _check(logits, tokens, uniforms, temperature, parents, draft_logits, counts)
     if work < 0:
         raise ValueError(f"{n} sequences of {T} nodes over a vocabulary of {V}: too large")
     return draft_logits, work
-
-
-def _launch(logits, tokens, uniforms, temperature, out, parents, counts, draft, work) -> Verified:
-    n, T, V = logits.shape
-    ws = torch.empty(work, device=logits.device, dtype=torch.float64)
-    per_row = isinstance(temperature, torch.Tensor)
-    s0, s1, _ = logits.stride()
-    d0, d1, _ = (0, 0, 1) if draft is None else draft.stride()
-    call("omni_spec_verify", logits.data_ptr(), _DTYPES[logits.dtype], s0, s1, ptr(draft), d0, d1,
-         tokens.data_ptr(), ptr(parents), ptr(counts), ptr(uniforms),
-         temperature.data_ptr() if per_row else None, 0.0 if per_row else float(temperature), n, T,
-         V, out.path.data_ptr(), out.tokens.data_ptr(), out.emitted.data_ptr(), ws.data_ptr(), work,
-         stream())
-    return out
 
 
 def _is(t, shape, dtype, name: str) -> None:
