@@ -188,8 +188,8 @@ int omni_tree_attention(const void* q, int64_t q_stride, const void* k_cache, co
  * NULL and temp for all (0: greedy, uniforms may then be NULL).  With p = softmax(logits /
  * temperature) a node's child x stands if u (1 - p(tried siblings)) < p(x), with a draft if u q(x)
  * < p(x); the next token is drawn with u_0 from what is left of p.  Writes path int32, out_tokens
- * int64 [n][n_nodes] (-1 past emitted[s]) and emitted int32 [n].  workspace: doubles, as many as
- * omni_spec_verify_work gives (-2: too many rows for one launch). */
+ * int64 [n][n_nodes] (-1 past emitted[s]) and emitted int32 [n], none of them over an input.
+ * workspace: doubles, as many as omni_spec_verify_work gives (-2: too many rows for one launch). */
 int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted);
 int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t row_stride,
                      const void* draft, int64_t draft_seq_stride, int64_t draft_row_stride,

@@ -772,6 +772,12 @@ extern "C" int omni_spec_verify_work(int n, int n_nodes, int vocab, int drafted)
   return work < 0 ? OMNI_EUNSUPPORTED : (int)work;
 }
 
+// Every workgroup of a sequence walks its tree while the first one writes the outcome.
+static bool sv_apart(const void* out, int64_t out_bytes, const void* in, int64_t in_bytes) {
+  const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+  return !in || o + out_bytes <= i || i + in_bytes <= o;
+}
+
 template <int DT>
 static void sv_launch(const SvArgs& a, hipStream_t st) {
   const int rows = (int)sv_rows(a.n, a.T, a.draft);
@@ -800,6 +806,16 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   const int64_t work = sv_work(n, n_nodes, vocab, draft != nullptr);
   if (work < 0) return OMNI_EUNSUPPORTED;
   if (!workspace || ((uintptr_t)workspace & 7) || workspace_doubles < work) return OMNI_EINVAL;
+  const int64_t nodes = (int64_t)n * n_nodes;
+  const void* outs[3] = {path, out_tokens, emitted};
+  const int64_t out_bytes[3] = {4 * nodes, 8 * nodes, 4 * (int64_t)n};
+  for (int k = 0; k < 3; ++k)
+    if (!sv_apart(outs[k], out_bytes[k], tokens, 8 * nodes) ||
+        !sv_apart(outs[k], out_bytes[k], parents, 4 * nodes) ||
+        !sv_apart(outs[k], out_bytes[k], counts, 4 * (int64_t)n) ||
+        !sv_apart(outs[k], out_bytes[k], uniforms, 4 * nodes) ||
+        !sv_apart(outs[k], out_bytes[k], temperature, 4 * (int64_t)n))
+      return OMNI_EINVAL;
   SvArgs a;
   a.logits = logits;
   a.seq_stride = seq_stride;

@@ -133,3 +133,23 @@ def test_launches_that_do_not_count_in_32_bits():
     # a merge of a wave's half a row, eight rows a workgroup
     cut = {"nodes": 64, "nkv": 8, "nh": 64, "form": (128, 2), "columns": 32760, "least": 1}
     assert attention_rc(n=(1 << 15) - 1, **cut) == -1 and attention_rc(n=1 << 15, **cut) == -2
+
+
+def test_verify_outputs_over_inputs():
+    """Outputs that lie over an input other workgroups still read: refused, before a launch."""
+    from omniserver_amd._lib import lib
+    n, T = 3, 8
+    at = {"tokens": (1 << 20, 8 * n * T), "parents": (2 << 20, 4 * n * T), "counts": (3 << 20, 4 * n),
+          "u": (4 << 20, 4 * n * T), "temps": (5 << 20, 4 * n)}
+    outs = {"path": 4 * n * T, "out": 8 * n * T, "emitted": 4 * n}
+
+    def rc(**kw):
+        a = {k: v[0] for k, v in at.items()} | {"path": 6 << 20, "out": 7 << 20, "emitted": 9 << 20} | kw
+        p = {k: ctypes.c_void_p(v) for k, v in a.items()}
+        return lib().omni_spec_verify(P, 0, 800, 100, None, 0, 0, p["tokens"], p["parents"],
+                                      p["counts"], p["u"], p["temps"], 0.0, n, T, 100, p["path"],
+                                      p["out"], p["emitted"], P, 1 << 20, None)
+
+    for name, (start, size) in at.items():
+        for o, osize in outs.items():
+            assert rc(**{o: start}) == rc(**{o: start + size - 4}) == rc(**{o: start - osize + 4}) == -1
