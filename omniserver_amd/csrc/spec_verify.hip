@@ -93,20 +93,22 @@ __device__ __forceinline__ int sv_used(const SvArgs& a, int s) {
 }
 
 // 2^t for -2100 <= t <= 0: t = n + f, |f| <= 1/2, n from the low word of t + 1.5 2^52, 2^f by the
-// polynomial through its values at the nine Chebyshev points of [-1/2, 1/2] (relative error
-// 1.1e-12), 2^n by the exponent (0 far below).  That error moves a border between two tokens of 1e-6
-// each across one draw in 10^6.
+// polynomial through its values at the eleven Chebyshev points of [-1/2, 1/2] (relative error 4e-16,
+// its roundings included), 2^n by the exponent (0 far below).  Nine points are off by 1.1e-12: a
+// random number that near to a border between two tokens would draw the other one.
 __device__ __forceinline__ double sv_exp2(double t) {
 #pragma clang fp contract(off)          // the same wherever it is inlined
   const double a = t + 0x1.8p52, f = t - (a - 0x1.8p52);
-  double r = 0x1.63d136366db24p-20;
-  r = fma(r, f, 0x1.00dc4a532fb8ep-16);
-  r = fma(r, f, 0x1.4308ac85aa947p-13);
-  r = fma(r, f, 0x1.5d8745a728441p-10);
-  r = fma(r, f, 0x1.3b2ab7181b755p-7);
-  r = fma(r, f, 0x1.c6b08dd6fd234p-5);
-  r = fma(r, f, 0x1.ebfbdff823cedp-3);
-  r = fma(r, f, 0x1.62e42fef84cf0p-1);
+  double r = 0x1.e6063f7217bc6p-28;
+  r = fma(r, f, 0x1.b675bca4eeebbp-24);
+  r = fma(r, f, 0x1.62bfd47773353p-20);
+  r = fma(r, f, 0x1.ffcb54062e698p-17);
+  r = fma(r, f, 0x1.430913096fd9fp-13);
+  r = fma(r, f, 0x1.5d87fe9d7a584p-10);
+  r = fma(r, f, 0x1.3b2ab6fba1ddap-7);
+  r = fma(r, f, 0x1.c6b08d703ce49p-5);
+  r = fma(r, f, 0x1.ebfbdff82c598p-3);
+  r = fma(r, f, 0x1.62e42fefa3a19p-1);
   r = fma(r, f, 1.0);
   return ldexp(r, (int)(uint32_t)__builtin_bit_cast(uint64_t, a));
 }

@@ -4,6 +4,7 @@ in which a sequence has nothing to draw from."""
 import math
 import random
 
+import numpy as np
 import pytest
 import torch
 
@@ -213,3 +214,31 @@ def test_runner_speculate_draft_logits_of_another_type(gpu):
                 r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=other)
         assert [s.output_token_ids for s in seqs] == before
         r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=draft.half())
+
+
+# ----------------------------------------------------------------------------- verification
+def test_verify_draws_with_64_bit_weights(gpu):
+    """Two tokens of weights 1 and w = exp(-x), random numbers 2e-14 to 4e-13 (relative) from the
+    border 1 / (1 + w): what 64-bit weights draw.  Their roundings come to some 1e-15."""
+    from omniserver_amd.speculative import verify
+    rng = np.random.default_rng(3)
+    rows, us, want = [], [], []
+    for _ in range(8):
+        x = rng.uniform(0.01, 3.0, 1 << 21).astype(np.float32)
+        total = 1.0 + np.exp(-x.astype(np.float64))
+        u = (1.0 / total).astype(np.float32)
+        gap = u.astype(np.float64) * total - 1.0
+        near = (np.abs(gap) > 2e-14) & (np.abs(gap) < 4e-13)
+        rows.append(-x[near])
+        us.append(u[near])
+        want.append(gap[near] >= 0)
+    x, u, want = (torch.from_numpy(np.concatenate(a)) for a in (rows, us, want))
+    n = x.numel()
+    say(f"{n} draws by the border")
+    assert n > 100
+    logits = torch.stack([torch.zeros(n), x], 1).view(n, 1, 2)
+    got = verify(logits.to(gpu), torch.zeros(n, 1, dtype=torch.int64, device=gpu),
+                 u.view(n, 1).to(gpu), 1.0)
+    off = (got.tokens[:, 0].cpu() != want.long()).sum().item()
+    say(f"  {off} differ")
+    assert off == 0
