@@ -24,7 +24,12 @@
 // max(p - q, 0) is summed without knowing both rows' 64-bit totals first: with weights p, q not yet
 // normalised it is max(p - r q, 0), r = the totals' ratio.  From the 32-bit ratio r0 the walk sums
 // max(p - r0 q, 0) and the q of its positive terms, and the draw moves the sums by (r0 - r) times
-// the latter: exact but for the terms whose sign changes between r0 and r, 1e-12 of the total.
+// the latter: exact but for terms that change sign between r0 and r.  The walk also sums the q of
+// the terms within 2^-20 r0 q of zero (what r0 is good to): a chunk where |r - r0| times these is
+// more than 2^-48 of the residual's total is summed anew by the draw, at r, and so are all where r
+// is further off.  151936 tokens have one such chunk in some 4 draws.  Where a draft is next to its
+// target the residual is hardly more than those terms and all chunks are: a call of 32 such
+// sequences takes 160-190 us, of others like them 43-46.
 #include "common.h"
 
 #define SV_MAX_NODES 64
@@ -33,6 +38,8 @@
 #define SV_CHUNK 1024              // tokens a wave sums in 64 bits: 16 a lane
 #define SV_PARTS 768              // workgroups of the walk in all: more walk again what others walk
 #define SV_ERR 0x1p-18             // relative error of a row's 32-bit sum, with a factor 4 to spare
+#define SV_BAND 0x1p-20            // of r0: what two 32-bit sums' ratio is mostly good to
+#define SV_SUMS 5                  // 64-bit sums of a chunk
 
 enum { SV_DONE = 0, SV_TARGET = 1, SV_RESIDUAL = 2 };   // where the next token comes from
 
@@ -53,7 +60,8 @@ struct SvArgs {
   int64_t* out_tokens;
   int* emitted;
   float2* rec;             // [n T target rows, n (T - 1) draft rows][blocks] (largest, sum or index)
-  double* sums;            // [4][n][chunks]: target, draft, residual at r0, its draft weights
+  double* sums;            // [SV_SUMS][n][chunks]: target, draft, residual at r0, its draft weights,
+                           // draft weights of the terms about zero
   struct SvSeq* seqs;      // [n]
 };
 
@@ -359,15 +367,16 @@ __device__ __forceinline__ double sv_chunk_sum(const void* row, int chunk, int V
   return wave_total(z[0] + z[1]);
 }
 
-// A chunk's 64-bit sums of p, of q, of max(p - r0 q, 0) and of the q of its positive terms.
+// A chunk's 64-bit sums of p, of q, of max(p - r0 q, 0), of the q of its positive terms and of the
+// q of those about zero.
 template <int DT>
 __device__ __forceinline__ void sv_residual_sums(const void* row, const void* drow, int chunk, int V,
                                                  int lane, const SvRow& wp, const SvRow& wq, double r0,
-                                                 double (&z)[4]) {
+                                                 double (&z)[SV_SUMS]) {
 #pragma clang fp contract(off)          // equal rows leave exactly nothing
   typedef SvPiece<DT> P;
   const int v0 = chunk * SV_CHUNK;
-  z[0] = z[1] = z[2] = z[3] = 0.0;
+  for (int k = 0; k < SV_SUMS; ++k) z[k] = 0.0;
   P nx, ny;
   nx.load(row, v0, V, lane, 0);
   ny.load(drow, v0, V, lane, 0);
@@ -380,15 +389,16 @@ __device__ __forceinline__ void sv_residual_sums(const void* row, const void* dr
     }
 #pragma unroll
     for (int e = 0; e < P::N; ++e) {
-      const double p = wp.weight(x.get(e)), q = wq.weight(y.get(e)), d = p - r0 * q;
+      const double p = wp.weight(x.get(e)), q = wq.weight(y.get(e)), rq = r0 * q, d = p - rq;
       z[0] += p;
       z[1] += q;
       z[2] += d > 0.0 ? d : 0.0;
       z[3] += d > 0.0 ? q : 0.0;
+      z[4] += fabs(d) <= SV_BAND * rq ? q : 0.0;
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) z[k] = wave_total(z[k]);
+  for (int k = 0; k < SV_SUMS; ++k) z[k] = wave_total(z[k]);
 }
 
 // ---------------------------------------------------------------------------
@@ -591,11 +601,11 @@ __global__ __launch_bounds__(64 * SV_WAVES) void sv_walk_kernel(SvArgs a) {
   const int64_t next = (int64_t)a.n * a.chunks;
   for (int k = mine * SV_WAVES + wave; k < a.chunks; k += a.parts * SV_WAVES) {
     if (residual) {
-      double z[4];
+      double z[SV_SUMS];
       sv_residual_sums<DT>(sv_row<DT>(a, s, last), sv_draft_row<DT>(a, s, last), k, a.V, lane, wp, wq,
                            r0, z);
       if (lane == 0)
-        for (int d = 0; d < 4; ++d) sums[d * next + k] = z[d];
+        for (int d = 0; d < SV_SUMS; ++d) sums[d * next + k] = z[d];
     } else {
       const double z = sv_chunk_sum<DT>(sv_row<DT>(a, s, last), k, a.V, lane, wp, tok, tried);
       if (lane == 0) sums[k] = z;
@@ -635,21 +645,42 @@ __global__ __launch_bounds__(256) void sv_draw_kernel(SvArgs a) {
       }
       __syncthreads();                                  // both turns' sums are this workgroup's
     }
+    const double r0 = q.r0;
     double ratio = 0.0;
     if (residual) {
-      double zp = 0.0, zq = 0.0;
-      for (int k = lane; k < a.chunks; k += 64) {
-        zp += sums[k];
-        zq += sums[next + k];
+      double z[SV_SUMS] = {};
+      for (int k = lane; k < a.chunks; k += 64)
+#pragma unroll
+        for (int d = 0; d < SV_SUMS; ++d) z[d] += sums[d * next + k];
+#pragma unroll
+      for (int d = 0; d < SV_SUMS; ++d) z[d] = wave_total(z[d]);
+      ratio = z[1] > 0.0 ? z[0] / z[1] : 0.0;
+      const double off = fabs(r0 - ratio), least = 0x1p-48 * (z[2] + (r0 - ratio) * z[3]);
+      const bool all = off > SV_BAND * r0;
+      if (all || off * z[4] > least) {                  // the same in every wave
+        __syncthreads();                                // all have read the sums
+        int turn_of = 0;
+        for (int k0 = 0; k0 < a.chunks; k0 += 64) {
+          const int k = k0 + lane;
+          uint64_t open = __ballot(k < a.chunks && (all || off * sums[4 * next + k] > least));
+          for (; open; open &= open - 1, ++turn_of) {
+            if ((turn_of & 3) != wave) continue;
+            const int c = k0 + __ffsll((unsigned long long)open) - 1;
+            sv_residual_sums<DT>(row, drow, c, a.V, lane, wp, wq, ratio, z);
+            if (lane == 0) {
+              sums[2 * next + c] = z[2];
+              sums[3 * next + c] = 0.0;                 // at the 64-bit ratio already
+            }
+          }
+        }
+        __syncthreads();
       }
-      zq = wave_total(zq);
-      ratio = zq > 0.0 ? wave_total(zp) / zq : 0.0;
     }
     auto chunk_sum = [&](int k) {
 #pragma clang fp contract(off)
       if (k >= a.chunks) return 0.0;
       if (!residual) return sums[k];
-      return fmax(sums[2 * next + k] + (q.r0 - ratio) * sums[3 * next + k], 0.0);
+      return fmax(sums[2 * next + k] + (r0 - ratio) * sums[3 * next + k], 0.0);
     };
     if (wave == 0) {
       // 256 chunks at a time: their sums' loads together
@@ -763,7 +794,7 @@ static int64_t sv_rows(int64_t n, int64_t T, bool drafted) {
 static int64_t sv_work(int64_t n, int64_t T, int64_t V, bool drafted) {
   const int64_t chunks = (V + SV_CHUNK - 1) / SV_CHUNK;
   const int64_t records = sv_rows(n, T, drafted) * ((V + SV_BLOCK - 1) / SV_BLOCK);
-  const int64_t work = records + 4 * n * chunks + 5 * n;        // records, sums, sequences
+  const int64_t work = records + SV_SUMS * n * chunks + 5 * n;  // records, sums, sequences
   return work > 0x7fffffff || records * 64 * SV_WAVES > 0xffffffff ? -1 : work;
 }
 
@@ -842,7 +873,7 @@ extern "C" int omni_spec_verify(const void* logits, int dtype, int64_t seq_strid
   a.emitted = emitted;
   a.rec = (float2*)workspace;
   a.sums = (double*)workspace + sv_rows(n, n_nodes, draft) * a.blocks;
-  a.seqs = (SvSeq*)(a.sums + 4 * (int64_t)n * a.chunks);
+  a.seqs = (SvSeq*)(a.sums + SV_SUMS * (int64_t)n * a.chunks);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) sv_launch<0>(a, st);
   else if (dtype == 1) sv_launch<1>(a, st);

@@ -242,3 +242,36 @@ def test_verify_draws_with_64_bit_weights(gpu):
     off = (got.tokens[:, 0].cpu() != want.long()).sum().item()
     say(f"  {off} differ")
     assert off == 0
+
+
+@pytest.mark.parametrize("V,noise", [(9001, 1e-6), (40000, 1e-6), (40000, 3e-7), (40000, 1e-4),
+                                     (40000, 0.0)])
+def test_verify_draft_next_to_the_target(gpu, V, noise):
+    """Drafts that are the target but for `noise` and one token of little mass that they overrate:
+    max(p - q, 0) comes to some 10^-6 of p, and its terms' signs hang on the totals' ratio in 64
+    bits.  The order of 64-bit sums moves a border by some 10^-10 of that total, one draw in 10^5."""
+    from omniserver_amd.speculative import verify
+    say(f"draft next to the target: V={V} noise={noise}")
+    g = torch.Generator().manual_seed(5)
+    m, draws = 24, 64
+    target = torch.randn(m, V, generator=g) * 2
+    target.scatter_add_(1, torch.randint(0, V, (m, 6), generator=g), torch.full((m, 6), 9.0))
+    draft = target + noise * torch.randn(m, V, generator=g)
+    p = torch.softmax(target.double(), -1)
+    x = (p - 1e-8).abs().argmin(-1)
+    draft[torch.arange(m), x] += 3.0
+    us = (torch.arange(draws) + 0.5) / draws
+    assert (0.9 * torch.softmax(draft.double(), -1)[torch.arange(m), x] > p[torch.arange(m), x]).all()
+    want = []
+    for t, d in zip(target, draft):
+        left = (ref.weights(t, 1.0) - ref.weights(d, 1.0)).clamp(min=0.0)
+        run = left.cumsum(0)
+        want += torch.searchsorted(run, us.double() * run[-1], right=True).tolist()
+    each = lambda y: y.to(gpu).repeat_interleave(draws, 0)  # noqa: E731
+    u = torch.stack([us.repeat(m), torch.full((m * draws,), 0.9)], 1).to(gpu)
+    tokens = torch.stack([torch.zeros_like(x), x], 1)
+    got = verify(each(torch.stack([target, target], 1)), each(tokens), u, 1.0,
+                 draft_logits=each(draft[:, None]))
+    off = (got.tokens[:, 0].cpu() != torch.tensor(want)).sum().item()
+    say(f"  {off} of {len(want)} draws differ")
+    assert got.emitted.eq(1).all() and off == 0
