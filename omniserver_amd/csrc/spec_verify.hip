@@ -15,7 +15,7 @@
 // -inf; a row without a token above -inf accepts nothing and gives -1.
 //
 // Every row is read once, in 32 bits: largest logit and sum of weights per 8192 tokens (the bound
-// is the rows' bytes).  A test that these sums leave open - they are good to 2^-18, so one in some
+// is the rows' bytes).  A test that these sums leave open - they are good to 2^-17, so one in some
 // 10^5 - is decided by a 64-bit sum of its row.  Where a random number falls among 151936 tokens
 // is a matter of borders 1e-6 apart and closer, which 32-bit sums would move across one draw in a
 // few hundred: the one row per sequence that the next token comes from is summed and searched in
@@ -37,7 +37,11 @@
 #define SV_BLOCK 8192              // tokens of a workgroup in 32 bits: 32 a lane
 #define SV_CHUNK 1024              // tokens a wave sums in 64 bits: 16 a lane
 #define SV_PARTS 768              // workgroups of the walk in all: more walk again what others walk
-#define SV_ERR 0x1p-18             // relative error of a row's 32-bit sum, with a factor 4 to spare
+// Relative error of a row's 32-bit sum.  A weight 2^t is off by |t| ln 2 of the roundings of its
+// exponent (difference, scale and its quotient, product: 1.9e-7), 1.2e-7 by its exponential and some
+// 14 additions by 6e-8 each; 2^30 tokens that together weigh against the largest have t = -30:
+// 5e-6 at worst.
+#define SV_ERR 0x1p-17
 #define SV_BAND 0x1p-20            // of r0: what two 32-bit sums' ratio is mostly good to
 #define SV_SUMS 5                  // 64-bit sums of a chunk
 

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import speculative_ref as ref
-from tests.test_gpu_speculative import HD, i32, say, trees
+from tests.test_gpu_speculative import HD, check_verify, i32, say, trees
 
 pytestmark = pytest.mark.gpu
 
@@ -275,3 +275,23 @@ def test_verify_draft_next_to_the_target(gpu, V, noise):
     off = (got.tokens[:, 0].cpu() != torch.tensor(want)).sum().item()
     say(f"  {off} of {len(want)} draws differ")
     assert got.emitted.eq(1).all() and off == 0
+
+
+def test_verify_open_tests_over_a_floor(gpu):
+    """One token against 151935 that together weigh as much: all of the 32-bit sums' error is there,
+    the same in every weight.  Random numbers on the test's border and beside it."""
+    g = torch.Generator().manual_seed(6)
+    n, V = 36, 151936
+    temps = (0.3 + torch.rand(n, generator=g) * 1.2).tolist()
+    temps = torch.tensor(temps, dtype=torch.float32)
+    floor = -11.9 * temps[:, None, None] + 0.02 * torch.randn(n, 2, V, generator=g)
+    floor[:, :, 777] = 0.01 * torch.randn(n, 2, generator=g)
+    p = torch.softmax(floor[:, 0].double() / temps.double()[:, None], -1)[:, 777]
+    assert 0.3 < p.min() and p.max() < 0.7
+    near = p.float()
+    step = torch.tensor([-1.0, 0.0, 1.0])[torch.arange(n) % 3]
+    u = torch.rand(n, 2, generator=g)
+    u[:, 1] = torch.where(step == 0, near, torch.nextafter(near, near + step))
+    say("tests on a border over a floor of equal tokens")
+    total = check_verify(gpu, floor, [[0, 777]] * n, u, temps.tolist(), parents=[[-1, 0]] * n)
+    assert 0 < (total == 2).sum() < n
