@@ -318,6 +318,9 @@ class PackedPrefillWriter:
     append (mixed batching) adapter of kv_prealloc.py:118-146: segment s writes its tokens
     at pool[slot, start:start+L] and attends to the slot's cached prefix as well."""
 
+    # whether attend_qkv may leave rows of its output as they were
+    leaves_rows = False
+
     def __init__(self, pool: PreallocatedKVCache, slots: Sequence[int],
                  seg_lengths: Sequence[int] | None, starts: Sequence[int] | None = None):
         self.pool = pool
@@ -571,6 +574,11 @@ class TreeCache(PackedPrefillWriter):
             dtype=torch.float32)
 
     @property
+    def leaves_rows(self) -> bool:
+        """Padding nodes and sequences outside the pool have no attention output."""
+        return self.counts is not None or self.slots is not None
+
+    @property
     def starts(self) -> torch.Tensor:
         """int64 [n]: the prefix lengths the trees stand behind."""
         return self._plan[:self.n]
@@ -645,7 +653,7 @@ class TreeCache(PackedPrefillWriter):
         call("omni_kv_write_rows", k.data_ptr(), ks, v.data_ptr(), vs,
              pool.k[layer_idx].data_ptr(), pool.v[layer_idx].data_ptr(), self._slot, self._pos,
              pool.max_batch, pool.max_len, nkv * hd, self.T, stream())
-        make = torch.empty if self.counts is None and self.slots is None else torch.zeros
+        make = torch.zeros if self.leaves_rows else torch.empty
         out = make(self.T, nh, hd, device=q.device, dtype=torch.float16)
         return self._attend(q.data_ptr(), qs, layer_idx, scale, out)
 

@@ -181,6 +181,13 @@ class DecoderLayer(nn.Module):
                 and not self.post_attention_layernorm.fp8_out)
 
 
+def _attention_rows(cache, T: int, cfg: Qwen2Config, device) -> torch.Tensor:
+    """The attention's output rows; zero where the adapter may leave some as they are (a
+    per-tensor FP8 linear behind it takes one scale from all of them)."""
+    make = torch.zeros if getattr(cache, "leaves_rows", False) else torch.empty
+    return make(T, cfg.num_heads, cfg.head_dim, device=device, dtype=torch.float16)
+
+
 class Qwen2LLM(nn.Module):
     def __init__(self, cfg: Qwen2Config, embed: torch.Tensor, final_norm: torch.Tensor,
                  layers: List[DecoderLayer], max_pos: int = 8192):
@@ -275,8 +282,7 @@ class Qwen2LLM(nn.Module):
             else:
                 cache.rope_and_write(qkv, i, pos, self.rope_cos, self.rope_sin,
                                      cfg.mrope_section)
-            attn = torch.empty(T, cfg.num_heads, cfg.head_dim, device=x.device,
-                               dtype=torch.float16)
+            attn = _attention_rows(cache, T, cfg, x.device)
             cache.attend_qkv(qkv, i, self.scale, attn)
             o = layer.self_attn.o_proj(attn.reshape(T, -1))
             h, residual = layer.post_attention_layernorm(o, residual)
@@ -338,7 +344,7 @@ class Qwen2LLM(nn.Module):
         residual = x.clone()
         h = torch.empty(T, H, device=dev, dtype=torch.float16)
         qkv = torch.empty(T, cfg.qkv_out, device=dev, dtype=torch.float16)
-        attn = torch.empty(T, cfg.num_heads, cfg.head_dim, device=dev, dtype=torch.float16)
+        attn = _attention_rows(cache, T, cfg, dev)
         act = torch.empty(T, cfg.intermediate_size, device=dev, dtype=torch.float16)
         Sd = 0
         for i, layer in enumerate(self.layers):

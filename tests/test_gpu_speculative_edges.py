@@ -1,5 +1,5 @@
 """Speculative decoding on the GPU at its edges: attention maxima that grow from tile to tile, steps
-in which a sequence has nothing to draw from."""
+that fail or have nothing to draw from, padded trees and FP8 linears, draws and tests on a border."""
 
 import math
 import random
@@ -214,6 +214,72 @@ def test_runner_speculate_draft_logits_of_another_type(gpu):
                 r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=other)
         assert [s.output_token_ids for s in seqs] == before
         r.speculate(seqs, [[1, 2], [3, 4]], draft_logits=draft.half())
+
+
+@pytest.mark.parametrize("quant", ["fp16", "fp8"])
+@pytest.mark.parametrize("n,T", [(3, 7), (9, 12)])
+def test_model_over_padded_trees(gpu, monkeypatch, quant, n, T):
+    """Padding nodes (counts=) take no part in what the others get: the used rows' logits do not
+    depend on what fresh memory holds, also behind linears that take one scale from all rows."""
+    from omniserver_amd import synth
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    from omniserver_amd.mixed_precision import apply_mixed
+    from omniserver_amd.qwen2_llm import Qwen2LLM
+    say(f"model over padded trees, {quant}, n={n} T={T}")
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=12, num_layers=2)
+    model = Qwen2LLM.from_fp16(w, shape, gpu, max_pos=512)
+    if quant == "fp8":
+        apply_mixed(model, {"qkv": "fp8", "o": "fp8", "gate_up": "fp8", "down": "fp8"})
+    rng = random.Random(n)
+    parents = i32(trees(rng, n, T, "tree"), gpu)
+    counts = i32([rng.randint(1, T - 1) for _ in range(n)], gpu)
+    ids = synth.random_ids(n * T, shape.vocab_size, 12, "pad").to(gpu)
+    pool = PreallocatedKVCache(2, n, 2, 128, HD, gpu, n_heads=12)
+    prefix = torch.randn(pool.storage.shape, device=gpu).half()
+    empty = torch.empty
+    got = []
+    for fill in (0.0, 3e4, math.nan):
+        def filled(*a, **kw):
+            t = empty(*a, **kw)
+            return t.fill_(fill) if t.dtype in (torch.float16, torch.float32) and t.is_cuda else t
+
+        pool.storage.copy_(prefix)
+        pool.lengths.fill_(40)
+        cache = pool.tree_cache(parents, counts=counts)
+        monkeypatch.setattr(torch, "empty", filled)
+        out = model(model.embed_tokens(ids).unsqueeze(0), cache.positions.view(3, 1, n * T), None,
+                    cache)[0]
+        monkeypatch.setattr(torch, "empty", empty)
+        used = torch.arange(T, device=gpu) < counts[:, None]
+        got.append(out.view(n, T, -1)[used])
+    assert got[0].isfinite().all()
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+def test_runner_speculates_with_fp8_linears(gpu):
+    """A decoder on FP8 linears, which decodes op by op: speculative steps, eager and as graphs,
+    give the same tokens, and decode() goes on from there."""
+    from omniserver_amd import synth
+    from omniserver_amd.mixed_precision import apply_mixed
+    say("runner speculates on FP8 linears")
+    shape = synth.DecoderShape()
+    w = synth.fp16_decoder(shape, seed=13, num_layers=2)
+    prompts = [synth.random_ids(L, shape.vocab_size, 13, f"q{L}").tolist() for L in (19, 30)]
+    streams = []
+    for use_graph in (False, True):
+        r, seqs = started(shape, w, prompts, use_graph=use_graph)
+        apply_mixed(r.adapter.model, {"qkv": "fp8", "o": "fp8", "gate_up": "fp8", "down": "fp8"})
+        r.drop_prefill_graphs()
+        assert not r.adapter.model.fused_decode_ready()
+        rng = random.Random(2)
+        for _ in range(4):
+            ids = [rng.randrange(shape.vocab_size) for _ in range(5)]
+            r.speculate(seqs, [ids[:3], (ids[3:], [-1, -1])])
+            r.decode(seqs)
+            assert r.pool.lengths[:2].tolist() == r._kv_len == [s.total_len - 1 for s in seqs]
+        streams.append([list(s.output_token_ids) for s in seqs])
+    assert streams[0] == streams[1]
 
 
 # ----------------------------------------------------------------------------- verification
