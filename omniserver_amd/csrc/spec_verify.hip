@@ -241,9 +241,9 @@ struct SvPiece {
 // ---------------------------------------------------------------------------
 // Row statistics: one workgroup 8192 tokens of a row, rec = (largest logit, sum of weights
 // relative to it), for greedy rows (largest logit, its first index).  32 x 16 nodes, half of them
-// in use, 80 MB: 20 us = 4.0 TB/s (a copy's rate is 4.9).  The whole call there 39.5 us; with 4096
-// or 16384 tokens a workgroup 44.5 / 41.4, with one round of workgroups that go over all rows,
-// loads one piece ahead, 44.5-52.
+// in use, 80 MB: 21 us = 3.8 TB/s (a large copy's rate is 4.7-5.2).  The whole call there 40 us; with
+// 4096 or 16384 tokens a workgroup 5 and 2 more, with one round of workgroups that go over all rows,
+// loads one piece ahead, 5-12 more.
 // ---------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(64 * SV_WAVES) void sv_stats_kernel(SvArgs a) {

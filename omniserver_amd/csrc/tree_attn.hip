@@ -212,12 +212,16 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const half_t* __restrict__
 // outputs are not all finite are taken again, key by key and without the keys they do not
 // attend to (tree_row).  That costs the others the check and a barrier.
 //
+// P is rounded to fp16 for the second product: outputs are off by 2.6e-4 of their size, 2.1e-4 of it
+// their own rounding.  The next bits of P would take the product's matrix instructions once more.
+//
 // MI355X, 12 / 2 heads.  A launch has some 8 us of its own (column and Q loads, first tile, LDS
-// merge).  128 rows: a step of 128 keys 1.85 us on up to 144 workgroups (matrix 40 %, vector 50 % of
-// the cycles, waits), 2.0 on 192, 2.4 on 240: the chip's power holds the products at 800
-// TFLOP/s, whether K and V come from memory or cache; wave priorities change nothing.
-// 64 rows: a step 1.3 us on 2 workgroups, 3.15 on 256 = 5.3 TB/s, memory's.  32 x 64 nodes at 4000
-// tokens 74 + 4.8 of merge, 32 x 8 at 2048 18 + 4.8, 1 x 26 at 4000 10.3 + 4.2.
+// merge).  128 rows: a step of 128 keys 1.84 us on up to 144 workgroups, 2.03 on 192, 2.53 on 240,
+// whether K and V come from memory or cache.  A workgroup takes the same cycles at any of them
+// (300000 at 8128 tokens, matrix busy 44 % of them, vector issue 48 %), but the clock falls: 2.50 GHz at
+// 48 workgroups, 2.39 at 144, 2.27 at 192, 2.10 at 240, with idle times between the launches.
+// 64 rows: a step 1.2 us on 2 workgroups, 3.15 on 256 = 5.3 TB/s, memory's.  32 x 64 nodes at 4000
+// tokens 74 + 4.8 of merge, 32 x 8 at 2048 18 + 4.1, 1 x 26 at 4000 10.7 + 4.3.
 // ---------------------------------------------------------------------------
 struct TreeArgs {
   const half_t* q;

@@ -463,13 +463,13 @@ def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) ->
 
     us, MI355X, 12 heads / 2 KV heads: fewer rows a workgroup and more key groups while the
     workgroups fit one round of the CUs, their key chains being the shorter.  Together where the
-    contexts are short (8 nodes at 250 keys 8.6 against 10.9 cut) or the workgroups many enough
-    (16 x 32 nodes at 1000 15.6 / 18.3), cut where they are few (8 x 8 at 4000 15.7, together 31)
-    or one long context would be all the others wait for (32 x 64 all at 4000 73, together 69, and
-    that also where one alone is so long).
+    contexts are short (8 nodes at 250 keys 8.8 against 10.9 cut) or the workgroups many enough
+    (16 x 32 nodes at 1000 16.2 / 18.8), cut where they are few (8 x 8 at 4000 16.1, together 33)
+    or one long context would be all the others wait for (32 x 64, one at 4000 and the others at
+    200 29, together 67; all at 4000 82 / 73).
     Cut: 64 rows; 128 where 64 would leave more than eight steps of 128 keys for every CU (4 x 64 at
-    4000 28, with 64 rows 23; at 32 x 16 they meet, 33 / 31); 32 where they suffice and many
-    sequences may be short (32 x 4 at 50-1000 11.8 against 13.1, all at 1000 14.0 / 13.5)."""
+    4000 29, with 64 rows 24; at 32 x 16 they meet, 33.1 / 32.9); 32 where they suffice and many
+    sequences may be short (32 x 4 at 50-1000 11.9 against 12.9, all at 1000 14.2 / 13.8)."""
     rows, items = nodes * (nh // nkv), n * nkv
     blocks = lambda r: -(-rows // r)
     form = next((f for f in ((32, 8), (64, 4)) if items * blocks(f[0]) <= cus), (128, 2))
@@ -481,7 +481,7 @@ def tree_plan(n: int, nodes: int, nh: int, nkv: int, capacity: int, cus: int) ->
     elif rows > 64 and steps > 8 * cus:
         form, unit, least = (128, 2), 128, 1
     else:
-        # no single steps where there are enough for every CU (16 x 8 at 1000 12.8 against 14.6)
+        # no single steps where there are enough for every CU (16 x 8 at 1000 13.1 against 14.9)
         form, unit, least = (64, 4), 128, 2 if steps >= cus else 1
     # one round of workgroups, in whole eights for the row blocks of a column to share an XCD, and
     # a multiple of the items, so that equal contexts are cut at their ends

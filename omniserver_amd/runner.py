@@ -447,9 +447,10 @@ class MultimodalRunner(ModelRunner):
         ``drafts``: per sequence (in the order of ``seqs``) either a list of tokens to follow one
         another, or (tokens, parents) with each token's parent in that list (-1: the sequence's
         last token), parents first; at most 63.  ``draft_logits`` fp16 [n, D, V] on the device (D =
-        the most tokens of a draft): row j of a sequence the logits its token j was
-        drawn from, for chains alone; without them the tokens are proposals.  Greedy sequences
-        keep the tokens that decode() would have produced, sampled ones are distributed as its.
+        the most tokens of a draft): row j of a sequence the logits its token j was drawn from, at
+        the sequence's temperature, for chains alone; without them the tokens are proposals.  Greedy
+        sequences keep the tokens that decode() would have produced, up to near ties (the forward
+        over a tree rounds otherwise than decode's), sampled ones are distributed as its.
         Returns the number of tokens each sequence has gained (a stop token or the length limit
         ends a sequence early).  Where nothing is left to draw a sequence's next token from (all
         of its logits NaN or -inf) every other one advances as ever, that one by the drafted tokens
