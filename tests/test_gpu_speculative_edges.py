@@ -361,3 +361,33 @@ def test_verify_open_tests_over_a_floor(gpu):
     say("tests on a border over a floor of equal tokens")
     total = check_verify(gpu, floor, [[0, 777]] * n, u, temps.tolist(), parents=[[-1, 0]] * n)
     assert 0 < (total == 2).sum() < n
+
+
+def test_verify_draft_next_to_the_target_replayed(gpu):
+    """The draw that sums what is left anew, in a graph: every replay as the eager call, also with
+    other numbers and ordinary drafts in between."""
+    from omniserver_amd.speculative import verify
+    g = torch.Generator().manual_seed(8)
+    n, V = 16, 20011
+    target = torch.randn(n, 2, V, generator=g) * 2
+    near, far = (target[:, :1] + noise * torch.randn(n, 1, V, generator=g) for noise in (1e-6, 0.5))
+    x = (torch.softmax(target[:, 0].double(), -1) - 1e-8).abs().argmin(-1)
+    for d in (near, far):
+        d[torch.arange(n), 0, x] = target[torch.arange(n), 0, x] + 3.0
+    tokens = torch.stack([torch.zeros_like(x), x], 1).to(gpu)
+    sets = [(d.to(gpu), torch.stack([torch.rand(n, generator=g), torch.full((n,), 0.97)], 1).to(gpu))
+            for d in (near, far, near)]
+    target = target.to(gpu)
+    want = [[t.clone() for t in verify(target, tokens, u, 1.0, draft_logits=d)] for d, u in sets]
+    draft, u = sets[0][0].clone(), sets[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = verify(target, tokens, u, 1.0, draft_logits=draft)
+    for turn in range(3):
+        for (d, uu), w in zip(sets, want):
+            draft.copy_(d)
+            u.copy_(uu)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, w)), turn
+            verify(target, tokens, uu, 1.0, draft_logits=d)
