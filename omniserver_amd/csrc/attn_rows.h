@@ -1,5 +1,5 @@
-// Attention on 32-row tiles: what the decoder's prefill (attn_rows.hip) and the vision
-// tower's attention (vit.hip) share.
+// Attention on 32-row tiles: what the decoder's prefill (attn_rows.hip), the drafted trees'
+// attention (tree_attn.hip) and the vision tower's (vit.hip) share.
 #pragma once
 
 #include "common.h"
