@@ -296,9 +296,10 @@ def _own_run(s):
         pool.reorder(s["parents"])
         return {"kv": pool.storage, "tables": pool.tables, "lengths": pool.lengths}
     if c["whole"]:
-        q, k, v = _split(s)
-        out = pool.decode_cache(c["n"]).flash_decode(q, k, v, 0, c["hd"] ** -0.5)
-        return {"out": out, "kv": pool.storage}
+        _, k, v = _split(s)
+        step = pool.decode_cache(c["n"])
+        step.write(k, v, 0)
+        return {"out": step.attend_qkv(s["qkv"], 0, c["hd"] ** -0.5, s["out"]), "kv": pool.storage}
     return {"out": s["step"].attend_qkv(s["qkv"], 0, c["hd"] ** -0.5, s["out"])}
 
 
