@@ -198,6 +198,69 @@ int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t 
                      int n_nodes, int vocab, int* path, int64_t* out_tokens, int* emitted,
                      void* workspace, int64_t workspace_doubles, void* stream);
 
+/* ---------------------------------------------------------------- paged cache */
+
+/* Pages of a paged KV cache.  Sequence r holds lengths[r] tokens (int64; taken as within [0,
+ * max_len]), token t in page tables[r][t / page_size] (int32 [seqs][width]), place t % page_size.  A
+ * page is free where no sequence's table names it within its length.  seqs up to 2048, pages up to
+ * 2^20, page_size a power of two from 16 to 1024, width * page_size at least max_len.
+ *
+ * Request i of n brings counts[i] tokens (int32; NULL: one; less than one: none) to sequence rows[i]
+ * (int64, all different; NULL: i), packed into `tokens` rows one request after another; dense:
+ * tokens = n, request i's one token is row i.  It is granted them where they fit max_len and the
+ * packed rows and their pages are there; the lowest free pages go to the requests in order, those
+ * of a request that goes without are left unused.  Writes the tables' new entries, starts and after
+ * int64 [n] (lengths before and with what is granted; lengths itself stays), token_page and
+ * token_pos int64 [tokens] (-1: nowhere), positions int64 [axes <= 3][tokens] (position + rope_delta
+ * of the sequence, int64 or NULL; -1 without a slot), granted int32 [n], cu int32 [n + 1] (sums of
+ * counts) and, for dense, schedule (int32 [4 (n + columns)], 16-byte aligned, or NULL) for
+ * omni_paged_attention. */
+int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int width, int pages, int page_size,
+                      int max_len, const int* counts, const int64_t* rows,
+                      const int64_t* rope_delta, int n, int tokens, int dense, int axes,
+                      int64_t* starts, int64_t* after, int64_t* token_page, int64_t* token_pos,
+                      int64_t* positions, int* granted, int* cu, int* schedule, int columns,
+                      void* stream);
+
+/* Beams after a choice: row s * beams + w of the first n * beams sequences goes on from row s * beams
+ * + parents[s][w] as it was (int32; outside [0, beams): empty).  Full pages are shared; a page that
+ * is filled in part stays with its first child, the others get the lowest free pages and a copy of
+ * its tokens in every layer of pool (16-bit elements [n_layers][2][pages][page_size][row_halfs],
+ * row_halfs a multiple of 8), or are empty where none is free.  work: int32, 16-byte aligned, 4 n
+ * beams of them. */
+int omni_page_reorder(void* pool, int n_layers, int row_halfs, int* tables, int64_t* lengths,
+                      int seqs, int width, int pages, int page_size, int max_len,
+                      const int* parents, int n, int beams, int* work, int64_t work_ints,
+                      void* stream);
+
+/* Attention of one new token per sequence over the pages: row i of q and out (dtype 0 fp16, 1 bf16;
+ * strides in elements, multiples of 8) attends to the keys that the schedule gives sequence i, the new
+ * token the last of them; a row without keys is zero.  k_cache / v_cache [pages][page_size]
+ * [n_kv_heads][head_dim 64 or 128].  The keys stand in one line cut into equal stretches, one a
+ * column of workgroups; the states of a sequence that several share go through workspace (fp32,
+ * (columns + n) n_heads (head_dim + 4) floats) to a second launch.  scale from 2^-126 to 2^126;
+ * operands 16-byte aligned. */
+int omni_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+                         int dtype, int pages, int page_size, const int* tables, int width, int n,
+                         const int* schedule, int columns, void* out, int64_t out_stride,
+                         int n_heads, int n_kv_heads, int head_dim, float scale, float* workspace,
+                         int64_t workspace_floats, void* stream);
+
+/* Beam search's choice: the k <= 64 best continuations of each of n requests over its beams <= 32
+ * and the vocabulary (up to 524288).  logits [n][beams][vocab] (dtype 0 fp16, 1 bf16, 2 fp32;
+ * strides in elements); a continuation is worth scores[s][b] (fp32) + logit - log sum exp of the
+ * row, compared in 64 bits, ties to the lower beam, then token; a beam with a score that is not
+ * finite is not in use; one with done[s][b] != 0 (bytes, or NULL) goes on as itself, with token pad.
+ * stop int64 [stops] (stop_stride 0) or [n][stops] (stop_stride its row stride): tokens that finish.
+ * Writes out_scores fp32, parents int32, tokens int64, out_done bytes [n][k], none of them over an
+ * input.  workspace: 8-byte words, 16-byte aligned, as many as omni_beam_select_work gives. */
+int omni_beam_select_work(int n, int beams, int vocab, int k);
+int omni_beam_select(const void* logits, int dtype, int64_t req_stride, int64_t row_stride,
+                     const float* scores, const void* done, const int64_t* stop, int stops,
+                     int64_t stop_stride, int64_t pad, int n, int beams, int vocab, int k,
+                     float* out_scores, int* parents, int64_t* tokens, void* out_done,
+                     void* workspace, int64_t workspace_words, void* stream);
+
 /* ---------------------------------------------------------------- attention */
 
 /* _CacheView.flash_decode (cache/kv_prealloc.py:272-290): GQA decode attention over the

@@ -1,0 +1,392 @@
+"""The paged cache's operators and beam search's choice on the GPU against plain forms in 64 bits:
+room for new tokens, attention of one new token per sequence, beams that take over their parents'
+pages, the best continuations."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def say(msg):
+    print(f"[gpu-test] {msg}", flush=True)
+
+
+def i32(x, gpu):
+    return torch.tensor(x, dtype=torch.int32, device=gpu)
+
+
+def make_cache(gpu, lengths, page, rng, nkv=2, nh=12, hd=128, layers=1, dtype=torch.float16, spare=0,
+               max_len=None, shared=1, seqs=None, room=0):
+    """A cache whose sequences hold `lengths` tokens in pages anywhere; groups of `shared` rows hold
+    their whole pages together.  Entries behind a sequence's length are anything at all."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    seqs = len(lengths) if seqs is None else seqs
+    lengths = list(lengths) + [0] * (seqs - len(lengths))
+    held = sum(ref.pages_of(m, page) for m in lengths)
+    pages = held + spare
+    max_len = max(max(lengths) + room, 1) if max_len is None else max_len
+    cache = PagedKVCache(layers, max(pages, 1), nkv, page, hd, gpu, max_seqs=seqs, max_len=max_len,
+                         dtype=dtype, n_heads=nh)
+    order = list(range(cache.num_pages))
+    rng.shuffle(order)
+    width = cache.tables.shape[1]
+    tables = [[rng.choice([-1, -7, 1 << 30, rng.randrange(max(pages, 1))]) for _ in range(width)]
+              for _ in range(seqs)]
+    for r, m in enumerate(lengths):
+        keep = 0
+        if shared > 1 and r % shared and lengths[r - 1] == m:
+            keep = m // page
+            tables[r][:keep] = tables[r - 1][:keep]
+        for j in range(keep, ref.pages_of(m, page)):
+            tables[r][j] = order.pop()
+    cache.tables.copy_(torch.tensor(tables, dtype=torch.int32))
+    cache.lengths.copy_(torch.tensor(lengths))
+    return cache, tables, lengths
+
+
+RESERVE = [
+    # sequences, asking, page, lengths, new tokens, spare pages, max_len
+    (1, 1, 16, (0, 0), (1, 1), 1, 1),
+    (1, 1, 16, (15, 15), (1, 1), 0, 16),
+    (1, 1, 16, (16, 16), (1, 1), 0, 64),              # no page left
+    (3, 3, 16, (0, 40), (1, 1), 3, 64),
+    (5, 4, 32, (0, 100), (0, 70), 9, 256),
+    (33, 33, 16, (0, 300), (-2, 3), 12, 400),
+    (64, 60, 16, (0, 90), (0, 40), 60, 100),          # too few pages, some past max_len
+    (100, 100, 256, (0, 2000), (1, 1), 20, 2048),
+    (300, 300, 16, (0, 64), (0, 30), 200, 80),        # more token rows than one workgroup writes
+    (1500, 1400, 16, (0, 50), (0, 2), 300, 64),       # more requests than a workgroup has threads
+    (2, 2, 1024, (1000, 1030), (1, 3000), 5, 8192),
+    (40, 40, 16, (2000, 4000), (1, 1), 40, 5000),
+]
+
+
+@pytest.mark.parametrize("seqs,n,page,span,new,spare,max_len", RESERVE)
+@pytest.mark.parametrize("kind", ["packed", "rows", "dense"])
+def test_reserve(gpu, seqs, n, page, span, new, spare, max_len, kind):
+    say(f"reserve {n} of {seqs} sequences, pages of {page}, lengths {span}, new {new} {kind}")
+    rng = random.Random(seqs * 31 + page)
+    lengths = [rng.randint(*span) for _ in range(seqs)]
+    cache, tables, lengths = make_cache(gpu, lengths, page, rng, spare=spare, max_len=max_len)
+    counts = [rng.randint(*new) for _ in range(n)]
+    rows = rng.sample(range(seqs), n) if kind == "rows" else list(range(n))
+    tokens = n if kind == "dense" else sum(max(c, 0) for c in counts)
+    if kind == "packed" and tokens > 8:
+        tokens -= 3                                     # not enough rows for the last ones
+    want = ref.reserve(tables, lengths, counts, rows, cache.num_pages, page, max_len, tokens,
+                       kind == "dense")
+    delta = torch.arange(seqs, device=gpu) * 7 if kind == "dense" else None
+    for turn in range(2):                               # the second finds what the first has written
+        if kind == "dense":
+            got = cache.decode_cache(n, i32(counts, gpu), delta)
+        else:
+            got = cache.reserve(i32(counts, gpu), rows if kind == "rows" else None, tokens)
+        new_tables, granted, starts, after, slots = want
+        assert got.granted.tolist() == granted
+        assert got.starts.tolist() == starts and got.after.tolist() == after
+        assert got.token_page.tolist() == [s[0] for s in slots]
+        assert got.token_pos.tolist() == [s[1] for s in slots]
+        if kind == "dense":
+            pos = [s[2] + 7 * i if s[2] >= 0 else -1 for i, s in enumerate(slots)]
+            assert got.positions.tolist() == [pos] * 3
+        else:
+            assert got.positions.tolist() == [s[2] for s in slots]
+        assert cache.tables.tolist() == new_tables
+    assert cache.lengths.tolist() == lengths            # they move in finish
+    got.finish()
+    for r, m in zip(rows, after):
+        lengths[r] = m
+    assert cache.lengths.tolist() == lengths
+    if kind == "rows":
+        cache.free(rows[:2])
+        for r in rows[:2]:
+            lengths[r] = 0
+        assert cache.lengths.tolist() == lengths
+
+
+def fill_pages(cache, tables, lengths, g):
+    """Random K/V where tokens are, NaN and infinities everywhere else; per sequence its K and V."""
+    page, dev = cache.page_size, cache.storage.device
+    cache.storage.fill_(math.nan)
+    cache.storage[:, :, ::2] = math.inf
+    content = torch.randn(cache.storage.shape, generator=g).to(cache.storage.dtype)
+    host = cache.storage.cpu()
+    for row, m in zip(tables, lengths):
+        for j in range(ref.pages_of(m, page)):
+            some = min(page, m - j * page)
+            host[:, :, row[j], :some] = content[:, :, row[j], :some]
+    cache.storage.copy_(host)
+    return host
+
+
+def tokens_of(host, layer, row, m, page):
+    """K and V [m, nkv, hd] of a sequence."""
+    pages = torch.tensor(row[:ref.pages_of(m, page)], dtype=torch.long)
+    return tuple(host[layer, i][pages].reshape(-1, *host.shape[4:])[:m] for i in (0, 1))
+
+
+def check_rows(out, q, host, layer, tables, keys, page, scale):
+    """out [n, nh, hd] against the plain form over keys[i] tokens of table i."""
+    worst = 0.0
+    out = out.cpu()
+    for i, m in enumerate(keys):
+        if m == 0:
+            assert (out[i] == 0).all(), f"row {i} has no keys"
+            continue
+        k, v = tokens_of(host, layer, tables[i], m, page)
+        want, mag = ref.attention(q[i].cpu(), k, v, scale)
+        bound = ref.attention_bound(want, mag, m, v.float().abs().max().item(), out.dtype)
+        err = ((out[i].double() - want).abs() / bound).max().item()
+        assert err <= 1.0, f"row {i} of {m} keys: {err:.2f} of the bound"
+        worst = max(worst, err)
+    say(f"  worst error {worst:.2f} of the bound")
+
+
+ATTENTION = [
+    # n, lengths, page, nh, nkv, hd, dtype, max_len
+    (1, (0, 0), 16, 12, 2, 128, torch.float16, None),
+    (2, (1, 15), 16, 12, 2, 128, torch.float16, None),
+    (3, (16, 32), 32, 12, 2, 128, torch.float16, None),
+    (4, (100, 130), 16, 12, 2, 128, torch.float16, None),
+    (5, (120, 140), 64, 12, 2, 128, torch.bfloat16, None),
+    (7, (0, 700), 16, 12, 2, 128, torch.float16, 4096),
+    (3, (0, 300), 128, 16, 16, 64, torch.bfloat16, None),
+    (4, (30, 400), 16, 8, 1, 64, torch.float16, 1000),
+    (2, (500, 600), 256, 28, 4, 128, torch.float16, None),
+    (3, (60, 70), 16, 40, 2, 128, torch.float16, None),       # 20 heads a KV head: two groups
+    (2, (128, 130), 32, 64, 1, 64, torch.bfloat16, None),     # four
+    (33, (0, 300), 16, 12, 2, 128, torch.float16, 8192),
+    (1, (5000, 5000), 64, 12, 2, 128, torch.float16, None),   # every column a piece of one row
+    (300, (0, 40), 16, 4, 2, 64, torch.float16, None),        # more rows than columns
+    (6, (127, 129), 1024, 6, 1, 128, torch.float16, None),
+    (9, (0, 1500), 16, 1, 1, 128, torch.bfloat16, 2000),
+]
+
+
+@pytest.mark.parametrize("n,span,page,nh,nkv,hd,dtype,max_len", ATTENTION)
+def test_decode_attention(gpu, n, span, page, nh, nkv, hd, dtype, max_len):
+    say(f"paged attention n={n} lengths {span} page {page} heads {nh}/{nkv} x {hd} {dtype}")
+    rng = random.Random(n * 131 + page)
+    lengths = [rng.randint(*span) for _ in range(n)]
+    lengths[0], lengths[-1] = span[1], span[0]
+    cache, tables, lengths = make_cache(gpu, lengths, page, rng, nkv, nh, hd, 2, dtype, spare=n,
+                                        max_len=max_len or max(lengths) + 1)
+    g = torch.Generator().manual_seed(n)
+    fill_pages(cache, tables, lengths, g)
+    counts = [1] * n if n < 4 else [int(rng.random() < 0.8) for _ in range(n)]
+    step = cache.decode_cache(n, counts)
+    tables = cache.tables.tolist()
+    rows = torch.randn(n, (nh + 2 * nkv) * hd, generator=g).to(dtype).to(gpu)
+    q, k, v = rows.view(n, nh + 2 * nkv, hd).split((nh, nkv, nkv), 1)
+    step.write(k, v, 1)
+    host = cache.storage.cpu()
+    keys = [m + 1 if c else 0 for m, c in zip(lengths, counts)]
+    for i, m in enumerate(keys):
+        if m:
+            assert torch.equal(host[1, 0, tables[i][(m - 1) // page], (m - 1) % page], k[i].cpu())
+    out = torch.full((n, nh, hd), 7.0, device=gpu, dtype=dtype)
+    assert step.attend_qkv(rows, 1, hd ** -0.5, out) is out
+    check_rows(out, q, host, 1, tables, keys, page, hd ** -0.5)
+    again = torch.full_like(out, 3.0)
+    step.attend_qkv(rows, 1, hd ** -0.5, again)
+    assert torch.equal(out, again)
+    # the protocol on separate tensors: the same rows, lengths move with the last layer
+    step = cache.decode_cache(n, i32(counts, gpu))
+    assert torch.equal(step.flash_decode(q, k, v, 1, hd ** -0.5), out)
+    assert cache.lengths.tolist() == [m + c for m, c in zip(lengths, counts)]
+
+
+def test_decode_attention_bad_pages(gpu):
+    """Table entries outside the pool: their tokens are not there, the others' attention is."""
+    rng = random.Random(5)
+    cache, tables, lengths = make_cache(gpu, [100, 70, 40], 16, rng, spare=3, max_len=128)
+    g = torch.Generator().manual_seed(1)
+    host = fill_pages(cache, tables, lengths, g)
+    cache.tables[0, 2], cache.tables[0, 3], cache.tables[2, 0] = -1, cache.num_pages, 1 << 30
+    cache.tables[2, 1:3] = -5
+    step = cache.decode_cache(3)
+    q = torch.randn(3, 12 * 128, generator=g).half().to(gpu)
+    rows = torch.randn(3, 2, 2, 128, generator=g).half().to(gpu)
+    step.write(rows[:, 0], rows[:, 1], 0)
+    host = cache.storage.cpu()
+    out = step.attend_qkv(q, 0, 128 ** -0.5, torch.empty(3, 12, 128, device=gpu, dtype=torch.float16))
+    tables, q = cache.tables.tolist(), q.view(3, 12, 128).cpu()
+    # sequence 0 without its pages 2 and 3
+    left = [t for j, t in enumerate(tables[0][:7]) if j not in (2, 3)]
+    k, v = tokens_of(host, 0, left, 101 - 32, 16)
+    want, mag = ref.attention(q[0], k, v, 128 ** -0.5)
+    bound = ref.attention_bound(want, mag, 101, 8.0, torch.float16)
+    assert ((out[0].cpu().double() - want).abs() <= bound).all()
+    check_rows(out[1:2], q[1:2], host, 0, tables[1:2], [71], 16, 128 ** -0.5)
+    assert (out[2] == 0).all()
+
+
+def test_decode_attention_far_pages(gpu):
+    """K and V of more than 2^31 elements each."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    pages = (1 << 31) // (64 * 2 * 128) + 40
+    cache = PagedKVCache(1, pages, 2, 64, 128, gpu, max_seqs=2, max_len=200)
+    g = torch.Generator().manual_seed(3)
+    table = [[pages - 1, 3, pages - 3], [pages - 2, pages - 4, 0]]
+    used = [p for row in table for p in row]
+    cache.storage[:, :, used] = torch.randn(1, 2, 6, 64, 2, 128, generator=g).half().to(gpu)
+    cache.tables[:, :3] = i32(table, gpu)
+    cache.lengths.copy_(torch.tensor([150, 180]))
+    step = cache.decode_cache(2)
+    q = torch.randn(2, 12 * 128, generator=g).half().to(gpu)
+    out = step.attend_qkv(q, 0, 0.1, torch.empty(2, 12, 128, device=gpu, dtype=torch.float16))
+    host = cache.storage[:, :, used].cpu()
+    check_rows(out, q.view(2, 12, 128), host, 0, [[0, 1, 2], [3, 4, 5]], [151, 181], 64, 0.1)
+
+
+REORDER = [
+    # requests, beams, page, lengths, spare pages, layers
+    (1, 1, 16, (5, 5), 0, 1),
+    (1, 4, 16, (33, 33), 4, 2),
+    (1, 4, 16, (32, 32), 0, 2),               # nothing in part
+    (3, 3, 32, (0, 70), 5, 3),
+    (2, 5, 16, (1, 200), 1, 2),               # too few pages
+    (8, 4, 64, (50, 300), 32, 1),
+    (100, 7, 16, (0, 30), 500, 1),
+    (300, 5, 16, (0, 20), 900, 1),            # more rows than a workgroup has threads
+    (2, 32, 128, (100, 500), 64, 1),
+]
+
+
+@pytest.mark.parametrize("n,W,page,span,spare,layers", REORDER)
+@pytest.mark.parametrize("shared", [False, True])
+def test_reorder(gpu, n, W, page, span, spare, layers, shared):
+    say(f"reorder {n} x {W} beams, pages of {page}, lengths {span}, shared={shared}")
+    rng = random.Random(n * 7 + W)
+    lengths = [rng.randint(*span) for _ in range(n) for _ in range(W)]
+    if shared:
+        lengths = [lengths[r - r % W] for r in range(n * W)]
+    cache, tables, lengths = make_cache(gpu, lengths, page, rng, nkv=1, nh=2, hd=64, layers=layers,
+                                        spare=spare, max_len=span[1] + 40, seqs=n * W + 3,
+                                        shared=W if shared else 1)
+    g = torch.Generator().manual_seed(W)
+    cache.storage.copy_(torch.randn(cache.storage.shape, generator=g))
+    for turn in range(3):
+        parents = [[rng.choice([-1, rng.randrange(W), rng.randrange(W), 0]) for _ in range(W)]
+                   for _ in range(n)]
+        if turn == 0:
+            parents[0][-1] = 0
+        before = cache.storage.clone()
+        new_tables, new_lengths, copies = ref.reorder(tables, lengths, parents, cache.num_pages, page)
+        if turn == 1:
+            cache.reorder(parents)
+        else:
+            given = i32(parents, gpu)
+            given[given < 0] = rng.choice([-1, -100, W, 1 << 30])
+            cache.reorder(given)
+        assert cache.lengths.tolist() == new_lengths
+        got = cache.tables.tolist()
+        for r, m in enumerate(new_lengths):
+            held = ref.pages_of(m, page)
+            assert got[r][:held] == new_tables[r][:held], f"row {r}"
+        for a, b, m in copies:
+            before[:, :, b, :m] = before[:, :, a, :m].clone()
+        assert torch.equal(cache.storage, before)
+        tables, lengths = got, new_lengths
+
+
+SELECT = [
+    # requests, beams, k, vocab, dtype, kind
+    (1, 1, 1, 1, torch.float32, "normal"),
+    (1, 1, 1, 7, torch.float16, "normal"),
+    (2, 3, 5, 2, torch.float16, "normal"),            # k near everything there is
+    (1, 4, 64, 5, torch.bfloat16, "normal"),          # fewer continuations than k
+    (3, 4, 4, 1000, torch.float16, "normal"),
+    (3, 4, 8, 1000, torch.float16, "ties"),
+    (2, 5, 10, 4097, torch.float32, "normal"),
+    (2, 5, 10, 8191, torch.bfloat16, "ties"),
+    (2, 4, 64, 20000, torch.float16, "sorted"),       # all of the best in one block
+    (2, 4, 64, 20000, torch.float32, "constant"),
+    (4, 32, 32, 3001, torch.float16, "ended"),
+    (5, 6, 12, 9999, torch.float32, "ended"),
+    (3, 4, 8, 5000, torch.float16, "odd"),            # NaN, infinities, empty rows
+    (3, 4, 8, 5000, torch.float32, "odd"),
+    (3, 4, 8, 5000, torch.bfloat16, "odd"),
+    (1, 4, 4, 151936, torch.float16, "normal"),
+    (40, 2, 4, 33333, torch.float16, "normal"),       # blocks of 8192
+    (1, 2, 16, 524288, torch.float16, "normal"),
+    (7, 16, 32, 32003, torch.bfloat16, "normal"),
+]
+
+
+def select_case(n, W, V, dtype, kind, g, rng):
+    logits = torch.randn(n, W, V, generator=g) * 3
+    if kind == "ties":
+        logits = (logits * 2).round() / 2
+    elif kind == "sorted":
+        logits = logits.sort(-1, descending=rng.random() < 0.5).values
+    elif kind == "constant":
+        logits = torch.full((n, W, V), 1.5)
+    scores = -torch.rand(n, W, generator=g) * 5
+    done = torch.zeros(n, W, dtype=torch.bool)
+    if kind == "ended":
+        done = torch.rand(n, W, generator=g) < 0.4
+        scores[torch.rand(n, W, generator=g) < 0.3] = -math.inf
+        scores[0] = -math.inf
+        scores[1, 0], done[1, 0] = -0.25, True
+        scores[2, :3] = torch.tensor([math.nan, math.inf, -1.0])
+    if kind == "odd":
+        logits[torch.rand(logits.shape, generator=g) < 0.5] = -math.inf
+        logits[torch.rand(logits.shape, generator=g) < 0.1] = math.nan
+        logits[0, 1] = -math.inf
+        logits[0, 2] = math.nan
+        logits[0, 3, 3:] = -math.inf
+        logits[0, 3, :3] = torch.tensor([math.nan, -2.0, -3.0])
+        logits[1, 0, [7, 90, 4000]] = math.inf
+        logits[2] = -math.inf
+        logits[2, 1, 4999] = -60000.0
+        logits[2, 3, 17] = 0.0
+        logits[2, 3, 16] = -0.0
+    return logits.to(dtype), scores, done
+
+
+@pytest.mark.parametrize("n,W,k,V,dtype,kind", SELECT)
+def test_select(gpu, n, W, k, V, dtype, kind):
+    from omniserver_amd.beam import select
+    say(f"select {k} of {n} x {W} beams over {V} {dtype} {kind}")
+    rng, g = random.Random(n + V), torch.Generator().manual_seed(V + k)
+    logits, scores, done = select_case(n, W, V, dtype, kind, g, rng)
+    stop = [[rng.randrange(V), -1, int(logits[s, 0].nan_to_num(nan=-9e4).argmax())] for s in range(n)]
+    want = ref.select(logits, scores, k, done, stop, pad=11)
+    got = select(logits.to(gpu), scores.to(gpu), k, done.to(gpu),
+                 torch.tensor(stop, device=gpu), pad=11)
+    pick = lambda i: [[row[i] for row in request] for request in want]
+    assert got.parents.tolist() == pick(1)
+    assert got.tokens.tolist() == pick(2)
+    assert got.done.tolist() == pick(3)
+    exact = torch.tensor(pick(0), dtype=torch.float64)
+    have = got.scores.cpu().double()
+    assert torch.equal(have == -math.inf, exact == -math.inf)
+    fine = exact > -math.inf
+    # one rounding to fp32, and 2^-30 for what is left of the 64-bit sums
+    assert ((have - exact).abs() <= exact.abs() * 2.0 ** -24 + 2.0 ** -30)[fine].all()
+    again = select(logits.to(gpu), scores.to(gpu), k, done.to(gpu), torch.tensor(stop, device=gpu), 11)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_select_defaults_and_strides(gpu):
+    """k defaults to the beams; rows that are views of wider ones; one list of stop tokens; nothing
+    finished."""
+    from omniserver_amd.beam import select
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(4, 3, 2, 1009, generator=g).half()
+    logits = wide[1:, :, 1, 5:1004]
+    scores = -torch.rand(3, 3, generator=g)
+    want = ref.select(logits, scores, 3, None, [4, 990])
+    got = select(wide.to(gpu)[1:, :, 1, 5:1004], scores.to(gpu), stop=[4, 990])
+    assert got.parents.tolist() == [[r[1] for r in q] for q in want]
+    assert got.tokens.tolist() == [[r[2] for r in q] for q in want]
+    assert got.done.tolist() == [[r[3] for r in q] for q in want]
+    one = select(logits[:1, :1].expand(2, 3, 999).to(gpu), torch.zeros(2, 3, device=gpu))
+    assert one.parents.tolist() == [[0, 1, 2]] * 2      # all alike: the lower beam first
