@@ -24,7 +24,7 @@ struct BeamArgs {
   int stops, n, W, V, k, blocks;
   int64_t pad;
   float2* lists;             // [n W][blocks][k] (logit, token), best first, -inf behind them
-  double2* sums;             // [n W][blocks] (largest logit, sum of weights relative to it)
+  float2* sums;              // [n W][blocks] (largest logit, sum of weights relative to it)
   float* out_scores;
   int* parents;
   int64_t* tokens;
@@ -41,6 +41,11 @@ __device__ __forceinline__ double bm_weight(float x, float m) {
   return sv_exp2(fmax(((double)x - (double)m) * 1.4426950408889634073599, -2000.0));
 }
 
+// Whether (logit, token) stands before another.
+__device__ __forceinline__ bool bm_before(float2 x, float2 y) {
+  return x.x > y.x || (x.x == y.x && __builtin_bit_cast(int, x.y) < __builtin_bit_cast(int, y.y));
+}
+
 // The lane that holds the largest v, of the lowest token among equals.
 __device__ __forceinline__ int bm_winner(float v, int token) {
   const float top = wave_top(v);
@@ -54,42 +59,144 @@ __device__ __forceinline__ int bm_winner(float v, int token) {
   return __ffsll((unsigned long long)best) - 1;
 }
 
+#define BM_LOG2E 1.4426950216f     // log2 e in 32 bits
+
+// Sum of a lane's N weights exp(x - m) in 32 bits, m finite.  Near zero one fma gives the exponent,
+// relative to the rounded product R = m log2 e instead of m: the caller's sum is then to be taken
+// times bm_shift(m).
+__device__ __forceinline__ bool bm_direct(float m) { return fabsf(m) <= 256.f; }
+__device__ __forceinline__ double bm_shift(float m) {
+  return bm_direct(m) ? 1.0 + 0.6931471805599453 * ((double)(m * BM_LOG2E) - (double)m * BM_LOG2E) : 1.0;
+}
+template <int N>
+__device__ __forceinline__ float bm_weights(const float (&x)[N], float m) {
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+  if (bm_direct(m)) {
+    const float R = m * BM_LOG2E;
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e & 3] += __builtin_amdgcn_exp2f(fmaf(x[e], BM_LOG2E, -R));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e & 3] += __builtin_amdgcn_exp2f((x[e] - m) * BM_LOG2E);
+  }
+  return (z[0] + z[1]) + (z[2] + z[3]);
+}
+
+// ---------------------------------------------------------------------------
+// A block of a row, EPT tokens a lane in registers.  Its k best: every wave finds the largest value
+// that at least k / 4 of its lanes reach; the smallest of the four waves' is reached by k tokens or
+// more, and mostly by few more.  Those go to LDS, where each counts the ones before it.
+// Where they are too many (equal logits, all of the best in a few lanes) the waves take out their k
+// best one after another, and the four lists are merged.
+// ---------------------------------------------------------------------------
+#define BM_CAP 256                 // tokens that are ranked, one a thread
+
 template <int DT, int EPT>
 __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
   typedef SvPiece<DT> P;
-  __shared__ float2 list[BM_WAVES][BM_MAX_K];
-  __shared__ float wm[BM_WAVES];
-  __shared__ double wz[BM_WAVES];
+  __shared__ float2 list[BM_CAP];
+  static_assert(BM_CAP >= BM_WAVES * BM_MAX_K && BM_CAP <= 64 * BM_WAVES, "one a thread");
+  __shared__ float wm[BM_WAVES], wz[BM_WAVES], wt[BM_WAVES];
+  __shared__ int found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = blockIdx.x / a.blocks, block = blockIdx.x - r * a.blocks;
-  if (bm_done(a, r) || !(fabsf(a.scores[r]) < INFINITY)) return;
-  const int s = r / a.W, b = r - s * a.W;
+  const int block = blockIdx.x, b = blockIdx.y, s = blockIdx.z, r = s * a.W + b;
+  const int64_t place = (int64_t)r * a.blocks + block;
+  const bool off = bm_done(a, r) || !(fabsf(a.scores[r]) < INFINITY);
   const void* row = (const char*)a.logits + (s * a.req_stride + b * a.row_stride) * sv_size<DT>();
-  const int v0 = (block * BM_WAVES + wave) * 64 * EPT;
+  constexpr int PIECE = 64 * P::N;                  // tokens of a wave's load; waves take turns
+  const int v0 = block * BM_WAVES * 64 * EPT + wave * PIECE;
+  if (threadIdx.x == 0) found = 0;
+  P p[EPT / P::N];
+#pragma unroll
+  for (int j = 0; j < EPT / P::N; ++j) p[j].load(row, v0 + j * BM_WAVES * PIECE, a.V, lane, 0);
   float x[EPT];
 #pragma unroll
-  for (int j = 0; j < EPT / P::N; ++j) {
-    P p;
-    p.load(row, v0, a.V, lane, j);
+  for (int e = 0; e < EPT; ++e)
+    x[e] = fmaxf(p[e / P::N].get(e % P::N), -INFINITY);       // leaves a NaN out
+  auto token = [&](int e) { return v0 + e / P::N * BM_WAVES * PIECE + lane * P::N + e % P::N; };
+  float best[EPT / P::N], own = -INFINITY;          // of a piece, of all
 #pragma unroll
-    for (int e = 0; e < P::N; ++e) {
-      const float y = p.get(e);
-      x[j * P::N + e] = y == y ? y : -INFINITY;
+  for (int j = 0; j < EPT / P::N; ++j) {
+    best[j] = x[j * P::N];
+#pragma unroll
+    for (int e = 1; e < P::N; ++e) best[j] = fmaxf(best[j], x[j * P::N + e]);
+    own = fmaxf(own, best[j]);
+  }
+  if (off) return;                                  // looked at once the logits are under way
+  const float m = wave_top(own);
+  // what k / nw lanes reach, of the nw waves with a token for every lane
+  const int nw = min(max((a.V - block * BM_WAVES * 64 * EPT) / PIECE, 1), BM_WAVES);
+  float least = wave < nw ? m : INFINITY;
+  if (wave < nw) {
+    float v = own;
+    for (int left = (a.k + nw - 1) / nw; least > -INFINITY;) {
+      const bool top = v == least;
+      left -= __popcll(__ballot(top));
+      if (left <= 0) break;
+      v = top ? -INFINITY : v;
+      least = wave_top(v);
     }
   }
-  auto token = [&](int e) { return v0 + P::at(lane, e / P::N) + e % P::N; };
-  float m = x[0];
-#pragma unroll
-  for (int e = 1; e < EPT; ++e) m = fmaxf(m, x[e]);
-  m = wave_top(m);
-  double z = 0.0;
-#pragma unroll 4
-  for (int e = 0; e < EPT; ++e) z += bm_weight(x[e], m);
-  z = wave_total(m > -INFINITY ? z : 0.0);
   if (lane == 0) {
     wm[wave] = m;
-    wz[wave] = z;
+    wt[wave] = least;
   }
+  __syncthreads();
+  const float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+  // the lowest finite number where -inf would do
+  const float from = fmaxf(fminf(fminf(wt[0], wt[1]), fminf(wt[2], wt[3])), -3.402823466e38f);
+  // a lane's pieces with such a token are read again, the first while the sum is made: registers
+  // have no index, and unrolled code is slow to fetch
+  uint32_t mine = 0;
+#pragma unroll
+  for (int j = 0; j < EPT / P::N; ++j) mine |= best[j] >= from ? 1u << j : 0u;
+  P again;
+  int piece = 0;
+  auto take = [&]() {
+    if (!mine) return;
+    piece = __ffs(mine) - 1;
+    again.load(row, v0 + piece * BM_WAVES * PIECE, a.V, lane, 0);
+  };
+  take();
+  float sum = 0.f;
+  if (fabsf(M) < INFINITY) {
+    sum = bm_weights(x, M);
+  } else if (M == INFINITY) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) sum += x[e] == M ? 1.f : 0.f;
+  }
+  sum = wave_total(sum);
+  if (lane == 0) wz[wave] = sum;
+  while (mine) {
+    const int t = v0 + piece * BM_WAVES * PIECE + lane * P::N;
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      const float v = again.get(e);
+      if (v >= from) {
+        const int at = atomicAdd(&found, 1);
+        if (at < BM_CAP) list[at] = make_float2(v, __builtin_bit_cast(float, t + e));
+      }
+    }
+    mine &= mine - 1;
+    take();
+  }
+  __syncthreads();
+  const int count = found;
+  float2* out = a.lists + place * a.k;
+  if (threadIdx.x == 0) a.sums[place] = make_float2(M, (wz[0] + wz[1]) + (wz[2] + wz[3]));
+  if (count <= BM_CAP) {
+    const int t = threadIdx.x;
+    if (t < count) {
+      const float2 own_t = list[t];
+      int rank = 0;
+      for (int i = 0; i < count; ++i) rank += bm_before(list[i], own_t);
+      if (rank < a.k) out[rank] = own_t;
+    } else if (t < a.k) {
+      out[t] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  __syncthreads();                                  // the list is read, and used again
   // the wave's k best, one after another: every lane's best behind the last one taken
   float lastv = INFINITY;
   int lastt = -1;
@@ -112,125 +219,317 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
     const int w = bm_winner(bv, bt);
     lastv = lane_of(bv, w);
     lastt = __builtin_amdgcn_readlane(bt, w);
-    if (lane == 0) list[wave][j] = make_float2(lastv, __builtin_bit_cast(float, lastt));
+    if (lane == 0) list[wave * BM_MAX_K + j] = make_float2(lastv, __builtin_bit_cast(float, lastt));
     if (!(lastv > -INFINITY)) {
-      for (int i = j + lane; i < a.k; i += 64) list[wave][i] = make_float2(-INFINITY, 0.f);
+      for (int i = j + lane; i < a.k; i += 64) list[wave * BM_MAX_K + i] = make_float2(-INFINITY, 0.f);
       break;
     }
     if (lane == w) next();
   }
   __syncthreads();
   if (wave) return;
-  float2* out = a.lists + (int64_t)blockIdx.x * a.k;
   int at = 0;
-  float2 head = lane < BM_WAVES ? list[lane][0] : make_float2(-INFINITY, 0.f);
+  float2 head = lane < BM_WAVES ? list[lane * BM_MAX_K] : make_float2(-INFINITY, 0.f);
   for (int j = 0; j < a.k; ++j) {
     const int w = bm_winner(head.x, __builtin_bit_cast(int, head.y));
     if (lane == w) {
       out[j] = head;
       ++at;
-      head = at < a.k && lane < BM_WAVES ? list[lane][at] : make_float2(-INFINITY, 0.f);
+      head = at < a.k && lane < BM_WAVES ? list[lane * BM_MAX_K + at] : make_float2(-INFINITY, 0.f);
     }
-  }
-  if (lane == 0) {
-    float M = wm[0];
-#pragma unroll
-    for (int w = 1; w < BM_WAVES; ++w) M = fmaxf(M, wm[w]);
-    double Z = 0.0;
-#pragma unroll
-    for (int w = 0; w < BM_WAVES; ++w) Z += wz[w] * bm_weight(wm[w], M);
-    a.sums[blockIdx.x] = make_double2((double)M, Z);
   }
 }
 
+// ---------------------------------------------------------------------------
+// The choice, one workgroup a request.  A wave merges the lists of a row (a list a lane, the next
+// four of it in registers) and makes values of their logits; then every value counts the ones before
+// it by a search in each other row.
+//
+// The rows' 32-bit sums are good to BM_ERR, and so are the values.  Where two rows' values stand
+// closer than twice that and one of them is among the k, the sums of those rows are made again in 64
+// bits, and the order with them.
+// ---------------------------------------------------------------------------
 #define BM_PICK_WAVES 8
+#define BM_AHEAD 4
+#define BM_FEW 8
+// Of a sum, relative: a weight 2^t is off by |t| ln 2 2^-24 of its exponent's rounding (and as
+// much of the difference's, or log2 e's), 2^-23 of its exponential; |t| up to 30 counts (2^19 tokens
+// 2^-30 weigh 2^-11), and EPT / 4 + 9 additions are off by 2^-24 each: 4e-6.
+#define BM_ERR 0x1p-17
 
+struct BmRow {
+  float m;
+  double z;
+};
+
+__device__ __forceinline__ double bm_value(float score, float x, const BmRow& r, double log_z) {
+#pragma clang fp contract(off)
+  return (double)score + ((x == r.m ? 0.0 : (double)x - (double)r.m) - log_z);
+}
+
+// A row's weights in 64 bits, by the whole workgroup.
+template <int DT>
+__device__ double bm_exact_sum(const BeamArgs& a, int s, int b, float m, double* lds) {
+  typedef SvPiece<DT> P;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const void* row = (const char*)a.logits + (s * a.req_stride + b * a.row_stride) * sv_size<DT>();
+  double z[2] = {0.0, 0.0};
+  for (int64_t v0 = wave * 64 * P::N; v0 < a.V; v0 += BM_PICK_WAVES * 64 * P::N) {
+    P p;
+    p.load(row, (int)v0, a.V, lane, 0);
+#pragma unroll
+    for (int e = 0; e < P::N; ++e) {
+      const float y = p.get(e);
+      z[e & 1] += bm_weight(y == y ? y : -INFINITY, m);
+    }
+  }
+  __syncthreads();
+  const double mine = wave_total(z[0] + z[1]);
+  if (lane == 0) lds[wave] = mine;
+  __syncthreads();
+  double total = 0.0;
+  for (int w = 0; w < BM_PICK_WAVES; ++w) total += lds[w];
+  return total;
+}
+
+// LDS that lanes of one wave hand each other: operations of a wave are in order.
+__device__ __forceinline__ void bm_wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The k best of a row's lists, a list a lane with its first entries in head; how many there are.
+// Entries below the k-th best head are out; the few that are left count the ones before them.  -1
+// where they are more than the lanes.
+__device__ __forceinline__ int bm_merge_few(const BeamArgs& a, const float2* list, const float2 (&head)[BM_AHEAD],
+                                            float* heads, float2* few, float2* out, float M) {
+  const int lane = threadIdx.x & 63;
+  const float h = head[0].x;
+  heads[lane] = h;
+  bm_wave_lds();
+  int above = 0;
+#pragma unroll 4
+  for (int j = 0; j < 64; j += 4) {
+    const float4 o = *(const float4*)(heads + j);
+    above += (o.x > h) + (o.y > h) + (o.z > h) + (o.w > h);
+  }
+  // as -(largest of the negated): the k-th best head, or the lowest finite number
+  float from = -wave_top(above < a.k && h > -INFINITY ? -h : -INFINITY);
+  if (__popcll(__ballot(h > -INFINITY)) < a.k || !(from < INFINITY)) from = -3.402823466e38f;
+  if (M == INFINITY) from = INFINITY;
+  int n = 0;
+  float2 e = head[0];
+#pragma unroll 1
+  for (int i = 0;;) {
+    const bool in = e.x >= from;
+    const uint64_t some = __ballot(in);
+    if (!some) break;
+    const int at = n + __popcll(some & ((1ull << lane) - 1));
+    if (in && at < 64) few[at] = e;
+    n += __popcll(some);
+    if (++i >= a.k) break;
+    if (!in) e.x = -INFINITY;
+    else e = i == 1 ? head[1] : i == 2 ? head[2] : i == 3 ? head[3] : list[i];
+  }
+  if (n > 64) return -1;
+  bm_wave_lds();
+  const float2 mine = few[lane < n ? lane : 0];
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) rank += bm_before(few[j], mine);
+  if (lane < n && rank < a.k) out[rank] = mine;
+  bm_wave_lds();
+  return min(n, a.k);
+}
+
+// The same, one entry after another.
+__device__ __forceinline__ int bm_merge(const BeamArgs& a, const float2* list, float2 (&head)[BM_AHEAD],
+                                        float2* out, float M) {
+  const int lane = threadIdx.x & 63;
+  const float2 none = make_float2(-INFINITY, 0.f);
+  int at = 0, got = 0;
+  for (; got < a.k; ++got) {
+    const int w = bm_winner(head[0].x, __builtin_bit_cast(int, head[0].y));
+    const float x = lane_of(head[0].x, w);
+    if (!(x > -INFINITY) || (M == INFINITY && x < M)) break;
+    if (lane == w) {
+      out[got] = head[0];
+      ++at;
+#pragma unroll
+      for (int j = 0; j + 1 < BM_AHEAD; ++j) head[j] = head[j + 1];
+      head[BM_AHEAD - 1] = none;
+      if (at % BM_AHEAD == 0) {
+#pragma unroll
+        for (int j = 0; j < BM_AHEAD; ++j)
+          if (at + j < a.k) head[j] = list[at + j];
+      }
+    }
+  }
+  bm_wave_lds();
+  return got;
+}
+
+template <int DT>
 __global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs a) {
   __shared__ double value[BM_MAX_BEAMS][BM_MAX_K];
-  __shared__ int token[BM_MAX_BEAMS][BM_MAX_K], count[BM_MAX_BEAMS];
-  __shared__ int pick_b[BM_MAX_K];
-  __shared__ int64_t pick_t[BM_MAX_K];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x;
+  __shared__ float2 cand[BM_MAX_BEAMS][BM_MAX_K];
+  __shared__ int count[BM_MAX_BEAMS];
+  __shared__ BmRow rows[BM_MAX_BEAMS];
+  __shared__ double lds[BM_PICK_WAVES];
+  __shared__ int pick_b[BM_MAX_K], pick_t[BM_MAX_K];
+  __shared__ int64_t stops[BM_MAX_K];
+  __shared__ bool ended[BM_MAX_BEAMS];
+  __shared__ double flat[64];                       // all values in a row, where they are few
+  __shared__ int ranks[64], order[64];
+  __shared__ uint32_t near;                         // a bit a beam
+  __shared__ float heads[BM_PICK_WAVES][64];
+  __shared__ float2 few[BM_PICK_WAVES][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = blockIdx.x;
+  if (tid == 0) near = 0;
+  if (tid < BM_MAX_K) pick_b[tid] = -1;
+  const int64_t own_stop = tid < min(a.stops, BM_MAX_K) ? a.stop[s * a.stop_stride + tid] : -1;
   for (int b = wave; b < a.W; b += BM_PICK_WAVES) {
     const int r = s * a.W + b;
+    const int64_t first = (int64_t)r * a.blocks;
+    const float2* list = a.lists + (first + lane) * a.k;
+    const float2 none = make_float2(-INFINITY, 0.f);
+    // all loads at once; what a row that is not in use has there is not looked at
     const float score = a.scores[r];
-    const bool in = fabsf(score) < INFINITY, over = bm_done(a, r);
+    const bool in = fabsf(score) < INFINITY, over = bm_done(a, r), mine = lane < a.blocks;
+    const float2 own = mine ? a.sums[first + lane] : make_float2(-INFINITY, 0.f);
+    float2 head[BM_AHEAD];
+#pragma unroll
+    for (int j = 0; j < BM_AHEAD; ++j) head[j] = mine && j < a.k ? list[j] : none;
+    if (lane == 0) ended[b] = over;
     if (!in || over) {
       if (lane == 0) {
         value[b][0] = (double)score;
+        cand[b][0] = make_float2(0.f, 0.f);
         count[b] = in ? 1 : 0;
       }
       continue;
     }
-    const int64_t first = (int64_t)r * a.blocks;
-    const double2 own = lane < a.blocks ? a.sums[first + lane] : make_double2(-INFINITY, 0.0);
-    const float M = wave_top((float)own.x);
-    const double Z = wave_total(M > -INFINITY ? own.y * bm_weight((float)own.x, M) : 0.0);
-    const double base = log(Z);
-    const float2* list = a.lists + (first + lane) * a.k;
-    int at = 0, got = 0;
-    float2 head = lane < a.blocks ? list[0] : make_float2(-INFINITY, 0.f);
-    for (; got < a.k; ++got) {
-      const int w = bm_winner(head.x, __builtin_bit_cast(int, head.y));
-      const float x = lane_of(head.x, w);
-      if (!(x > -INFINITY) || (M == INFINITY && x < M)) break;
-      if (lane == w) {
-        value[b][got] = (double)score + ((x == M ? 0.0 : (double)x - (double)M) - base);
-        token[b][got] = __builtin_bit_cast(int, head.y);
-        ++at;
-        head = at < a.k ? list[at] : make_float2(-INFINITY, 0.f);
-      }
+    const float M = wave_top(own.x);
+    BmRow row = {M, wave_total(M > -INFINITY ? (double)own.y * bm_shift(own.x) * bm_weight(own.x, M) : 0.0)};
+    int got = -1;
+    if (a.k >= BM_FEW && a.blocks >= a.k) got = bm_merge_few(a, list, head, heads[wave], few[wave], cand[b], M);
+    if (got < 0) got = bm_merge(a, list, head, cand[b], M);
+    const double log_z = log(row.z);
+    for (int i = lane; i < got; i += 64) value[b][i] = bm_value(score, cand[b][i].x, row, log_z);
+    if (lane == 0) {
+      count[b] = got;
+      rows[b] = row;
     }
-    if (lane == 0) count[b] = got;
   }
+  if (tid < BM_MAX_K) stops[tid] = own_stop;
   __syncthreads();
-  if (wave == 0) {
-    int at = 0;
-    const int have = lane < a.W ? count[lane] : 0;
-    double head = have ? value[lane][0] : -INFINITY;
-    for (int j = 0; j < a.k; ++j) {
-      double top = head;
+  for (int turn = 0; turn < 2; ++turn) {
+    const int all = a.W * a.k;
+    if (all <= 64) {
+      if (wave == 0) {
+        const int b = (int)(((float)lane + 0.5f) * (1.f / (float)a.k)), i = lane - b * a.k;
+        flat[lane] = lane < all && i < count[b] ? value[b][i] : -INFINITY;
+        ranks[lane] = 0;
+      }
+      __syncthreads();
+      // a value a lane; every wave counts eight of the others
+      const double v = flat[lane];
+      int before = 0;
 #pragma unroll
-      for (int o = 32; o; o >>= 1) top = fmax(top, __shfl_xor(top, o));
-      const uint64_t best = __ballot(head == top);
-      const int w = __ffsll((unsigned long long)best) - 1;
-      if (lane == w) {
-        const bool found = top > -INFINITY;
-        const int64_t t = !found ? -1 : bm_done(a, s * a.W + lane) ? a.pad : token[lane][at];
-        pick_b[j] = found ? lane : -1;
-        pick_t[j] = t;
-        a.out_scores[s * a.k + j] = (float)top;
-        if (found) {
-          ++at;
-          head = at < have ? value[lane][at] : -INFINITY;
+      for (int j = 0; j < 8; ++j) {
+        const double y = flat[wave * 8 + j];
+        before += y > v || (y == v && wave * 8 + j < lane);    // of one row the lists are in order
+      }
+      if (before) atomicAdd(&ranks[lane], before);
+      __syncthreads();
+      if (wave == 0) {
+        order[ranks[lane]] = lane;                         // a permutation: equal values by lane
+        bm_wave_lds();
+        const int up = order[lane], down = order[min(lane + 1, 63)];
+        const double vu = flat[up], vd = flat[down], vk = flat[order[a.k - 1]];
+        const int bu = (int)(((float)up + 0.5f) * (1.f / (float)a.k));
+        if (lane < a.k && vu > -INFINITY) {
+          pick_b[lane] = bu;
+          pick_t[lane] = up - bu * a.k;
+        }
+        // next to one another, of two rows, and one of them may be among the k
+        if (turn == 0 && vd > -INFINITY && vu - vd <= 2 * BM_ERR && vk - vd <= 2 * BM_ERR) {
+          const int bd = (int)(((float)down + 0.5f) * (1.f / (float)a.k));
+          if (bu != bd && !(ended[bu] && ended[bd])) atomicOr(&near, 1u << bu | 1u << bd);
         }
       }
+    } else
+    for (int c = tid; c < all; c += 64 * BM_PICK_WAVES) {
+      const int b = c / a.k, i = c - b * a.k;
+      if (i >= count[b]) continue;
+      const double v = value[b][i];
+      const bool over = ended[b];
+      int rank = i;
+      uint32_t close = 0;
+      for (int o = 0; o < a.W; ++o) {
+        if (o == b) continue;
+        // values of row o before this one
+        int lo = 0, hi = count[o];
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          const double y = value[o][mid];
+          if (y > v || (y == v && o < b)) lo = mid + 1;
+          else hi = mid;
+        }
+        rank += lo;
+        const bool tight = (lo > 0 && value[o][lo - 1] - v <= 2 * BM_ERR) ||
+                           (lo < count[o] && v - value[o][lo] <= 2 * BM_ERR);
+        if (tight && !(over && ended[o])) close |= 1u << o | 1u << b;
+      }
+      if (rank >= a.k) continue;
+      pick_b[rank] = b;
+      pick_t[rank] = i;
+      if (turn == 0 && close) atomicOr(&near, close);
     }
+    __syncthreads();
+    const uint32_t again = turn ? 0 : near;
+    if (!again) break;
+    for (int b = 0; b < a.W; ++b) {
+      if (!(again >> b & 1) || ended[b]) continue;
+      BmRow row = rows[b];
+      row.z = bm_exact_sum<DT>(a, s, b, row.m, lds);
+      const double log_z = log(row.z);
+      const float score = a.scores[s * a.W + b];
+      for (int i = tid; i < count[b]; i += 64 * BM_PICK_WAVES)
+        value[b][i] = bm_value(score, cand[b][i].x, row, log_z);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int j = threadIdx.x; j < a.k; j += 64 * BM_PICK_WAVES) {
+  for (int j = tid; j < a.k; j += 64 * BM_PICK_WAVES) {
     const int b = pick_b[j];
-    const int64_t t = pick_t[j];
-    bool over = b < 0 || bm_done(a, s * a.W + b);
-    for (int i = 0; i < a.stops; ++i) over |= a.stop[s * a.stop_stride + i] == t;
+    int64_t t = -1;
+    bool over = true;
+    float v = -INFINITY;
+    if (b >= 0) {
+      over = ended[b];
+      t = over ? a.pad : __builtin_bit_cast(int, cand[b][pick_t[j]].y);
+      v = (float)value[b][pick_t[j]];
+    }
+    for (int i = 0; i < min(a.stops, BM_MAX_K); ++i) over |= stops[i] == t;
+    for (int i = BM_MAX_K; i < a.stops; ++i) over |= a.stop[s * a.stop_stride + i] == t;
     const int64_t o = (int64_t)s * a.k + j;
+    a.out_scores[o] = v;
     a.parents[o] = b;
     a.tokens[o] = t;
     a.out_done[o] = over;
   }
 }
 
-// Tokens of a block: 4096 where rows are few, 8192 else.
+// Tokens of a block, 256 times this: as many as leave a workgroup for every CU twice, or as few.
 static int bm_ept(int64_t rows, int V) {
-  return rows * ceil_div(V, 8192) < 512 && V <= 4096 * BM_MAX_BLOCKS ? 16 : 32;
+  for (int ept = 32; ept > 8; ept /= 2)
+    if (rows * ceil_div(V, 256 * ept) >= 512 || V > 128 * ept * BM_MAX_BLOCKS) return ept;
+  return 8;
 }
 
 static int64_t bm_work(int n, int W, int V, int k) {
   if (n < 0 || W < 1 || V < 1 || k < 1) return OMNI_EINVAL;
-  if (W > BM_MAX_BEAMS || k > BM_MAX_K || V > 8192 * BM_MAX_BLOCKS) return OMNI_EUNSUPPORTED;
+  if (n > 65535 || W > BM_MAX_BEAMS || k > BM_MAX_K || V > 8192 * BM_MAX_BLOCKS) return OMNI_EUNSUPPORTED;
   const int64_t rows = (int64_t)n * W;
   const int64_t blocks = ceil_div(V, 64 * BM_WAVES * bm_ept(rows, V));
-  const int64_t work = rows * blocks * (k + 2);
+  const int64_t work = rows * blocks * (k + 1);
   return rows * blocks > 0x7fffffff || work > 0x7fffffff ? OMNI_EUNSUPPORTED : work;
 }
 
@@ -254,23 +553,29 @@ extern "C" int omni_beam_select(const void* logits, int dtype, int64_t req_strid
     return OMNI_EINVAL;
   const int64_t rows = (int64_t)n * beams;
   const int ept = bm_ept(rows, vocab), blocks = ceil_div(vocab, 64 * BM_WAVES * ept);
-  double2* sums = (double2*)workspace;
+  float2* sums = (float2*)workspace;
   const BeamArgs a = {logits, req_stride, row_stride, scores, (const uint8_t*)done, stop, stop_stride,
-                      stops, n, beams, vocab, k, blocks, pad, (float2*)(sums + rows * blocks), sums,
+                      stops, n, beams, vocab, k, blocks, pad, sums + rows * blocks, sums,
                       out_scores, parents, tokens, (uint8_t*)out_done};
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(rows * blocks)), block(64 * BM_WAVES);
-  if (ept == 16) {
-    if (dtype == 0) hipLaunchKernelGGL((beam_scan_kernel<0, 16>), grid, block, 0, st, a);
-    else if (dtype == 1) hipLaunchKernelGGL((beam_scan_kernel<1, 16>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((beam_scan_kernel<2, 16>), grid, block, 0, st, a);
+  const dim3 grid(blocks, beams, n), block(64 * BM_WAVES);
+#define BM_SCAN(DT)                                                                          \
+  if (ept == 8) hipLaunchKernelGGL((beam_scan_kernel<DT, 8>), grid, block, 0, st, a);        \
+  else if (ept == 16) hipLaunchKernelGGL((beam_scan_kernel<DT, 16>), grid, block, 0, st, a); \
+  else hipLaunchKernelGGL((beam_scan_kernel<DT, 32>), grid, block, 0, st, a);
+  if (dtype == 0) {
+    BM_SCAN(0)
+  } else if (dtype == 1) {
+    BM_SCAN(1)
   } else {
-    if (dtype == 0) hipLaunchKernelGGL((beam_scan_kernel<0, 32>), grid, block, 0, st, a);
-    else if (dtype == 1) hipLaunchKernelGGL((beam_scan_kernel<1, 32>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((beam_scan_kernel<2, 32>), grid, block, 0, st, a);
+    BM_SCAN(2)
   }
+#undef BM_SCAN
   OMNI_CHECK_LAUNCH();
-  hipLaunchKernelGGL(beam_pick_kernel, dim3(n), dim3(64 * BM_PICK_WAVES), 0, st, a);
+  const dim3 picks(64 * BM_PICK_WAVES);
+  if (dtype == 0) hipLaunchKernelGGL(beam_pick_kernel<0>, dim3(n), picks, 0, st, a);
+  else if (dtype == 1) hipLaunchKernelGGL(beam_pick_kernel<1>, dim3(n), picks, 0, st, a);
+  else hipLaunchKernelGGL(beam_pick_kernel<2>, dim3(n), picks, 0, st, a);
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }

@@ -7,6 +7,14 @@
 template <int DT>
 __device__ __forceinline__ constexpr int sv_size() { return DT == 2 ? 4 : 2; }
 
+template <int DT>   // 0 fp16, 1 bf16, 2 fp32; NaN as -inf
+__device__ __forceinline__ float sv_logit(const void* row, int64_t v) {
+  float x;
+  if (DT == 2) x = ((const float*)row)[v];
+  else x = ld16f<DT == 1>(((const unsigned short*)row)[v]);
+  return x == x ? x : -INFINITY;
+}
+
 // 2^t for -2100 <= t <= 0: t = n + f, |f| <= 1/2, n from the low word of t + 1.5 2^52, 2^f by the
 // polynomial through its values at the eleven Chebyshev points of [-1/2, 1/2] (relative error 4e-16,
 // its roundings included), 2^n by the exponent (0 far below).  Nine points are off by 1.1e-12: a

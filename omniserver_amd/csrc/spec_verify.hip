@@ -77,14 +77,6 @@ struct SvSeq {             // what the walk leaves for the draw
   double r0;               // the drawn rows' ratio of 32-bit sums, target / draft
 };
 
-template <int DT>   // 0 fp16, 1 bf16, 2 fp32; NaN as -inf
-__device__ __forceinline__ float sv_logit(const void* row, int64_t v) {
-  float x;
-  if (DT == 2) x = ((const float*)row)[v];
-  else x = ld16f<DT == 1>(((const unsigned short*)row)[v]);
-  return x == x ? x : -INFINITY;
-}
-
 template <int DT>
 __device__ __forceinline__ const void* sv_row(const SvArgs& a, int s, int i) {
   return (const char*)a.logits + (s * a.seq_stride + i * a.row_stride) * sv_size<DT>();
