@@ -203,7 +203,7 @@ int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t 
 /* Pages of a paged KV cache.  Sequence r holds lengths[r] tokens (int64; taken as within [0,
  * max_len]), token t in page tables[r][t / page_size] (int32 [seqs][width]), place t % page_size.  A
  * page is free where no sequence's table names it within its length.  seqs up to 2048, pages up to
- * 2^20, page_size a power of two from 16 to 1024, width * page_size at least max_len.
+ * 2^19, page_size a power of two from 16 to 1024, width * page_size at least max_len.
  *
  * Request i of n brings counts[i] tokens (int32; NULL: one; less than one: none) to sequence rows[i]
  * (int64, all different; NULL: i), packed into `tokens` rows one request after another; dense:

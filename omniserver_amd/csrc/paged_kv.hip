@@ -9,7 +9,7 @@
 
 #define PG_THREADS 1024
 #define PG_WAVES (PG_THREADS / 64)
-#define PG_MAX_PAGES (1 << 20)     // a bit each in LDS: 128 KB
+#define PG_MAX_PAGES (1 << 19)     // a bit each in LDS: 64 KB
 #define PG_MAX_SEQS 2048
 
 struct PageTables {
@@ -29,26 +29,33 @@ __device__ __forceinline__ int pg_pages(const PageTables& t, int64_t tokens) {
 
 // Sums of non-negative numbers up to 2^30, which they stay at.
 __device__ __forceinline__ int pg_add(int a, int b) { return min(a + b, 1 << 30); }
+// What the lane CTRL moves here holds, in the rows of 16 lanes that ROWS names; else 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int pg_move(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
 
-// Inclusive prefix sum over the workgroup; total in all threads.  lds: PG_WAVES ints.
+// Inclusive prefix sum over the workgroup; total in all threads.  lds: PG_WAVES ints, free for a new
+// call after the caller's next barrier.
 __device__ __forceinline__ int pg_scan(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int x = __shfl_up(v, o);
-    if (lane >= o) v = pg_add(v, x);
-  }
-  __syncthreads();                                 // the last call's sums are read
+  v = pg_add(v, pg_move<0x111>(v));                // from 1, 2, 4, 8 lanes below
+  v = pg_add(v, pg_move<0x112>(v));
+  v = pg_add(v, pg_move<0x114>(v));
+  v = pg_add(v, pg_move<0x118>(v));
+  v = pg_add(v, pg_move<0x142, 0xa>(v));           // a row's total into the next row
+  v = pg_add(v, pg_move<0x143, 0xc>(v));           // the lower half's into the upper
   if (lane == 63) lds[wave] = v;
   __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < PG_WAVES; ++w) {
-    if (w == wave) before = total;
-    total = pg_add(total, lds[w]);
-  }
-  return pg_add(v, before);
+  // a wave's sum a lane, the same way
+  int sums = lane < PG_WAVES ? lds[lane] : 0;
+  sums = pg_add(sums, pg_move<0x111>(sums));
+  sums = pg_add(sums, pg_move<0x112>(sums));
+  sums = pg_add(sums, pg_move<0x114>(sums));
+  sums = pg_add(sums, pg_move<0x118>(sums));
+  total = __builtin_amdgcn_readlane(sums, PG_WAVES - 1);
+  const int w = __builtin_amdgcn_readfirstlane(wave);
+  return pg_add(v, w ? __builtin_amdgcn_readlane(sums, w - 1) : 0);
 }
 
 // First i in [0, n) with ends[i] > x (ends ascends), n if there is none.
@@ -63,52 +70,68 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
 }
 
 // Set the bits of the pages that sequences hold; held(row) gives how many of a row's entries count
-// and which one of them does not.  2^group lanes a row, four entries a lane.
+// and which one of them does not.  2^group lanes a row, four entries a lane at a time.
 template <typename Held>
 __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held) {
   const int lanes = 1 << group, l = threadIdx.x & (lanes - 1);
+#pragma unroll 1
   for (int row = threadIdx.x >> group; row < t.seqs; row += PG_THREADS >> group) {
     int but;
     const int count = held(row, but);
     const int* entry = t.tables + (int64_t)row * t.width;
-#pragma unroll 4
-    for (int j = l; j < count; j += lanes) {
-      const int p = entry[j];
-      if (j != but && p >= 0 && p < t.pages) atomicOr(&used[p >> 5], 1u << (p & 31));
+    auto mark = [&](int j, int p) {
+      if (j < count && j != but && p >= 0 && p < t.pages) atomicOr(&used[p >> 5], 1u << (p & 31));
+    };
+#pragma unroll 1
+    for (int j0 = 4 * l; j0 < count; j0 += 16 * lanes) {
+      i32x4 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + 4 * lanes * u;
+        p[u] = (i32x4){-1, -1, -1, -1};
+        if (j + 4 <= t.width) {
+          if (j < count) __builtin_memcpy(&p[u], entry + j, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 3; ++e)
+            if (j + e < count) p[u][e] = entry[j + e];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mark(j0 + 4 * lanes * u + e, p[u][e]);
     }
   }
 }
 
-// The free pages counted in order: first[t] of them are below thread t's words; returns how many
+// The free pages counted in order: `first` of them are below this thread's words; returns how many
 // there are.  Bits past the pool count as used.
-__device__ __forceinline__ int pg_count_free(const PageTables& t, uint32_t* used, int* first, int* lds) {
+__device__ __forceinline__ int pg_count_free(const PageTables& t, uint32_t* used, int& first, int* lds) {
   const int words = (t.pages + 31) >> 5, per = ceil_div(words, PG_THREADS);
+  const int end = min((int)(threadIdx.x + 1) * per, words);
   int mine = 0;
-  for (int w = threadIdx.x * per; w < min((int)(threadIdx.x + 1) * per, words); ++w) {
+#pragma unroll 1
+  for (int w = threadIdx.x * per; w < end; ++w) {
     if (w == words - 1 && (t.pages & 31)) used[w] |= ~0u << (t.pages & 31);
     mine += 32 - __popc(used[w]);
   }
   int total;
-  const int upto = pg_scan(mine, lds, total);
-  first[threadIdx.x] = upto - mine;
-  __syncthreads();
+  first = pg_scan(mine, lds, total) - mine;
   return total;
 }
 
-// give(rank, page) for the `want` lowest free pages; half a wave a word, a lane a bit.
+// give(rank, page) for the `want` lowest free pages, by the threads that counted them, in order.
 template <typename Give>
-__device__ __forceinline__ void pg_deal(const PageTables& t, const uint32_t* used, const int* first,
-                                        int want, Give give) {
+__device__ __forceinline__ void pg_deal(const PageTables& t, const uint32_t* used, int first, int want,
+                                        Give give) {
   const int words = (t.pages + 31) >> 5, per = ceil_div(words, PG_THREADS);
-  const int bit = threadIdx.x & 31;
-  for (int w = threadIdx.x >> 5; w < words; w += PG_THREADS / 32) {
-    int rank = first[w / per];
-    if (rank >= want) break;
-    for (int x = w / per * per; x < w; ++x) rank += 32 - __popc(used[x]);
-    const uint32_t free = ~used[w];
-    rank += __popc(free & ((1u << bit) - 1));
-    if ((free >> bit & 1) && rank < want) give(rank, w * 32 + bit);
-  }
+  const int end = min((int)(threadIdx.x + 1) * per, words);
+#pragma unroll 1
+  for (int w = threadIdx.x * per; w < end && first < want; ++w)
+#pragma unroll 1
+    for (uint32_t free = ~used[w]; free && first < want; free &= free - 1, ++first)
+      give(first, w * 32 + __ffs(free) - 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -144,131 +167,137 @@ struct ReserveArgs {
   int group, slots_here;
 };
 
-__device__ __forceinline__ void pg_slot(const PageTables& t, const ReserveArgs& r, int tok, int i,
-                                        int row, int L, int at, bool ok) {
-  int64_t page = -1, place = -1, pos = -1;
-  if (ok) {
-    const int p = L + at;
-    page = t.tables[(int64_t)row * t.width + (p >> t.shift)];
-    place = p & ((1 << t.shift) - 1);
-    pos = p + (r.rope_delta ? r.rope_delta[row] : 0);
-  }
+// Token row tok is position p of the sequence, in that page (-1: it has no slot).
+__device__ __forceinline__ void pg_slot(const PageTables& t, const ReserveArgs& r, int tok, int page,
+                                        int p, int64_t delta) {
+  const bool ok = page >= 0;
   r.token_page[tok] = page;
-  r.token_pos[tok] = place;
-  for (int a = 0; a < r.axes; ++a) r.positions[(int64_t)a * r.T + tok] = pos;
+  r.token_pos[tok] = ok ? p & ((1 << t.shift) - 1) : -1;
+  for (int a = 0; a < r.axes; ++a) r.positions[(int64_t)a * r.T + tok] = ok ? p + delta : -1;
 }
 
 __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, ReserveArgs r) {
   extern __shared__ uint32_t pg_smem[];
-  __shared__ int first[PG_THREADS], lds[PG_WAVES];
+  __shared__ int lds[4][PG_WAVES];
   const int tid = threadIdx.x, words = (t.pages + 31) >> 5;
   uint32_t* used = pg_smem;
   int* ends = (int*)pg_smem + words;                // new pages up to and with request i
-  int* last = ends + r.n;                           // token rows up to and with request i
+  int* last = ends + r.n;                           // token rows up to and with request i, then units
+  int* len = last + r.n;                            // length, and tokens that it may be granted
+  int* ask = len + r.n;
+  int* at = ask + r.n;                              // dense: the token's page
+#pragma unroll 1
   for (int w = tid; w < words; w += PG_THREADS) used[w] = 0;
-  auto row_of = [&](int i) { return r.rows ? r.rows[i] : (int64_t)i; };
-  // tokens of request i: none where they do not fit
-  auto ask = [&](int i, int& L, int& asked) {
-    const int64_t row = row_of(i);
-    const bool in = row >= 0 && row < t.seqs;
-    L = in ? pg_length(t, row) : 0;
-    asked = max(r.counts ? r.counts[i] : 1, 0);
-    if (r.dense) asked = min(asked, 1);
-    return in && asked <= t.max_len - L ? asked : 0;
-  };
   int wanted = 0, rows_sum = 0;
+#pragma unroll 1
   for (int base = 0; base < r.n; base += PG_THREADS) {
     const int i = base + tid;
-    int need = 0, asked = 0, L;
+    int need = 0, asked = 0, total;
     if (i < r.n) {
-      const int c = ask(i, L, asked);
+      const int64_t row = r.rows ? r.rows[i] : (int64_t)i;
+      const bool in = row >= 0 && row < t.seqs;
+      const int L = in ? pg_length(t, row) : 0;
+      asked = max(r.counts ? r.counts[i] : 1, 0);
+      if (r.dense) asked = min(asked, 1);
+      const int c = in && asked <= t.max_len - L ? asked : 0;
       need = pg_pages(t, L + c) - pg_pages(t, L);
+      if (r.dense) at[i] = c && !need ? t.tables[row * t.width + (L >> t.shift)] : -1;
+      len[i] = L;
+      ask[i] = c;
+      last[i] = i + 1;
     }
-    // a request whose token rows run past T needs nothing: sums of token rows first
-    int total;
-    const int upto = pg_add(pg_scan(min(asked, 1 << 30), lds, total), rows_sum);
-    rows_sum = pg_add(rows_sum, total);
-    if (!r.dense && upto > r.T) need = 0;
-    const int pages = pg_add(pg_scan(need, lds, total), wanted);
+    if (!r.dense) {
+      // a request whose token rows run past T gets none
+      const int upto = pg_add(pg_scan(min(asked, 1 << 30), lds[0], total), rows_sum);
+      rows_sum = pg_add(rows_sum, total);
+      if (i < r.n) {
+        last[i] = upto;
+        if (upto > r.T) need = ask[i] = 0;
+      }
+    }
+    const int pages = pg_add(pg_scan(need, lds[1], total), wanted);
     wanted = pg_add(wanted, total);
-    if (i < r.n) {
-      ends[i] = pages;
-      last[i] = r.dense ? i + 1 : upto;
-    }
+    if (i < r.n) ends[i] = pages;
+    __syncthreads();                                // the sums are read
   }
-  __syncthreads();
   pg_mark(t, used, r.group, [&](int row, int& but) {
     but = -1;
     return pg_pages(t, pg_length(t, row));
   });
   __syncthreads();
-  const int left = pg_count_free(t, used, first, lds);
+  int first;
+  const int left = pg_count_free(t, used, first, lds[2]);
+  int to = -1, low = 0, high = 0;                   // the request of this thread's next page
   pg_deal(t, used, first, min(left, wanted), [&](int rank, int page) {
-    const int i = pg_find(ends, r.n, rank);
-    if (i >= r.n || ends[i] > left) return;
-    const int64_t row = row_of(i);
-    const int j = pg_pages(t, pg_length(t, row)) + rank - (i ? ends[i - 1] : 0);
-    t.tables[row * t.width + j] = page;
+    if (rank >= high) {
+      to = to < 0 ? pg_find(ends, r.n, rank) : to + 1;
+      while (to < r.n && ends[to] <= rank) ++to;
+      if (to >= r.n) return;
+      low = to ? ends[to - 1] : 0;
+      high = ends[to];
+    }
+    if (to >= r.n || high > left) return;
+    const int64_t row = r.rows ? r.rows[to] : (int64_t)to;
+    t.tables[row * t.width + pg_pages(t, len[to]) + rank - low] = page;
+    if (r.dense) at[to] = page;
   });
-  auto grant = [&](int i, int& L) {
-    int asked;
-    const int c = ask(i, L, asked);
-    const bool fits = r.dense || last[i] <= r.T;
-    const bool paid = ends[i] == (i ? ends[i - 1] : 0) || ends[i] <= left;
-    return fits && paid ? c : 0;
-  };
   __syncthreads();                                  // the tables are written
-  for (int i = tid; i < r.n; i += PG_THREADS) {
-    int L;
-    const int c = grant(i, L);
-    r.granted[i] = c;
-    r.starts[i] = L;
-    r.after[i] = L + c;
-    r.cu[i + 1] = last[i];
-    if (i == 0) r.cu[0] = 0;
-    if (r.dense) pg_slot(t, r, i, i, (int)row_of(i), L, 0, c > 0);
+  int units = 0;
+#pragma unroll 1
+  for (int base = 0; base < r.n; base += PG_THREADS) {
+    const int i = base + tid;
+    int mine = 0, total;
+    if (i < r.n) {
+      const int L = len[i], low_i = i ? ends[i - 1] : 0;
+      const int c = ends[i] == low_i || ends[i] <= left ? ask[i] : 0;
+      ask[i] = c;
+      r.granted[i] = c;
+      r.starts[i] = L;
+      r.after[i] = L + c;
+      r.cu[i + 1] = last[i];
+      if (i == 0) r.cu[0] = 0;
+      if (r.dense) {
+        const int64_t row = r.rows ? r.rows[i] : (int64_t)i;
+        pg_slot(t, r, i, c ? at[i] : -1, L, c && r.rope_delta ? r.rope_delta[row] : 0);
+        mine = c ? ceil_div(L + c, PG_UNIT) : 0;
+      }
+    }
+    if (r.schedule) {
+      const int upto = pg_scan(mine, lds[3], total) + units;
+      units += total;
+      if (i < r.n) last[i] = upto;
+    }
+    __syncthreads();
   }
   if (!r.dense && r.slots_here) {
+#pragma unroll 1
     for (int tok = tid; tok < r.T; tok += PG_THREADS) {
       const int i = pg_find(last, r.n, tok);
-      int L = 0, c = 0;
-      if (i < r.n) c = grant(i, L);
-      pg_slot(t, r, tok, i, c ? (int)row_of(i) : 0, L, c ? tok - (i ? last[i - 1] : 0) : 0, c > 0);
+      int page = -1, p = 0;
+      int64_t row = 0;
+      if (i < r.n && ask[i]) {
+        row = r.rows ? r.rows[i] : (int64_t)i;
+        p = len[i] + tok - (i ? last[i - 1] : 0);
+        page = t.tables[row * t.width + (p >> t.shift)];
+      }
+      pg_slot(t, r, tok, page, p, page >= 0 && r.rope_delta ? r.rope_delta[row] : 0);
     }
   }
   if (!r.schedule) return;
-  // the schedule, over the sums of units (in place of the sums of token rows)
-  int units = 0;
-  __syncthreads();
-  for (int base = 0; base < r.n; base += PG_THREADS) {
-    const int i = base + tid;
-    int L, c = 0, mine = 0, total;
-    if (i < r.n && (c = grant(i, L)) > 0) mine = ceil_div(L + c, PG_UNIT);
-    const int upto = pg_scan(mine, lds, total) + units;
-    units += total;
-    if (i < r.n) last[i] = upto;
-  }
-  __syncthreads();
   const int cols = min(r.ncols, units);
-  auto cut = [&](int c) { return (int)((int64_t)c * units / cols); };
   auto column_of = [&](int x) { return (int)((((int64_t)x + 1) * cols - 1) / units); };
-  for (int i = tid; i < r.n; i += PG_THREADS) {
-    int L;
-    const int c = grant(i, L), lo = i ? last[i - 1] : 0, hi = last[i];
-    i32x4 v = {c ? L + c : 0, 0, 0, 0};
-    if (hi > lo) {
-      v[1] = column_of(lo);
-      v[2] = column_of(hi - 1);
+#pragma unroll 1
+  for (int i = tid; i < r.n + r.ncols; i += PG_THREADS) {
+    i32x4 v = {0, 0, 0, 0};
+    if (i < r.n) {
+      const int lo = i ? last[i - 1] : 0, hi = last[i];
+      if (hi > lo) v = (i32x4){len[i] + ask[i], column_of(lo), column_of(hi - 1), 0};
+    } else if (i - r.n < cols) {
+      const int64_t c = i - r.n;
+      const int lo = (int)(c * units / cols), s = pg_find(last, r.n, lo);
+      v = (i32x4){s, lo - (s ? last[s - 1] : 0), (int)((c + 1) * units / cols) - lo, 0};
     }
     *(i32x4*)(r.schedule + 4 * i) = v;
-  }
-  for (int c = tid; c < r.ncols; c += PG_THREADS) {
-    i32x4 v = {0, 0, 0, 0};
-    if (c < cols) {
-      const int lo = cut(c), i = pg_find(last, r.n, lo);
-      v = (i32x4){i, lo - (i ? last[i - 1] : 0), cut(c + 1) - lo, 0};
-    }
-    *(i32x4*)(r.schedule + 4 * r.n + 4 * c) = v;
   }
 }
 
@@ -280,16 +309,21 @@ __global__ __launch_bounds__(256) void page_slots_kernel(PageTables t, ReserveAr
   const int tok = blockIdx.x * 256 + threadIdx.x;
   if (tok >= r.T) return;
   const int i = pg_find(last, r.n, tok);
-  const int c = i < r.n ? r.granted[i] : 0;
-  const int L = c ? (int)r.starts[i] : 0;
-  pg_slot(t, r, tok, i, c ? (int)(r.rows ? r.rows[i] : i) : 0, L, c ? tok - (i ? last[i - 1] : 0) : 0,
-          c > 0);
+  int page = -1, p = 0;
+  int64_t row = 0;
+  if (i < r.n && r.granted[i]) {
+    row = r.rows ? r.rows[i] : (int64_t)i;
+    p = (int)r.starts[i] + tok - (i ? last[i - 1] : 0);
+    page = t.tables[row * t.width + (p >> t.shift)];
+  }
+  pg_slot(t, r, tok, page, p, page >= 0 && r.rope_delta ? r.rope_delta[row] : 0);
 }
 
 __global__ void page_gather_kernel(PageTables t, const int* __restrict__ parents, int rows, int W);
 struct CopyItem {
   int from, to, rows, pad;       // pages, token rows
 };
+template <bool HERE>
 __global__ void page_fork_kernel(PageTables t, const int* __restrict__ parents, int rows, int W,
                                  CopyItem* __restrict__ items, int group);
 
@@ -321,8 +355,8 @@ static int pg_tables_ok(const int* tables, const int64_t* lengths, int seqs, int
 static int pg_allow_lds() {
   static const int rc = [] {
     hipError_t e = hipSuccess;
-    for (const void* k : {(const void*)page_reserve_kernel, (const void*)page_fork_kernel,
-                          (const void*)page_gather_kernel})
+    for (const void* k : {(const void*)page_reserve_kernel, (const void*)page_fork_kernel<false>,
+                          (const void*)page_fork_kernel<true>, (const void*)page_gather_kernel})
       if (e == hipSuccess)
         e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 152 << 10);
     return (int)e;
@@ -354,7 +388,7 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
   ReserveArgs r = {counts, rows, rope_delta, n, tokens, dense, axes, starts, after, token_page,
                    token_pos, positions, granted, cu, schedule, columns, pg_group(seqs),
                    tokens <= PG_SLOTS_HERE};
-  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 2 * (size_t)n);
+  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 5 * (size_t)n);
   if (smem > (32 << 10) && pg_allow_lds()) return pg_allow_lds();
   hipLaunchKernelGGL(page_reserve_kernel, dim3(1), dim3(PG_THREADS), smem, (hipStream_t)stream, t, r);
   OMNI_CHECK_LAUNCH();
@@ -375,6 +409,7 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
 // and new pages, one workgroup; the copies.
 // ---------------------------------------------------------------------------
 #define PG_COLS 16
+#define PG_TILE 8192               // table entries that one workgroup moves
 
 __global__ __launch_bounds__(256) void page_gather_kernel(PageTables t, const int* __restrict__ parents,
                                                           int rows, int W) {
@@ -391,61 +426,92 @@ __global__ __launch_bounds__(256) void page_gather_kernel(PageTables t, const in
   }
 }
 
+// HERE: the tables are few enough for this workgroup's LDS, and it moves them itself.
+template <bool HERE>
 __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, const int* __restrict__ parents,
                                                                int rows, int W, CopyItem* __restrict__ items,
                                                                int group) {
   extern __shared__ uint32_t pg_smem[];
-  __shared__ int first[PG_THREADS], lds[PG_WAVES];
+  __shared__ int lds[2][PG_WAVES];
   const int tid = threadIdx.x, words = (t.pages + 31) >> 5, page = 1 << t.shift;
   uint32_t* used = pg_smem;
   int* len = (int*)pg_smem + words;                 // lengths after; ~length: with a page of its own
   int* ends = len + rows;                           // pages up to and with row r
+  int* from = ends + rows;                          // the page that is filled in part
+  int* up = from + rows;                            // the row that row r goes on from, or -1
+  int* tile = up + rows;                            // HERE: [rows][width], the tables before
+#pragma unroll 1
   for (int w = tid; w < words; w += PG_THREADS) used[w] = 0;
+  if (HERE) {
+#pragma unroll 4
+    for (int e = tid; e < rows * t.width; e += PG_THREADS) tile[e] = t.tables[e];
+  }
   int wanted = 0;
+#pragma unroll 1
   for (int base = 0; base < rows; base += PG_THREADS) {
     const int r = base + tid;
     int L = 0, total;
     bool later = false;
     if (r < rows) {
       const int w = r % W, p = parents[r];
+      up[r] = -1;
       if (p >= 0 && p < W) {
+        up[r] = r - w + p;
         L = pg_length(t, r - w + p);
         for (int x = 0; x < w; ++x) later |= parents[r - w + x] == p;
         later &= (L & (page - 1)) != 0;
+        // moved tables are this row's own by now
+        if (later && !HERE) from[r] = t.tables[(int64_t)r * t.width + (L >> t.shift)];
       }
       len[r] = later ? ~L : L;
     }
-    const int upto = pg_scan(later ? 1 : 0, lds, total) + wanted;
+    const int upto = pg_scan(later ? 1 : 0, lds[0], total) + wanted;
     wanted += total;
     if (r < rows) ends[r] = upto;
+    __syncthreads();                                // the sums are read
   }
-  __syncthreads();
+  if (HERE) {
+    // a wave a row: its new table, and the pages in it
+#pragma unroll 1
+    for (int r = tid >> 6; r < rows; r += PG_WAVES) {
+      const int v = len[r], L = v < 0 ? ~v : v, source = up[r];
+      if (source < 0) continue;
+      const int held = pg_pages(t, L), but = v < 0 ? L >> t.shift : -1;
+#pragma unroll 2
+      for (int c = tid & 63; c < held; c += 64) {
+        const int p = tile[source * t.width + c];
+        if (source != r) t.tables[r * t.width + c] = p;
+        if (c == but) from[r] = p;
+        else if (p >= 0 && p < t.pages) atomicOr(&used[p >> 5], 1u << (p & 31));
+      }
+    }
+  }
   pg_mark(t, used, group, [&](int row, int& but) {
     but = -1;
     if (row >= rows) return pg_pages(t, pg_length(t, row));
+    if (HERE) return 0;
     const int v = len[row], L = v < 0 ? ~v : v;
     if (v < 0) but = L >> t.shift;
     return pg_pages(t, L);
   });
   __syncthreads();
-  const int left = pg_count_free(t, used, first, lds);
+  int first;
+  const int left = pg_count_free(t, used, first, lds[1]);
+#pragma unroll 1
   for (int r = tid; r < rows; r += PG_THREADS) {
     const int v = len[r];
-    if (v >= 0 || ends[r] > left) {
-      t.lengths[r] = v >= 0 ? v : 0;
-      items[r] = {0, 0, 0, 0};
-    }
+    const bool copies = v < 0 && ends[r] <= left;
+    t.lengths[r] = v >= 0 ? v : copies ? ~v : 0;
+    if (!copies) items[r] = {0, 0, 0, 0};
   }
-  pg_deal(t, used, first, min(left, wanted), [&](int rank, int to) {
-    const int r = pg_find(ends, rows, rank);
-    if (r >= rows) return;
-    const int L = ~len[r];
-    int* entry = t.tables + (int64_t)r * t.width + (L >> t.shift);
-    const int from = *entry;
-    *entry = to;
-    t.lengths[r] = L;
-    const bool in = from >= 0 && from < t.pages;
-    items[r] = {in ? from : 0, to, in ? L & (page - 1) : 0, 0};
+  int to = -1;
+  pg_deal(t, used, first, min(left, wanted), [&](int rank, int own) {
+    to = to < 0 ? pg_find(ends, rows, rank) : to + 1;
+    while (len[to] >= 0) ++to;                      // the next row with a page of its own
+    const int L = ~len[to], p = from[to];
+    t.tables[(int64_t)to * t.width + (L >> t.shift)] = own;
+    const bool in = p >= 0 && p < t.pages;
+    items[to] = {in ? p : 0, own, in ? L & (page - 1) : 0, 0};
   });
 }
 
@@ -479,12 +545,19 @@ extern "C" int omni_page_reorder(void* pool, int n_layers, int row_halfs, int* t
   const PageTables t = {tables, lengths, seqs, width, pages, pg_shift(page_size), max_len};
   hipStream_t st = (hipStream_t)stream;
   if (const int e = pg_allow_lds()) return e;
-  hipLaunchKernelGGL(page_gather_kernel, dim3(ceil_div(width, PG_COLS)), dim3(256),
-                     (size_t)rows * PG_COLS * 4, st, t, parents, rows, beams);
-  OMNI_CHECK_LAUNCH();
-  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 2 * (size_t)rows);
-  hipLaunchKernelGGL(page_fork_kernel, dim3(1), dim3(PG_THREADS), smem, st, t, parents, rows, beams,
-                     (CopyItem*)work, pg_group(seqs));
+  const bool here = (int64_t)rows * width <= PG_TILE;
+  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 4 * (size_t)rows + (here ? (size_t)rows * width : 0));
+  const int group = pg_group(seqs);
+  if (here) {
+    hipLaunchKernelGGL(page_fork_kernel<true>, dim3(1), dim3(PG_THREADS), smem, st, t, parents, rows,
+                       beams, (CopyItem*)work, group);
+  } else {
+    hipLaunchKernelGGL(page_gather_kernel, dim3(ceil_div(width, PG_COLS)), dim3(256),
+                       (size_t)rows * PG_COLS * 4, st, t, parents, rows, beams);
+    OMNI_CHECK_LAUNCH();
+    hipLaunchKernelGGL(page_fork_kernel<false>, dim3(1), dim3(PG_THREADS), smem, st, t, parents, rows,
+                       beams, (CopyItem*)work, group);
+  }
   OMNI_CHECK_LAUNCH();
   const int64_t page_halfs = (int64_t)page_size * row_halfs;
   hipLaunchKernelGGL(page_copy_kernel, dim3(2 * n_layers, rows), dim3(256), 0, st, (half_t*)pool,

@@ -23,7 +23,7 @@ from .attention import num_cus, prefill_attention_pool
 from .hostio import to_device
 from .kv_cache import PreallocatedKVCache, _head_rows, _ints
 
-MAX_PAGES = 1 << 20
+MAX_PAGES = 1 << 19
 MAX_SEQS = 2048
 PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
 UNIT = 128                         # keys of a workgroup's step in omni_paged_attention
