@@ -213,56 +213,67 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attn_kernel(PagedArgs a) 
   }
 }
 
-// The states of a row that several columns share, merged: one workgroup a row and head, 32 lanes a
-// state.  Rows without keys are zero.
-template <bool BF, int HD>
+// The states of a row that several columns share, merged: one workgroup a row, head and DIMS of its
+// columns, DIMS / 4 lanes a state.  All maxima first, a state a thread, then every state's outputs
+// once, by its factor: no load waits for another state's.  Rows without keys are zero.
+#define PA_PARTS 256               // states in a round
+template <bool BF, int HD, int DIMS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  constexpr int PER = HD / 32, OS = HD + 4, SETS = 8;
-  __shared__ float part[SETS][HD], ml[SETS][2];
-  const int i = blockIdx.y, head = blockIdx.x, heads = a.nkv * a.G;
+  constexpr int OS = HD + 4, LANES = DIMS / 4, SETS = 256 / LANES, DEEP = 4;
+  __shared__ float factor[PA_PARTS], wred[2][4];
+  __shared__ __attribute__((aligned(16))) float part[SETS][DIMS];
+  const int i = blockIdx.y, head = blockIdx.x, heads = a.nkv * a.G, tid = threadIdx.x;
+  const int d0 = blockIdx.z * DIMS;
   typedef const __attribute__((address_space(4))) int plan_int;
   const plan_int* row = (const plan_int*)a.schedule + 4 * i;
   const int keys = row[0], first = row[1], last = row[2];
   if (keys && first == last) return;
-  const int set = threadIdx.x >> 5, c = (threadIdx.x & 31) * PER;
-  float M = -INFINITY, L = 0.f, v[PER];
+  const int n = keys ? last - first + 1 : 0, set = tid / LANES, c = (tid % LANES) * 4;
+  const float* rec = a.states + ((int64_t)(first + i) * heads + head) * OS;
+  const int64_t next = (int64_t)heads * OS;
+  float M = -INFINITY, L = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int base = 0; base < n; base += PA_PARTS) {
+    const int here = min(n - base, PA_PARTS);
+    float2 s = make_float2(-INFINITY, 0.f);
+    if (tid < here) s = *(const float2*)(rec + (base + tid) * next + HD);
+    // the first states' outputs are on their way meanwhile
+    f32x4 x[DEEP];
 #pragma unroll
-  for (int t = 0; t < PER; ++t) v[t] = 0.f;
-  if (keys) {
-    for (int col = first + set; col <= last; col += SETS) {
-      const float* rec = a.states + ((int64_t)(col + i) * heads + head) * OS;
-      const float2 s = *(const float2*)(rec + HD);
-      float x[PER];
-      __builtin_memcpy(x, rec + c, 4 * PER);
-      const float mn = fmaxf(M, s.x), ref = mn == -INFINITY ? 0.f : mn;
-      const float fa = exp2f(M - ref), fb = exp2f(s.x - ref);
-      M = mn;
-      L = L * fa + s.y * fb;
+    for (int u = 0; u < DEEP; ++u)
+      if (set + u * SETS < here) x[u] = *(const f32x4*)(rec + (base + set + u * SETS) * next + d0 + c);
+    const float top = wave_max(s.x);
+    if ((tid & 63) == 0) wred[0][tid >> 6] = top;
+    __syncthreads();
+    const float mn = fmaxf(M, fmaxf(fmaxf(wred[0][0], wred[0][1]), fmaxf(wred[0][2], wred[0][3])));
+    const float ref = mn == -INFINITY ? 0.f : mn, old = exp2f(M - ref), f = exp2f(s.x - ref);
+    factor[tid] = f;
+    const float sum = wave_sum(f * s.y);
+    if ((tid & 63) == 0) wred[1][tid >> 6] = sum;
+    __syncthreads();
+    L = L * old + ((wred[1][0] + wred[1][1]) + (wred[1][2] + wred[1][3]));
+    M = mn;
+    v *= old;
 #pragma unroll
-      for (int t = 0; t < PER; ++t) v[t] = v[t] * fa + x[t] * fb;
-    }
+    for (int u = 0; u < DEEP; ++u)
+      if (set + u * SETS < here) v += x[u] * factor[set + u * SETS];
+#pragma unroll 4
+    for (int p = set + DEEP * SETS; p < here; p += SETS)
+      v += *(const f32x4*)(rec + (base + p) * next + d0 + c) * factor[p];
   }
-#pragma unroll
-  for (int t = 0; t < PER; ++t) part[set][c + t] = v[t];
-  if (c == 0) {
-    ml[set][0] = M;
-    ml[set][1] = L;
-  }
+  *(f32x4*)&part[set][c] = v;
   __syncthreads();
-  if (threadIdx.x >= HD / 2) return;
-  float MM = -INFINITY, LL = 0.f, y0 = 0.f, y1 = 0.f;
-#pragma unroll
-  for (int k = 0; k < SETS; ++k) MM = fmaxf(MM, ml[k][0]);
+  if (tid >= DIMS / 2) return;
+  float y0 = 0.f, y1 = 0.f;
 #pragma unroll
   for (int k = 0; k < SETS; ++k) {
-    const float f = MM == -INFINITY ? 0.f : exp2f(ml[k][0] - MM);
-    LL = fmaf(f, ml[k][1], LL);
-    y0 = fmaf(f, part[k][2 * threadIdx.x], y0);
-    y1 = fmaf(f, part[k][2 * threadIdx.x + 1], y1);
+    const float2 y = *(const float2*)&part[k][2 * tid];
+    y0 += y.x;
+    y1 += y.y;
   }
-  const float inv = LL == 0.f ? 0.f : 1.f / LL;
-  *(uint32_t*)(a.out + i * a.out_stride + (int64_t)head * HD + 2 * threadIdx.x) =
-      pa_pack<BF>(y0 * inv, y1 * inv);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *(uint32_t*)(a.out + i * a.out_stride + (int64_t)head * HD + d0 + 2 * tid) = pa_pack<BF>(y0 * inv, y1 * inv);
 }
 
 template <bool BF, int HD>
@@ -271,7 +282,10 @@ static int pa_launch(const PagedArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((paged_attn_kernel<BF, HD>), dim3(a.ncols, a.nkv, groups), dim3(64 * PA_WAVES), 0,
                      st, a);
   OMNI_CHECK_LAUNCH();
-  hipLaunchKernelGGL((paged_merge_kernel<BF, HD>), dim3(a.nkv * a.G, a.n), dim3(256), 0, st, a);
+  // few rows have many states each
+  const dim3 rows(a.nkv * a.G, a.n, a.n * a.nkv * a.G < 256 && a.ncols >= 64 ? HD / 32 : 1);
+  if (rows.z > 1) hipLaunchKernelGGL((paged_merge_kernel<BF, HD, 32>), rows, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((paged_merge_kernel<BF, HD, HD>), rows, dim3(256), 0, st, a);
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }

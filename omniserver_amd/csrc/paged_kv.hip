@@ -69,19 +69,17 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
   return lo;
 }
 
-// Set the bits of the pages that sequences hold; held(row) gives how many of a row's entries count
-// and which one of them does not.  2^group lanes a row, four entries a lane at a time.
-template <typename Held>
+// Set the bits of the pages that sequences hold; held(row, but) gives how many of a row's entries
+// count and, for FORK, which one of them does not.  2^group lanes a row, four entries a lane at a
+// time.
+template <bool FORK, typename Held>
 __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held) {
   const int lanes = 1 << group, l = threadIdx.x & (lanes - 1);
 #pragma unroll 1
   for (int row = threadIdx.x >> group; row < t.seqs; row += PG_THREADS >> group) {
-    int but;
+    int but = -1;
     const int count = held(row, but);
     const int* entry = t.tables + (int64_t)row * t.width;
-    auto mark = [&](int j, int p) {
-      if (j < count && j != but && p >= 0 && p < t.pages) atomicOr(&used[p >> 5], 1u << (p & 31));
-    };
 #pragma unroll 1
     for (int j0 = 4 * l; j0 < count; j0 += 16 * lanes) {
       i32x4 p[4];
@@ -89,8 +87,8 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
       for (int u = 0; u < 4; ++u) {
         const int j = j0 + 4 * lanes * u;
         p[u] = (i32x4){-1, -1, -1, -1};
-        if (j + 4 <= t.width) {
-          if (j < count) __builtin_memcpy(&p[u], entry + j, 16);
+        if (j + 4 <= count) {
+          __builtin_memcpy(&p[u], entry + j, 16);
         } else {
 #pragma unroll
           for (int e = 0; e < 3; ++e)
@@ -100,38 +98,62 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mark(j0 + 4 * lanes * u + e, p[u][e]);
+        for (int e = 0; e < 4; ++e) {
+          const int x = p[u][e];
+          bool in = (unsigned)x < (unsigned)t.pages;
+          if (FORK) in &= j0 + 4 * lanes * u + e != but;
+          if (in) atomicOr(&used[x >> 5], 1u << (x & 31));
+        }
     }
   }
 }
 
-// The free pages counted in order: `first` of them are below this thread's words; returns how many
-// there are.  Bits past the pool count as used.
-__device__ __forceinline__ int pg_count_free(const PageTables& t, uint32_t* used, int& first, int* lds) {
-  const int words = (t.pages + 31) >> 5, per = ceil_div(words, PG_THREADS);
-  const int end = min((int)(threadIdx.x + 1) * per, words);
-  int mine = 0;
-#pragma unroll 1
-  for (int w = threadIdx.x * per; w < end; ++w) {
-    if (w == words - 1 && (t.pages & 31)) used[w] |= ~0u << (t.pages & 31);
-    mine += 32 - __popc(used[w]);
+// A thread's share of the pages: 2^k of one word's bits, or whole words where they are many.
+struct PgShare {
+  int word, end, shift;
+  uint32_t mask;
+  __device__ __forceinline__ explicit PgShare(const PageTables& t) {
+    const int words = (t.pages + 31) >> 5, per = ceil_div(words, PG_THREADS);
+    int bits = 32;
+    while (bits > 1 && (bits / 2) * PG_THREADS >= t.pages) bits /= 2;
+    const int at = threadIdx.x * (bits < 32 ? bits : 32 * per);
+    word = at >> 5;
+    end = min(bits < 32 ? word + 1 : word + per, words);
+    shift = at & 31;
+    mask = bits < 32 ? (1u << bits) - 1 : ~0u;
   }
-  int total;
+  __device__ __forceinline__ uint32_t free(const uint32_t* used, int w) const {
+    return ~used[w] >> shift & mask;
+  }
+};
+
+// The free pages counted in order: `first` of them are below this thread's; returns how many there
+// are.
+__device__ __forceinline__ int pg_count_free(const PgShare& own, const uint32_t* used, int& first, int* lds) {
+  int mine = 0, total;
+#pragma unroll 1
+  for (int w = own.word; w < own.end; ++w) mine += __popc(own.free(used, w));
   first = pg_scan(mine, lds, total) - mine;
   return total;
 }
 
+// Bits to start with: none held, those past the pool not there.
+__device__ __forceinline__ void pg_clear(const PageTables& t, uint32_t* used) {
+  const int words = (t.pages + 31) >> 5;
+#pragma unroll 1
+  for (int w = threadIdx.x; w < words; w += PG_THREADS)
+    used[w] = w == words - 1 && (t.pages & 31) ? ~0u << (t.pages & 31) : 0u;
+}
+
 // give(rank, page) for the `want` lowest free pages, by the threads that counted them, in order.
 template <typename Give>
-__device__ __forceinline__ void pg_deal(const PageTables& t, const uint32_t* used, int first, int want,
+__device__ __forceinline__ void pg_deal(const PgShare& own, const uint32_t* used, int first, int want,
                                         Give give) {
-  const int words = (t.pages + 31) >> 5, per = ceil_div(words, PG_THREADS);
-  const int end = min((int)(threadIdx.x + 1) * per, words);
 #pragma unroll 1
-  for (int w = threadIdx.x * per; w < end && first < want; ++w)
+  for (int w = own.word; w < own.end && first < want; ++w)
 #pragma unroll 1
-    for (uint32_t free = ~used[w]; free && first < want; free &= free - 1, ++first)
-      give(first, w * 32 + __ffs(free) - 1);
+    for (uint32_t free = own.free(used, w); free && first < want; free &= free - 1, ++first)
+      give(first, w * 32 + own.shift + __ffs(free) - 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -186,8 +208,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   int* len = last + r.n;                            // length, and tokens that it may be granted
   int* ask = len + r.n;
   int* at = ask + r.n;                              // dense: the token's page
-#pragma unroll 1
-  for (int w = tid; w < words; w += PG_THREADS) used[w] = 0;
+  pg_clear(t, used);
   int wanted = 0, rows_sum = 0;
 #pragma unroll 1
   for (int base = 0; base < r.n; base += PG_THREADS) {
@@ -220,15 +241,15 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
     if (i < r.n) ends[i] = pages;
     __syncthreads();                                // the sums are read
   }
-  pg_mark(t, used, r.group, [&](int row, int& but) {
-    but = -1;
+  pg_mark<false>(t, used, r.group, [&](int row, int& but) {
     return pg_pages(t, pg_length(t, row));
   });
   __syncthreads();
+  const PgShare own(t);
   int first;
-  const int left = pg_count_free(t, used, first, lds[2]);
+  const int left = pg_count_free(own, used, first, lds[2]);
   int to = -1, low = 0, high = 0;                   // the request of this thread's next page
-  pg_deal(t, used, first, min(left, wanted), [&](int rank, int page) {
+  pg_deal(own, used, first, min(left, wanted), [&](int rank, int page) {
     if (rank >= high) {
       to = to < 0 ? pg_find(ends, r.n, rank) : to + 1;
       while (to < r.n && ends[to] <= rank) ++to;
@@ -440,8 +461,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, con
   int* from = ends + rows;                          // the page that is filled in part
   int* up = from + rows;                            // the row that row r goes on from, or -1
   int* tile = up + rows;                            // HERE: [rows][width], the tables before
-#pragma unroll 1
-  for (int w = tid; w < words; w += PG_THREADS) used[w] = 0;
+  pg_clear(t, used);
   if (HERE) {
 #pragma unroll 4
     for (int e = tid; e < rows * t.width; e += PG_THREADS) tile[e] = t.tables[e];
@@ -486,8 +506,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, con
       }
     }
   }
-  pg_mark(t, used, group, [&](int row, int& but) {
-    but = -1;
+  pg_mark<true>(t, used, group, [&](int row, int& but) {
     if (row >= rows) return pg_pages(t, pg_length(t, row));
     if (HERE) return 0;
     const int v = len[row], L = v < 0 ? ~v : v;
@@ -495,8 +514,9 @@ __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, con
     return pg_pages(t, L);
   });
   __syncthreads();
+  const PgShare share(t);
   int first;
-  const int left = pg_count_free(t, used, first, lds[1]);
+  const int left = pg_count_free(share, used, first, lds[1]);
 #pragma unroll 1
   for (int r = tid; r < rows; r += PG_THREADS) {
     const int v = len[r];
@@ -505,7 +525,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, con
     if (!copies) items[r] = {0, 0, 0, 0};
   }
   int to = -1;
-  pg_deal(t, used, first, min(left, wanted), [&](int rank, int own) {
+  pg_deal(share, used, first, min(left, wanted), [&](int rank, int own) {
     to = to < 0 ? pg_find(ends, rows, rank) : to + 1;
     while (len[to] >= 0) ++to;                      // the next row with a page of its own
     const int L = ~len[to], p = from[to];
