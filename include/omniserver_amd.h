@@ -213,14 +213,15 @@ int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t 
  * int64 [n] (lengths before and with what is granted; lengths itself stays), token_page and
  * token_pos int64 [tokens] (-1: nowhere), positions int64 [axes <= 3][tokens] (position + rope_delta
  * of the sequence, int64 or NULL; -1 without a slot), granted int32 [n], cu int32 [n + 1] (sums of
- * counts) and, for dense, schedule (int32 [4 (n + columns)], 16-byte aligned, or NULL) for
- * omni_paged_attention. */
+ * counts) and, for dense without rows, schedule (int32 [8 n + 4 columns], 16-byte aligned, or NULL)
+ * for omni_paged_attention with the same columns and most: up to `most` neighbouring sequences whose
+ * tables begin alike are taken together. */
 int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int width, int pages, int page_size,
                       int max_len, const int* counts, const int64_t* rows,
                       const int64_t* rope_delta, int n, int tokens, int dense, int axes,
                       int64_t* starts, int64_t* after, int64_t* token_page, int64_t* token_pos,
                       int64_t* positions, int* granted, int* cu, int* schedule, int columns,
-                      void* stream);
+                      int most, void* stream);
 
 /* Beams after a choice: row s * beams + w of the first n * beams sequences goes on from row s * beams
  * + parents[s][w] as it was (int32; outside [0, beams): empty).  Full pages are shared; a page that
@@ -237,13 +238,14 @@ int omni_page_reorder(void* pool, int n_layers, int row_halfs, int* tables, int6
  * strides in elements, multiples of 8) attends to the keys that the schedule gives sequence i, the new
  * token the last of them; a row without keys is zero.  k_cache / v_cache [pages][page_size]
  * [n_kv_heads][head_dim 64 or 128].  The keys stand in one line cut into equal stretches, one a
- * column of workgroups; the states of a sequence that several share go through workspace (fp32,
- * (columns + n) n_heads (head_dim + 4) floats) to a second launch.  scale from 2^-126 to 2^126;
- * operands 16-byte aligned. */
+ * column of workgroups; the states of a sequence in several pieces go through workspace (fp32,
+ * n_heads ((most > 1 ? columns most + n : 0) + columns + n) (head_dim + 4) floats) to a second
+ * launch.  most: 1, or up to 32 / (n_heads / n_kv_heads).  scale from 2^-126 to 2^126; operands
+ * 16-byte aligned. */
 int omni_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                          int dtype, int pages, int page_size, const int* tables, int width, int n,
-                         const int* schedule, int columns, void* out, int64_t out_stride,
-                         int n_heads, int n_kv_heads, int head_dim, float scale, float* workspace,
+                         const int* schedule, int columns, int most, void* out,
+                         int64_t out_stride, int n_heads, int n_kv_heads, int head_dim, float scale, float* workspace,
                          int64_t workspace_floats, void* stream);
 
 /* Beam search's choice: the k <= 64 best continuations of each of n requests over its beams <= 32

@@ -82,10 +82,10 @@ SIGNATURES = {
     "omni_spec_verify": [_P, _I, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _F, _I, _I, _I,
                          _P, _P, _P, _P, _I64, _P],
     "omni_page_reserve": [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P,
-                          _P, _P, _P, _P, _I, _P],
+                          _P, _P, _P, _P, _I, _I, _P],
     "omni_page_reorder": [_P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P, _I, _I, _P, _I64, _P],
-    "omni_paged_attention": [_P, _I64, _P, _P, _I, _I, _I, _P, _I, _I, _P, _I, _P, _I64, _I, _I, _I,
-                             _F, _P, _I64, _P],
+    "omni_paged_attention": [_P, _I64, _P, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _P, _I64, _I, _I,
+                             _I, _F, _P, _I64, _P],
     "omni_beam_select_work": [_I, _I, _I, _I],
     "omni_beam_select": [_P, _I, _I64, _I64, _P, _P, _P, _I, _I64, _I64, _I, _I, _I, _I, _P, _P, _P,
                          _P, _P, _I64, _P],

@@ -29,33 +29,36 @@ __device__ __forceinline__ int pg_pages(const PageTables& t, int64_t tokens) {
 
 // Sums of non-negative numbers up to 2^30, which they stay at.
 __device__ __forceinline__ int pg_add(int a, int b) { return min(a + b, 1 << 30); }
-// What the lane CTRL moves here holds, in the rows of 16 lanes that ROWS names; else 0.
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ int pg_move(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+template <bool MAX>
+__device__ __forceinline__ int pg_join(int a, int b) { return MAX ? max(a, b) : pg_add(a, b); }
+// v with what the lane CTRL moves here holds, in the rows of 16 lanes that ROWS names.
+template <bool MAX, int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int pg_step(int v) {
+  return pg_join<MAX>(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false));
 }
 
-// Inclusive prefix sum over the workgroup; total in all threads.  lds: PG_WAVES ints, free for a new
-// call after the caller's next barrier.
+// Inclusive prefix sum (or maximum) of non-negative numbers over the workgroup; total in all
+// threads.  lds: PG_WAVES ints, free for a new call after the caller's next barrier.
+template <bool MAX = false>
 __device__ __forceinline__ int pg_scan(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = pg_add(v, pg_move<0x111>(v));                // from 1, 2, 4, 8 lanes below
-  v = pg_add(v, pg_move<0x112>(v));
-  v = pg_add(v, pg_move<0x114>(v));
-  v = pg_add(v, pg_move<0x118>(v));
-  v = pg_add(v, pg_move<0x142, 0xa>(v));           // a row's total into the next row
-  v = pg_add(v, pg_move<0x143, 0xc>(v));           // the lower half's into the upper
+  v = pg_step<MAX, 0x111>(v);                      // from 1, 2, 4, 8 lanes below
+  v = pg_step<MAX, 0x112>(v);
+  v = pg_step<MAX, 0x114>(v);
+  v = pg_step<MAX, 0x118>(v);
+  v = pg_step<MAX, 0x142, 0xa>(v);                 // a row's total into the next row
+  v = pg_step<MAX, 0x143, 0xc>(v);                 // the lower half's into the upper
   if (lane == 63) lds[wave] = v;
   __syncthreads();
   // a wave's sum a lane, the same way
   int sums = lane < PG_WAVES ? lds[lane] : 0;
-  sums = pg_add(sums, pg_move<0x111>(sums));
-  sums = pg_add(sums, pg_move<0x112>(sums));
-  sums = pg_add(sums, pg_move<0x114>(sums));
-  sums = pg_add(sums, pg_move<0x118>(sums));
+  sums = pg_step<MAX, 0x111>(sums);
+  sums = pg_step<MAX, 0x112>(sums);
+  sums = pg_step<MAX, 0x114>(sums);
+  sums = pg_step<MAX, 0x118>(sums);
   total = __builtin_amdgcn_readlane(sums, PG_WAVES - 1);
   const int w = __builtin_amdgcn_readfirstlane(wave);
-  return pg_add(v, w ? __builtin_amdgcn_readlane(sums, w - 1) : 0);
+  return pg_join<MAX>(v, w ? __builtin_amdgcn_readlane(sums, w - 1) : 0);
 }
 
 // First i in [0, n) with ends[i] > x (ends ascends), n if there is none.
@@ -71,18 +74,37 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
 
 // Set the bits of the pages that sequences hold; held(row, but) gives how many of a row's entries
 // count and, for FORK, which one of them does not.  2^group lanes a row, four entries a lane at a
-// time.
+// time.  common[row] of the first n rows becomes the number of entries before the first one that the
+// row above has otherwise, of those that both hold (it comes as that many or more).
 template <bool FORK, typename Held>
-__device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held) {
+__device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held,
+                                        int* common = nullptr, int n = 0) {
   const int lanes = 1 << group, l = threadIdx.x & (lanes - 1);
 #pragma unroll 1
   for (int row = threadIdx.x >> group; row < t.seqs; row += PG_THREADS >> group) {
     int but = -1;
     const int count = held(row, but);
     const int* entry = t.tables + (int64_t)row * t.width;
+    int both = 0;
+    if (common && row && row < n) {
+      int x;
+      both = min(count, held(row - 1, x));
+    }
 #pragma unroll 1
     for (int j0 = 4 * l; j0 < count; j0 += 16 * lanes) {
-      i32x4 p[4];
+      i32x4 p[4], above[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + 4 * lanes * u;
+        above[u] = (i32x4){-1, -1, -1, -1};
+        if (j + 4 <= both) {
+          __builtin_memcpy(&above[u], entry - t.width + j, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 3; ++e)
+            if (j + e < both) above[u][e] = entry[j + e - t.width];
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int j = j0 + 4 * lanes * u;
@@ -104,6 +126,15 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
           if (FORK) in &= j0 + 4 * lanes * u + e != but;
           if (in) atomicOr(&used[x >> 5], 1u << (x & 31));
         }
+      if (j0 < both) {
+        int other = both;
+#pragma unroll
+        for (int u = 3; u >= 0; --u)
+#pragma unroll
+          for (int e = 3; e >= 0; --e)
+            if (p[u][e] != above[u][e]) other = min(other, j0 + 4 * lanes * u + e);
+        if (other < both) atomicMin(&common[row], other);
+      }
     }
   }
 }
@@ -163,11 +194,16 @@ __device__ __forceinline__ void pg_deal(const PgShare& own, const uint32_t* used
 // that one that needs none is never turned down for another.
 //
 // One workgroup: bits of the held pages, how many are free below each, then every free page of
-// low enough rank looks up the request that it goes to.  And the attention's schedule for single
-// tokens (paged_attn.hip): the sequences' keys in units of PG_UNIT stand in one line that is cut into
-// at most ncols equal stretches, one a column of workgroups; a row of the schedule is
-//   (keys, first column, last column, 0)
-// and a column (sequence, first unit there, units in all, 0).
+// low enough rank goes to the request whose sum of new pages it falls into.
+//
+// And the attention's schedule for single tokens (paged_attn.hip).  Neighbouring sequences whose
+// tables begin with the same pages, for half of the shorter one's length or more, form groups of up to
+// `most`: what they share, in whole units of PG_UNIT keys, is one item, read once for all of them, and
+// the rest of each is another.  The items stand in one line, every group's shared one before its
+// rows', that is cut into at most ncols equal stretches, one a column of workgroups:
+//   row     (keys, shared units, the group's first row, its rows,
+//            first and last column of the shared item, of the row's own)
+//   column  (2 row + (1: its own, 0: its group's shared item), first unit there, units in all, 0)
 // ---------------------------------------------------------------------------
 #define PG_UNIT 128
 
@@ -184,8 +220,8 @@ struct ReserveArgs {
   int64_t* positions;          // [axes][T]
   int* granted;                // [n]
   int* cu;                     // [n + 1]
-  int* schedule;               // [n][4] then [ncols][4], or null
-  int ncols;
+  int* schedule;               // [n][8] then [ncols][4], or null
+  int ncols, most;
   int group, slots_here;
 };
 
@@ -207,7 +243,10 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   int* last = ends + r.n;                           // token rows up to and with request i, then units
   int* len = last + r.n;                            // length, and tokens that it may be granted
   int* ask = len + r.n;
-  int* at = ask + r.n;                              // dense: the token's page
+  int* at = ask + r.n;                              // dense: the token's page, then the group
+  int* common = at + r.n;                           // dense: pages, then units, as the row above
+  int* share = common + r.n;                        // dense: a group's shared units
+  int* size = share + r.n;                          // dense: its rows
   pg_clear(t, used);
   int wanted = 0, rows_sum = 0;
 #pragma unroll 1
@@ -226,6 +265,11 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
       len[i] = L;
       ask[i] = c;
       last[i] = i + 1;
+      if (r.dense) {
+        common[i] = pg_pages(t, L);
+        share[i] = 1 << 30;
+        size[i] = 0;
+      }
     }
     if (!r.dense) {
       // a request whose token rows run past T gets none
@@ -243,7 +287,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   }
   pg_mark<false>(t, used, r.group, [&](int row, int& but) {
     return pg_pages(t, pg_length(t, row));
-  });
+  }, r.schedule ? common : nullptr, r.n);
   __syncthreads();
   const PgShare own(t);
   int first;
@@ -263,33 +307,22 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
     if (r.dense) at[to] = page;
   });
   __syncthreads();                                  // the tables are written
-  int units = 0;
 #pragma unroll 1
-  for (int base = 0; base < r.n; base += PG_THREADS) {
-    const int i = base + tid;
-    int mine = 0, total;
-    if (i < r.n) {
-      const int L = len[i], low_i = i ? ends[i - 1] : 0;
-      const int c = ends[i] == low_i || ends[i] <= left ? ask[i] : 0;
-      ask[i] = c;
-      r.granted[i] = c;
-      r.starts[i] = L;
-      r.after[i] = L + c;
-      r.cu[i + 1] = last[i];
-      if (i == 0) r.cu[0] = 0;
-      if (r.dense) {
-        const int64_t row = r.rows ? r.rows[i] : (int64_t)i;
-        pg_slot(t, r, i, c ? at[i] : -1, L, c && r.rope_delta ? r.rope_delta[row] : 0);
-        mine = c ? ceil_div(L + c, PG_UNIT) : 0;
-      }
+  for (int i = tid; i < r.n; i += PG_THREADS) {
+    const int L = len[i], low_i = i ? ends[i - 1] : 0;
+    const int c = ends[i] == low_i || ends[i] <= left ? ask[i] : 0;
+    r.granted[i] = c;
+    r.starts[i] = L;
+    r.after[i] = L + c;
+    r.cu[i + 1] = last[i];
+    if (i == 0) r.cu[0] = 0;
+    ask[i] = c;
+    if (r.dense) {
+      const int64_t row = r.rows ? r.rows[i] : (int64_t)i;
+      pg_slot(t, r, i, c ? at[i] : -1, L, c && r.rope_delta ? r.rope_delta[row] : 0);
     }
-    if (r.schedule) {
-      const int upto = pg_scan(mine, lds[3], total) + units;
-      units += total;
-      if (i < r.n) last[i] = upto;
-    }
-    __syncthreads();
   }
+  __syncthreads();
   if (!r.dense && r.slots_here) {
 #pragma unroll 1
     for (int tok = tid; tok < r.T; tok += PG_THREADS) {
@@ -305,20 +338,70 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
     }
   }
   if (!r.schedule) return;
+  // groups: a row that goes on from its neighbour, and the places in such a run cut at `most`
+  int units = 0, start = 0;
+#pragma unroll 1
+  for (int base = 0; base < r.n; base += PG_THREADS) {
+    const int i = base + tid;
+    int total, shared = 0;
+    if (i && i < r.n && ask[i] && ask[i - 1]) {
+      const int least = min(len[i], len[i - 1]);
+      shared = min(least, (int)min((int64_t)common[i] << t.shift, (int64_t)1 << 30)) / PG_UNIT;
+      if (shared * PG_UNIT < least - shared * PG_UNIT) shared = 0;
+    }
+    const int run = max(pg_scan<true>(shared ? 0 : i, lds[3], total), start);
+    start = max(start, total);
+    if (i < r.n) {
+      const int group = i - (i - run) % r.most;
+      at[i] = group;
+      atomicAdd(&size[group], 1);
+      if (group != i) atomicMin(&share[group], shared);
+    }
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (int base = 0; base < r.n; base += PG_THREADS) {
+    const int i = base + tid;
+    int mine = 0, total;
+    if (i < r.n) {
+      const int group = at[i], S = size[group] > 1 ? share[group] : 0;
+      common[i] = S;
+      mine = ask[i] ? ceil_div(len[i] + ask[i], PG_UNIT) - (group == i ? 0 : S) : 0;
+    }
+    const int upto = pg_scan(mine, lds[0], total) + units;
+    units += total;
+    if (i < r.n) last[i] = upto;
+    __syncthreads();
+  }
   const int cols = min(r.ncols, units);
   auto column_of = [&](int x) { return (int)((((int64_t)x + 1) * cols - 1) / units); };
 #pragma unroll 1
-  for (int i = tid; i < r.n + r.ncols; i += PG_THREADS) {
-    i32x4 v = {0, 0, 0, 0};
-    if (i < r.n) {
-      const int lo = i ? last[i - 1] : 0, hi = last[i];
-      if (hi > lo) v = (i32x4){len[i] + ask[i], column_of(lo), column_of(hi - 1), 0};
-    } else if (i - r.n < cols) {
-      const int64_t c = i - r.n;
-      const int lo = (int)(c * units / cols), s = pg_find(last, r.n, lo);
-      v = (i32x4){s, lo - (s ? last[s - 1] : 0), (int)((c + 1) * units / cols) - lo, 0};
+  for (int i = tid; i < r.n; i += PG_THREADS) {
+    const int group = at[i], S = common[i], first_i = i ? last[i - 1] : 0, first_g = group ? last[group - 1] : 0;
+    i32x4 v = {0, 0, group, size[group]}, w = {0, 0, 0, 0};
+    if (last[i] > first_i) {
+      v[0] = len[i] + ask[i];
+      v[1] = S;
+      if (S) {
+        w[0] = column_of(first_g);
+        w[1] = column_of(first_g + S - 1);
+      }
+      w[2] = column_of(first_i + (group == i ? S : 0));
+      w[3] = column_of(last[i] - 1);
     }
-    *(i32x4*)(r.schedule + 4 * i) = v;
+    *(i32x4*)(r.schedule + 8 * i) = v;
+    *(i32x4*)(r.schedule + 8 * i + 4) = w;
+  }
+#pragma unroll 1
+  for (int c = tid; c < r.ncols; c += PG_THREADS) {
+    i32x4 v = {0, 0, 0, 0};
+    if (c < cols) {
+      const int lo = (int)((int64_t)c * units / cols), hi = (int)(((int64_t)c + 1) * units / cols);
+      const int i = pg_find(last, r.n, lo), in = lo - (i ? last[i - 1] : 0);
+      const int S = at[i] == i ? common[i] : 0;
+      v = in < S ? (i32x4){2 * i, in, hi - lo, 0} : (i32x4){2 * i + 1, in - S, hi - lo, 0};
+    }
+    *(i32x4*)(r.schedule + 8 * r.n + 4 * c) = v;
   }
 }
 
@@ -393,7 +476,7 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
                                  const int64_t* rope_delta, int n, int tokens, int dense, int axes,
                                  int64_t* starts, int64_t* after, int64_t* token_page,
                                  int64_t* token_pos, int64_t* positions, int* granted, int* cu,
-                                 int* schedule, int columns, void* stream) {
+                                 int* schedule, int columns, int most, void* stream) {
   if (n < 0 || tokens < 0 || axes < 1) return OMNI_EINVAL;
   const int rc = pg_tables_ok(tables, lengths, seqs, width, pages, page_size, max_len);
   if (rc) return rc;
@@ -402,14 +485,15 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
   if (n == 0) return OMNI_OK;
   if (!starts || !after || !granted || !cu) return OMNI_EINVAL;
   if (tokens && (!token_page || !token_pos || !positions)) return OMNI_EINVAL;
-  if (schedule && (!dense || columns <= 0 || ((uintptr_t)schedule & 15))) return OMNI_EINVAL;
+  if (schedule && (!dense || rows || columns <= 0 || most <= 0 || ((uintptr_t)schedule & 15)))
+    return OMNI_EINVAL;
   if (schedule && (columns > 65535 || (int64_t)n * ceil_div(max_len, PG_UNIT) > (1 << 30)))
     return OMNI_EUNSUPPORTED;
   const PageTables t = {tables, lengths, seqs, width, pages, pg_shift(page_size), max_len};
   ReserveArgs r = {counts, rows, rope_delta, n, tokens, dense, axes, starts, after, token_page,
-                   token_pos, positions, granted, cu, schedule, columns, pg_group(seqs),
+                   token_pos, positions, granted, cu, schedule, columns, most, pg_group(seqs),
                    tokens <= PG_SLOTS_HERE};
-  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 5 * (size_t)n);
+  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + (dense ? 8 : 4) * (size_t)n);
   if (smem > (32 << 10) && pg_allow_lds()) return pg_allow_lds();
   hipLaunchKernelGGL(page_reserve_kernel, dim3(1), dim3(PG_THREADS), smem, (hipStream_t)stream, t, r);
   OMNI_CHECK_LAUNCH();

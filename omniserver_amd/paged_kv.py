@@ -32,8 +32,13 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 def attention_columns(n: int, nh: int, nkv: int, max_len: int, cus: int) -> int:
     """Columns of workgroups that n sequences' keys are cut over."""
-    per = nkv * -(-(nh // nkv) // 16)
+    per = nkv * -(-(nh // nkv) // 32)
     return max(1, min(2 * cus // per, n * -(-max_len // UNIT)))
+
+
+def attention_group(nh: int, nkv: int) -> int:
+    """How many sequences a workgroup takes together where they share pages: 32 queries in all."""
+    return 32 // (nh // nkv) if nh // nkv <= 16 else 1
 
 
 class PagedKVCache:
@@ -150,7 +155,7 @@ class PageSlots:
     object, so two captured graphs never share them."""
 
     def __init__(self, pool: PagedKVCache, counts, rows=None, tokens=None, dense: bool = False,
-                 n: int | None = None, rope_delta=None, columns: int = 0):
+                 n: int | None = None, rope_delta=None, columns: int = 0, most: int = 0):
         dev = pool.device
         if rows is not None:
             rows = pool._checked_rows(rows)
@@ -182,7 +187,7 @@ class PageSlots:
         # the attention's schedule on a 16-byte boundary
         words = 2 * n + (2 + axes) * T
         ints = 2 * n + 1 + (-(2 * words + 2 * n + 1) % 4)
-        self._plan = torch.empty(words + (ints + (4 * (n + columns) if columns else 0) + 1) // 2,
+        self._plan = torch.empty(words + (ints + (8 * n + 4 * columns if columns else 0) + 1) // 2,
                                  device=dev, dtype=torch.int64)
         p = self._plan.data_ptr()
         self._granted = p + 8 * words
@@ -193,7 +198,7 @@ class PageSlots:
         call("omni_page_reserve", *pool._geometry(), ptr(self.counts), ptr(self.rows),
              ptr(rope_delta), n, T, int(dense), axes, p, p + 8 * n, self._page, self._place,
              p + 16 * (n + T), self._granted, self._granted + 4 * n, self._schedule, columns,
-             stream())
+             most, stream())
 
     @property
     def starts(self) -> torch.Tensor:
@@ -341,7 +346,9 @@ class PagedDecode(PageSlots):
     a page for it, gets zeros.
 
     The sequences' keys stand in one line that is cut into equal stretches for the attention's
-    workgroups, so that one long sequence among short ones takes no longer than its share."""
+    workgroups, so that one long sequence among short ones takes no longer than its share; the pages
+    that the tables of neighbours begin with alike (beams of one prompt) stand there, and are read,
+    once for several of them."""
 
     leaves_rows = False
 
@@ -350,11 +357,13 @@ class PagedDecode(PageSlots):
             raise ValueError(f"{n} sequences, the cache has {pool.max_seqs}")
         self._columns = attention_columns(n, pool.n_heads, pool.n_kv_heads, pool.max_len,
                                           num_cus(pool.device))
+        self._most = most = attention_group(pool.n_heads, pool.n_kv_heads)
         super().__init__(pool, counts, dense=True, n=n, rope_delta=rope_delta,
-                         columns=self._columns)
+                         columns=self._columns, most=most)
         # the attention's split states, for all layers (launches on one stream are ordered)
-        self._ws = torch.empty((self._columns + n) * pool.n_heads * (pool.head_dim + 4),
-                               device=pool.device, dtype=torch.float32)
+        states = self._columns + n + (self._columns * most + n if most > 1 else 0)
+        self._ws = torch.empty(states * pool.n_heads * (pool.head_dim + 4), device=pool.device,
+                               dtype=torch.float32)
 
     @property
     def positions(self) -> torch.Tensor:
@@ -386,7 +395,7 @@ class PagedDecode(PageSlots):
         call("omni_paged_attention", q, q_stride, pool.k[layer_idx].data_ptr(),
              pool.v[layer_idx].data_ptr(), _DTYPES[pool.storage.dtype], pool.num_pages,
              pool.page_size, pool.tables.data_ptr(), pool.tables.shape[1], self.n, self._schedule,
-             self._columns, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd, float(scale),
+             self._columns, self._most, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd, float(scale),
              self._ws.data_ptr(), self._ws.numel(), stream())
         return out
 

@@ -202,6 +202,62 @@ def test_decode_attention(gpu, n, span, page, nh, nkv, hd, dtype, max_len):
     assert cache.lengths.tolist() == [m + c for m, c in zip(lengths, counts)]
 
 
+SHARED = [
+    # requests, beams, prompt, own tokens, page, nh, nkv, hd, dtype
+    (1, 4, 500, (1, 40), 16, 12, 2, 128, torch.float16),
+    (3, 4, 1000, (1, 200), 32, 12, 2, 128, torch.float16),
+    (2, 16, 700, (0, 30), 64, 12, 2, 128, torch.bfloat16),     # groups of five, the last of one
+    (5, 3, 300, (0, 300), 16, 8, 1, 64, torch.float16),
+    (2, 32, 400, (1, 9), 16, 4, 4, 128, torch.float16),        # 32 queries of 32 rows
+    (4, 2, 2000, (1, 20), 128, 16, 1, 128, torch.float16),     # two rows of sixteen heads
+    (2, 4, 600, (1, 20), 16, 34, 2, 64, torch.bfloat16),       # seventeen heads: none together
+    (40, 5, 260, (0, 300), 16, 6, 1, 64, torch.float16),
+]
+
+
+@pytest.mark.parametrize("n,W,prompt,own,page,nh,nkv,hd,dtype", SHARED)
+def test_decode_attention_shared(gpu, n, W, prompt, own, page, nh, nkv, hd, dtype):
+    """Beams that hold their prompt's pages together, some requests' prompts almost all of it, others
+    hardly any, some rows idle; and what a row gets does not depend on its neighbours."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    say(f"shared pages: {n} x {W} beams, prompt {prompt}, heads {nh}/{nkv} x {hd} {dtype}")
+    rng = random.Random(n * 17 + W)
+    rows, g = n * W, torch.Generator().manual_seed(prompt)
+    most = prompt + own[1] + 2
+    pages = rows * ref.pages_of(most, page) + 4
+    cache = PagedKVCache(1, pages, nkv, page, hd, gpu, max_seqs=rows, max_len=most, dtype=dtype,
+                         n_heads=nh)
+    order = list(range(pages))
+    rng.shuffle(order)
+    tables, lengths = [], []
+    for s in range(n):
+        shared = prompt // rng.choice([1, 1, 1, 3]) // page
+        common = [order.pop() for _ in range(shared)]
+        for w in range(W):
+            m = max(0, prompt + rng.randint(*own) - (prompt if rng.random() < 0.05 else 0))
+            held = ref.pages_of(m, page)
+            keep = common[:min(held, shared) if held > shared or m % page == 0 else max(held - 1, 0)]
+            row = keep + [order.pop() for _ in range(held - len(keep))]
+            tables.append(row + [0] * (cache.tables.shape[1] - held))
+            lengths.append(m)
+    cache.tables.copy_(torch.tensor(tables, dtype=torch.int32))
+    cache.lengths.copy_(torch.tensor(lengths))
+    fill_pages(cache, tables, lengths, g)
+    counts = [int(rng.random() < 0.95) for _ in range(rows)]
+    step = cache.decode_cache(rows, counts)
+    tables = cache.tables.tolist()
+    qkv = torch.randn(rows, (nh + 2 * nkv) * hd, generator=g).to(dtype).to(gpu)
+    q, k, v = qkv.view(rows, nh + 2 * nkv, hd).split((nh, nkv, nkv), 1)
+    step.write(k, v, 0)
+    out = torch.full((rows, nh, hd), 7.0, device=gpu, dtype=dtype)
+    step.attend_qkv(qkv, 0, hd ** -0.5, out)
+    keys = [m + 1 if c else 0 for m, c in zip(lengths, counts)]
+    check_rows(out, q, cache.storage.cpu(), 0, tables, keys, page, hd ** -0.5)
+    again = torch.full_like(out, 3.0)
+    step.attend_qkv(qkv, 0, hd ** -0.5, again)
+    assert torch.equal(out, again)
+
+
 def test_decode_attention_bad_pages(gpu):
     """Table entries outside the pool: their tokens are not there, the others' attention is."""
     rng = random.Random(5)
