@@ -42,16 +42,16 @@ struct PagedArgs {
   int64_t out_stride;
   float scale_log2;
   float* states;                 // [nkv][shared_recs] then [nkv][own_recs] records of HD + 4
-  int64_t shared_recs, own_recs;
+  int shared_recs, own_recs;
 };
 
 // The record of a row's head in a column: the columns and rows of an item ascend together, so that
 // column times the most records of a column, plus those of the rows before, is a place of its own.
-__device__ __forceinline__ int64_t pa_shared_rec(const PagedArgs& a, int g, int col, int row, int h) {
-  return g * a.shared_recs + ((int64_t)col * a.most + row) * a.G + h;
+__device__ __forceinline__ int pa_shared_rec(const PagedArgs& a, int g, int col, int row, int h) {
+  return g * a.shared_recs + (col * a.most + row) * a.G + h;
 }
-__device__ __forceinline__ int64_t pa_own_rec(const PagedArgs& a, int g, int col, int row, int h) {
-  return a.nkv * a.shared_recs + g * a.own_recs + ((int64_t)col + row) * a.G + h;
+__device__ __forceinline__ int pa_own_rec(const PagedArgs& a, int g, int col, int row, int h) {
+  return a.nkv * a.shared_recs + g * a.own_recs + (col + row) * a.G + h;
 }
 
 typedef const __attribute__((address_space(4))) int plan_int;
@@ -302,16 +302,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   constexpr int OS = HD + 4, LANES = DIMS / 4, SETS = 256 / LANES, DEEP = 4;
   __shared__ float factor[PA_PARTS], wred[2][4];
   __shared__ __attribute__((aligned(16))) float part[SETS][DIMS];
-  const int i = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, d0 = blockIdx.z * DIMS;
+  const int i = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, g = blockIdx.z / (HD / DIMS);
+  const int head = g * a.G + h, d0 = blockIdx.z % (HD / DIMS) * DIMS;
   const plan_int* row = (const plan_int*)a.schedule + 8 * i;
   const int keys = row[0], S = row[1];
   const int shared = S ? row[5] - row[4] + 1 : 0, n = keys ? shared + row[7] - row[6] + 1 : 0;
   if (n == 1) return;                               // written where it was made
-  const int set = tid / LANES, c = (tid % LANES) * 4, g = head / a.G, h = head - g * a.G;
-  const int64_t rec0 = pa_shared_rec(a, g, row[4], i, h), rec1 = pa_own_rec(a, g, row[6] - shared, i, h);
-  auto rec = [&](int p) {
-    return a.states + (p < shared ? rec0 + (int64_t)p * a.most * a.G : rec1 + (int64_t)p * a.G) * OS;
-  };
+  const int set = tid / LANES, c = (tid % LANES) * 4;
+  const int rec0 = pa_shared_rec(a, g, row[4], i, h) * OS, next0 = a.most * a.G * OS;
+  const int rec1 = pa_own_rec(a, g, row[6] - shared, i, h) * OS, next1 = a.G * OS;
+  auto rec = [&](int p) { return a.states + (p < shared ? rec0 + p * next0 : rec1 + p * next1); };
   float M = -INFINITY, L = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -357,6 +357,50 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   *(uint32_t*)(a.out + i * a.out_stride + (int64_t)head * HD + d0 + 2 * tid) = pa_pack<BF>(y0 * inv, y1 * inv);
 }
 
+// The same where rows have few states: one wave a row and head, two columns a lane, sixteen states at
+// a time.
+template <bool BF, int HD>
+__global__ __launch_bounds__(256) void paged_merge_few_kernel(PagedArgs a) {
+  constexpr int OS = HD + 4;
+  const int lane = threadIdx.x & 63, heads = a.nkv * a.G, c = 2 * (lane & (HD / 2 - 1));
+  const int i = blockIdx.y, head = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (head >= heads) return;
+  const plan_int* row = (const plan_int*)a.schedule + 8 * i;
+  const int keys = row[0], S = row[1];
+  const int shared = S ? row[5] - row[4] + 1 : 0, n = keys ? shared + row[7] - row[6] + 1 : 0;
+  if (n == 1) return;                               // written where it was made
+  const int g = head / a.G, h = head - g * a.G;
+  const int rec0 = pa_shared_rec(a, g, row[4], i, h) * OS, next0 = a.most * a.G * OS;
+  const int rec1 = pa_own_rec(a, g, row[6] - shared, i, h) * OS, next1 = a.G * OS;
+  auto rec = [&](int p) { return a.states + (p < shared ? rec0 + p * next0 : rec1 + p * next1); };
+  float M = -INFINITY, L = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll 1
+  for (int base = 0; base < n; base += 16) {
+    float2 x[16], s = make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (base + u < n) x[u] = *(const float2*)(rec(base + u) + c);
+    if (base + (lane & 15) < n) s = *(const float2*)(rec(base + (lane & 15)) + HD);
+    const float mn = fmaxf(M, wave_max(s.x)), ref = mn == -INFINITY ? 0.f : mn;
+    const float old = exp2f(M - ref), f = exp2f(s.x - ref), fl = f * s.y;
+    M = mn;
+    L *= old;
+    y0 *= old;
+    y1 *= old;
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      if (base + u < n) {
+        const float fu = __shfl(f, u);
+        L += __shfl(fl, u);
+        y0 = fmaf(fu, x[u].x, y0);
+        y1 = fmaf(fu, x[u].y, y1);
+      }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (lane < HD / 2)
+    *(uint32_t*)(a.out + i * a.out_stride + (int64_t)head * HD + c) = pa_pack<BF>(y0 * inv, y1 * inv);
+}
+
 template <bool BF, int HD>
 static int pa_launch(const PagedArgs& a, hipStream_t st) {
   const int groups = ceil_div(a.G, 32);
@@ -364,9 +408,11 @@ static int pa_launch(const PagedArgs& a, hipStream_t st) {
                      st, a);
   OMNI_CHECK_LAUNCH();
   // few rows have many states each
-  const dim3 rows(a.nkv * a.G, a.n, a.n * a.nkv * a.G < 256 && a.ncols >= 64 ? HD / 32 : 1);
-  if (rows.z > 1) hipLaunchKernelGGL((paged_merge_kernel<BF, HD, 32>), rows, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((paged_merge_kernel<BF, HD, HD>), rows, dim3(256), 0, st, a);
+  const int heads = a.nkv * a.G;
+  if (a.ncols <= 16 * a.n)
+    hipLaunchKernelGGL((paged_merge_few_kernel<BF, HD>), dim3(ceil_div(heads, 4), a.n), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<BF, HD, 32>), dim3(a.G, a.n, a.nkv * (HD / 32)), dim3(256), 0, st, a);
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }
@@ -400,11 +446,13 @@ extern "C" int omni_paged_attention(const void* q, int64_t q_stride, const void*
   if (most > 1 && most * G > 32) return OMNI_EUNSUPPORTED;
   const int64_t shared_recs = most > 1 ? ((int64_t)columns * most + n) * G : 0;
   const int64_t own_recs = ((int64_t)columns + n) * G;
-  if (workspace_floats < n_kv_heads * (shared_recs + own_recs) * (head_dim + 4)) return OMNI_EINVAL;
+  const int64_t floats = n_kv_heads * (shared_recs + own_recs) * (head_dim + 4);
+  if (floats > 0x7fffffff) return OMNI_EUNSUPPORTED;
+  if (workspace_floats < floats) return OMNI_EINVAL;
   const PagedArgs a = {(const unsigned short*)q, q_stride, (const unsigned short*)k_cache,
                        (const unsigned short*)v_cache, pages, shift, n_kv_heads, G, n, columns, width,
                        most, tables, schedule, (unsigned short*)out, out_stride,
-                       scale * 1.4426950408889634f, workspace, shared_recs, own_recs};
+                       scale * 1.4426950408889634f, workspace, (int)shared_recs, (int)own_recs};
   hipStream_t st = (hipStream_t)stream;
   if (dtype) return head_dim == 64 ? pa_launch<true, 64>(a, st) : pa_launch<true, 128>(a, st);
   return head_dim == 64 ? pa_launch<false, 64>(a, st) : pa_launch<false, 128>(a, st);

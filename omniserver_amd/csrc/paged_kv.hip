@@ -287,7 +287,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   }
   pg_mark<false>(t, used, r.group, [&](int row, int& but) {
     return pg_pages(t, pg_length(t, row));
-  }, r.schedule ? common : nullptr, r.n);
+  }, r.schedule && r.most > 1 && r.n > 1 ? common : nullptr, r.n);
   __syncthreads();
   const PgShare own(t);
   int first;
@@ -340,8 +340,9 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   if (!r.schedule) return;
   // groups: a row that goes on from its neighbour, and the places in such a run cut at `most`
   int units = 0, start = 0;
+  const bool groups = r.most > 1 && r.n > 1;
 #pragma unroll 1
-  for (int base = 0; base < r.n; base += PG_THREADS) {
+  for (int base = 0; base < r.n && groups; base += PG_THREADS) {
     const int i = base + tid;
     int total, shared = 0;
     if (i && i < r.n && ask[i] && ask[i - 1]) {
@@ -364,7 +365,11 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
     const int i = base + tid;
     int mine = 0, total;
     if (i < r.n) {
-      const int group = at[i], S = size[group] > 1 ? share[group] : 0;
+      const int group = groups ? at[i] : i, S = groups && size[group] > 1 ? share[group] : 0;
+      if (!groups) {
+        at[i] = i;
+        size[i] = 1;
+      }
       common[i] = S;
       mine = ask[i] ? ceil_div(len[i] + ask[i], PG_UNIT) - (group == i ? 0 : S) : 0;
     }
