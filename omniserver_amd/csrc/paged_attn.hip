@@ -9,6 +9,10 @@
 
 #define PA_WAVES 4
 #define PA_UNIT 128                // keys of a workgroup's step: 32 a wave
+// KV heads from which on a column's heads are neighbouring workgroups, on XCDs of their own, and not
+// its columns: 32 x 2048 tokens of 16 heads 97.6 us, the other way 105; 32 x 4096 of 8 heads 103 and
+// 107; 200 x 1000 of 4 heads 88.7 and 87.0; 32 x 2048 of 2 heads 19.5 and 18.6.
+#define PA_BY_HEAD 8
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
@@ -18,6 +22,12 @@ __device__ __forceinline__ f32x4 pa_mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                    __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
   return mfma16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
+}
+// The lower and upper half of a packed pair as fp32.
+template <bool BF>
+__device__ __forceinline__ float pa_half(uint32_t v, bool upper) {
+  if (BF) return __builtin_bit_cast(float, upper ? v & 0xffff0000u : v << 16);
+  return (float)__builtin_bit_cast(half2_t, v)[upper ? 1 : 0];
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
@@ -43,6 +53,7 @@ struct PagedArgs {
   float scale_log2;
   float* states;                 // [nkv][shared_recs] then [nkv][own_recs] records of HD + 4
   int shared_recs, own_recs;
+  int by_head;                   // workgroups in the order of KV heads, not of columns
 };
 
 // The record of a row's head in a column: the columns and rows of an item ascend together, so that
@@ -60,6 +71,25 @@ typedef const __attribute__((address_space(4))) int plan_int;
 struct PaItem {
   int row, rows, heads, keys0, end, h0, g;
   const plan_int* table;
+};
+
+// Where 32 keys are: two runs of 16, each in one page, and how many of each there are.
+struct PaPlace {
+  int64_t at[2];
+  int there[2];
+  __device__ __forceinline__ PaPlace(const PagedArgs& a, const PaItem& it, int kb, int HD) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int k0 = min(kb, it.end - 1) + 16 * b;
+      there[b] = min(it.end - k0, 16);
+      int page = it.table[min(min(k0, it.end - 1) >> a.shift, a.width - 1)];
+      if (page < 0 || page >= a.pages) {
+        page = 0;
+        there[b] = 0;
+      }
+      at[b] = (((int64_t)page << a.shift) + (k0 & ((1 << a.shift) - 1))) * a.nkv * HD + it.g * HD;
+    }
+  }
 };
 
 // ---------------------------------------------------------------------------
@@ -100,62 +130,52 @@ struct PaState {
     }
   }
 
-  __device__ __forceinline__ void step(const PagedArgs& a, const PaItem& it, int kb, int l16, int g4) {
-    const int64_t tstride = (int64_t)a.nkv * HD;
-    const unsigned short *kp[2], *vp[2];
-    int there[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int k0 = kb + 16 * b;
-      there[b] = min(it.end - k0, 16);
-      int page = it.table[min(min(k0, it.end - 1) >> a.shift, a.width - 1)];
-      if (page < 0 || page >= a.pages) {
-        page = 0;
-        there[b] = 0;
-      }
-      const int64_t at = (((int64_t)page << a.shift) + (k0 & ((1 << a.shift) - 1))) * tstride + it.g * HD;
-      kp[b] = a.k_cache + at;
-      vp[b] = a.v_cache + at;
-    }
-    u32x4 kf[2][KC];
+  u32x4 kf[2][KC];
+  uint32_t vf[8][CV / 2];
+
+  __device__ __forceinline__ void load_k(const PagedArgs& a, const PaPlace& at, int l16, int g4) {
+    const int tstride = a.nkv * HD;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int j = 0; j < KC; ++j) kf[b][j] = *(const u32x4*)(kp[b] + l16 * tstride + j * 32 + g4 * 8);
-    uint32_t vf[8][CV / 2];
+      for (int j = 0; j < KC; ++j)
+        kf[b][j] = *(const u32x4*)(a.k_cache + at.at[b] + l16 * tstride + j * 32 + g4 * 8);
+  }
+  __device__ __forceinline__ void load_v(const PagedArgs& a, const PaPlace& at, int l16, int g4) {
+    const int tstride = a.nkv * HD;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      __builtin_memcpy(vf[e], vp[e >> 2] + (4 * g4 + (e & 3)) * tstride + l16 * CV, 2 * CV);
-    const bool part = there[0] < 16 || there[1] < 16;
-    if (part) {
+      __builtin_memcpy(vf[e], a.v_cache + at.at[e >> 2] + (4 * g4 + (e & 3)) * tstride + l16 * CV, 2 * CV);
+  }
+
+  // The keys at kb; the next step's K goes out once this one's is used up, and V likewise.
+  __device__ __forceinline__ void step(const PagedArgs& a, const PaPlace& at, const PaPlace& then, bool more,
+                                       int l16, int g4) {
+    const bool part = at.there[0] < 16 || at.there[1] < 16;
+    f32x4 s[NT][2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool off = 4 * g4 + (e & 3) >= there[e >> 2];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int d = 0; d < CV / 2; ++d) vf[e][d] = off ? 0 : vf[e][d];
+      for (int b = 0; b < 2; ++b) {
+        s[n][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KC; ++j) s[n][b] = pa_mfma<BF>(kf[b][j], qf[n][j], s[n][b]);
       }
-    }
-    u32x4 pf[NT];
+    if (more) load_k(a, then, l16, g4);
+    u32x4 pf[NT], rest[NT];
     float alpha[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      f32x4 s[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        s[b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < KC; ++j) s[b] = pa_mfma<BF>(kf[b][j], qf[n][j], s[b]);
-      }
       if (part) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (4 * g4 + (e & 3) >= there[e >> 2]) s[e >> 2][e & 3] = -INFINITY;
+          if (4 * g4 + (e & 3) >= at.there[e >> 2]) s[n][e >> 2][e & 3] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s[e >> 2][e & 3] *= a.scale_log2;
-        top = fmaxf(top, s[e >> 2][e & 3]);
+        s[n][e >> 2][e & 3] *= a.scale_log2;
+        top = fmaxf(top, s[n][e >> 2][e & 3]);
       }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -166,11 +186,23 @@ struct PaState {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = exp2f(s[e >> 2][e & 3] - ref);
+        p[e] = exp2f(s[n][e >> 2][e & 3] - ref);
         l[n] += p[e];
       }
-      pf[n] = (u32x4){pa_pack<BF>(p[0], p[1]), pa_pack<BF>(p[2], p[3]), pa_pack<BF>(p[4], p[5]),
-                      pa_pack<BF>(p[6], p[7])};
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const uint32_t w = pa_pack<BF>(p[2 * d], p[2 * d + 1]);
+        pf[n][d] = w;
+        rest[n][d] = pa_pack<BF>(p[2 * d] - pa_half<BF>(w, false), p[2 * d + 1] - pa_half<BF>(w, true));
+      }
+    }
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool off = 4 * g4 + (e & 3) >= at.there[e >> 2];
+#pragma unroll
+        for (int d = 0; d < CV / 2; ++d) vf[e][d] = off ? 0 : vf[e][d];
+      }
     }
 #pragma unroll
     for (int t = 0; t < CV; ++t) {
@@ -183,8 +215,10 @@ struct PaState {
       for (int n = 0; n < NT; ++n) {
         o[n][t] *= alpha[n];
         o[n][t] = pa_mfma<BF>(vt, pf[n], o[n][t]);
+        o[n][t] = pa_mfma<BF>(vt, rest[n], o[n][t]);
       }
     }
+    if (more) load_v(a, then, l16, g4);
   }
 };
 
@@ -196,12 +230,12 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedArgs 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
-  const int col = blockIdx.x;
+  const int col = a.by_head ? blockIdx.y : blockIdx.x;
   const plan_int* schedule = (const plan_int*)a.schedule;
   const plan_int* column = schedule + 8 * a.n + 4 * col;
   int item = column[0], u0 = column[1], left = column[2];
   PaItem it;
-  it.g = blockIdx.y;
+  it.g = a.by_head ? blockIdx.x : blockIdx.y;
   it.h0 = blockIdx.z * 32;
   it.heads = min(32, a.G - it.h0);
   while (left > 0) {
@@ -221,7 +255,18 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedArgs 
       constexpr int NT = decltype(tiles)::value;
       PaState<BF, HD, NT> st;
       st.load(a, it, l16, g4);
-      for (int kb = from + wave * 32; kb < to; kb += PA_UNIT) st.step(a, it, kb, l16, g4);
+      int kb = from + wave * 32;
+      if (kb < to) {
+        PaPlace at(a, it, kb, HD);
+        st.load_k(a, at, l16, g4);
+        st.load_v(a, at, l16, g4);
+        for (; kb < to; kb += PA_UNIT) {
+          const bool more = kb + PA_UNIT < to;
+          const PaPlace then(a, it, more ? kb + PA_UNIT : kb, HD);
+          st.step(a, at, then, more, l16, g4);
+          at = then;
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float l = st.l[n];
@@ -404,8 +449,8 @@ __global__ __launch_bounds__(256) void paged_merge_few_kernel(PagedArgs a) {
 template <bool BF, int HD>
 static int pa_launch(const PagedArgs& a, hipStream_t st) {
   const int groups = ceil_div(a.G, 32);
-  hipLaunchKernelGGL((paged_attn_kernel<BF, HD>), dim3(a.ncols, a.nkv, groups), dim3(64 * PA_WAVES), 0,
-                     st, a);
+  const dim3 grid = a.by_head ? dim3(a.nkv, a.ncols, groups) : dim3(a.ncols, a.nkv, groups);
+  hipLaunchKernelGGL((paged_attn_kernel<BF, HD>), grid, dim3(64 * PA_WAVES), 0, st, a);
   OMNI_CHECK_LAUNCH();
   // few rows have many states each
   const int heads = a.nkv * a.G;
@@ -452,7 +497,8 @@ extern "C" int omni_paged_attention(const void* q, int64_t q_stride, const void*
   const PagedArgs a = {(const unsigned short*)q, q_stride, (const unsigned short*)k_cache,
                        (const unsigned short*)v_cache, pages, shift, n_kv_heads, G, n, columns, width,
                        most, tables, schedule, (unsigned short*)out, out_stride,
-                       scale * 1.4426950408889634f, workspace, (int)shared_recs, (int)own_recs};
+                       scale * 1.4426950408889634f, workspace, (int)shared_recs, (int)own_recs,
+                       n_kv_heads >= PA_BY_HEAD};
   hipStream_t st = (hipStream_t)stream;
   if (dtype) return head_dim == 64 ? pa_launch<true, 64>(a, st) : pa_launch<true, 128>(a, st);
   return head_dim == 64 ? pa_launch<false, 64>(a, st) : pa_launch<false, 128>(a, st);
