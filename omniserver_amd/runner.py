@@ -30,21 +30,52 @@ is copied into the next decode slot.
 Speculative decoding: ``speculate`` takes a drafted tree of tokens per running sequence (from
 any draft: prompt lookup, extra heads, a smaller model), scores all of them in one forward and
 advances every sequence by the drafted tokens that stand and one more.
+
+Beam search: ``beam_search`` finds the best continuations of prompts, in a paged cache beside the
+pool.
 """
 
 from __future__ import annotations
 
 import abc
-from typing import Dict, List
+from typing import Dict, List, NamedTuple
 
 import numpy as np
 import torch
 
+from .beam import MAX_BEAMS, select
 from .hostio import to_device
 from .kv_cache import PreallocatedKVCache
 from .linear import weights_epoch
+from .paged_kv import MAX_SEQS, PAGE_SIZES, PagedKVCache
 from .request import Sequence, Status
 from .speculative import MAX_NODES, verify
+
+
+class Beam(NamedTuple):
+    """A continuation that beam search has found."""
+    tokens: List[int]      # with its stop token, if it ended with one
+    logprob: float         # sum of the tokens' log-probabilities
+    score: float           # logprob / len(tokens) ** length_penalty
+
+
+def _beams_of(tokens, parents, scores, length_penalty: float) -> List[List[Beam]]:
+    """Each request's beams, the best first, from every step's choices [t][request][beam]."""
+    out = []
+    for s, row in enumerate(scores):
+        found = []
+        for w, logprob in enumerate(row):
+            if logprob == -float("inf"):
+                continue
+            line, b = [], w
+            for t in range(len(tokens) - 1, -1, -1):
+                line.append(tokens[t][s][b])
+                b = parents[t][s][b]
+            line = [x for x in reversed(line) if x >= 0]          # a finished beam goes on with -1
+            found.append(Beam(line, logprob, logprob / len(line) ** length_penalty))
+        found.sort(key=lambda b: -b.score)
+        out.append(found)
+    return out
 
 
 class ModelRunner(abc.ABC):
@@ -165,18 +196,9 @@ class MultimodalRunner(ModelRunner):
         self._pool.lengths[:n] -= 1
         self._dev_ids_for = None
 
-    @torch.inference_mode()
-    def prefill(self, seqs: List[Sequence]) -> None:
-        """Packed prefill, compute branch (multimodal.py:116-144): every prompt in one
-        forward, causal within its segment, K/V written to its slot, logits only at
-        segment ends."""
-        if not seqs:
-            return
-        self.settle()
-        base = len(self._slot_seq)
-        if base + len(seqs) > self.max_running:
-            raise RuntimeError(f"KV pool full: {base} running + {len(seqs)} new > "
-                               f"{self.max_running}")
+    def _pack_prompts(self, seqs: List[Sequence]):
+        """(embeddings [1, T, H], positions [3, 1, T], prompt lengths, rope deltas, the deltas on
+        the device) of the sequences' prompts, one after another."""
         dev = self.device
         # The packed prompt's host-side inputs are gathered as numpy arrays and uploaded in
         # one pinned copy (ids, image row indices, positions, rope deltas): the GPU is idle
@@ -208,7 +230,6 @@ class MultimodalRunner(ModelRunner):
             seg_lens.append(L)
             deltas.append(int(delta))
             T += L
-        slots = [base + i for i in range(len(seqs))]
         nr = sum(int(r.shape[0]) for r in img_rows)
         host = np.concatenate(ids_l + img_rows + [np.concatenate(pos_l, axis=1).reshape(-1),
                                                   np.asarray(deltas, dtype=np.int64)])
@@ -218,13 +239,29 @@ class MultimodalRunner(ModelRunner):
             emb.index_copy_(0, up[T:T + nr], torch.cat(vis, 0).to(emb.dtype))
         packed = emb.unsqueeze(0)
         pos = up[T + nr:T + nr + 3 * T].view(3, 1, T)                           # [3, 1, T]
+        return packed, pos, seg_lens, deltas, up[T + nr + 3 * T:]
+
+    @torch.inference_mode()
+    def prefill(self, seqs: List[Sequence]) -> None:
+        """Packed prefill, compute branch (multimodal.py:116-144): every prompt in one
+        forward, causal within its segment, K/V written to its slot, logits only at
+        segment ends."""
+        if not seqs:
+            return
+        self.settle()
+        base = len(self._slot_seq)
+        if base + len(seqs) > self.max_running:
+            raise RuntimeError(f"KV pool full: {base} running + {len(seqs)} new > "
+                               f"{self.max_running}")
+        packed, pos, seg_lens, deltas, delta_rows = self._pack_prompts(seqs)
+        slots = [base + i for i in range(len(seqs))]
         if self._use_graph and self.prefill_graph_layouts > 0:
             logits = self._prefill_graphed(packed, pos, slots, seg_lens)
         else:
             last = torch.tensor(seg_lens).cumsum(0) - 1
             cache = self._pool.packed_prefill_cache(slots, seg_lens)
             logits = self.adapter.llm(packed, pos, None, cache, logits_indices=last.tolist())[0]
-        self._rope_delta[base:base + len(seqs)].copy_(up[T + nr + 3 * T:])
+        self._rope_delta[base:base + len(seqs)].copy_(delta_rows)
         toks = self._sample_rows(logits, seqs)
         for i, seq in enumerate(seqs):
             slot = slots[i]
@@ -581,6 +618,89 @@ class MultimodalRunner(ModelRunner):
         while len(self._spec_graphs) > self.spec_graph_layouts:
             self._spec_graphs.pop(next(iter(self._spec_graphs)))
         return v
+
+    # ---- beam search -----------------------------------------------------------------
+    @torch.inference_mode()
+    def beam_search(self, seqs: List[Sequence], beams: int = 4, length_penalty: float = 1.0,
+                    page_size: int = 32) -> List[List["Beam"]]:
+        """The best continuations of each prompt, ``beams`` of them, the best first.
+
+        Every step keeps the ``beams`` continuations of a request with the largest sums of
+        log-probabilities, over all of its beams and the vocabulary (``beam.select``); a beam ends with
+        one of the request's stop tokens, after max_new_tokens, or at the runner's max_len, and holds
+        its place from then on.  They are ranked by sum / tokens ** length_penalty.  The sequences'
+        prompts are read, nothing else of them is changed, and running sequences go on as ever: the
+        beams live in a paged cache of their own, in which those of a request share its prompt's pages.
+        With ``use_graph=True`` the steps of a call behind its first are one captured graph."""
+        if not seqs:
+            return []
+        if not 1 <= beams <= MAX_BEAMS or len(seqs) * beams > MAX_SEQS:
+            raise ValueError(f"{len(seqs)} x {beams} beams: 1 to {MAX_BEAMS} each, {MAX_SEQS} in all")
+        if any(not s.request.sampling.greedy for s in seqs):
+            raise ValueError("beam search draws nothing: temperature has to be 0")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"pages of {page_size} tokens: one of {PAGE_SIZES}")
+        self.settle()
+        n, W, dev = len(seqs), beams, self.device
+        packed, pos, lens, _, deltas = self._pack_prompts(seqs)
+        limits = [min(max(s.request.sampling.max_new_tokens, 1), self._pool.max_len - L)
+                  for s, L in zip(seqs, lens)]
+        steps = max(limits)
+        # whole pages of the prompts are shared; behind them every beam has its own
+        held = lambda tokens: -(-tokens // page_size)
+        own = W * (held(steps) + 1)
+        pool = self._pool
+        with torch.inference_mode(False):                         # (captured outside of it)
+            cache = PagedKVCache(pool.n_layers, sum(held(L) + own for L in lens), pool.n_kv_heads,
+                                 page_size, pool.head_dim, dev, max_seqs=n * W,
+                                 max_len=max(lens) + steps, n_heads=pool.n_heads)
+        last = torch.tensor(lens).cumsum(0) - 1
+        logits = self.adapter.llm(packed, pos, None, cache.prefill_cache(range(0, n * W, W), lens),
+                                  logits_indices=last.tolist())[0]
+        stops = [list(s.request.sampling.stop_token_ids) for s in seqs]
+        most = max(1, max(map(len, stops)))
+        st = {"stop": to_device([t + [-1] * (most - len(t)) for t in stops], torch.int64, dev),
+              "delta": deltas.repeat_interleave(W)}
+        scores = torch.full((n, W), -float("inf"), device=dev)
+        scores[:, 0] = 0.0                      # one beam to begin with
+        first = select(logits.view(n, 1, -1).expand(n, W, -1), scores, stop=st["stop"], pad=-1)
+        cache.reorder(first.parents)
+        limit = to_device(limits, torch.int64, dev).unsqueeze(1)
+        st.update(scores=first.scores, tokens=first.tokens, parents=first.parents,
+                  done=first.done | (limit <= 1))
+        tokens = torch.empty(steps, n, W, device=dev, dtype=torch.int64)
+        parents = torch.empty(steps, n, W, device=dev, dtype=torch.int32)
+        graph, t = None, 0
+        while True:
+            tokens[t].copy_(st["tokens"])
+            parents[t].copy_(st["parents"])
+            t += 1
+            if t == steps or bool(st["done"].all()):
+                break
+            if graph is not None:
+                graph.replay()
+            else:
+                self._beam_step(cache, st)
+                if self._use_graph and t == 1 and steps > 4:
+                    with torch.inference_mode(False):
+                        st = {name: v.clone() for name, v in st.items()}
+                        graph = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph):
+                            self._beam_step(cache, st)
+            st["done"].logical_or_(limit <= t + 1)
+        return _beams_of(tokens[:t].tolist(), parents[:t].tolist(), st["scores"].tolist(),
+                         length_penalty)
+
+    def _beam_step(self, cache: PagedKVCache, st: dict) -> None:
+        """One token for every beam, on device tensors: forward, choice, the cache after it."""
+        n, W = st["tokens"].shape
+        emb = self.adapter.embed_tokens(st["tokens"].reshape(-1).clamp(min=0)).unsqueeze(0)
+        step = cache.decode_cache(n * W, rope_delta=st["delta"])
+        logits = self.adapter.llm(emb, step.positions.view(3, 1, n * W), None, step)[0]
+        b = select(logits.view(n, W, -1), st["scores"], done=st["done"], stop=st["stop"], pad=-1)
+        cache.reorder(b.parents)
+        for name, v in zip(("scores", "parents", "tokens", "done"), b):
+            st[name].copy_(v)
 
     # ---- decode paths ----------------------------------------------------------------
     def _load_ids(self, seqs, n, dst: torch.Tensor) -> None:

@@ -450,3 +450,337 @@ def test_select_defaults_and_strides(gpu):
     assert got.done.tolist() == [[r[3] for r in q] for q in want]
     one = select(logits[:1, :1].expand(2, 3, 999).to(gpu), torch.zeros(2, 3, device=gpu))
     assert one.parents.tolist() == [[0, 1, 2]] * 2      # all alike: the lower beam first
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_select_close_values(gpu, dtype):
+    """Beams whose continuations differ by less than 32-bit sums resolve: the order is that of 64-bit
+    values, and of the lower beam where these are equal."""
+    from omniserver_amd.beam import select
+    say(f"select close values {dtype}")
+    g = torch.Generator().manual_seed(8)
+    V, W, n = 20011, 5, 6
+    row = (torch.randn(1, 1, V, generator=g) * 3).to(dtype)
+    logits = row.expand(n, W, V).contiguous()
+    # the same logits; scores a rounding step or two apart, or equal
+    steps = torch.tensor([[0, 1, 2, 3, 4], [4, 3, 2, 1, 0], [1, 1, 0, 0, 1], [0] * 5, [2, 0, 2, 1, 0],
+                          [3, 3, 3, 0, 3]])
+    scores = (-1.0 - steps * 2.0 ** -23).float()
+    # rows that differ by one small logit: sums apart by 1e-9 of themselves and less
+    for s in (3, 4):
+        for b in range(W):
+            logits[s, b, 100 + b] = (-14.0 - 0.01 * ((b * 3) % 5))
+    done = torch.zeros(n, W, dtype=torch.bool)
+    done[5, 1] = True
+    for k in (5, 12, 40):
+        want = ref.select(logits, scores, k, done)
+        got = select(logits.to(gpu), scores.to(gpu), k, done.to(gpu))
+        assert got.parents.tolist() == [[r[1] for r in q] for q in want], k
+        assert got.tokens.tolist() == [[r[2] for r in q] for q in want], k
+
+
+def test_select_vector_of_values(gpu):
+    """More beams times continuations than lanes, close ones among them."""
+    from omniserver_amd.beam import select
+    g = torch.Generator().manual_seed(9)
+    n, W, V = 3, 24, 5003
+    row = (torch.randn(n, 1, V, generator=g) * 3).half()
+    logits = row.expand(n, W, V).contiguous()
+    logits[:, 12:] = (torch.randn(n, 12, V, generator=g) * 3).half()
+    scores = (-2.0 - torch.randint(0, 3, (n, W), generator=g) * 2.0 ** -22).float()
+    for k in (8, 48):
+        want = ref.select(logits, scores, k)
+        got = select(logits.to(gpu), scores.to(gpu), k)
+        assert got.parents.tolist() == [[r[1] for r in q] for q in want], k
+        assert got.tokens.tolist() == [[r[2] for r in q] for q in want], k
+
+
+# ----------------------------------------------------------------------------- as a step runs them
+def beam_step(cache, x, n, W, nh, nkv, hd):
+    """One step of beam search on the operators alone: x holds the tensors that a model would give."""
+    from omniserver_amd.beam import select
+    rows = n * W
+    step = cache.decode_cache(rows)
+    q, k, v = x["qkv"].view(rows, nh + 2 * nkv, hd).split((nh, nkv, nkv), 1)
+    for layer in range(cache.n_layers):
+        step.write(k, v, layer)
+        step.attend_qkv(x["qkv"], layer, hd ** -0.5, x["out"][layer])
+    step.finish()
+    b = select(x["logits"], x["scores"], done=x["done"], stop=x["stop"], pad=-1)
+    cache.reorder(b.parents)
+    x["scores"].copy_(b.scores)
+    x["done"].copy_(b.done)
+    return b
+
+
+def beam_inputs(rng, g, n, W, nh, nkv, hd, layers, V, gpu):
+    x = {"qkv": torch.randn(n * W, (nh + 2 * nkv) * hd, generator=g).half(),
+         "logits": torch.randn(n, W, V, generator=g).half() * 3,
+         "stop": torch.tensor([rng.randrange(V)])}
+    return x
+
+
+def test_beam_steps_follow_their_tokens(gpu):
+    """Ten steps of beam search on random K/V: what every beam holds is what a list of its tokens' K/V
+    rows holds, and its attention that of the list."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    say("beam steps against lists")
+    n, W, nh, nkv, hd, layers, page, V = 3, 4, 6, 2, 64, 2, 16, 700
+    rng, g = random.Random(3), torch.Generator().manual_seed(4)
+    prompts = [37, 16, 5]
+    cache = PagedKVCache(layers, 60, nkv, page, hd, gpu, max_seqs=n * W, max_len=80, n_heads=nh)
+    slots = cache.reserve(prompts, rows=range(0, n * W, W))
+    kv = torch.randn(layers, 2, sum(prompts), nkv, hd, generator=g).half()
+    for layer in range(layers):
+        slots.write(kv[layer, 0].to(gpu), kv[layer, 1].to(gpu), layer)
+    slots.finish()
+    held, at = [], 0
+    for L in prompts:
+        held.append([kv[:, :, at:at + L]] + [kv[:, :, :0]] * (W - 1))
+        at += L
+    state = {"scores": torch.full((n, W), -math.inf), "done": torch.zeros(n, W, dtype=torch.bool),
+             "out": torch.zeros(layers, n * W, nh, hd).half()}
+    state["scores"][:, 0] = 0.0
+    state = {name: v.to(gpu) for name, v in state.items()}
+    for turn in range(10):
+        x = beam_inputs(rng, g, n, W, nh, nkv, hd, layers, V, gpu)
+        want = ref.select(x["logits"], state["scores"].cpu(), W, state["done"].cpu(), x["stop"].tolist(), -1)
+        rows = x["qkv"].view(n * W, nh + 2 * nkv, hd)
+        state.update({name: v.to(gpu) for name, v in x.items()})
+        b = beam_step(cache, state, n, W, nh, nkv, hd)
+        for s in range(n):
+            for w in range(W):
+                r = s * W + w
+                new = rows[r, nh:].reshape(2, 1, nkv, hd)
+                held[s][w] = torch.cat([held[s][w], new.expand(layers, 2, 1, nkv, hd)], 2)
+                for layer in range(layers):
+                    k, v = held[s][w][layer]
+                    exact, mag = ref.attention(rows[r, :nh], k, v, hd ** -0.5)
+                    bound = ref.attention_bound(exact, mag, k.shape[0], v.float().abs().max().item(),
+                                                torch.float16)
+                    err = (state["out"][layer, r].cpu().double() - exact).abs()
+                    assert (err <= bound).all(), (turn, s, w, layer)
+        assert b.parents.tolist() == [[e[1] for e in q] for q in want], turn
+        assert b.tokens.tolist() == [[e[2] for e in q] for q in want], turn
+        assert b.done.tolist() == [[e[3] for e in q] for q in want], turn
+        held = [[held[s][e[1]] if e[1] >= 0 else kv[:, :, :0] for e in q] for s, q in enumerate(want)]
+        tables, host = cache.tables.tolist(), cache.storage.cpu()
+        assert cache.lengths.tolist() == [h.shape[2] for q in held for h in q], turn
+        for r, h in enumerate(h for q in held for h in q):
+            for layer in range(layers):
+                k, v = tokens_of(host, layer, tables[r], h.shape[2], page)
+                assert torch.equal(k, h[layer, 0]) and torch.equal(v, h[layer, 1]), (turn, r)
+
+
+def test_beam_step_in_graphs(gpu):
+    """A step captured on one cache, and another on a second one, replayed in turn with eager work
+    between: each does what an eager twin does."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    say("beam steps in two graphs")
+    n, W, nh, nkv, hd, layers, page, V = 2, 3, 12, 2, 128, 1, 16, 3001
+    rng, g = random.Random(5), torch.Generator().manual_seed(6)
+
+    def start():
+        cache = PagedKVCache(layers, 40, nkv, page, hd, gpu, max_seqs=n * W, max_len=96, n_heads=nh)
+        cache.storage.copy_(torch.randn(cache.storage.shape, generator=torch.Generator().manual_seed(1)))
+        for s, L in enumerate((30, 47)):
+            cache.reserve([L], rows=[s * W]).finish()
+        x = {"scores": torch.full((n, W), -math.inf, device=gpu),
+             "done": torch.zeros(n, W, dtype=torch.bool, device=gpu),
+             "out": torch.zeros(layers, n * W, nh, hd, device=gpu, dtype=torch.float16),
+             "qkv": torch.zeros(n * W, (nh + 2 * nkv) * hd, device=gpu, dtype=torch.float16),
+             "logits": torch.zeros(n, W, V, device=gpu, dtype=torch.float16),
+             "stop": torch.tensor([5], device=gpu)}
+        x["scores"][:, 0] = 0.0
+        return cache, x
+
+    twins = [(start(), start()) for _ in range(2)]
+    graphs = []
+    for (cache, x), _ in twins:
+        keep = {name: t.clone() for name, t in
+                list(x.items()) + [("l", cache.lengths), ("t", cache.tables), ("s", cache.storage)]}
+        beam_step(cache, x, n, W, nh, nkv, hd)                 # warm
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            b = beam_step(cache, x, n, W, nh, nkv, hd)
+        for name, t in list(x.items()) + [("l", cache.lengths), ("t", cache.tables), ("s", cache.storage)]:
+            t.copy_(keep[name])
+        graphs.append((graph, b))
+    for turn in range(8):
+        which = turn % 2
+        (cache, x), (twin, y) = twins[which]
+        new = beam_inputs(rng, g, n, W, nh, nkv, hd, layers, V, gpu)
+        for name, v in new.items():
+            x[name].copy_(v)
+            y[name].copy_(v)
+        graphs[which][0].replay()
+        want = beam_step(twin, y, n, W, nh, nkv, hd)
+        torch.cuda.synchronize()
+        for a, b in zip(graphs[which][1], want):
+            assert torch.equal(a, b), turn
+        for name in x:
+            assert torch.equal(x[name], y[name]), (turn, name)
+        assert torch.equal(cache.tables, twin.tables) and torch.equal(cache.lengths, twin.lengths)
+        assert torch.equal(cache.storage, twin.storage), turn
+
+
+def test_another_stream(gpu):
+    """Launches go to the current stream: a step on a side stream behind a long kernel of its own."""
+    rng = random.Random(7)
+    cache, tables, lengths = make_cache(gpu, [90, 33], 16, rng, spare=4, max_len=128)
+    g = torch.Generator().manual_seed(2)
+    host = fill_pages(cache, tables, lengths, g)
+    rows = torch.randn(2, 16 * 128, generator=g).half()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        x = torch.randn(3000, 3000, device=gpu)
+        for _ in range(5):
+            x = x @ x / 3000
+        qkv = rows.to(gpu)
+        step = cache.decode_cache(2)
+        q, k, v = qkv.view(2, 16, 128).split((12, 2, 2), 1)
+        out = step.flash_decode(q, k, v, 0, 0.1)
+    side.synchronize()
+    check_rows(out, rows.view(2, 16, 128)[:, :12], cache.storage.cpu(), 0, cache.tables.tolist(),
+               [91, 34], 16, 0.1)
+
+
+def test_superseded_reservations(gpu):
+    """A later reservation or reordering may give the same pages away: the older one says so."""
+    rng = random.Random(8)
+    cache, _, _ = make_cache(gpu, [20, 7, 9], 16, rng, spare=6, max_len=128)
+    first = cache.decode_cache(3)
+    second = cache.reserve([1, 2], rows=[2, 0])
+    k = torch.zeros(3, 2, 128, device=gpu, dtype=torch.float16)
+    out = torch.empty(3, 12, 128, device=gpu, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="later"):
+        first.write(k, k, 0)
+    with pytest.raises(RuntimeError, match="later"):
+        first.attend_qkv(torch.zeros(3, 1536, device=gpu).half(), 0, 0.1, out)
+    with pytest.raises(RuntimeError, match="later"):
+        first.finish()
+    second.finish()
+    assert cache.lengths.tolist() == [22, 7, 10]
+    third = cache.reserve([3])
+    cache.reorder([[0, 0, 2]])
+    with pytest.raises(RuntimeError, match="later"):
+        third.finish()
+    assert cache.lengths.tolist() == [22, 22, 10]
+
+
+# ----------------------------------------------------------------------------- the model
+@pytest.mark.parametrize("quant", [None, "gptq"])
+def test_model_over_pages(gpu, quant):
+    """The decoder's forward over a paged cache against the same over the preallocated pool: packed
+    prompts, then single tokens, for which the pool's view runs the same linears."""
+    from omniserver_amd import synth
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    from omniserver_amd.paged_kv import PagedKVCache
+    from omniserver_amd.qwen2_llm import Qwen2LLM
+    from tests.helpers import compare_logits
+    say(f"model over pages quant={quant}")
+    shape = synth.DecoderShape()
+    gen, build = ((synth.gptq_decoder, Qwen2LLM.from_gptq) if quant
+                  else (synth.fp16_decoder, Qwen2LLM.from_fp16))
+    shape.num_layers = 2
+    llm = build(gen(shape, seed=5, num_layers=2), shape, gpu)
+    lens = [40, 17, 65, 100]
+    T, n = sum(lens), len(lens)
+    ids = [synth.random_ids(L, shape.vocab_size, 5, f"p{L}") for L in lens]
+    pool = PreallocatedKVCache(2, n, 2, 160, 128, gpu, n_heads=12)
+    pages = PagedKVCache(2, 40, 2, 16, 128, gpu, max_seqs=n, max_len=160, n_heads=12)
+    pos = torch.cat([torch.arange(L) for L in lens]).expand(3, 1, T).contiguous().to(gpu)
+    last = [sum(lens[:i + 1]) - 1 for i in range(n)]
+    with torch.inference_mode():
+        emb = llm.embed_tokens(torch.cat(ids).to(gpu)).unsqueeze(0)
+        a = llm(emb, pos, None, pool.packed_prefill_cache(range(n), lens), logits_indices=last)[0]
+        b = llm(emb, pos, None, pages.prefill_cache(range(n), lens), logits_indices=last)[0]
+        assert torch.equal(a, b)
+        assert pages.lengths.tolist() == lens == pool.lengths.tolist()
+        for turn in range(20):                        # over pages' borders
+            new = a.argmax(-1)
+            emb = llm.embed_tokens(new)
+            a = llm(emb.unsqueeze(1), pool.lengths[:n].expand(3, n).unsqueeze(-1), None,
+                    pool.view(n))[:, -1]
+            step = pages.decode_cache(n)
+            b = llm(emb.unsqueeze(0), step.positions.view(3, 1, n), None, step)[0]
+            compare_logits(b, a)
+        assert pages.lengths.tolist() == [L + 20 for L in lens] == pool.lengths.tolist()
+
+
+def oracle_beams(orc, prompt, W, steps, stops):
+    """Beam search on the oracle's logits: (sum of log-probabilities, tokens), the best first."""
+    from tests.helpers import oracle_stream_logits
+    beams = [(0.0, [], False)]
+    for _ in range(steps):
+        every = []
+        for score, line, over in beams:
+            if over:
+                every.append((score, line, True))
+                continue
+            rows = oracle_stream_logits(orc, prompt, line + [0], 256)
+            lp = torch.log_softmax(rows[len(line)].double(), -1)
+            best = lp.topk(W)
+            every += [(score + v, line + [t], t in stops)
+                      for v, t in zip(best.values.tolist(), best.indices.tolist())]
+        every.sort(key=lambda e: -e[0])
+        beams = every[:W]
+    return beams
+
+
+@pytest.mark.parametrize("quant,use_graph", [(None, False), (None, True), ("gptq", True)])
+def test_runner_beam_search(gpu, quant, use_graph):
+    """Beams of two prompts: their sums of log-probabilities are the oracle's for their tokens, the
+    best is as good as the oracle's beam search finds, one beam alone is the greedy stream, and running
+    sequences are left alone."""
+    from omniserver_amd import synth
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    from omniserver_amd.runner import NativeQwenVLRunner
+    from tests.helpers import oracle_from_fp16, oracle_from_gptq, oracle_stream_logits
+    say(f"runner beam search quant={quant} use_graph={use_graph}")
+    shape = synth.DecoderShape()
+    w = (synth.gptq_decoder if quant else synth.fp16_decoder)(shape, seed=5, num_layers=2)
+    prompts = [synth.random_ids(L, shape.vocab_size, 5, f"p{L}").tolist() for L in (40, 17)]
+    orc = oracle_from_gptq(w, shape) if quant else oracle_from_fp16(w, shape)
+    r = NativeQwenVLRunner(max_running=2, max_len=128, use_graph=use_graph, weights=w, quant=quant)
+    mk = lambda p, steps: Sequence(Request(prompt=p, sampling=SamplingParams(max_new_tokens=steps)))  # noqa: E731
+    running = [mk(p, 30) for p in prompts]
+    for s in running:
+        r.tokenize(s)
+    r.prefill(running)
+    r.decode(running)
+    before = [list(s.output_token_ids) for s in running]
+    W, steps = 3, 6
+    seqs = [mk(prompts[0], steps), mk(prompts[1], steps - 1)]
+    found = r.beam_search(seqs, beams=W, page_size=16)
+    for s, beams in zip(seqs, found):
+        p, limit = s.request.prompt, s.request.sampling.max_new_tokens
+        assert len(beams) == W and not s.output_token_ids
+        assert [b.score for b in beams] == sorted((b.score for b in beams), reverse=True)
+        assert len({tuple(b.tokens) for b in beams}) == W
+        want = oracle_beams(orc, p, W, limit, s.request.sampling.stop_token_ids)
+        # logits within 2e-2 of the oracle's: a log-probability within twice that
+        slack = 2 * 2e-2 * limit
+        for b in beams:
+            rows = oracle_stream_logits(orc, p, b.tokens, 256)
+            lp = torch.log_softmax(torch.as_tensor(rows).double(), -1)
+            exact = sum(float(lp[i, t]) for i, t in enumerate(b.tokens))
+            assert abs(b.logprob - exact) <= slack
+            assert abs(b.score - b.logprob / len(b.tokens)) < 1e-6 and len(b.tokens) == limit
+        assert max(b.logprob for b in beams) >= want[0][0] - slack
+    stop = found[0][0].tokens[2]
+    seq = mk(prompts[0], steps)
+    seq.request.sampling.stop_token_ids = [stop]
+    for b in r.beam_search([seq], beams=W)[0]:
+        assert stop not in b.tokens[:-1] and (b.tokens[-1] == stop or len(b.tokens) == steps)
+    greedy = r.beam_search([mk(prompts[0], steps)], beams=1)[0]
+    assert len(greedy) == 1 and len(greedy[0].tokens) == steps
+    r.decode(running)
+    assert [s.output_token_ids[:len(b)] for s, b in zip(running, before)] == before
+    for bad in ({"beams": 0}, {"beams": 33}, {"page_size": 24}):
+        with pytest.raises(ValueError):
+            r.beam_search([mk(prompts[0], 4)], **bad)
+    with pytest.raises(ValueError):
+        r.beam_search([Sequence(Request(prompt=prompts[0], sampling=SamplingParams(temperature=0.5)))])
+    assert r.beam_search([]) == []
