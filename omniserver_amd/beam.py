@@ -33,8 +33,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int | None = None,
     logits [n, W, V] (fp16, bf16 or fp32, columns contiguous); scores fp32 [n, W]: the beams' sums of
     log-probabilities.  Going on with token v is worth scores + logits[v] - log sum exp logits; a beam
     whose score is not finite is not in use (so a request's first step has one beam in use).  ``done``
-    bool [n, W]: a finished beam goes on only as itself, with token ``pad`` at its score, and its
-    logits are not read.  ``stop``: tokens that finish a beam, a list, or int64 [m] or [n, m] on the
+    bool [n, W]: a finished beam goes on only as itself, with token ``pad`` at its score, whatever its
+    logits.  ``stop``: tokens that finish a beam, a list, or int64 [m] or [n, m] on the
     device (-1: none).
 
     Ties go to the lower beam, then to the lower token.  A NaN logit counts as -inf, infinite ones

@@ -89,13 +89,13 @@ __device__ __forceinline__ float bm_weights(const float (&x)[N], float m) {
 // Where they are too many (equal logits, all of the best in a few lanes) the waves take out their k
 // best one after another, and the four lists are merged.
 // ---------------------------------------------------------------------------
-#define BM_CAP 256                 // tokens that are ranked, one a thread
+#define BM_CAP 512                 // tokens that are ranked
 
 template <int DT, int EPT>
 __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
   typedef SvPiece<DT> P;
   __shared__ float2 list[BM_CAP];
-  static_assert(BM_CAP >= BM_WAVES * BM_MAX_K && BM_CAP <= 64 * BM_WAVES, "one a thread");
+  static_assert(BM_CAP >= BM_WAVES * BM_MAX_K, "the waves' lists");
   __shared__ float wm[BM_WAVES], wz[BM_WAVES], wt[BM_WAVES];
   __shared__ int found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -185,15 +185,15 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
   float2* out = a.lists + place * a.k;
   if (threadIdx.x == 0) a.sums[place] = make_float2(M, (wz[0] + wz[1]) + (wz[2] + wz[3]));
   if (count <= BM_CAP) {
-    const int t = threadIdx.x;
-    if (t < count) {
+#pragma unroll 1
+    for (int t = threadIdx.x; t < count; t += 64 * BM_WAVES) {
       const float2 own_t = list[t];
       int rank = 0;
+#pragma unroll 8
       for (int i = 0; i < count; ++i) rank += bm_before(list[i], own_t);
       if (rank < a.k) out[rank] = own_t;
-    } else if (t < a.k) {
-      out[t] = make_float2(-INFINITY, 0.f);
     }
+    if (threadIdx.x >= count && threadIdx.x < a.k) out[threadIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
   __syncthreads();                                  // the list is read, and used again
@@ -249,7 +249,6 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
 // closer than twice that and one of them is among the k, the sums of those rows are made again in 64
 // bits, and the order with them.
 // ---------------------------------------------------------------------------
-#define BM_PICK_WAVES 8
 #define BM_AHEAD 4
 #define BM_FEW 8
 // Of a sum, relative: a weight 2^t is off by |t| ln 2 2^-24 of its exponent's rounding (and as
@@ -268,13 +267,13 @@ __device__ __forceinline__ double bm_value(float score, float x, const BmRow& r,
 }
 
 // A row's weights in 64 bits, by the whole workgroup.
-template <int DT>
+template <int DT, int WAVES>
 __device__ double bm_exact_sum(const BeamArgs& a, int s, int b, float m, double* lds) {
   typedef SvPiece<DT> P;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const void* row = (const char*)a.logits + (s * a.req_stride + b * a.row_stride) * sv_size<DT>();
   double z[2] = {0.0, 0.0};
-  for (int64_t v0 = wave * 64 * P::N; v0 < a.V; v0 += BM_PICK_WAVES * 64 * P::N) {
+  for (int64_t v0 = wave * 64 * P::N; v0 < a.V; v0 += WAVES * 64 * P::N) {
     P p;
     p.load(row, (int)v0, a.V, lane, 0);
 #pragma unroll
@@ -288,53 +287,80 @@ __device__ double bm_exact_sum(const BeamArgs& a, int s, int b, float m, double*
   if (lane == 0) lds[wave] = mine;
   __syncthreads();
   double total = 0.0;
-  for (int w = 0; w < BM_PICK_WAVES; ++w) total += lds[w];
+  for (int w = 0; w < WAVES; ++w) total += lds[w];
   return total;
 }
 
 // LDS that lanes of one wave hand each other: operations of a wave are in order.
 __device__ __forceinline__ void bm_wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The k best of a row's lists, a list a lane with its first entries in head; how many there are.
-// Entries below the k-th best head are out; the few that are left count the ones before them.  -1
-// where they are more than the lanes.
-__device__ __forceinline__ int bm_merge_few(const BeamArgs& a, const float2* list, const float2 (&head)[BM_AHEAD],
-                                            float* heads, float2* few, float2* out, float M) {
-  const int lane = threadIdx.x & 63;
-  const float h = head[0].x;
-  heads[lane] = h;
-  bm_wave_lds();
-  int above = 0;
-#pragma unroll 4
-  for (int j = 0; j < 64; j += 4) {
-    const float4 o = *(const float4*)(heads + j);
-    above += (o.x > h) + (o.y > h) + (o.z > h) + (o.w > h);
+// The k best of a row's lists (`lists`: the first of them); how many there are.  At least k entries
+// reach the k-th best of the lists' first few, 3 k entries in all or more; what reaches that, mostly
+// little more than k, goes to LDS and counts the entries before it.  -1 where it is more than fits.
+#define BM_MANY 256
+#define BM_FIRSTS 256              // 3 k + lists at most
+#define BM_BATCH 10
+__device__ __forceinline__ int bm_merge_many(const BeamArgs& a, const float2* lists, float* firsts, float2* many,
+                                             float2* out, float M) {
+  const int lane = threadIdx.x & 63, q = min(ceil_div(3 * a.k, a.blocks), a.k), heads = a.blocks * q;
+  // all loads at once, here and below: they come from other XCDs' stores, a microsecond away
+  float h[BM_FIRSTS / 64];
+#pragma unroll
+  for (int u = 0; u < BM_FIRSTS / 64; ++u) {
+    const int e = min(lane + 64 * u, heads - 1), l = e / q;
+    h[u] = lists[l * a.k + e - l * q].x;
   }
-  // as -(largest of the negated): the k-th best head, or the lowest finite number
-  float from = -wave_top(above < a.k && h > -INFINITY ? -h : -INFINITY);
-  if (__popcll(__ballot(h > -INFINITY)) < a.k || !(from < INFINITY)) from = -3.402823466e38f;
+  int filled = 0;
+#pragma unroll
+  for (int u = 0; u < BM_FIRSTS / 64; ++u) {
+    if (lane + 64 * u >= heads) h[u] = -INFINITY;
+    firsts[lane + 64 * u] = h[u];
+    filled += __popcll(__ballot(h[u] > -INFINITY));
+  }
+  bm_wave_lds();
+  // as -(largest of the negated): the k-th best, or the lowest finite number
+  float least = -INFINITY;
+#pragma unroll 1
+  for (int e = lane; e < ceil_div(heads, 64) * 64; e += 64) {
+    const float h = firsts[e];
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < heads; j += 4) {
+      const float4 o = *(const float4*)(firsts + j);
+      above += (o.x > h) + (o.y > h) + (o.z > h) + (o.w > h);
+    }
+    if (above < a.k && h > -INFINITY) least = fmaxf(least, -h);
+  }
+  float from = -wave_top(least);
+  if (filled < a.k || !(from < INFINITY)) from = -3.402823466e38f;
   if (M == INFINITY) from = INFINITY;
   int n = 0;
-  float2 e = head[0];
+  const int all = a.blocks * a.k;
 #pragma unroll 1
-  for (int i = 0;;) {
-    const bool in = e.x >= from;
-    const uint64_t some = __ballot(in);
-    if (!some) break;
-    const int at = n + __popcll(some & ((1ull << lane) - 1));
-    if (in && at < 64) few[at] = e;
-    n += __popcll(some);
-    if (++i >= a.k) break;
-    if (!in) e.x = -INFINITY;
-    else e = i == 1 ? head[1] : i == 2 ? head[2] : i == 3 ? head[3] : list[i];
+  for (int e0 = lane; e0 - lane < all; e0 += 64 * BM_BATCH) {
+    float2 e[BM_BATCH];
+#pragma unroll
+    for (int u = 0; u < BM_BATCH; ++u) e[u] = lists[min(e0 + 64 * u, all - 1)];
+#pragma unroll
+    for (int u = 0; u < BM_BATCH; ++u) {
+      const bool in = e[u].x >= from && e0 + 64 * u < all;
+      const uint64_t some = __ballot(in);
+      if (!some) continue;
+      const int at = n + __popcll(some & ((1ull << lane) - 1));
+      if (in && at < BM_MANY) many[at] = e[u];
+      n += __popcll(some);
+    }
   }
-  if (n > 64) return -1;
+  if (n > BM_MANY) return -1;
   bm_wave_lds();
-  const float2 mine = few[lane < n ? lane : 0];
-  int rank = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) rank += bm_before(few[j], mine);
-  if (lane < n && rank < a.k) out[rank] = mine;
+#pragma unroll 1
+  for (int c = lane; c < n; c += 64) {
+    const float2 mine = many[c];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += bm_before(many[j], mine);
+    if (rank < a.k) out[rank] = mine;
+  }
   bm_wave_lds();
   return min(n, a.k);
 }
@@ -366,26 +392,29 @@ __device__ __forceinline__ int bm_merge(const BeamArgs& a, const float2* list, f
   return got;
 }
 
-template <int DT>
-__global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs a) {
+template <int DT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
   __shared__ double value[BM_MAX_BEAMS][BM_MAX_K];
   __shared__ float2 cand[BM_MAX_BEAMS][BM_MAX_K];
   __shared__ int count[BM_MAX_BEAMS];
   __shared__ BmRow rows[BM_MAX_BEAMS];
-  __shared__ double lds[BM_PICK_WAVES];
+  __shared__ double lds[WAVES];
   __shared__ int pick_b[BM_MAX_K], pick_t[BM_MAX_K];
   __shared__ int64_t stops[BM_MAX_K];
   __shared__ bool ended[BM_MAX_BEAMS];
   __shared__ double flat[64];                       // all values in a row, where they are few
   __shared__ int ranks[64], order[64];
+  __shared__ uint16_t line[BM_MAX_BEAMS * BM_MAX_K], place[BM_MAX_BEAMS * BM_MAX_K];    // where they are many
+  __shared__ double reach[BM_MAX_BEAMS * BM_MAX_K], least;
+  __shared__ int asked;
   __shared__ uint32_t near;                         // a bit a beam
-  __shared__ float heads[BM_PICK_WAVES][64];
-  __shared__ float2 few[BM_PICK_WAVES][64];
+  __shared__ __attribute__((aligned(16))) float firsts[WAVES][BM_FIRSTS];
+  __shared__ float2 many[WAVES][BM_MANY];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = blockIdx.x;
   if (tid == 0) near = 0;
   if (tid < BM_MAX_K) pick_b[tid] = -1;
   const int64_t own_stop = tid < min(a.stops, BM_MAX_K) ? a.stop[s * a.stop_stride + tid] : -1;
-  for (int b = wave; b < a.W; b += BM_PICK_WAVES) {
+  for (int b = wave; b < a.W; b += WAVES) {
     const int r = s * a.W + b;
     const int64_t first = (int64_t)r * a.blocks;
     const float2* list = a.lists + (first + lane) * a.k;
@@ -409,7 +438,7 @@ __global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs 
     const float M = wave_top(own.x);
     BmRow row = {M, wave_total(M > -INFINITY ? (double)own.y * bm_shift(own.x) * bm_weight(own.x, M) : 0.0)};
     int got = -1;
-    if (a.k >= BM_FEW && a.blocks >= a.k) got = bm_merge_few(a, list, head, heads[wave], few[wave], cand[b], M);
+    if (a.k >= BM_FEW) got = bm_merge_many(a, a.lists + first * a.k, firsts[wave], many[wave], cand[b], M);
     if (got < 0) got = bm_merge(a, list, head, cand[b], M);
     const double log_z = log(row.z);
     for (int i = lane; i < got; i += 64) value[b][i] = bm_value(score, cand[b][i].x, row, log_z);
@@ -429,13 +458,14 @@ __global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs 
         ranks[lane] = 0;
       }
       __syncthreads();
-      // a value a lane; every wave counts eight of the others
+      // a value a lane; every wave counts some of the others
       const double v = flat[lane];
       int before = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const double y = flat[wave * 8 + j];
-        before += y > v || (y == v && wave * 8 + j < lane);    // of one row the lists are in order
+      for (int j = 0; j < 64 / WAVES; ++j) {
+        const int o = wave * (64 / WAVES) + j;
+        const double y = flat[o];
+        before += y > v || (y == v && o < lane);    // of one row the lists are in order
       }
       if (before) atomicAdd(&ranks[lane], before);
       __syncthreads();
@@ -455,33 +485,66 @@ __global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs 
           if (bu != bd && !(ended[bu] && ended[bd])) atomicOr(&near, 1u << bu | 1u << bd);
         }
       }
-    } else
-    for (int c = tid; c < all; c += 64 * BM_PICK_WAVES) {
-      const int b = c / a.k, i = c - b * a.k;
-      if (i >= count[b]) continue;
-      const double v = value[b][i];
-      const bool over = ended[b];
-      int rank = i;
-      uint32_t close = 0;
-      for (int o = 0; o < a.W; ++o) {
-        if (o == b) continue;
-        // values of row o before this one
-        int lo = 0, hi = count[o];
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          const double y = value[o][mid];
-          if (y > v || (y == v && o < b)) lo = mid + 1;
-          else hi = mid;
-        }
-        rank += lo;
-        const bool tight = (lo > 0 && value[o][lo - 1] - v <= 2 * BM_ERR) ||
-                           (lo < count[o] && v - value[o][lo] <= 2 * BM_ERR);
-        if (tight && !(over && ended[o])) close |= 1u << o | 1u << b;
+    } else {
+      // the k-th best of the rows' first few values, 3 k in all or more: what reaches that, or
+      // stands close below, is in question
+      const int q = min((3 * a.k + a.W - 1) / a.W, a.k), firsts_n = a.W * q;
+      if (tid < firsts_n) {
+        const int b = tid / q, i = tid - b * q;
+        reach[tid] = i < count[b] ? value[b][i] : -INFINITY;
       }
-      if (rank >= a.k) continue;
-      pick_b[rank] = b;
-      pick_t[rank] = i;
-      if (turn == 0 && close) atomicOr(&near, close);
+      if (tid == 0) {
+        asked = 0;
+        least = -INFINITY;
+      }
+      __syncthreads();
+      if (tid < firsts_n) {
+        const double v = reach[tid];
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < firsts_n; ++j) above += reach[j] > v || (reach[j] == v && j < tid);
+        if (above == a.k - 1) least = v;
+      }
+      __syncthreads();
+      const double from = least - 4 * BM_ERR;
+      __syncthreads();
+      for (int c = tid; c < all; c += 64 * WAVES) {
+        const int b = c / a.k, i = c - b * a.k;
+        const double v = i < count[b] ? value[b][i] : -INFINITY;
+        if (v > -INFINITY && v >= from) {
+          const int x = atomicAdd(&asked, 1);
+          line[x] = (uint16_t)c;
+          reach[x] = v;
+        }
+      }
+      __syncthreads();
+      const int n = asked;
+      for (int x = tid; x < n; x += 64 * WAVES) {
+        const int c = line[x];
+        const double v = reach[x];
+        int rank = 0;
+#pragma unroll 8
+        for (int y = 0; y < n; ++y) rank += reach[y] > v || (reach[y] == v && line[y] < c);
+        place[rank] = (uint16_t)c;
+      }
+      __syncthreads();
+      auto at = [&](int r) {
+        const int c = place[r], b = c / a.k;
+        return value[b][c - b * a.k];
+      };
+      const double vk = n ? at(min(a.k, n) - 1) : 0.0;
+      for (int r = tid; r < n; r += 64 * WAVES) {
+        const int bu = place[r] / a.k;
+        if (r < a.k) {
+          pick_b[r] = bu;
+          pick_t[r] = place[r] - bu * a.k;
+        }
+        // next to one another, of two rows, and one of them may be among the k
+        if (turn == 0 && r + 1 < n && at(r) - at(r + 1) <= 2 * BM_ERR && vk - at(r + 1) <= 2 * BM_ERR) {
+          const int bd = place[r + 1] / a.k;
+          if (bu != bd && !(ended[bu] && ended[bd])) atomicOr(&near, 1u << bu | 1u << bd);
+        }
+      }
     }
     __syncthreads();
     const uint32_t again = turn ? 0 : near;
@@ -489,15 +552,15 @@ __global__ __launch_bounds__(64 * BM_PICK_WAVES) void beam_pick_kernel(BeamArgs 
     for (int b = 0; b < a.W; ++b) {
       if (!(again >> b & 1) || ended[b]) continue;
       BmRow row = rows[b];
-      row.z = bm_exact_sum<DT>(a, s, b, row.m, lds);
+      row.z = bm_exact_sum<DT, WAVES>(a, s, b, row.m, lds);
       const double log_z = log(row.z);
       const float score = a.scores[s * a.W + b];
-      for (int i = tid; i < count[b]; i += 64 * BM_PICK_WAVES)
+      for (int i = tid; i < count[b]; i += 64 * WAVES)
         value[b][i] = bm_value(score, cand[b][i].x, row, log_z);
     }
     __syncthreads();
   }
-  for (int j = tid; j < a.k; j += 64 * BM_PICK_WAVES) {
+  for (int j = tid; j < a.k; j += 64 * WAVES) {
     const int b = pick_b[j];
     int64_t t = -1;
     bool over = true;
@@ -572,10 +635,17 @@ extern "C" int omni_beam_select(const void* logits, int dtype, int64_t req_strid
   }
 #undef BM_SCAN
   OMNI_CHECK_LAUNCH();
-  const dim3 picks(64 * BM_PICK_WAVES);
-  if (dtype == 0) hipLaunchKernelGGL(beam_pick_kernel<0>, dim3(n), picks, 0, st, a);
-  else if (dtype == 1) hipLaunchKernelGGL(beam_pick_kernel<1>, dim3(n), picks, 0, st, a);
-  else hipLaunchKernelGGL(beam_pick_kernel<2>, dim3(n), picks, 0, st, a);
+#define BM_PICK(DT)                                                                                      \
+  if (beams > 8) hipLaunchKernelGGL((beam_pick_kernel<DT, 16>), dim3(n), dim3(64 * 16), 0, st, a);       \
+  else hipLaunchKernelGGL((beam_pick_kernel<DT, 8>), dim3(n), dim3(64 * 8), 0, st, a);
+  if (dtype == 0) {
+    BM_PICK(0)
+  } else if (dtype == 1) {
+    BM_PICK(1)
+  } else {
+    BM_PICK(2)
+  }
+#undef BM_PICK
   OMNI_CHECK_LAUNCH();
   return OMNI_OK;
 }

@@ -248,6 +248,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedArgs 
     it.end = own ? keys : S * PA_UNIT;
     it.table = (const plan_int*)(a.tables + (int64_t)i * a.width);
     const int units = ceil_div(it.end - it.keys0, PA_UNIT), steps = min(left, units - u0);
+    if (steps <= 0) break;                          // no schedule of omni_page_reserve's
     const int from = it.keys0 + u0 * PA_UNIT, to = min(from + steps * PA_UNIT, it.end);
     const int queries = it.rows * it.heads;
     const bool whole = own && !S && u0 == 0 && steps == units;
@@ -329,6 +330,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedArgs 
         int next = i;
         do ++next;
         while (next < a.n - 1 && schedule[8 * next] == 0);
+        if (next >= a.n) break;
         const plan_int* after = schedule + 8 * next;
         item = 2 * next + (after[1] && after[2] == next ? 0 : 1);
       } else {

@@ -74,9 +74,9 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
 
 // Set the bits of the pages that sequences hold; held(row, but) gives how many of a row's entries
 // count and, for FORK, which one of them does not.  2^group lanes a row, four entries a lane at a
-// time.  common[row] of the first n rows becomes the number of entries before the first one that the
+// time.  For COMMON, common[row] of the first n rows becomes the number of entries before the first one that the
 // row above has otherwise, of those that both hold (it comes as that many or more).
-template <bool FORK, typename Held>
+template <bool FORK, bool COMMON, typename Held>
 __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held,
                                         int* common = nullptr, int n = 0) {
   const int lanes = 1 << group, l = threadIdx.x & (lanes - 1);
@@ -86,7 +86,7 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
     const int count = held(row, but);
     const int* entry = t.tables + (int64_t)row * t.width;
     int both = 0;
-    if (common && row && row < n) {
+    if (COMMON && row && row < n) {
       int x;
       both = min(count, held(row - 1, x));
     }
@@ -94,7 +94,7 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
     for (int j0 = 4 * l; j0 < count; j0 += 16 * lanes) {
       i32x4 p[4], above[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < (COMMON ? 4 : 0); ++u) {
         const int j = j0 + 4 * lanes * u;
         above[u] = (i32x4){-1, -1, -1, -1};
         if (j + 4 <= both) {
@@ -126,7 +126,7 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
           if (FORK) in &= j0 + 4 * lanes * u + e != but;
           if (in) atomicOr(&used[x >> 5], 1u << (x & 31));
         }
-      if (j0 < both) {
+      if (COMMON && j0 < both) {
         int other = both;
 #pragma unroll
         for (int u = 3; u >= 0; --u)
@@ -285,9 +285,9 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
     if (i < r.n) ends[i] = pages;
     __syncthreads();                                // the sums are read
   }
-  pg_mark<false>(t, used, r.group, [&](int row, int& but) {
-    return pg_pages(t, pg_length(t, row));
-  }, r.schedule && r.most > 1 && r.n > 1 ? common : nullptr, r.n);
+  auto held = [&](int row, int& but) { return pg_pages(t, pg_length(t, row)); };
+  if (r.schedule && r.most > 1 && r.n > 1) pg_mark<false, true>(t, used, r.group, held, common, r.n);
+  else pg_mark<false, false>(t, used, r.group, held);
   __syncthreads();
   const PgShare own(t);
   int first;
@@ -460,17 +460,19 @@ static int pg_tables_ok(const int* tables, const int64_t* lengths, int seqs, int
   return OMNI_OK;
 }
 
-// Workgroups of these kernels may take more dynamic LDS than a launch allows by default.
+// Workgroups of these kernels may take more dynamic LDS than a launch allows by default; said once
+// per device.
 static int pg_allow_lds() {
-  static const int rc = [] {
-    hipError_t e = hipSuccess;
-    for (const void* k : {(const void*)page_reserve_kernel, (const void*)page_fork_kernel<false>,
-                          (const void*)page_fork_kernel<true>, (const void*)page_gather_kernel})
-      if (e == hipSuccess)
-        e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 152 << 10);
-    return (int)e;
-  }();
-  return rc;
+  static bool said[64];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return (int)e;
+  if (dev >= 0 && dev < 64 && said[dev]) return OMNI_OK;
+  for (const void* k : {(const void*)page_reserve_kernel, (const void*)page_fork_kernel<false>,
+                        (const void*)page_fork_kernel<true>, (const void*)page_gather_kernel})
+    if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 152 << 10);
+  if (e == hipSuccess && dev >= 0 && dev < 64) said[dev] = true;
+  return (int)e;
 }
 
 // How many tokens the slots are written for by the workgroup that deals the pages.
@@ -499,7 +501,8 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
                    token_pos, positions, granted, cu, schedule, columns, most, pg_group(seqs),
                    tokens <= PG_SLOTS_HERE};
   const size_t smem = 4 * ((size_t)(pages + 31) / 32 + (dense ? 8 : 4) * (size_t)n);
-  if (smem > (32 << 10) && pg_allow_lds()) return pg_allow_lds();
+  if (smem > (32 << 10))
+    if (const int e = pg_allow_lds()) return e;
   hipLaunchKernelGGL(page_reserve_kernel, dim3(1), dim3(PG_THREADS), smem, (hipStream_t)stream, t, r);
   OMNI_CHECK_LAUNCH();
   if (!dense && !r.slots_here) {
@@ -595,7 +598,7 @@ __global__ __launch_bounds__(PG_THREADS) void page_fork_kernel(PageTables t, con
       }
     }
   }
-  pg_mark<true>(t, used, group, [&](int row, int& but) {
+  pg_mark<true, false>(t, used, group, [&](int row, int& but) {
     if (row >= rows) return pg_pages(t, pg_length(t, row));
     if (HERE) return 0;
     const int v = len[row], L = v < 0 ? ~v : v;

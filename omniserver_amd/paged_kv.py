@@ -79,7 +79,7 @@ class PagedKVCache:
         self.tables = torch.zeros(max_seqs, -(-max_len // page_size), device=device,
                                   dtype=torch.int32)
         self.lengths = torch.zeros(max_seqs, device=device, dtype=torch.int64)
-        self._step = 0             # the newest reservation, or reorder, of pages
+        self._step = 0             # counts what may give pages away
 
     def _geometry(self) -> tuple:
         return (self.tables.data_ptr(), self.lengths.data_ptr(), self.max_seqs,
@@ -105,6 +105,7 @@ class PagedKVCache:
     def free(self, rows: Sequence[int]) -> None:
         """Forget the sequences ``rows``; pages that no other one holds are free."""
         rows = self._checked_rows(rows)
+        self._step += 1
         if rows:
             self.lengths.index_fill_(0, to_device(rows, torch.int64, self.device), 0)
 
@@ -236,7 +237,8 @@ class PageSlots:
 
     def _current(self) -> None:
         if self._step != self.pool._step:
-            raise RuntimeError("a later reservation or reordering may have given these pages away")
+            raise RuntimeError("a later reservation, reordering or freeing of sequences may have given "
+                               "these pages away")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, layer_idx: int) -> None:
         """K/V rows [T, n_kv_heads, head_dim] of the packed tokens to their places."""
@@ -297,9 +299,9 @@ class PagedPrefill(PageSlots):
     def __init__(self, pool: PagedKVCache, rows: Sequence[int], seg_lengths: Sequence[int]):
         if pool.storage.dtype != torch.float16 or pool.head_dim != 128:
             raise ValueError("prompts are for fp16 pages of head_dim 128")
-        seg = [int(L) for L in seg_lengths]
+        rows, seg = list(rows), [int(L) for L in seg_lengths]
         if not seg or len(seg) != len(rows) or any(not 1 <= L <= pool.max_len for L in seg):
-            raise ValueError(f"prompts of {seg} tokens for rows {list(rows)}: 1 to {pool.max_len} each")
+            raise ValueError(f"prompts of {seg} tokens for rows {rows}: 1 to {pool.max_len} each")
         pool.free(rows)
         super().__init__(pool, seg, rows)
         one = PreallocatedKVCache(1, len(seg), pool.n_kv_heads, max(seg), 128, pool.device,

@@ -667,6 +667,11 @@ def test_superseded_reservations(gpu):
     with pytest.raises(RuntimeError, match="later"):
         third.finish()
     assert cache.lengths.tolist() == [22, 22, 10]
+    fourth = cache.decode_cache(3)
+    cache.free([1])
+    with pytest.raises(RuntimeError, match="later"):
+        fourth.finish()
+    assert cache.lengths.tolist() == [22, 0, 10]
 
 
 # ----------------------------------------------------------------------------- the model
