@@ -250,7 +250,6 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
 // bits, and the order with them.
 // ---------------------------------------------------------------------------
 #define BM_AHEAD 4
-#define BM_FEW 8
 // Of a sum, relative: a weight 2^t is off by |t| ln 2 2^-24 of its exponent's rounding (and as
 // much of the difference's, or log2 e's), 2^-23 of its exponential; |t| up to 30 counts (2^19 tokens
 // 2^-30 weigh 2^-11), and EPT / 4 + 9 additions are off by 2^-24 each: 4e-6.
@@ -294,78 +293,10 @@ __device__ double bm_exact_sum(const BeamArgs& a, int s, int b, float m, double*
 // LDS that lanes of one wave hand each other: operations of a wave are in order.
 __device__ __forceinline__ void bm_wave_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The k best of a row's lists (`lists`: the first of them); how many there are.  At least k entries
-// reach the k-th best of the lists' first few, 3 k entries in all or more; what reaches that, mostly
-// little more than k, goes to LDS and counts the entries before it.  -1 where it is more than fits.
-#define BM_MANY 256
-#define BM_FIRSTS 256              // 3 k + lists at most
-#define BM_BATCH 10
-__device__ __forceinline__ int bm_merge_many(const BeamArgs& a, const float2* lists, float* firsts, float2* many,
-                                             float2* out, float M) {
-  const int lane = threadIdx.x & 63, q = min(ceil_div(3 * a.k, a.blocks), a.k), heads = a.blocks * q;
-  // all loads at once, here and below: they come from other XCDs' stores, a microsecond away
-  float h[BM_FIRSTS / 64];
-#pragma unroll
-  for (int u = 0; u < BM_FIRSTS / 64; ++u) {
-    const int e = min(lane + 64 * u, heads - 1), l = e / q;
-    h[u] = lists[l * a.k + e - l * q].x;
-  }
-  int filled = 0;
-#pragma unroll
-  for (int u = 0; u < BM_FIRSTS / 64; ++u) {
-    if (lane + 64 * u >= heads) h[u] = -INFINITY;
-    firsts[lane + 64 * u] = h[u];
-    filled += __popcll(__ballot(h[u] > -INFINITY));
-  }
-  bm_wave_lds();
-  // as -(largest of the negated): the k-th best, or the lowest finite number
-  float least = -INFINITY;
-#pragma unroll 1
-  for (int e = lane; e < ceil_div(heads, 64) * 64; e += 64) {
-    const float h = firsts[e];
-    int above = 0;
-#pragma unroll 4
-    for (int j = 0; j < heads; j += 4) {
-      const float4 o = *(const float4*)(firsts + j);
-      above += (o.x > h) + (o.y > h) + (o.z > h) + (o.w > h);
-    }
-    if (above < a.k && h > -INFINITY) least = fmaxf(least, -h);
-  }
-  float from = -wave_top(least);
-  if (filled < a.k || !(from < INFINITY)) from = -3.402823466e38f;
-  if (M == INFINITY) from = INFINITY;
-  int n = 0;
-  const int all = a.blocks * a.k;
-#pragma unroll 1
-  for (int e0 = lane; e0 - lane < all; e0 += 64 * BM_BATCH) {
-    float2 e[BM_BATCH];
-#pragma unroll
-    for (int u = 0; u < BM_BATCH; ++u) e[u] = lists[min(e0 + 64 * u, all - 1)];
-#pragma unroll
-    for (int u = 0; u < BM_BATCH; ++u) {
-      const bool in = e[u].x >= from && e0 + 64 * u < all;
-      const uint64_t some = __ballot(in);
-      if (!some) continue;
-      const int at = n + __popcll(some & ((1ull << lane) - 1));
-      if (in && at < BM_MANY) many[at] = e[u];
-      n += __popcll(some);
-    }
-  }
-  if (n > BM_MANY) return -1;
-  bm_wave_lds();
-#pragma unroll 1
-  for (int c = lane; c < n; c += 64) {
-    const float2 mine = many[c];
-    int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) rank += bm_before(many[j], mine);
-    if (rank < a.k) out[rank] = mine;
-  }
-  bm_wave_lds();
-  return min(n, a.k);
-}
-
-// The same, one entry after another.
+// The k best of a row's lists, a list a lane with its first entries in head, one after another; how
+// many there are.  (Counting, among the entries that reach the k-th best of the lists' first ones, those
+// before each, costs more fetched code than it saves: 1 x 4 beams, k = 4 13.1 us a call, this 11.5; 1 x 8,
+// k = 16 23.4 and 22.2; only 8 x 16, k = 32 47.3 and 49.5.)
 __device__ __forceinline__ int bm_merge(const BeamArgs& a, const float2* list, float2 (&head)[BM_AHEAD],
                                         float2* out, float M) {
   const int lane = threadIdx.x & 63;
@@ -408,8 +339,6 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
   __shared__ double reach[BM_MAX_BEAMS * BM_MAX_K], least;
   __shared__ int asked;
   __shared__ uint32_t near;                         // a bit a beam
-  __shared__ __attribute__((aligned(16))) float firsts[WAVES][BM_FIRSTS];
-  __shared__ float2 many[WAVES][BM_MANY];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = blockIdx.x;
   if (tid == 0) near = 0;
   if (tid < BM_MAX_K) pick_b[tid] = -1;
@@ -437,9 +366,7 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
     }
     const float M = wave_top(own.x);
     BmRow row = {M, wave_total(M > -INFINITY ? (double)own.y * bm_shift(own.x) * bm_weight(own.x, M) : 0.0)};
-    int got = -1;
-    if (a.k >= BM_FEW) got = bm_merge_many(a, a.lists + first * a.k, firsts[wave], many[wave], cand[b], M);
-    if (got < 0) got = bm_merge(a, list, head, cand[b], M);
+    const int got = bm_merge(a, list, head, cand[b], M);
     const double log_z = log(row.z);
     for (int i = lane; i < got; i += 64) value[b][i] = bm_value(score, cand[b][i].x, row, log_z);
     if (lane == 0) {

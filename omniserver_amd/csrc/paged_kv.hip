@@ -11,6 +11,8 @@
 #define PG_WAVES (PG_THREADS / 64)
 #define PG_MAX_PAGES (1 << 19)     // a bit each in LDS: 64 KB
 #define PG_MAX_SEQS 2048
+#define PG_TILE 16384              // table entries that the dealing workgroup moves itself
+#define PG_LDS (152 << 10)
 
 struct PageTables {
   int* tables;             // [seqs][width]
@@ -470,7 +472,7 @@ static int pg_allow_lds() {
   if (dev >= 0 && dev < 64 && said[dev]) return OMNI_OK;
   for (const void* k : {(const void*)page_reserve_kernel, (const void*)page_fork_kernel<false>,
                         (const void*)page_fork_kernel<true>, (const void*)page_gather_kernel})
-    if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, 152 << 10);
+    if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, PG_LDS);
   if (e == hipSuccess && dev >= 0 && dev < 64) said[dev] = true;
   return (int)e;
 }
@@ -522,7 +524,6 @@ extern "C" int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int wi
 // and new pages, one workgroup; the copies.
 // ---------------------------------------------------------------------------
 #define PG_COLS 16
-#define PG_TILE 8192               // table entries that one workgroup moves
 
 __global__ __launch_bounds__(256) void page_gather_kernel(PageTables t, const int* __restrict__ parents,
                                                           int rows, int W) {
@@ -657,8 +658,9 @@ extern "C" int omni_page_reorder(void* pool, int n_layers, int row_halfs, int* t
   const PageTables t = {tables, lengths, seqs, width, pages, pg_shift(page_size), max_len};
   hipStream_t st = (hipStream_t)stream;
   if (const int e = pg_allow_lds()) return e;
-  const bool here = (int64_t)rows * width <= PG_TILE;
-  const size_t smem = 4 * ((size_t)(pages + 31) / 32 + 4 * (size_t)rows + (here ? (size_t)rows * width : 0));
+  const size_t base = 4 * ((size_t)(pages + 31) / 32 + 4 * (size_t)rows), tile = 4 * (size_t)rows * width;
+  const bool here = tile <= 4 * PG_TILE && base + tile <= PG_LDS;
+  const size_t smem = here ? base + tile : base;
   const int group = pg_group(seqs);
   if (here) {
     hipLaunchKernelGGL(page_fork_kernel<true>, dim3(1), dim3(PG_THREADS), smem, st, t, parents, rows,
