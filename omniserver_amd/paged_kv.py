@@ -84,10 +84,22 @@ class PagedKVCache:
                                   dtype=torch.int32)
         self.lengths = torch.zeros(max_seqs, device=device, dtype=torch.int64)
         self._step = 0             # counts what may give pages away
+        self._plans = {}
 
     def _geometry(self) -> tuple:
         return (self.tables.data_ptr(), self.lengths.data_ptr(), self.max_seqs,
                 self.tables.shape[1], self.num_pages, self.page_size, self.max_len)
+
+    def _attention_plan(self, n: int) -> tuple:
+        """(columns, rows taken together, floats of split states) for n sequences."""
+        plan = self._plans.get(n)
+        if plan is None:
+            columns = attention_columns(n, self.n_heads, self.n_kv_heads, self.max_len,
+                                        num_cus(self.device))
+            most = attention_group(self.n_heads, self.n_kv_heads)
+            states = columns + n + (columns * most + n if most > 1 else 0)
+            plan = self._plans[n] = (columns, most, states * self.n_heads * (self.head_dim + 4))
+        return plan
 
     # ---- room for new tokens ---------------------------------------------------------
     def reserve(self, counts, rows: Sequence[int] | None = None,
@@ -160,7 +172,8 @@ class PageSlots:
     object, so two captured graphs never share them."""
 
     def __init__(self, pool: PagedKVCache, counts, rows=None, tokens=None, dense: bool = False,
-                 n: int | None = None, rope_delta=None, columns: int = 0, most: int = 0):
+                 n: int | None = None, rope_delta=None, columns: int = 0, most: int = 0,
+                 floats: int = 0):
         dev = pool.device
         if rows is not None:
             rows = pool._checked_rows(rows)
@@ -188,15 +201,18 @@ class PageSlots:
         require_here(pool.lengths, self.counts, rope_delta)
         self.pool, self.n, self.T = pool, n, T
         self._axes = axes = 3 if dense else 1
-        # int64: starts, lengths after, pages, places, positions; int32: granted, sums of rows, and
-        # the attention's schedule on a 16-byte boundary
+        # int64: starts, lengths after, pages, places, positions; int32: granted, sums of rows; on
+        # 16-byte boundaries the attention's schedule, int32, and its split states, fp32 (for all layers:
+        # launches on one stream are ordered)
         words = 2 * n + (2 + axes) * T
         ints = 2 * n + 1 + (-(2 * words + 2 * n + 1) % 4)
-        self._plan = torch.empty(words + (ints + (8 * n + 4 * columns if columns else 0) + 1) // 2,
-                                 device=dev, dtype=torch.int64)
+        more = 8 * n + 4 * columns if columns else 0
+        self._plan = torch.empty(words + (ints + more + floats + 1) // 2, device=dev,
+                                 dtype=torch.int64)
         p = self._plan.data_ptr()
         self._granted = p + 8 * words
         self._schedule = self._granted + 4 * ints if columns else None
+        self._states = self._granted + 4 * (ints + more)
         self._page, self._place = p + 16 * n, p + 16 * n + 8 * T
         pool._step += 1
         self._step = pool._step
@@ -361,15 +377,9 @@ class PagedDecode(PageSlots):
     def __init__(self, pool: PagedKVCache, n: int, counts=None, rope_delta=None):
         if not 1 <= n <= pool.max_seqs:
             raise ValueError(f"{n} sequences, the cache has {pool.max_seqs}")
-        self._columns = attention_columns(n, pool.n_heads, pool.n_kv_heads, pool.max_len,
-                                          num_cus(pool.device))
-        self._most = most = attention_group(pool.n_heads, pool.n_kv_heads)
-        super().__init__(pool, counts, dense=True, n=n, rope_delta=rope_delta,
-                         columns=self._columns, most=most)
-        # the attention's split states, for all layers (launches on one stream are ordered)
-        states = self._columns + n + (self._columns * most + n if most > 1 else 0)
-        self._ws = torch.empty(states * pool.n_heads * (pool.head_dim + 4), device=pool.device,
-                               dtype=torch.float32)
+        self._columns, self._most, self._floats = pool._attention_plan(n)
+        super().__init__(pool, counts, dense=True, n=n, rope_delta=rope_delta, columns=self._columns,
+                         most=self._most, floats=self._floats)
 
     @property
     def positions(self) -> torch.Tensor:
@@ -402,7 +412,7 @@ class PagedDecode(PageSlots):
              pool.v[layer_idx].data_ptr(), _DTYPES[pool.storage.dtype], pool.num_pages,
              pool.page_size, pool.tables.data_ptr(), pool.tables.shape[1], self.n, self._schedule,
              self._columns, self._most, out.data_ptr(), nh * hd, nh, pool.n_kv_heads, hd, float(scale),
-             self._ws.data_ptr(), self._ws.numel(), stream())
+             self._states, self._floats, stream())
         return out
 
     def flash_decode(self, q, key, value, layer_idx, scale):
