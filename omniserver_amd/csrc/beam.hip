@@ -254,7 +254,7 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
 // closer than twice that and one of them is among the k, the sums of those rows are made again in 64
 // bits, and the order with them.
 //
-// A chain of waits: 4 beams, k = 4, 6.5 us; 5 beams, k = 10, 8.5.  Loads of the lists and sums (1 us),
+// A chain of waits: 4 beams, k = 4, 5.9 us; 5 beams, k = 10, 7.8.  Loads of the lists and sums (1 us),
 // sums and logarithm in 64 bits (1), k entries (0.2 each), the count (1.3).  Sixteen waves where the beams
 // are more than eight: 12 beams, k = 12 21.2 us a call, with eight 24.4; 8 x 16, k = 32 47 and 52.
 // ---------------------------------------------------------------------------

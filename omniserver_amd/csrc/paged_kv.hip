@@ -83,6 +83,7 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
 template <bool FORK, bool COMMON, typename Held>
 __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held,
                                         int* common = nullptr, int n = 0) {
+  constexpr int DEEP = 4;                           // loads of a lane under way; 8 took no less
   const int lanes = 1 << group, l = threadIdx.x & (lanes - 1);
 #pragma unroll 1
   for (int row = threadIdx.x >> group; row < t.seqs; row += PG_THREADS >> group) {
@@ -94,51 +95,37 @@ __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int
       int x;
       both = min(count, held(row - 1, x));
     }
+    auto take = [&](int j, int x, int above) {
+      bool in = j < count && (unsigned)x < (unsigned)t.pages;
+      if (FORK) in &= j != but;
+      if (in) atomicOr(&used[x >> 5], 1u << (x & 31));
+      return COMMON && j < both && x != above;
+    };
+    if (t.width < 4) {
+      for (int j = l; j < count; j += lanes)
+        if (take(j, entry[j], j < both ? entry[j - t.width] : 0)) atomicMin(&common[row], j);
+      continue;
+    }
+    // whole pieces of the row, the last ones moved back into it: an entry may come twice
 #pragma unroll 1
-    for (int j0 = 4 * l; j0 < count; j0 += 16 * lanes) {
-      i32x4 p[4], above[4];
+    for (int j0 = 4 * l; j0 < count; j0 += 4 * DEEP * lanes) {
+      i32x4 p[DEEP], above[DEEP];
 #pragma unroll
-      for (int u = 0; u < (COMMON ? 4 : 0); ++u) {
-        const int j = j0 + 4 * lanes * u;
-        above[u] = (i32x4){-1, -1, -1, -1};
-        if (j + 4 <= both) {
-          __builtin_memcpy(&above[u], entry - t.width + j, 16);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (j + e < both) above[u][e] = entry[j + e - t.width];
-        }
+      for (int u = 0; u < DEEP; ++u) {
+        const int j = min(j0 + 4 * lanes * u, t.width - 4);
+        __builtin_memcpy(&p[u], entry + j, 16);
+        if (COMMON) __builtin_memcpy(&above[u], entry - (row ? t.width : 0) + j, 16);
       }
+      int other = both;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = j0 + 4 * lanes * u;
-        p[u] = (i32x4){-1, -1, -1, -1};
-        if (j + 4 <= count) {
-          __builtin_memcpy(&p[u], entry + j, 16);
-        } else {
+      for (int u = DEEP - 1; u >= 0; --u) {
+        const int from = j0 + 4 * lanes * u, j = min(from, t.width - 4);
+        if (from >= count) continue;
 #pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (j + e < count) p[u][e] = entry[j + e];
-        }
+        for (int e = 3; e >= 0; --e)
+          if (take(j + e, p[u][e], COMMON ? above[u][e] : 0)) other = min(other, j + e);
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = p[u][e];
-          bool in = (unsigned)x < (unsigned)t.pages;
-          if (FORK) in &= j0 + 4 * lanes * u + e != but;
-          if (in) atomicOr(&used[x >> 5], 1u << (x & 31));
-        }
-      if (COMMON && j0 < both) {
-        int other = both;
-#pragma unroll
-        for (int u = 3; u >= 0; --u)
-#pragma unroll
-          for (int e = 3; e >= 0; --e)
-            if (p[u][e] != above[u][e]) other = min(other, j0 + 4 * lanes * u + e);
-        if (other < both) atomicMin(&common[row], other);
-      }
+      if (COMMON && other < both) atomicMin(&common[row], other);
     }
   }
 }
@@ -200,8 +187,8 @@ __device__ __forceinline__ void pg_deal(const PgShare& own, const uint32_t* used
 // One workgroup: bits of the held pages, how many are free below each, then every free page of
 // low enough rank goes to the request whose sum of new pages it falls into.  What it takes is a chain:
 // fetched code, loads of lengths and tables (1 us each from other XCDs' stores), sums over the
-// workgroup.  32 tokens behind 2048 6.2 us (half of it before the pages are counted); 384 requests among
-// 512 sequences of up to 4096 tokens 20, of which marking 65000 entries in LDS takes 11.  Bits in LDS
+// workgroup.  32 tokens behind 2048 5.8 us (half of it before the pages are counted); 384 requests among
+// 512 sequences of up to 4096 tokens 16.5, most of it the marks of 65000 entries in LDS.  Bits in LDS
 // rather than counts kept in memory: nothing has to be given back, and a captured step can be repeated.
 //
 // And the attention's schedule for single tokens (paged_attn.hip).  Neighbouring sequences whose
