@@ -78,8 +78,8 @@ __device__ __forceinline__ int pg_find(const int* ends, int n, int x) {
 
 // Set the bits of the pages that sequences hold; held(row, but) gives how many of a row's entries
 // count and, for FORK, which one of them does not.  2^group lanes a row, four entries a lane at a
-// time.  For COMMON, common[row] of the first n rows becomes the number of entries before the first one that the
-// row above has otherwise, of those that both hold (it comes as that many or more).
+// time.  For COMMON, common[row] of the first n rows becomes the number of entries before the first
+// one that the row above has otherwise, of those that both hold (it comes as that many or more).
 template <bool FORK, bool COMMON, typename Held>
 __device__ __forceinline__ void pg_mark(const PageTables& t, uint32_t* used, int group, Held held,
                                         int* common = nullptr, int n = 0) {

@@ -674,6 +674,29 @@ def test_superseded_reservations(gpu):
     assert cache.lengths.tolist() == [22, 0, 10]
 
 
+def test_prompts_short_of_pages(gpu):
+    """Prompts whose pages are not there are attended to like the others and leave nothing behind; rows
+    that held something before are begun anew; more packed rows than tokens."""
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    from omniserver_amd.paged_kv import PagedKVCache
+    cache = PagedKVCache(1, 4, 2, 16, 128, gpu, max_seqs=5, max_len=40, n_heads=12)
+    cache.reserve([40, 3], rows=[1, 4]).finish()                 # all four pages
+    assert cache.lengths.tolist() == [0, 40, 0, 0, 3]
+    pool = PreallocatedKVCache(1, 3, 2, 40, 128, gpu, n_heads=12)
+    g = torch.Generator().manual_seed(3)
+    lens, T = [20, 30, 10], 60
+    q, k, v = (torch.randn(T, h, 128, generator=g).half().to(gpu) for h in (12, 2, 2))
+    want = pool.packed_prefill_cache(range(3), lens).flash_prefill(q, k, v, 0, 0.1)
+    prompts = cache.prefill_cache([1, 0, 3], lens)               # row 1's three pages are free for it
+    assert prompts.granted.tolist() == [20, 0, 0]
+    assert torch.equal(prompts.flash_prefill(q, k, v, 0, 0.1), want)
+    assert cache.lengths.tolist() == [0, 20, 0, 0, 3]
+    kk, vv = tokens_of(cache.storage.cpu(), 0, cache.tables[1].tolist(), 20, 16)
+    assert torch.equal(kk, k[:20].cpu()) and torch.equal(vv, v[:20].cpu())
+    more = cache.reserve([2, 1], rows=[1, 4], tokens=6)
+    assert more.token_pos.tolist() == [4, 5, 3, -1, -1, -1] and more.granted.tolist() == [2, 1]
+
+
 # ----------------------------------------------------------------------------- the model
 @pytest.mark.parametrize("quant", [None, "gptq"])
 def test_model_over_pages(gpu, quant):
