@@ -286,6 +286,27 @@ class PageSlots:
             self.pool.lengths.index_copy_(0, self.rows, self.after)
 
     # ---- the adapters' protocol ------------------------------------------------------
+    def _check_rows(self, qkv: torch.Tensor, heads: int, out: torch.Tensor | None = None) -> None:
+        """Rows of a projection with the first ``heads`` heads, and a place for the attention's."""
+        pool = self.pool
+        width = heads * pool.head_dim
+        if qkv.dim() != 2 or qkv.shape[0] != self.T or qkv.shape[1] < width or qkv.stride(1) != 1:
+            raise ValueError(f"rows of shape {tuple(qkv.shape)}: expected [{self.T}, >= {width}] with "
+                             f"contiguous columns")
+        if qkv.dtype != pool.storage.dtype or (out is not None and out.dtype != qkv.dtype):
+            raise TypeError(f"the pages are {pool.storage.dtype} (got {qkv.dtype}"
+                            f"{'' if out is None else f' -> {out.dtype}'})")
+        if out is not None and (out.numel() != self.T * width or not out.is_contiguous()):
+            raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
+                             f"[{self.T}, {heads}, {pool.head_dim}]")
+
+    def _check_heads(self, q: torch.Tensor) -> None:
+        pool = self.pool
+        if q.shape != (self.T, pool.n_heads, pool.head_dim) or q.dtype != pool.storage.dtype:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype}: expected [{self.T}, {pool.n_heads}, "
+                             f"{pool.head_dim}] {pool.storage.dtype}")
+        require_here(pool.storage, q)
+
     def bind(self, T: int) -> None:
         if T != self.T:
             raise ValueError(f"the forward brings {T} tokens, the adapter was made for {self.T}")
@@ -298,6 +319,12 @@ class PageSlots:
         self._current()
         if pool.storage.dtype != torch.float16 or pool.head_dim != 128:
             raise ValueError("rotary embedding is for fp16 pages of head_dim 128")
+        self._check_rows(qkv, pool.n_heads + 2 * pool.n_kv_heads)
+        if positions.numel() != 3 * self.T or positions.dtype != torch.int64 or \
+                not positions.is_contiguous():
+            raise ValueError(f"positions {tuple(positions.shape)} {positions.dtype}: expected a "
+                             f"contiguous int64 [3, {self.T}]")
+        require_here(pool.storage, qkv, positions)
         if parts is None:
             fn, extra = "omni_mrope_kv_write", ()
         else:
@@ -343,6 +370,9 @@ class PagedPrefill(PageSlots):
 
     def attend_qkv(self, qkv: torch.Tensor, layer_idx: int, scale: float,
                    out: torch.Tensor) -> torch.Tensor:
+        """As PackedPrefillWriter.attend_qkv."""
+        self._check_rows(qkv, self.pool.n_heads, out)
+        require_here(self.pool.storage, qkv, out)
         return prefill_attention_pool(self._prompt, qkv, 0, scale, out)
 
     def flash_prefill(self, q, k, v, layer_idx, scale):
@@ -350,6 +380,7 @@ class PagedPrefill(PageSlots):
         the last layer."""
         pool = self.pool
         self.bind(q.shape[0])
+        self._check_heads(q)
         self.write(k, v, layer_idx)
         (k, ks), (v, vs) = _head_rows(k), _head_rows(v)
         self._copy(k.data_ptr(), ks, v.data_ptr(), vs)
@@ -391,18 +422,11 @@ class PagedDecode(PageSlots):
         """out [n, nh, hd] (contiguous): attention of the rows whose queries are the first nh * hd
         columns of the rows qkv; their K/V is in the pages (rope_and_write)."""
         pool = self.pool
-        width = pool.n_heads * pool.head_dim
-        if qkv.dim() != 2 or qkv.shape[0] != self.n or qkv.shape[1] < width or qkv.stride(1) != 1:
-            raise ValueError(f"query rows of shape {tuple(qkv.shape)}: expected [{self.n}, >= "
-                             f"{width}] with contiguous columns")
-        if not qkv.dtype == out.dtype == pool.storage.dtype:
-            raise TypeError(f"the pages are {pool.storage.dtype} (got {qkv.dtype} -> {out.dtype})")
-        if out.numel() != self.n * width or not out.is_contiguous():
-            raise ValueError(f"attention output of shape {tuple(out.shape)}: expected a contiguous "
-                             f"[{self.n}, {pool.n_heads}, {pool.head_dim}]")
+        self._check_rows(qkv, pool.n_heads, out)
         self._current()
         require_here(pool.storage, qkv, out)
-        stride = qkv.stride(0) if self.n > 1 else max(qkv.stride(0), width)
+        width = pool.n_heads * pool.head_dim
+        stride = qkv.stride(0) if self.n > 1 else width
         return self._attend(qkv.data_ptr(), stride, layer_idx, scale, out)
 
     def _attend(self, q: int, q_stride: int, layer_idx: int, scale: float, out):
@@ -419,9 +443,7 @@ class PagedDecode(PageSlots):
         """The decode views' protocol on rotated tensors: q [n, nh, hd], key / value [n, nkv, hd].
         Writes the K/V rows, attends; lengths on the last layer."""
         pool = self.pool
-        if q.shape != (self.n, pool.n_heads, pool.head_dim) or q.dtype != pool.storage.dtype:
-            raise ValueError(f"q {tuple(q.shape)} {q.dtype}: expected [{self.n}, {pool.n_heads}, "
-                             f"{pool.head_dim}] {pool.storage.dtype}")
+        self._check_heads(q)
         self.write(key, value, layer_idx)
         q, qs = _head_rows(q)
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)

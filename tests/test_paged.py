@@ -148,6 +148,39 @@ def test_cache_checks_its_arguments():
         cache(dtype=torch.bfloat16).prefill_cache([0], [4])
 
 
+def test_adapters_check_their_rows():
+    """Rows, outputs and positions of other sizes or types never reach a kernel."""
+    from omniserver_amd.paged_kv import PagedDecode, PagedPrefill
+    c = cache()
+    qkv, out = torch.zeros(3, 16 * 128).half(), torch.empty(3, 12, 128).half()
+    pos = torch.zeros(3, 3, dtype=torch.int64)
+    q, k = torch.zeros(3, 12, 128).half(), torch.zeros(3, 2, 128).half()
+    for kind in (PagedDecode, PagedPrefill):
+        step = object.__new__(kind)
+        step.pool, step.n, step.T, step._step = c, 3, 3, c._step
+        attend = lambda x, y: step.attend_qkv(x, 0, 0.1, y)
+        rotate = lambda x, p: step.rope_and_write(x, 0, p, None, None, (16, 24, 24))
+        flash = step.flash_decode if kind is PagedDecode else step.flash_prefill
+        for x, y in ((qkv[:2], out), (qkv[:, :1535], out), (qkv.view(-1), out), (qkv, out[:2]),
+                     (qkv.t().contiguous().t(), out), (qkv, out.transpose(0, 1))):
+            with pytest.raises(ValueError):
+                attend(x, y)
+        for x, y in ((qkv.float(), out), (qkv, out.float()), (qkv.bfloat16(), out.bfloat16())):
+            with pytest.raises(TypeError):
+                attend(x, y)
+        for x, p in ((qkv[:, :2047], pos), (qkv[:2], pos), (qkv, pos[:2]), (qkv, pos.int()), (qkv, pos.t()[:2])):
+            with pytest.raises(ValueError):
+                rotate(x, p)
+        with pytest.raises(TypeError):
+            rotate(qkv.float(), pos)
+        for bad in (q[:2], q[:, :11], q[..., :64], q.float()):
+            with pytest.raises(ValueError):
+                flash(bad, k, k, 0, 0.1)
+        for call in (lambda: attend(qkv, out), lambda: rotate(qkv, pos), lambda: flash(q, k, k, 0, 0.1)):
+            with pytest.raises(RuntimeError, match="GPU only"):
+                call()
+
+
 def test_select_checks_its_arguments():
     from omniserver_amd.beam import select
     logits, scores = torch.zeros(2, 3, 50), torch.zeros(2, 3)
