@@ -38,9 +38,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int | None = None,
     device (-1: none).
 
     Ties go to the lower beam, then to the lower token.  A NaN logit counts as -inf, infinite ones
-    share all the weight; tokens at -inf are no continuations, and where a request has fewer than
-    k the rest is -inf, -1, -1, finished.  Values are compared in 64 bits, those within a beam by
-    their logits; the same inputs give the same choice."""
+    share all the weight; tokens at -inf, or whose sum is too low for fp32, are no continuations, and
+    where a request has fewer than k the rest is -inf, -1, -1, finished.  Values are compared in 64
+    bits, those within a beam by their logits; the same inputs give the same choice."""
     if logits.dim() != 3:
         raise ValueError(f"logits of shape {tuple(logits.shape)}: expected [n, beams, vocab]")
     n, W, V = logits.shape

@@ -497,14 +497,16 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
     __syncthreads();
   }
   for (int j = tid; j < a.k; j += 64 * WAVES) {
-    const int b = pick_b[j];
+    int b = pick_b[j];
     int64_t t = -1;
     bool over = true;
     float v = -INFINITY;
-    if (b >= 0) {
+    if (b >= 0) v = (float)value[b][pick_t[j]];
+    if (v > -INFINITY) {
       over = ended[b];
       t = over ? a.pad : __builtin_bit_cast(int, cand[b][pick_t[j]].y);
-      v = (float)value[b][pick_t[j]];
+    } else {
+      b = -1;                                       // also a sum that is too low for 32 bits
     }
     for (int i = 0; i < min(a.stops, BM_MAX_K); ++i) over |= stops[i] == t;
     for (int i = BM_MAX_K; i < a.stops; ++i) over |= a.stop[s * a.stop_stride + i] == t;

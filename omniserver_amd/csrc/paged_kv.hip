@@ -223,8 +223,8 @@ struct ReserveArgs {
 // Token row tok is position p of the sequence, in that page (-1: it has no slot).
 __device__ __forceinline__ void pg_slot(const PageTables& t, const ReserveArgs& r, int tok, int page,
                                         int p, int64_t delta) {
-  const bool ok = page >= 0;
-  r.token_page[tok] = page;
+  const bool ok = page >= 0 && page < t.pages;
+  r.token_page[tok] = ok ? page : -1;
   r.token_pos[tok] = ok ? p & ((1 << t.shift) - 1) : -1;
   for (int a = 0; a < r.axes; ++a) r.positions[(int64_t)a * r.T + tok] = ok ? p + delta : -1;
 }

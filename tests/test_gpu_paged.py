@@ -283,6 +283,23 @@ def test_decode_attention_bad_pages(gpu):
     assert (out[2] == 0).all()
 
 
+def test_reserve_in_a_bad_page(gpu):
+    """A sequence whose last, partly filled page is an entry outside the pool: its new tokens have no
+    place until a page of their own begins."""
+    rng = random.Random(6)
+    cache, tables, lengths = make_cache(gpu, [20, 30, 5], 16, rng, spare=3, max_len=64)
+    cache.tables[0, 1], cache.tables[1, 1] = -7, cache.num_pages
+    free = sorted(set(range(cache.num_pages)) - {tables[0][0], tables[1][0], tables[2][0]})
+    got = cache.reserve([14, 1, 1])
+    assert got.granted.tolist() == [14, 1, 1]
+    assert got.token_page.tolist() == [-1] * 12 + [free[0]] * 2 + [-1, tables[2][0]]
+    assert got.token_pos.tolist() == [-1] * 12 + [0, 1, -1, 5]
+    assert got.positions.tolist() == [-1] * 12 + [32, 33, -1, 5]
+    got = cache.decode_cache(3)
+    assert got.token_page.tolist() == [-1, -1, tables[2][0]]
+    assert got.positions.tolist() == [[-1, -1, 5]] * 3
+
+
 def test_decode_attention_far_pages(gpu):
     """K and V of more than 2^31 elements each."""
     from omniserver_amd.paged_kv import PagedKVCache
@@ -477,6 +494,30 @@ def test_select_close_values(gpu, dtype):
         got = select(logits.to(gpu), scores.to(gpu), k, done.to(gpu))
         assert got.parents.tolist() == [[r[1] for r in q] for q in want], k
         assert got.tokens.tolist() == [[r[2] for r in q] for q in want], k
+
+
+def test_select_lowest_values(gpu):
+    """Logits masked by the type's lowest number are continuations while their sums fit fp32; a sum
+    that does not is none: no parent, no token, finished."""
+    from omniserver_amd.beam import select
+    low = torch.finfo(torch.float32).min
+    logits = torch.full((1, 2, 40), low)
+    logits[0, :, 7] = 1.0
+    got = select(logits.to(gpu), torch.tensor([[0.0, low]], device=gpu), 5)
+    # beam 0: token 7 at 0, the others at low - 1, which is low in 64 bits too; beam 1: token 7 at low,
+    # behind those, the others at 2 low
+    assert got.scores.tolist() == [[0.0] + [low] * 4]
+    assert got.parents.tolist() == [[0] * 5] and got.tokens.tolist() == [[7, 0, 1, 2, 3]]
+    assert got.done.tolist() == [[False] * 5]
+    for W in (1, 2):                                  # one unfinished row; many values in question
+        scores = torch.full((1, 2), low)[:, :W].contiguous().to(gpu)
+        for k in (3, 50):
+            got = select(logits[:, :W].contiguous().to(gpu), scores, k)
+            none = k - W
+            assert got.scores.tolist() == [[low] * W + [-math.inf] * none]
+            assert got.parents.tolist() == [[0, 1][:W] + [-1] * none]
+            assert got.tokens.tolist() == [[7] * W + [-1] * none]
+            assert got.done.tolist() == [[False] * W + [True] * none]
 
 
 def test_select_vector_of_values(gpu):
