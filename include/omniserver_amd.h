@@ -255,7 +255,8 @@ int omni_paged_attention(const void* q, int64_t q_stride, const void* k_cache, c
  * finite is not in use; one with done[s][b] != 0 (bytes, or NULL) goes on as itself, with token pad.
  * stop int64 [stops] (stop_stride 0) or [n][stops] (stop_stride its row stride): tokens that finish.
  * Writes out_scores fp32, parents int32, tokens int64, out_done bytes [n][k], none of them over an
- * input; where there is no continuation, or none whose sum fits fp32, -inf, -1, -1, 1.  workspace: 8-byte words, 16-byte aligned, as many as omni_beam_select_work gives. */
+ * input; where there is no continuation, or none whose sum fits fp32, -inf, -1, -1, 1.  workspace:
+ * 8-byte words, 16-byte aligned, as many as omni_beam_select_work gives. */
 int omni_beam_select_work(int n, int beams, int vocab, int k);
 int omni_beam_select(const void* logits, int dtype, int64_t req_stride, int64_t row_stride,
                      const float* scores, const void* done, const int64_t* stop, int stops,
