@@ -89,15 +89,15 @@ __device__ __forceinline__ float bm_weights(const float (&x)[N], float m) {
 // Where they are too many (equal logits, all of the best in a few lanes) the waves take out their k
 // best one after another, and the four lists are merged.
 //
-// 128 rows of 151936 fp16 logits, 39 MB, 15 us where a copy's rate is 8: of a lane's 32 logits each takes
-// some 9 vector operations (conversion, maximum, fma, a quarter-rate exp2, sum, comparison), 8 us in
-// all, and a workgroup's start, two barriers and list stand beside them.  With weights in 64 bits and
-// the lists taken out one after another it was 59.  4 rows 6.1 us.
+// 128 rows of 151936 fp16 logits, 39 MB, 13.5 us where a copy's rate is 8.  A workgroup is a chain (loads,
+// largest, thresholds, sum, list, with two barriers), and eight waves a SIMD hide it from one another:
+// with five 15, and fewer vector operations (maxima and fma of fp16 pairs as they are) change nothing.
+// With weights in 64 bits and the lists taken out one after another it was 59.  4 rows 6.1 us.
 // ---------------------------------------------------------------------------
 #define BM_CAP 512                 // tokens that are ranked
 
 template <int DT, int EPT>
-__global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
+__global__ __launch_bounds__(64 * BM_WAVES, 8) void beam_scan_kernel(BeamArgs a) {
   typedef SvPiece<DT> P;
   __shared__ float2 list[BM_CAP];
   static_assert(BM_CAP >= BM_WAVES * BM_MAX_K, "the waves' lists");
@@ -118,7 +118,6 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
 #pragma unroll
   for (int e = 0; e < EPT; ++e)
     x[e] = fmaxf(p[e / P::N].get(e % P::N), -INFINITY);       // leaves a NaN out
-  auto token = [&](int e) { return v0 + e / P::N * BM_WAVES * PIECE + lane * P::N + e % P::N; };
   float best[EPT / P::N], own = -INFINITY;          // of a piece, of all
 #pragma unroll
   for (int j = 0; j < EPT / P::N; ++j) {
@@ -208,16 +207,19 @@ __global__ __launch_bounds__(64 * BM_WAVES) void beam_scan_kernel(BeamArgs a) {
   float bv;
   int bt;
   auto next = [&]() {
+    const int first = v0 + lane * P::N, taken = lastt - first;
     bv = -INFINITY;
-    bt = 0x7fffffff;
+    bt = 0;
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
-      const bool behind = x[e] < lastv || (x[e] == lastv && token(e) > lastt);
+      const int t = e / P::N * BM_WAVES * PIECE + e % P::N;
+      const bool behind = x[e] < lastv || (x[e] == lastv && t > taken);
       if (behind && x[e] > bv) {
         bv = x[e];
-        bt = token(e);
+        bt = t;
       }
     }
+    bt += first;
   };
   next();
   for (int j = 0; j < a.k; ++j) {
