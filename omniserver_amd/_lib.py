@@ -179,12 +179,15 @@ def require_cuda(*tensors, dtype=None, contiguous=True) -> None:
 
 def require_here(*tensors) -> None:
     """Refuse tensors off the current device: launches go to its current stream."""
+    here = None
     for t in tensors:
         if t is None:
             continue
         at = t.get_device()
+        if at == here:
+            continue
         if at < 0:
             raise RuntimeError("omniserver_amd ops run on the GPU only (got a CPU tensor)")
-        if at != torch._C._cuda_getDevice():
-            raise RuntimeError(f"tensor on {t.device}, but the current device is "
-                               f"cuda:{torch._C._cuda_getDevice()}")
+        here = torch._C._cuda_getDevice()
+        if at != here:
+            raise RuntimeError(f"tensor on {t.device}, but the current device is cuda:{here}")

@@ -7,6 +7,7 @@ these continue.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -24,6 +25,14 @@ class Selected(NamedTuple):
     parents: torch.Tensor    # int32 [n, k]: the beams they continue, or -1
     tokens: torch.Tensor     # int64 [n, k]: by which token, or -1
     done: torch.Tensor       # bool [n, k]: finished (or none)
+
+
+@lru_cache(maxsize=256)
+def _work(n: int, W: int, V: int, k: int) -> int:
+    work = lib().omni_beam_select_work(n, W, V, k)
+    if work < 0:
+        raise ValueError(f"{n} requests of {W} beams over a vocabulary of {V}: too large")
+    return work
 
 
 def select(logits: torch.Tensor, scores: torch.Tensor, k: int | None = None,
@@ -66,9 +75,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int | None = None,
                    torch.empty(n, k, device=dev, dtype=torch.int32),
                    torch.empty(n, k, device=dev, dtype=torch.int64),
                    torch.empty(n, k, device=dev, dtype=torch.bool))
-    work = lib().omni_beam_select_work(n, W, V, k)
-    if work < 0:
-        raise ValueError(f"{n} requests of {W} beams over a vocabulary of {V}: too large")
+    work = _work(n, W, V, k)
     ws = torch.empty(work, device=dev, dtype=torch.float64)
     call("omni_beam_select", logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0),
          logits.stride(1), scores.data_ptr(), ptr(done), ptr(stop), m,
