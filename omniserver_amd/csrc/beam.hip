@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * BM_WAVES, 8) void beam_scan_kernel(BeamArgs a)
 //
 // A chain of waits: 4 beams, k = 4, 5.9 us; 5 beams, k = 10, 7.8.  Loads of the lists and sums (1 us),
 // sums and logarithm in 64 bits (1), k entries (0.2 each), the count (1.3).  Sixteen waves where the beams
-// are more than eight: 12 beams, k = 12 21.2 us a call, with eight 24.4; 8 x 16, k = 32 47 and 52.
+// are more than eight: 12 beams, k = 12 21.2 us a call, with eight 24.4; 8 x 16, k = 32 48 and 52.
 // ---------------------------------------------------------------------------
 #define BM_AHEAD 4
 // Of a sum, relative: a weight 2^t is off by |t| ln 2 2^-24 of its exponent's rounding (and as
@@ -521,8 +521,8 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
 }
 
 // Tokens of a block, 256 times this: as many as leave a workgroup for every CU twice, or as few.  A call of
-// 8 x 16 beams, k = 16, with 8192 tokens 34.9 us, with 4096 38.7 (more lists to merge); 32 x 4 21.2 and
-// 22.0; 4 x 4 beams over 32003 tokens with 2048 12.4, with 4096 12.9.
+// 8 x 16 beams, k = 16, with 8192 tokens 34.3 us, with 4096 38.2 (more lists to merge); 32 x 4 19.2 and
+// 21.8; 4 x 4 beams over 32003 tokens with 2048 12.4, with 4096 12.9.
 static int bm_ept(int64_t rows, int V) {
   for (int ept = 32; ept > 8; ept /= 2)
     if (rows * ceil_div(V, 256 * ept) >= 512 || V > 128 * ept * BM_MAX_BLOCKS) return ept;
