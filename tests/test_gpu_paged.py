@@ -452,6 +452,28 @@ def test_select(gpu, n, W, k, V, dtype, kind):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("V,dtype", [(300001, torch.float16), (300001, torch.bfloat16), (270000, torch.float32),
+                                     (140003, torch.float16), (9001, torch.float16)])
+def test_select_level_rows(gpu, V, dtype):
+    """Rows of one value with a few above it, in blocks of every size: more equal logits than a block ranks,
+    so that its best are taken out one after another."""
+    from omniserver_amd.beam import select
+    say(f"select level rows {V} {dtype}")
+    g = torch.Generator().manual_seed(V)
+    logits = torch.full((1, 3, V), -0.75)
+    for b, few in enumerate((2, 7, 30)):
+        at = torch.randperm(V, generator=g)[:few]
+        logits[0, b, at] = torch.randint(0, 4, (few,), generator=g).float()
+    logits[0, 2, 5:50] = -math.inf
+    logits[0, 1, 3] = math.nan
+    logits, scores = logits.to(dtype), torch.tensor([[-1.0, -2.5, -0.5]])
+    for k in (3, 40):
+        want = ref.select(logits, scores, k)
+        got = select(logits.to(gpu), scores.to(gpu), k)
+        assert got.parents.tolist() == [[r[1] for r in q] for q in want], k
+        assert got.tokens.tolist() == [[r[2] for r in q] for q in want], k
+
+
 def test_select_defaults_and_strides(gpu):
     """k defaults to the beams; rows that are views of wider ones; one list of stop tokens; nothing
     finished."""
