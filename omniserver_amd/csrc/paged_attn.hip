@@ -104,10 +104,14 @@ struct PaPlace {
 // Keys that are not there (of a page outside the pool, or past the item) have probability 0 and
 // their V taken as 0, whatever the memory holds.
 //
-// P goes into the second product in two 16-bit parts, rounded and rest: the matrix cores are idle
-// otherwise, and the outputs are off by their own rounding alone (2.1e-4 of their size in fp16; with the
-// rounded part alone 2.6e-4, in bf16 1.7e-3 and 2.1e-3).  That costs 3 % (32 x 2048 tokens 15.1 -> 15.7
-// us), which the next step's loads, issued as soon as this one's K and V are used up, give back.
+// P goes into the second product in 16-bit parts that hold its 24 bits (bf16: three) or 22 (fp16: two),
+// rounded, rest, and the rest's rest: the matrix cores are idle otherwise, and the outputs are off by
+// their own rounding alone (2.1e-4 of their size in fp16, 1.7e-3 in bf16; with the rounded part alone
+// 2.6e-4 and 2.1e-3).  The second part costs 3 % (32 x 2048 tokens 15.1 -> 15.7 us), which the next
+// step's loads, issued as soon as this one's K and V are used up, give back.  bf16's third costs up to 3 %
+// (32 x 4096 tokens of 8 KV heads 101.5 -> 103.6 us, 128 x 4096 in groups of 4 beams 32.9 -> 33.7, 64 x
+// 20-4000 of 16 97.1 both): of 65536 outputs 13 are rounded to the other neighbour instead of 128, and
+// where terms cancel an output is no longer off by 2^-18 of them, many of its own steps.
 //
 // The bound is the K/V bytes.  MI355X: a kernel that only reads takes 10.4 us for 64 MB, 19.3 for 128 MB
 // (which the cache holds), 88 for 512 MB (6.1 TB/s).  Here, us with the merge, launches in a row: 32 x
@@ -120,6 +124,7 @@ template <bool BF, int HD, int NT>
 struct PaState {
   static constexpr int CV = HD / 16;                // columns of a V row a lane reads
   static constexpr int KC = HD / 32;                // matrix operands of a K row
+  static constexpr int PARTS = BF ? 3 : 2;          // of a probability
   u32x4 qf[NT][KC];
   f32x4 o[NT][CV];
   float m[NT], l[NT];
@@ -174,7 +179,7 @@ struct PaState {
         for (int j = 0; j < KC; ++j) s[n][b] = pa_mfma<BF>(kf[b][j], qf[n][j], s[n][b]);
       }
     if (more) load_k(a, then, l16, g4);
-    u32x4 pf[NT], rest[NT];
+    u32x4 pf[NT][PARTS];
     float alpha[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -203,9 +208,13 @@ struct PaState {
       }
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const uint32_t w = pa_pack<BF>(p[2 * d], p[2 * d + 1]);
-        pf[n][d] = w;
-        rest[n][d] = pa_pack<BF>(p[2 * d] - pa_half<BF>(w, false), p[2 * d + 1] - pa_half<BF>(w, true));
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const uint32_t w = pa_pack<BF>(p[2 * d], p[2 * d + 1]);
+          pf[n][i][d] = w;
+          p[2 * d] -= pa_half<BF>(w, false);
+          p[2 * d + 1] -= pa_half<BF>(w, true);
+        }
       }
     }
     if (part) {
@@ -226,8 +235,8 @@ struct PaState {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         o[n][t] *= alpha[n];
-        o[n][t] = pa_mfma<BF>(vt, pf[n], o[n][t]);
-        o[n][t] = pa_mfma<BF>(vt, rest[n], o[n][t]);
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) o[n][t] = pa_mfma<BF>(vt, pf[n][i], o[n][t]);
       }
     }
     if (more) load_v(a, then, l16, g4);

@@ -1,0 +1,51 @@
+"""The paged cache's operators and beam search where terms cancel, counts overflow, rows are many or have
+no more room, and what a runner's own sequences keep of a search beside them."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from tests.test_gpu_paged import make_cache, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,parts", [(torch.float16, 2.0 ** -22), (torch.bfloat16, 2.0 ** -24)])
+def test_decode_attention_cancelling_terms(gpu, dtype, parts):
+    """Two keys of nearly the same weight and opposite V: the output is their weights' difference, which
+    a weight held in fewer bits than fp32 would show."""
+    say(f"paged attention of cancelling terms {dtype}")
+    n, nh, nkv, hd = 64, 12, 2, 128
+    rng, g = random.Random(4), torch.Generator().manual_seed(5)
+    cache, tables, lengths = make_cache(gpu, [2] * n, 16, rng, nkv, nh, hd, 1, dtype, spare=1, max_len=16)
+    # scores x + y 2^-13 and x + z 2^-13 of the two keys, exact in fp32, and 0 of the new one, the largest
+    k, v = torch.zeros(n, 3, nkv, hd), torch.zeros(n, 3, nkv, hd)
+    x = -0.25 - 0.5 * torch.rand(n, nkv, generator=g)
+    k[:, 0, :, 0] = k[:, 1, :, 0] = x
+    k[:, :2, :, 1] = torch.rand(n, 2, nkv, generator=g)
+    v[:, 0], v[:, 1] = 1.0, -1.0
+    q = torch.zeros(n, nh, hd)
+    q[:, :, 0], q[:, :, 1] = 1.0, 2.0 ** -13
+    k, v, q = k.to(dtype), v.to(dtype), q.to(dtype)
+    for i, row in enumerate(tables):
+        cache.storage[0, 0, row[0], :2] = k[i, :2].to(gpu)
+        cache.storage[0, 1, row[0], :2] = v[i, :2].to(gpu)
+    step = cache.decode_cache(n)
+    step.write(k[:, 2].contiguous().to(gpu), v[:, 2].contiguous().to(gpu), 0)
+    out = step.attend_qkv(q.view(n, -1).to(gpu), 0, 1.0, torch.empty(n, nh, hd, device=gpu, dtype=dtype))
+    s = k[:, :, :, 0].double() + k[:, :, :, 1].double() * 2.0 ** -13          # [n, 3, nkv]
+    p = torch.exp(s - s.amax(1, keepdim=True))
+    L = p.sum(1)
+    exact = ((p[:, 0] - p[:, 1]) / L).repeat_interleave(nh // nkv, 1)[..., None].expand(n, nh, hd)
+    # a weight: its exponent, below 1.45, off by log2 e's rounding and the product's, 2^-24 of it each, ln 2 of
+    # that relative; 2^-23 for the exponential; and the parts.  Six products added up, sums below 1, are off
+    # by 2^-24 each.  All over L; then the output's rounding, and L's and its reciprocal's
+    weight = 2 * 1.45 * math.log(2) * 2.0 ** -24 + 2.0 ** -23 + parts
+    bound = (((p[:, 0] + p[:, 1]) * weight + 6 * 2.0 ** -24) / L).repeat_interleave(nh // nkv, 1)[..., None]
+    low = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    bound = bound + exact.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -20) + low
+    err = ((out.cpu().double() - exact).abs() / bound).max().item()
+    say(f"  worst error {err:.2f} of the bound")
+    assert err <= 1.0
