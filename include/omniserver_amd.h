@@ -213,7 +213,7 @@ int omni_spec_verify(const void* logits, int dtype, int64_t seq_stride, int64_t 
  * int64 [n] (lengths before and with what is granted; lengths itself stays), token_page and
  * token_pos int64 [tokens] (-1: nowhere), positions int64 [axes <= 3][tokens] (position + rope_delta
  * of the sequence, int64 or NULL; -1 without a slot), granted int32 [n], cu int32 [n + 1] (sums of
- * counts) and, for dense without rows, schedule (int32 [8 n + 4 columns], 16-byte aligned, or NULL)
+ * counts, at most 2^30) and, for dense without rows, schedule (int32 [8 n + 4 columns], 16-byte aligned, or NULL)
  * for omni_paged_attention with the same columns and most: up to `most` neighbouring sequences whose
  * tables begin alike are taken together. */
 int omni_page_reserve(int* tables, int64_t* lengths, int seqs, int width, int pages, int page_size,

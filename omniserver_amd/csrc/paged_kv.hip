@@ -31,8 +31,11 @@ __device__ __forceinline__ int pg_pages(const PageTables& t, int64_t tokens) {
   return (int)((tokens + (1 << t.shift) - 1) >> t.shift);
 }
 
-// Sums of non-negative numbers up to 2^30, which they stay at.
-__device__ __forceinline__ int pg_add(int a, int b) { return min(a + b, 1 << 30); }
+// Sums of non-negative numbers up to 2^30, which they stay at (two of those add up to 2^31, which is
+// no int).
+__device__ __forceinline__ int pg_add(int a, int b) {
+  return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)1 << 30);
+}
 template <bool MAX>
 __device__ __forceinline__ int pg_join(int a, int b) { return MAX ? max(a, b) : pg_add(a, b); }
 // v with what the lane CTRL moves here holds, in the rows of 16 lanes that ROWS names.
@@ -321,12 +324,12 @@ __global__ __launch_bounds__(PG_THREADS) void page_reserve_kernel(PageTables t, 
   if (!r.dense && r.slots_here) {
 #pragma unroll 1
     for (int tok = tid; tok < r.T; tok += PG_THREADS) {
-      const int i = pg_find(last, r.n, tok);
+      const int i = pg_find(last, r.n, tok), in = tok - (i ? last[i - 1] : 0);
       int page = -1, p = 0;
       int64_t row = 0;
-      if (i < r.n && ask[i]) {
+      if (i < r.n && in < ask[i]) {
         row = r.rows ? r.rows[i] : (int64_t)i;
-        p = len[i] + tok - (i ? last[i - 1] : 0);
+        p = len[i] + in;
         page = t.tables[row * t.width + (p >> t.shift)];
       }
       pg_slot(t, r, tok, page, p, page >= 0 && r.rope_delta ? r.rope_delta[row] : 0);
@@ -413,12 +416,12 @@ __global__ __launch_bounds__(256) void page_slots_kernel(PageTables t, ReserveAr
   __syncthreads();
   const int tok = blockIdx.x * 256 + threadIdx.x;
   if (tok >= r.T) return;
-  const int i = pg_find(last, r.n, tok);
+  const int i = pg_find(last, r.n, tok), in = tok - (i ? last[i - 1] : 0);
   int page = -1, p = 0;
   int64_t row = 0;
-  if (i < r.n && r.granted[i]) {
+  if (i < r.n && in < r.granted[i]) {
     row = r.rows ? r.rows[i] : (int64_t)i;
-    p = (int)r.starts[i] + tok - (i ? last[i - 1] : 0);
+    p = (int)r.starts[i] + in;
     page = t.tables[row * t.width + (p >> t.shift)];
   }
   pg_slot(t, r, tok, page, p, page >= 0 && r.rope_delta ? r.rope_delta[row] : 0);

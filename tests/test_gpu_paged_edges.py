@@ -7,7 +7,8 @@ import random
 import pytest
 import torch
 
-from tests.test_gpu_paged import make_cache, say
+from oracle import paged_ref as ref
+from tests.test_gpu_paged import i32, make_cache, say
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,35 @@ def test_decode_attention_cancelling_terms(gpu, dtype, parts):
     err = ((out.cpu().double() - exact).abs() / bound).max().item()
     say(f"  worst error {err:.2f} of the bound")
     assert err <= 1.0
+
+
+@pytest.mark.parametrize("kind", ["packed", "rows", "dense"])
+@pytest.mark.parametrize("n,tokens,where", [(3, 8, (0, 1)), (8, 64, (0, 1, 4, 5)), (8, 64, (2,)), (200, 1500, (60, 61, 62, 130)),
+                                            (200, 4000, (3, 199)), (200, 4000, (150, 151, 152)),
+                                            (1500, 5000, (1100, 1101, 1499)), (1500, 1500, (0, 63, 64, 1030))])
+def test_reserve_counts_beyond_all_sums(gpu, n, tokens, where, kind):
+    """Counts on the device that no sum in 32 bits holds: those requests and the ones behind them in the packed
+    rows go without, whatever the sums, and no row behind them has a place."""
+    say(f"reserve {n} requests, {tokens} rows, counts of 2^30 and more at {where} {kind}")
+    rng = random.Random(n + tokens)
+    lengths = [rng.randint(0, 60) for _ in range(n)]
+    cache, tables, lengths = make_cache(gpu, lengths, 16, rng, spare=3 * n, max_len=128)
+    counts = [rng.randint(0, 5) for _ in range(n)]
+    counts[-1] = 15
+    for j, i in enumerate(where):
+        counts[i] = [(1 << 31) - 1, 1 << 30, (1 << 30) + 5][j % 3]
+    rows = rng.sample(range(n), n) if kind == "rows" else list(range(n))
+    tokens = n if kind == "dense" else tokens
+    new_tables, granted, starts, after, slots = ref.reserve(tables, lengths, counts, rows, cache.num_pages, 16, 128,
+                                                            tokens, kind == "dense")
+    if kind == "dense":
+        got = cache.decode_cache(n, i32(counts, gpu))
+    else:
+        got = cache.reserve(i32(counts, gpu), rows if kind == "rows" else None, tokens)
+    assert got.granted.tolist() == granted
+    assert got.starts.tolist() == starts and got.after.tolist() == after
+    assert got.token_page.tolist() == [s[0] for s in slots]
+    assert got.token_pos.tolist() == [s[1] for s in slots]
+    positions = [s[2] for s in slots]
+    assert got.positions.tolist() == ([positions] * 3 if kind == "dense" else positions)
+    assert cache.tables.tolist() == new_tables
