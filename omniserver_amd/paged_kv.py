@@ -9,7 +9,8 @@ A step asks for room first (``reserve``, or the adapters for a model's forward: 
 ``decode_cache``), writes and attends, and moves the lengths last (``finish``).  ``reorder`` makes
 rows go on from their parents' tables after a beam search's choice (``beam.select``).  All of it
 runs on the device from device tensors, without a host synchronisation, and can be captured in a
-graph: omni_page_reserve, omni_paged_attention, omni_page_reorder.
+graph: omni_page_reserve, omni_paged_attention, omni_page_reorder.  Lists in their place are uploaded,
+which a capture refuses.
 """
 
 from __future__ import annotations

@@ -82,3 +82,46 @@ def test_reserve_counts_beyond_all_sums(gpu, n, tokens, where, kind):
     positions = [s[2] for s in slots]
     assert got.positions.tolist() == ([positions] * 3 if kind == "dense" else positions)
     assert cache.tables.tolist() == new_tables
+
+
+def test_lists_are_refused_in_captured_steps(gpu):
+    """A captured upload would read its staging memory at every replay, when other values are there: lists
+    are refused while a graph is captured, device tensors in their place are not."""
+    from omniserver_amd.beam import select
+    from omniserver_amd.hostio import to_device
+    say("lists while a graph is captured")
+    rng = random.Random(3)
+    cache, tables, lengths = make_cache(gpu, [20, 7, 9, 3], 16, rng, spare=8, max_len=64)
+    logits = torch.randn(2, 2, 50, generator=torch.Generator().manual_seed(1)).half().to(gpu)
+    scores = torch.zeros(2, 2, device=gpu)
+    listed = [lambda: cache.reserve([1, 1]), lambda: cache.reserve(i_counts, rows=[1, 0], tokens=2),
+              lambda: cache.decode_cache(4, [1, 0, 1, 1]), lambda: cache.reorder([[0, 0], [1, 0]]),
+              lambda: cache.free([1]), lambda: cache.prefill_cache([0], [5]),
+              lambda: select(logits, scores, stop=[3]), lambda: to_device([1, 2], torch.int64, gpu)]
+    i_counts, parents, stop = i32([1, 1], gpu), i32([[0, 0], [1, 0]], gpu), torch.tensor([3], device=gpu)
+    select(logits, scores, stop=stop)
+    keep = cache.tables.clone(), cache.lengths.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in listed:
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        got = select(logits, scores, stop=stop)
+        slots = cache.reserve(i_counts, tokens=2)
+        cache.reorder(parents)
+    assert torch.equal(cache.tables, keep[0]) and torch.equal(cache.lengths, keep[1])
+    want = select(logits, scores, stop=[3])
+    new_tables, granted, _, _, places = ref.reserve(tables, lengths, [1, 1], [0, 1], cache.num_pages, 16, 64, 2)
+    for turn in range(3):
+        cache.tables.copy_(keep[0])
+        cache.lengths.copy_(keep[1])
+        [to_device([90 + turn] * 8, torch.int64, gpu) for _ in range(4)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+        assert slots.token_page.tolist() == [p[0] for p in places], turn
+        after, m, _ = ref.reorder(new_tables, lengths, [[0, 0], [1, 0]], cache.num_pages, 16)
+        assert cache.lengths.tolist() == m, turn
+        for r in range(4):
+            held = ref.pages_of(m[r], 16)
+            assert cache.tables[r, :held].tolist() == after[r][:held], (turn, r)
