@@ -26,6 +26,7 @@ from .kv_cache import PreallocatedKVCache, _head_rows, _ints
 
 MAX_PAGES = 1 << 19
 MAX_SEQS = 2048
+MAX_TOKENS = 1 << 28               # packed rows of a reservation
 PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
 UNIT = 128                         # keys of a workgroup's step in omni_paged_attention
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
@@ -192,8 +193,8 @@ class PageSlots:
             raise ValueError(f"{n} requests for {pool.max_seqs if rows is None else len(rows)} "
                              f"sequences")
         T = n if dense else int(tokens)
-        if not 0 <= T <= 1 << 28:
-            raise ValueError(f"{T} packed rows: 0 to {1 << 28}")
+        if not 0 <= T <= MAX_TOKENS:
+            raise ValueError(f"{T} packed rows: 0 to {MAX_TOKENS}")
         self.counts = _ints(counts, (n,), torch.int32, dev, "counts")
         self.rows = _ints(rows, (n,), torch.int64, dev, "rows")
         rope_delta = _ints(rope_delta, None, torch.int64, dev, "rope_delta")
@@ -339,22 +340,27 @@ class PageSlots:
 
 class PagedPrefill(PageSlots):
     """Packed prompts that become sequences ``rows`` (whatever those held is forgotten): causal
-    attention within each.  It runs over a copy of the layer's K/V in rows of one prompt each, by the
-    pool's prefill kernels.  fp16, head_dim 128."""
+    attention within each.  It runs over a copy of the layer's K/V in rows of one prompt each, all as
+    long as the longest, by the pool's prefill kernels.  A call that is refused leaves the rows as they
+    were.  fp16, head_dim 128."""
 
     leaves_rows = False
 
     def __init__(self, pool: PagedKVCache, rows: Sequence[int], seg_lengths: Sequence[int]):
         if pool.storage.dtype != torch.float16 or pool.head_dim != 128:
             raise ValueError("prompts are for fp16 pages of head_dim 128")
-        rows, seg = list(rows), [int(L) for L in seg_lengths]
+        rows, seg = pool._checked_rows(rows), [int(L) for L in seg_lengths]
         if not seg or len(seg) != len(rows) or any(not 1 <= L <= pool.max_len for L in seg):
             raise ValueError(f"prompts of {seg} tokens for rows {rows}: 1 to {pool.max_len} each")
-        pool.free(rows)
-        super().__init__(pool, seg, rows)
+        if sum(seg) > MAX_TOKENS:
+            raise ValueError(f"prompts of {sum(seg)} tokens: up to {MAX_TOKENS} in all")
+        require_here(pool.storage)
+        # all that may be refused before the rows' sequences are forgotten
         one = PreallocatedKVCache(1, len(seg), pool.n_kv_heads, max(seg), 128, pool.device,
                                   n_heads=pool.n_heads)
         self._prompt = one.packed_prefill_cache(range(len(seg)), seg)
+        pool.free(rows)
+        super().__init__(pool, seg, rows)
 
     def rope_and_write(self, qkv, layer_idx, positions, cos_tab, sin_tab, mrope_section,
                        parts=None) -> None:

@@ -148,6 +148,18 @@ def test_cache_checks_its_arguments():
         cache(dtype=torch.bfloat16).prefill_cache([0], [4])
 
 
+def test_refused_prompts_leave_their_rows():
+    """Sequences are forgotten for prompts that are taken, not for those that are refused."""
+    c = cache(page_size=1024, max_len=1 << 28)
+    c.lengths.fill_(5)
+    step = c._step
+    for error, rows, lens in ((ValueError, [0, 1], [1 << 28, 1]), (ValueError, [0, 4], [1, 1]),
+                              (ValueError, [2, 2], [1, 1]), (RuntimeError, [0, 3], [4, 7])):
+        with pytest.raises(error):
+            c.prefill_cache(rows, lens)
+        assert c.lengths.tolist() == [5] * 4 and c._step == step, rows
+
+
 def test_adapters_check_their_rows():
     """Rows, outputs and positions of other sizes or types never reach a kernel."""
     from omniserver_amd.paged_kv import PagedDecode, PagedPrefill
