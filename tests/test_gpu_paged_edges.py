@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from oracle import paged_ref as ref
-from tests.test_gpu_paged import i32, make_cache, say
+from tests import test_gpu_paged as paged
+from tests.test_gpu_paged import check_rows, fill_pages, i32, make_cache, say
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +126,222 @@ def test_lists_are_refused_in_captured_steps(gpu):
         for r in range(4):
             held = ref.pages_of(m[r], 16)
             assert cache.tables[r, :held].tolist() == after[r][:held], (turn, r)
+
+
+def tables_cache(gpu, tables, lengths, pages, page, nkv, nh, hd, dtype, max_len):
+    """A cache that holds these tables (lists as long as the rows' pages) and lengths."""
+    from omniserver_amd.paged_kv import PagedKVCache
+    cache = PagedKVCache(1, pages, nkv, page, hd, gpu, max_seqs=len(tables), max_len=max_len, dtype=dtype,
+                         n_heads=nh)
+    width = cache.tables.shape[1]
+    cache.tables.copy_(torch.tensor([row + [0] * (width - len(row)) for row in tables], dtype=torch.int32))
+    cache.lengths.copy_(torch.tensor(lengths))
+    return cache
+
+
+def common_prompt_rows(layout, page, order):
+    """Tables and lengths of requests (own prompt, beams, new tokens) behind one common prompt."""
+    system, requests = layout
+    first = [order.pop() for _ in range(system // page)]
+    tables, lengths = [], []
+    for prompt, beams, new in requests:
+        shared = first + [order.pop() for _ in range(prompt // page)]
+        for w in range(beams):
+            m = len(shared) * page + new + w
+            tables.append(shared + [order.pop() for _ in range(ref.pages_of(m, page) - len(shared))])
+            lengths.append(m)
+    return tables, lengths
+
+
+COMMON = [
+    # (tokens of the common prompt, (a request's own prompt, beams, new tokens behind it)), heads
+    (512, ((3500, 2, 3), (0, 1, 88), (3500, 2, 3)), 12, 2, 128),
+    (512, tuple((900, 4, 5) for _ in range(6)), 12, 2, 128),
+    (256, tuple((0, 3, 1 + 7 * i) for i in range(9)), 8, 1, 64),
+    (1024, ((128, 5, 0), (2000, 1, 9), (0, 4, 127), (128, 16, 1)), 4, 2, 64),
+]
+
+
+@pytest.mark.parametrize("system,requests,nh,nkv,hd", COMMON)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_decode_attention_common_prompt(gpu, system, requests, nh, nkv, hd, dtype):
+    """Requests that share a common prompt's pages, and each request's beams its own prompt's behind them: groups
+    of rows go over the requests' borders.  And the same rows with copies of all pages to themselves."""
+    say(f"shared pages: common prompt {system}, {len(requests)} requests, heads {nh}/{nkv} x {hd} {dtype}")
+    page, rng, g = 32, random.Random(system + nh), torch.Generator().manual_seed(system)
+    held = sum((system + p + 200) // page * b for p, b, _ in requests) + 8
+    order = list(range(held))
+    rng.shuffle(order)
+    tables, lengths = common_prompt_rows((system, requests), page, order)
+    n, max_len = len(tables), max(lengths) + 1
+    cache = tables_cache(gpu, tables, lengths, held, page, nkv, nh, hd, dtype, max_len)
+    host = fill_pages(cache, cache.tables.tolist(), lengths, g)
+    own = list(range(sum(map(len, tables)) + n))
+    rng.shuffle(own)
+    apart = [[own.pop() for _ in row] for row in tables]
+    alone = tables_cache(gpu, apart, lengths, len(own) + sum(map(len, tables)), page, nkv, nh, hd, dtype, max_len)
+    for row, copy in zip(tables, apart):
+        alone.storage[:, :, copy] = host[:, :, row].to(gpu)
+    qkv = torch.randn(n, (nh + 2 * nkv) * hd, generator=g).to(dtype).to(gpu)
+    q, k, v = qkv.view(n, nh + 2 * nkv, hd).split((nh, nkv, nkv), 1)
+    for c in (cache, alone):
+        step = c.decode_cache(n)
+        step.write(k, v, 0)
+        out = step.attend_qkv(qkv, 0, hd ** -0.5, torch.full((n, nh, hd), 7.0, device=gpu, dtype=dtype))
+        check_rows(out, q, c.storage.cpu(), 0, c.tables.tolist(), [m + 1 for m in lengths], page, hd ** -0.5)
+
+
+def test_decode_attention_many_rows(gpu):
+    """More rows than the scheduling workgroup has threads, in groups, some over its turns' borders."""
+    paged.test_decode_attention_shared(gpu, 260, 5, 300, (0, 40), 16, 6, 1, 64, torch.float16)
+
+
+@pytest.mark.parametrize("rows,length", [(1, 40000), (2, 40001), (3, 65400)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_decode_attention_many_states(gpu, rows, length, dtype):
+    """More states of a row than the merge takes at once: one KV head and a sequence of more than 32768 tokens,
+    alone, and several that share all whole pages."""
+    say(f"{rows} rows of {length} tokens {dtype}")
+    page, nh, nkv, hd = 64, 4, 1, 64
+    shared = length // page
+    order = list(range(shared + rows * 3))
+    random.Random(length).shuffle(order)
+    first = [order.pop() for _ in range(shared)]
+    tables = [first + [order.pop() for _ in range(ref.pages_of(length, page) - shared)] for _ in range(rows)]
+    cache = tables_cache(gpu, tables, [length] * rows, shared + rows * 3, page, nkv, nh, hd, dtype, length + 1)
+    g = torch.Generator().manual_seed(length)
+    fill_pages(cache, cache.tables.tolist(), [length] * rows, g)
+    step = cache.decode_cache(rows)
+    assert step._columns > 256
+    qkv = (2 * torch.randn(rows, (nh + 2 * nkv) * hd, generator=g)).to(dtype).to(gpu)
+    q, k, v = qkv.view(rows, nh + 2 * nkv, hd).split((nh, nkv, nkv), 1)
+    step.write(k, v, 0)
+    out = step.attend_qkv(qkv, 0, hd ** -0.5, torch.full((rows, nh, hd), 7.0, device=gpu, dtype=dtype))
+    check_rows(out, q, cache.storage.cpu(), 0, cache.tables.tolist(), [length + 1] * rows, page, hd ** -0.5)
+
+
+def test_select_stop_lists(gpu):
+    """More stop tokens than a workgroup keeps at hand, the same for all requests or each its own; none."""
+    from omniserver_amd.beam import select
+    g = torch.Generator().manual_seed(6)
+    n, W, V = 3, 3, 400
+    logits = torch.randn(n, W, V, generator=g).half() * 3
+    scores = -torch.rand(n, W, generator=g)
+    stops = torch.stack([torch.randperm(V, generator=g)[:150] for _ in range(n)])
+    for stop in ([], stops[0].tolist(), stops):
+        want = ref.select(logits, scores, 8, None, stop.tolist() if torch.is_tensor(stop) else stop or None)
+        got = select(logits.to(gpu), scores.to(gpu), 8, stop=stop.to(gpu) if torch.is_tensor(stop) else stop)
+        for name, i in (("parents", 1), ("tokens", 2), ("done", 3)):
+            assert getattr(got, name).tolist() == [[r[i] for r in q] for q in want], (name, len(stop))
+
+
+# ----------------------------------------------------------------------------- the runner
+def runner_of(shape, w, quant, use_graph, running=2):
+    from omniserver_amd.runner import NativeQwenVLRunner
+    return NativeQwenVLRunner(max_running=running, max_len=160, use_graph=use_graph, weights=w, quant=quant)
+
+
+def sequence(prompt, steps, images=None):
+    from omniserver_amd.request import Request, SamplingParams, Sequence
+    return Sequence(Request(prompt=list(prompt), sampling=SamplingParams(max_new_tokens=steps), images=images))
+
+
+@pytest.mark.parametrize("quant,use_graph", [(None, False), (None, True), ("gptq", False), ("gptq", True)])
+def test_beam_search_leaves_running_sequences(gpu, quant, use_graph):
+    """Two runners of the same weights decode the same sequences; one of them searches beams in between (with
+    graphs behind a step that is enqueued ahead): the same tokens, lengths and K/V rows."""
+    from omniserver_amd import synth
+    say(f"beam search beside running sequences quant={quant} use_graph={use_graph}")
+    shape = synth.DecoderShape()
+    w = (synth.gptq_decoder if quant else synth.fp16_decoder)(shape, seed=7, num_layers=2)
+    prompts = [synth.random_ids(L, shape.vocab_size, 7, f"p{L}").tolist() for L in (33, 50, 20)]
+    runners = [runner_of(shape, w, quant, use_graph) for _ in range(2)]
+    running = [[sequence(p, 60) for p in prompts[:2]] for _ in runners]
+    for r, seqs in zip(runners, running):
+        r.prefill(seqs)
+    for turn in range(4):
+        for i, (r, seqs) in enumerate(zip(runners, running)):
+            for _ in range(3):
+                r.decode(seqs)
+            if i == 0 and turn < 3:
+                assert len(r.beam_search([sequence(p, 7 + turn) for p in prompts[turn:]], beams=3,
+                                         page_size=16)) == 3 - turn
+    for r in runners:
+        r.settle()
+    torch.cuda.synchronize()
+    assert [s.output_token_ids for s in running[0]] == [s.output_token_ids for s in running[1]]
+    assert len(running[0][0].output_token_ids) == 13
+    a, b = (r.pool for r in runners)
+    lengths = a.lengths.tolist()
+    assert lengths[:2] == [33 + 12, 50 + 12] and lengths[:2] == b.lengths.tolist()[:2]
+    for slot in range(2):
+        assert torch.equal(a.storage[:, :, slot, :lengths[slot]].view(torch.int16),
+                           b.storage[:, :, slot, :lengths[slot]].view(torch.int16))
+
+
+@pytest.mark.parametrize("quant,use_graph", [(None, True), ("gptq", False)])
+def test_one_beam_is_the_greedy_stream(gpu, quant, use_graph):
+    """One beam takes, at every step, the token that the oracle's logits behind the same tokens put first, wherever
+    their margin is larger than what logits may be off."""
+    from omniserver_amd import synth
+    from tests.helpers import check_stream, oracle_from_fp16, oracle_from_gptq, oracle_stream_logits
+    say(f"one beam quant={quant} use_graph={use_graph}")
+    shape = synth.DecoderShape()
+    w = (synth.gptq_decoder if quant else synth.fp16_decoder)(shape, seed=7, num_layers=2)
+    orc = oracle_from_gptq(w, shape) if quant else oracle_from_fp16(w, shape)
+    r = runner_of(shape, w, quant, use_graph)
+    prompts = [synth.random_ids(L, shape.vocab_size, 7, f"p{L}").tolist() for L in (31, 12)]
+    found = r.beam_search([sequence(p, 8) for p in prompts], beams=1)
+    for p, (beam,) in zip(prompts, found):
+        rows = torch.as_tensor(oracle_stream_logits(orc, p, beam.tokens, 256))
+        # logits within 2e-2 of the oracle's: two of them within twice that of each other
+        check_stream(beam.tokens, rows, 2 * 2e-2, 4, "beam")
+
+
+def test_beam_search_with_images(gpu):
+    """Prompts with images, whose rotary positions do not follow their lengths: every step's positions are those of
+    the prompt's continuation, and the beams' log-probabilities those of one forward over prompt and beam."""
+    from omniserver_amd import synth
+    from omniserver_amd.kv_cache import PreallocatedKVCache
+    from omniserver_amd.positions import IMAGE_TOKEN_ID, VISION_START_TOKEN_ID
+    from omniserver_amd.request import VisionInput
+    say("beam search with images")
+    shape = synth.DecoderShape()
+    r = runner_of(shape, synth.fp16_decoder(shape, seed=9, num_layers=2), None, False)
+    images = [VisionInput(synth.randn16((16, shape.hidden_size), 1.0, 9, "img").to(gpu), (1, 8, 8))]
+    prompts = [synth.random_ids(L, shape.vocab_size, 9, f"p{L}").tolist() for L in (45, 30)]
+    prompts[0][10:27] = [VISION_START_TOKEN_ID] + [IMAGE_TOKEN_ID] * 16
+    W, steps = 3, 6
+    seqs = [sequence(prompts[0], steps, images), sequence(prompts[1], steps)]
+    seen, llm = [], r.adapter.llm
+
+    def watched(emb, pos, *rest, **kw):
+        seen.append(pos.cpu())
+        return llm(emb, pos, *rest, **kw)
+
+    r.adapter.llm = watched
+    try:
+        found = r.beam_search(seqs, beams=W, page_size=16)
+    finally:
+        r.adapter.llm = llm
+    assert len(seen) == steps
+    deltas = [r.adapter.prefill_positions(torch.tensor(s.prompt_token_ids).numpy(),
+                                          [im.grid for im in s.request.images] if s.request.images else None)[1]
+              for s in seqs]
+    assert int(deltas[0]) < 0 == int(deltas[1])
+    for t, pos in enumerate(seen[1:]):
+        want = [len(p) + t + int(d) for p, d in zip(prompts, deltas) for _ in range(W)]
+        assert pos.view(3, -1).tolist() == [want] * 3, t
+    for s, beams in zip(seqs, found):
+        L = len(s.prompt_token_ids)
+        for b in beams:
+            line = sequence(list(s.prompt_token_ids) + b.tokens[:-1], 1, s.request.images)
+            with torch.inference_mode():
+                packed, pos, lens, _, _ = r._pack_prompts([line])
+                pool = PreallocatedKVCache(2, 1, 2, lens[0], 128, gpu, n_heads=12)
+                rows = llm(packed, pos, None, pool.packed_prefill_cache([0], lens),
+                           logits_indices=list(range(L - 1, lens[0])))[0]
+            lp = torch.log_softmax(rows.double(), -1).cpu()
+            exact = sum(float(lp[i, t]) for i, t in enumerate(b.tokens))
+            # two routes of the model, logits within 2e-2 each: log-probabilities within four times that
+            assert abs(b.logprob - exact) <= 4 * 2e-2 * len(b.tokens)
