@@ -245,8 +245,8 @@ int omni_page_reorder(void* pool, int n_layers, int row_halfs, int* tables, int6
 int omni_paged_attention(const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
                          int dtype, int pages, int page_size, const int* tables, int width, int n,
                          const int* schedule, int columns, int most, void* out,
-                         int64_t out_stride, int n_heads, int n_kv_heads, int head_dim, float scale, float* workspace,
-                         int64_t workspace_floats, void* stream);
+                         int64_t out_stride, int n_heads, int n_kv_heads, int head_dim, float scale,
+                         float* workspace, int64_t workspace_floats, void* stream);
 
 /* Beam search's choice: the k <= 64 best continuations of each of n requests over its beams <= 32
  * and the vocabulary (up to 524288).  logits [n][beams][vocab] (dtype 0 fp16, 1 bf16, 2 fp32;
@@ -254,9 +254,10 @@ int omni_paged_attention(const void* q, int64_t q_stride, const void* k_cache, c
  * row, compared in 64 bits, ties to the lower beam, then token; a beam with a score that is not
  * finite is not in use; one with done[s][b] != 0 (bytes, or NULL) goes on as itself, with token pad.
  * stop int64 [stops] (stop_stride 0) or [n][stops] (stop_stride its row stride): tokens that finish.
- * Writes out_scores fp32, parents int32, tokens int64, out_done bytes [n][k], none of them over an
- * input; where there is no continuation, or none whose sum fits fp32, -inf, -1, -1, 1.  workspace:
- * 8-byte words, 16-byte aligned, as many as omni_beam_select_work gives. */
+ * Writes out_scores fp32 (with the logarithm of a 32-bit sum where no other beam's value stood close:
+ * off by 4e-6 at most beside their rounding), parents int32, tokens int64, out_done bytes [n][k],
+ * none of them over an input; where there is no continuation, or none whose sum fits fp32, -inf, -1,
+ * -1, 1.  workspace: 8-byte words, 16-byte aligned, as many as omni_beam_select_work gives. */
 int omni_beam_select_work(int n, int beams, int vocab, int k);
 int omni_beam_select(const void* logits, int dtype, int64_t req_stride, int64_t row_stride,
                      const float* scores, const void* done, const int64_t* stop, int stops,

@@ -49,7 +49,10 @@ def select(logits: torch.Tensor, scores: torch.Tensor, k: int | None = None,
     Ties go to the lower beam, then to the lower token.  A NaN logit counts as -inf, infinite ones
     share all the weight; tokens at -inf, or whose sum is too low for fp32, are no continuations, and
     where a request has fewer than k the rest is -inf, -1, -1, finished.  Values are compared in 64
-    bits, those within a beam by their logits; the same inputs give the same choice."""
+    bits, those within a beam by their logits; the same inputs give the same choice.  The scores given
+    out are fp32, and where no other beam's value stood close they have the logarithm of a sum in 32 bits
+    in them: off by 4e-6 at most beside their rounding.  A list of stop tokens is uploaded, which a
+    capture refuses."""
     if logits.dim() != 3:
         raise ValueError(f"logits of shape {tuple(logits.shape)}: expected [n, beams, vocab]")
     n, W, V = logits.shape

@@ -250,11 +250,13 @@ __global__ __launch_bounds__(64 * BM_WAVES, 8) void beam_scan_kernel(BeamArgs a)
 // ---------------------------------------------------------------------------
 // The choice, one workgroup a request.  A wave merges the lists of a row (a list a lane, the next
 // four of it in registers) and makes values of their logits; then every value counts the ones before
-// it by a search in each other row.
+// it: among all, where these are 64 at most, a value a lane; else among those that reach the k-th best
+// of the rows' first few values, or stand close below it.
 //
 // The rows' 32-bit sums are good to BM_ERR, and so are the values.  Where two rows' values stand
 // closer than twice that and one of them is among the k, the sums of those rows are made again in 64
-// bits, and the order with them.
+// bits, and the order with them.  The scores of rows that are not stay as they are, 4e-6 off at most
+// (3e-8 on a language model's rows, which is fp32's rounding).
 //
 // A chain of waits: 4 beams, k = 4, 5.9 us; 5 beams, k = 10, 7.8.  Loads of the lists and sums (1 us),
 // sums and logarithm in 64 bits (1), k entries (0.2 each), the count (1.3).  Sixteen waves where the beams
@@ -520,9 +522,10 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(BeamArgs a) {
   }
 }
 
-// Tokens of a block, 256 times this: as many as leave a workgroup for every CU twice, or as few.  A call of
-// 8 x 16 beams, k = 16, with 8192 tokens 34.3 us, with 4096 38.2 (more lists to merge); 32 x 4 19.2 and
-// 21.8; 4 x 4 beams over 32003 tokens with 2048 12.4, with 4096 12.9.
+// Tokens of a block, 256 times this: as many as leave a workgroup for every CU twice, or as few.  A call in
+// a graph of ten (among others, with its outputs' allocation, 32 x 4 take 20.9) of 8 x 16 beams, k = 16, with
+// 8192 tokens 34.3 us, with 4096 38.2 (more lists to merge); 32 x 4 19.2 and 21.8; 4 x 4 beams over 32003
+// tokens with 2048 12.4, with 4096 12.9.
 static int bm_ept(int64_t rows, int V) {
   for (int ept = 32; ept > 8; ept /= 2)
     if (rows * ceil_div(V, 256 * ept) >= 512 || V > 128 * ept * BM_MAX_BLOCKS) return ept;

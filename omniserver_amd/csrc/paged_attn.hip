@@ -1,8 +1,8 @@
 // Attention of one new token per sequence over a paged KV cache, split over the cache's length.
 //
 // Row i of the schedule (omni_page_reserve) attends to keys [0, keys_i) of the sequence whose block
-// table is tables[i]: softmax(scale q K^T) V, heads grouped.  What the tables of neighbours share is
-// read once for all of them.
+// table is tables[i]: softmax(scale q K^T) V, heads grouped.  What the tables of a group of neighbours
+// share is read once for all of them.
 #include "common.h"
 
 #include <type_traits>
@@ -114,9 +114,11 @@ struct PaPlace {
 // where terms cancel an output is no longer off by 2^-18 of them, many of its own steps.
 //
 // The bound is the K/V bytes.  MI355X: a kernel that only reads takes 10.4 us for 64 MB, 19.3 for 128 MB
-// (which the cache holds), 88 for 512 MB (6.1 TB/s).  Here, us with the merge, launches in a row: 32 x
-// 2048 tokens of 2 KV heads 18.8 (67 MB; 15.5 + 3.9), 32 x 2048 of 16 96 (538 MB, 5.5 TB/s), 32 x 4096 of
-// 8 102, 200 x 1000 of 4 83, 128 x 4096 of 2 in groups of 4 beams 32.3 (131 MB; each row for itself 79).
+// (which the cache holds), 88 for 512 MB (6.1 TB/s).  Here, us with the merge, launches in a row over one
+// layer's K/V (of which the cache holds 256 MB): 32 x 2048 tokens of 2 KV heads 18.8 (67 MB; 15.5 + 3.9),
+// 32 x 2048 of 16 96 (538 MB, 5.5 TB/s), 32 x 4096 of 8 102, 200 x 1000 of 4 83, 128 x 4096 of 2 in groups
+// of 4 beams 32 (131 MB; each row for itself 79).  Over 28 layers one after another, as a step has it: 32 x
+// 2048 22, the groups 38, one row of 32000 tokens of 4 heads 20 (66 MB; 18 from the cache).
 // What is left of the small ones is start and end: schedule, table and Q loads behind each other (3 us),
 // the waves' merge through LDS, the merging launch.
 // ---------------------------------------------------------------------------

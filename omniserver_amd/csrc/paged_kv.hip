@@ -196,8 +196,10 @@ __device__ __forceinline__ void pg_deal(const PgShare& own, const uint32_t* used
 //
 // And the attention's schedule for single tokens (paged_attn.hip).  Neighbouring sequences whose
 // tables begin with the same pages, for half of the shorter one's length or more, form groups of up to
-// `most`: what they share, in whole units of PG_UNIT keys, is one item, read once for all of them, and
-// the rest of each is another.  The items stand in one line, every group's shared one before its
+// `most`: what they all share, in whole units of PG_UNIT keys, is one item, read once for all of them,
+// and the rest of each is another.  Runs are cut at multiples of `most` whatever they share, and the least
+// that two neighbours of a group share is what counts for it: beams of two requests in a group share the
+// requests' common prompt and no more.  The items stand in one line, every group's shared one before its
 // rows', that is cut into at most ncols equal stretches, one a column of workgroups:
 //   row     (keys, shared units, the group's first row, its rows,
 //            first and last column of the shared item, of the row's own)

@@ -408,7 +408,9 @@ class PagedDecode(PageSlots):
     The sequences' keys stand in one line that is cut into equal stretches for the attention's
     workgroups, so that one long sequence among short ones takes no longer than its share; the pages
     that the tables of neighbours begin with alike (beams of one prompt) stand there, and are read,
-    once for several of them."""
+    once for a group of up to 32 queries a KV head.  What a group shares is the least that two neighbours
+    in it do: keep rows that share most next to each other.  The split states are the adapter's own, one
+    for all layers: its calls go to one stream at a time."""
 
     leaves_rows = False
 
