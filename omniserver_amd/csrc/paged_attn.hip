@@ -113,6 +113,11 @@ struct PaPlace {
 // 20-4000 of 16 97.1 both): of 65536 outputs 13 are rounded to the other neighbour instead of 128, and
 // where terms cancel an output is no longer off by 2^-18 of them, many of its own steps.
 //
+// In fp16 all of them, and the sums with them, are 2^15 times as large: its steps end at 2^-24, and of a
+// largest probability of 1 the keys below 2^-25 that a wave has beside it would be gone from the product
+// though not from the sum (60 keys of 2^-20 to 2^-35 beside one of 1: an output 2.5 times as far off as
+// fp32's would be).  Of 2^15 a step is 2^-39.
+//
 // The bound is the K/V bytes.  MI355X: a kernel that only reads takes 10.4 us for 64 MB, 19.3 for 128 MB
 // (which the cache holds), 88 for 512 MB (6.1 TB/s).  Here, us with the merge, launches in a row over one
 // layer's K/V (of which the cache holds 256 MB): 32 x 2048 tokens of 2 KV heads 18.8 (67 MB; 15.5 + 3.9),
@@ -127,6 +132,7 @@ struct PaState {
   static constexpr int CV = HD / 16;                // columns of a V row a lane reads
   static constexpr int KC = HD / 32;                // matrix operands of a K row
   static constexpr int PARTS = BF ? 3 : 2;          // of a probability
+  static constexpr float UNIT_P = BF ? 1.f : 0x1p15f;   // the largest probability, and what l counts in
   u32x4 qf[NT][KC];
   f32x4 o[NT][CV];
   float m[NT], l[NT];
@@ -205,7 +211,7 @@ struct PaState {
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = exp2f(s[n][e >> 2][e & 3] - ref);
+        p[e] = __builtin_amdgcn_exp2f(s[n][e >> 2][e & 3] - ref) * UNIT_P;   // 0 below 2^-126
         l[n] += p[e];
       }
 #pragma unroll

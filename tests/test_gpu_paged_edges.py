@@ -53,6 +53,47 @@ def test_decode_attention_cancelling_terms(gpu, dtype, parts):
     assert err <= 1.0
 
 
+@pytest.mark.parametrize("rows,length", [(1, 60), (3, 3000), (1, 40000), (2, 65000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_decode_attention_small_weights(gpu, rows, length, dtype):
+    """One key far above all others, whose weights are 2^-20 to 2^-35 of its own: they count with their V, however
+    small a type's smallest number leaves them."""
+    say(f"paged attention of small weights, {rows} x {length} {dtype}")
+    page, nh, nkv, hd = 64, 4, 1, 64
+    rng, g = random.Random(length), torch.Generator().manual_seed(length)
+    cache, tables, lengths = make_cache(gpu, [length] * rows, page, rng, nkv, nh, hd, 1, dtype, spare=rows,
+                                        max_len=length + 1, shared=rows)
+    k = torch.zeros(rows, length, nkv, hd)
+    # scores of whole sixteenths, exact; those of a shared page are the same rows'
+    k[..., 0] = -14 - torch.randint(0, 160, (1, length, 1), generator=g) / 16.0
+    k[:, 0] = 0.0
+    v = torch.rand(1, length, nkv, hd, generator=g).expand(rows, -1, -1, -1).clone()
+    v[:, 0] = 0.0
+    k, v = k.to(dtype), v.to(dtype)
+    for r, row in enumerate(tables):
+        pages = torch.tensor(row[:ref.pages_of(length, page)], device=gpu)
+        for i, x in enumerate((k, v)):
+            full = torch.zeros(len(pages) * page, nkv, hd, dtype=dtype)
+            full[:length] = x[r]
+            cache.storage[0, i, pages] = full.view(-1, page, nkv, hd).to(gpu)
+    q = torch.zeros(rows, nh, hd, dtype=dtype)
+    q[..., 0] = 1.0
+    new = torch.zeros(rows, nkv, hd, dtype=dtype)
+    low = new.clone()
+    low[..., 0] = -18.0
+    step = cache.decode_cache(rows)
+    step.write(low.to(gpu), (new + 1).to(gpu), 0)
+    out = step.attend_qkv(q.view(rows, -1).to(gpu), 0, 1.0, torch.empty(rows, nh, hd, device=gpu, dtype=dtype)).cpu()
+    for r in range(rows):
+        want, mag = ref.attention(q[r], torch.cat([k[r], low[r:r + 1]]), torch.cat([v[r], new[r:r + 1] + 1]), 1.0)
+        # the output's rounding; fp32 scores, sums and exponentials, 2^-13 of the weights; and a weight 2^-40 of
+        # the largest away from what it is: fp16's step of 2^-24, halved, where the largest weight is 2^15
+        bound = want.abs() * torch.finfo(dtype).eps / 2 + mag * 2.0 ** -13 + (length + 1) * 2.0 ** -40 + 2.0 ** -25
+        err = ((out[r].double() - want).abs() / bound).max().item()
+        say(f"  row {r}: output {float(want[0, 0]):.2e}, error {err:.2f} of the bound")
+        assert err <= 1.0
+
+
 @pytest.mark.parametrize("kind", ["packed", "rows", "dense"])
 @pytest.mark.parametrize("n,tokens,where", [(3, 8, (0, 1)), (8, 64, (0, 1, 4, 5)), (8, 64, (2,)), (200, 1500, (60, 61, 62, 130)),
                                             (200, 4000, (3, 199)), (200, 4000, (150, 151, 152)),
